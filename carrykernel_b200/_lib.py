@@ -24,7 +24,7 @@ F32, BF16, F16 = 0, 1, 2
 RES_FP32, RES_FP16, RES_FP8, RES_INT8, RES_INT4, RES_NONE = 0, 1, 2, 3, 4, 5
 SCALE_PER_V, SCALE_PER_HEAD = 0, 1
 EPS_ON_AMAX, EPS_ON_SCALE = 0, 1
-STATUS_BAD_SLOT, STATUS_TIMEOUT = 1, 2
+STATUS_BAD_SLOT, STATUS_TIMEOUT, STATUS_BAD_RANGE = 1, 2, 4
 
 _DTYPE_ID = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
@@ -130,11 +130,56 @@ class PoolCopyLayersArgs(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p), ("k_scale", C.c_void_p), ("v_codes", C.c_void_p), ("v_scale", C.c_void_p),
+        ("stride_k_page", C.c_int64), ("stride_ks_page", C.c_int64),
+        ("stride_v_page", C.c_int64), ("stride_vs_page", C.c_int64),
+        ("block_table", C.c_void_p), ("stride_table", C.c_int64), ("lengths", C.c_void_p),
+        ("num_pages", C.c_int32), ("HKV", C.c_int32), ("page", C.c_int32), ("block", C.c_int32),
+        ("D", C.c_int32), ("max_pages", C.c_int32),
+    ]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("query_start", C.c_void_p), ("B", C.c_int32), ("N", C.c_int32), ("max_query", C.c_int32)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [
+        ("cache", KvCache), ("rows", KvRows), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("stride_k_tok", C.c_int64), ("stride_k_head", C.c_int64),
+        ("stride_v_tok", C.c_int64), ("stride_v_head", C.c_int64),
+        ("dtype", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
+class KvAttentionArgs(C.Structure):
+    _fields_ = [
+        ("cache", KvCache), ("rows", KvRows),
+        ("q", C.c_void_p), ("stride_q_tok", C.c_int64), ("stride_q_head", C.c_int64),
+        ("out", C.c_void_p), ("stride_out_tok", C.c_int64), ("stride_out_head", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("scale", C.c_float), ("HQ", C.c_int32), ("dtype", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("residual_out", C.c_void_p), ("weight", C.c_void_p),
+        ("codes", C.c_void_p), ("scale", C.c_void_p),
+        ("stride_x", C.c_int64), ("stride_residual", C.c_int64), ("stride_residual_out", C.c_int64),
+        ("stride_codes", C.c_int64), ("eps", C.c_float), ("N", C.c_int32), ("W", C.c_int32), ("group", C.c_int32),
+        ("x_dtype", C.c_int32), ("residual_dtype", C.c_int32), ("weight_dtype", C.c_int32),
+    ]
+
+
 ERR_UNSUPPORTED = -5
 
 EXPORTS = ("carry_gdn_quant_step", "carry_gdn_quant_decode", "carry_gdn_fp32_step", "carry_gdn_packed_decode",
            "carry_gdn_packed_decode_multi", "carry_gdn_pool_store", "carry_gdn_pool_load",
-           "carry_gdn_pool_copy", "carry_gdn_pool_copy_layers", "carry_gdn_strerror",
+           "carry_gdn_pool_copy", "carry_gdn_pool_copy_layers", "carry_gdn_kv_append", "carry_gdn_kv_attention",
+           "carry_gdn_kv_attention_workspace", "carry_gdn_add_rms_norm_quant", "carry_gdn_strerror",
            "carry_gdn_abi_version", "carry_gdn_last_kernel")
 # what the native call path is given the addresses of, in the order it expects them (csrc/host_native.cpp, Table)
 _NATIVE_ENTRIES = ("carry_gdn_quant_step", "carry_gdn_fp32_step", "carry_gdn_packed_decode",
@@ -198,9 +243,15 @@ def load_library(path: str | None = None):
         lib.carry_gdn_pool_load.argtypes = [C.POINTER(PoolLoadArgs), C.c_void_p]
         lib.carry_gdn_pool_copy.argtypes = [C.POINTER(PoolCopyArgs), C.c_void_p]
         lib.carry_gdn_pool_copy_layers.argtypes = [C.POINTER(PoolCopyLayersArgs), C.c_void_p]
+        lib.carry_gdn_kv_append.argtypes = [C.POINTER(KvAppendArgs), C.c_void_p]
+        lib.carry_gdn_kv_attention.argtypes = [C.POINTER(KvAttentionArgs), C.c_void_p]
+        lib.carry_gdn_kv_attention_workspace.argtypes = [C.POINTER(KvAttentionArgs)]
+        lib.carry_gdn_kv_attention_workspace.restype = C.c_int64
+        lib.carry_gdn_add_rms_norm_quant.argtypes = [C.POINTER(NormArgs), C.c_void_p]
         for fn in (lib.carry_gdn_quant_step, lib.carry_gdn_fp32_step, lib.carry_gdn_packed_decode,
                    lib.carry_gdn_packed_decode_multi, lib.carry_gdn_pool_store, lib.carry_gdn_pool_load,
-                   lib.carry_gdn_pool_copy, lib.carry_gdn_pool_copy_layers, lib.carry_gdn_quant_decode):
+                   lib.carry_gdn_pool_copy, lib.carry_gdn_pool_copy_layers, lib.carry_gdn_quant_decode,
+                   lib.carry_gdn_kv_append, lib.carry_gdn_kv_attention, lib.carry_gdn_add_rms_norm_quant):
             fn.restype = C.c_int
         lib.native, lib.native_table = _NoNative(), None
         try:
@@ -270,7 +321,8 @@ def raise_for_status(status: torch.Tensor, what: str = "carry_gdn"):
     bits = int(status.item())
     if bits:
         names = [n for b, n in ((STATUS_BAD_SLOT, "slot id beyond the pool (treated as padding)"),
-                                (STATUS_TIMEOUT, "a wait on data in flight ran out (tiles left untouched)"))
+                                (STATUS_TIMEOUT, "a wait on data in flight ran out (tiles left untouched)"),
+                                (STATUS_BAD_RANGE, "a page id, length or query range outside the call's bounds (skipped)"))
                  if bits & b]
         raise RuntimeError(f"{what}: device status {bits}: " + "; ".join(names))
 

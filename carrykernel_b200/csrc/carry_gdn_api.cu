@@ -1,6 +1,7 @@
 // C ABI of libcarry_gdn.so: argument checks and kernel selection.  See
 // include/carry_gdn.h for the contract of every entry point.
 #include "carry_gdn_common.cuh"
+#include "carry_hybrid.cuh"
 
 #include <initializer_list>
 
@@ -288,6 +289,84 @@ int carry_gdn_pool_copy_layers(const CarryGdnPoolCopyLayersArgs* a, void* stream
   }
   const int rc = carry::launch_pool_copy_layers(*a, static_cast<cudaStream_t>(stream));
   if (rc == CARRY_GDN_OK) g_last_kernel = 4;
+  return rc;
+}
+
+namespace {
+// what append and attention share: the cache and the rows, pointers apart
+int kv_ok(const CarryGdnKvCache& c, const CarryGdnKvRows& r) {
+  if (c.num_pages < 0 || c.max_pages < 0 || c.HKV <= 0 || c.page <= 0 || c.block <= 0 || c.D <= 0) return CARRY_GDN_ERR_SHAPE;
+  if (c.page % 16 || c.block % 16 || c.page % c.block) return CARRY_GDN_ERR_SHAPE;
+  if ((c.D != 64 && c.D != 128) || c.block > 128) return CARRY_GDN_ERR_UNSUPPORTED;
+  if (r.B < 0 || r.N < 0 || r.max_query < 0) return CARRY_GDN_ERR_SHAPE;
+  if (!r.query_start && (long long)r.B * r.max_query != r.N) return CARRY_GDN_ERR_SHAPE;
+  if (r.B > 65535 || c.HKV > 65535) return CARRY_GDN_ERR_TOO_LARGE;
+  return CARRY_GDN_OK;
+}
+int kv_pointers_ok(const CarryGdnKvCache& c) {
+  if (!c.lengths) return CARRY_GDN_ERR_NULL;
+  if (c.max_pages > 0 && c.num_pages > 0 && (!c.k_codes || !c.k_scale || !c.v_codes || !c.v_scale || !c.block_table))
+    return CARRY_GDN_ERR_NULL;
+  for (const uint8_t* p : {c.k_codes, c.v_codes})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return CARRY_GDN_ERR_SHAPE;
+  if (c.stride_k_page % 16 || c.stride_v_page % 16) return CARRY_GDN_ERR_SHAPE;
+  return CARRY_GDN_OK;
+}
+int kv_attention_ok(const CarryGdnKvAttentionArgs* a) {
+  if (!a) return CARRY_GDN_ERR_NULL;
+  const int rc = kv_ok(a->cache, a->rows);
+  if (rc != CARRY_GDN_OK) return rc;
+  if (a->HQ <= 0 || a->HQ % a->cache.HKV) return CARRY_GDN_ERR_SHAPE;
+  return dtype_ok(a->dtype) ? CARRY_GDN_OK : CARRY_GDN_ERR_DTYPE;
+}
+}  // namespace
+
+int carry_gdn_kv_append(const CarryGdnKvAppendArgs* a, void* stream) {
+  clear_stale_error();
+  if (!a) return CARRY_GDN_ERR_NULL;
+  int rc = kv_ok(a->cache, a->rows);
+  if (rc != CARRY_GDN_OK) return rc;
+  if (!dtype_ok(a->dtype)) return CARRY_GDN_ERR_DTYPE;
+  if (a->rows.N == 0 || a->rows.B == 0 || a->rows.max_query == 0) return CARRY_GDN_OK;
+  if (!a->k || !a->v) return CARRY_GDN_ERR_NULL;
+  rc = kv_pointers_ok(a->cache);
+  if (rc == CARRY_GDN_OK) rc = carry::launch_kv_append(*a, static_cast<cudaStream_t>(stream));
+  if (rc == CARRY_GDN_OK) g_last_kernel = 9;
+  return rc;
+}
+
+int64_t carry_gdn_kv_attention_workspace(const CarryGdnKvAttentionArgs* a) {
+  const int rc = kv_attention_ok(a);
+  return rc == CARRY_GDN_OK ? carry::kv_attention_workspace(*a) : rc;
+}
+
+int carry_gdn_kv_attention(const CarryGdnKvAttentionArgs* a, void* stream) {
+  clear_stale_error();
+  int rc = kv_attention_ok(a);
+  if (rc != CARRY_GDN_OK) return rc;
+  if (a->rows.N == 0 || a->rows.B == 0 || a->rows.max_query == 0) return CARRY_GDN_OK;
+  if (!a->q || !a->out) return CARRY_GDN_ERR_NULL;
+  rc = kv_pointers_ok(a->cache);
+  if (rc != CARRY_GDN_OK) return rc;
+  const int64_t need = carry::kv_attention_workspace(*a);
+  if (need < 0) return static_cast<int>(need);
+  if (need > 0 && !a->workspace) return CARRY_GDN_ERR_NULL;
+  if (need > 0 && (a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)) return CARRY_GDN_ERR_SHAPE;
+  rc = carry::launch_kv_attention(*a, static_cast<cudaStream_t>(stream));
+  if (rc == CARRY_GDN_OK) g_last_kernel = 10;
+  return rc;
+}
+
+int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* a, void* stream) {
+  clear_stale_error();
+  if (!a) return CARRY_GDN_ERR_NULL;
+  if (a->N < 0 || a->W <= 0 || (a->group != 0 && a->group != 128)) return CARRY_GDN_ERR_SHAPE;
+  if (!dtype_ok(a->x_dtype) || !dtype_ok(a->residual_dtype) || !dtype_ok(a->weight_dtype)) return CARRY_GDN_ERR_DTYPE;
+  if (a->W > 32768) return CARRY_GDN_ERR_TOO_LARGE;
+  if (a->N == 0) return CARRY_GDN_OK;
+  if (!a->x || !a->weight || !a->codes || !a->scale) return CARRY_GDN_ERR_NULL;
+  const int rc = carry::launch_norm(*a, static_cast<cudaStream_t>(stream));
+  if (rc == CARRY_GDN_OK) g_last_kernel = 11;
   return rc;
 }
 

@@ -61,8 +61,10 @@ enum {
 /* bits of the optional device-side status word (OR-ed in by the kernels) */
 enum {
   CARRY_GDN_STATUS_BAD_SLOT = 1,   /* a slot id was >= num_slots; that request was treated as padding */
-  CARRY_GDN_STATUS_TIMEOUT = 2     /* an asynchronous copy did not complete within the wait limit: that CTA
+  CARRY_GDN_STATUS_TIMEOUT = 2,    /* an asynchronous copy did not complete within the wait limit: that CTA
                                       stopped loading and storing and left its remaining tiles untouched */
+  CARRY_GDN_STATUS_BAD_RANGE = 4   /* key/value cache: a page id, a length or a query range lay outside of what the
+                                      call was given; what lay outside was skipped */
 };
 
 /*
@@ -319,6 +321,121 @@ typedef struct CarryGdnPoolCopyLayersArgs {
 
 int carry_gdn_pool_copy_layers(const CarryGdnPoolCopyLayersArgs* args, void* stream);
 
+/*
+ * The key/value cache of one full-attention layer, in 8 bits: pages of `page`
+ * tokens, e4m3 codes [pages, HKV, page, D] and one fp32 scale for every `block`
+ * tokens of a head, [pages, HKV, page / block]; a value is code * scale.  The
+ * scales that carry_gdn_kv_append writes are powers of two, 2^-100 to 2^119.
+ * Request b holds lengths[b] tokens, token j of it in page
+ * block_table[b][j / page]; a page id <= 0 is padding, its tokens are not
+ * there.  A page id >= num_pages and a length beyond max_pages * page are
+ * flagged with CARRY_GDN_STATUS_BAD_RANGE and treated as padding and as that
+ * bound.  Within a page the tensors are contiguous; strides between pages and
+ * between the table's rows are in elements.  D is 64 or 128, page and block are
+ * multiples of 16, block divides page and is at most 128; code pages start on
+ * 16-byte boundaries.  B and HKV are at most 65535, a request's tokens 2^30.
+ */
+typedef struct CarryGdnKvCache {
+  uint8_t* k_codes;
+  float* k_scale;
+  uint8_t* v_codes;
+  float* v_scale;
+  int64_t stride_k_page, stride_ks_page, stride_v_page, stride_vs_page;
+  const int32_t* block_table; /* [B, max_pages] */
+  int64_t stride_table;
+  const int32_t* lengths;     /* [B], with the call's own tokens among them */
+  int32_t num_pages, HKV, page, block, D, max_pages;
+} CarryGdnKvCache;
+
+/*
+ * The new tokens of a call: N rows, those of request b being
+ * query_start[b] .. query_start[b + 1] - 1 (at most max_query of them; more,
+ * and rows outside 0 .. N - 1, are skipped and flagged), or, with query_start
+ * NULL, max_query = N / B rows each.  Row i of n of a request stands at
+ * position lengths[b] - n + i of its context.
+ */
+typedef struct CarryGdnKvRows {
+  const int32_t* query_start; /* [B + 1], or NULL */
+  int32_t B, N, max_query;
+} CarryGdnKvRows;
+
+/*
+ * Append: the rows' keys and values become codes at their positions.  The scale
+ * of a block is the smallest power of two s with amax / s <= 448, amax over the
+ * block's tokens so far; where it grows, the codes of the block's earlier
+ * tokens are rounded to it (exactly, down to e4m3's subnormals).  A block whose
+ * first token is among the new ones is started afresh.  A token whose key or
+ * value has a number that is not finite gets a NaN key and takes no part in the
+ * scale: the queries that see it become NaN, no others.  Rows at a negative
+ * position or in a padding page are skipped.  No two requests may append to one
+ * page.
+ */
+typedef struct CarryGdnKvAppendArgs {
+  CarryGdnKvCache cache;
+  CarryGdnKvRows rows;
+  const void* k;          /* [N, HKV, D], D contiguous */
+  const void* v;
+  int64_t stride_k_tok, stride_k_head, stride_v_tok, stride_v_head;
+  int32_t dtype;          /* CARRY_F32 | CARRY_BF16 | CARRY_F16 */
+  int32_t* status;        /* optional device word, may be NULL */
+} CarryGdnKvAppendArgs;
+
+int carry_gdn_kv_append(const CarryGdnKvAppendArgs* args, void* stream);
+
+/*
+ * Attention of the rows' queries over the cache: out = sum_j softmax_j(scale *
+ * q . k_j) v_j over the tokens j of the request up to the row's own position.
+ * HQ is a multiple of HKV; query head h reads key/value head h / (HQ / HKV).  A
+ * row that sees no token is zero.  Value codes have to be finite where they are
+ * within a request's length.  `workspace` holds partial results and is at least
+ * carry_gdn_kv_attention_workspace() bytes, 16-byte aligned; nothing is kept
+ * in it between calls.
+ */
+typedef struct CarryGdnKvAttentionArgs {
+  CarryGdnKvCache cache;  /* read only */
+  CarryGdnKvRows rows;
+  const void* q;          /* [N, HQ, D], D contiguous */
+  int64_t stride_q_tok, stride_q_head;
+  void* out;              /* [N, HQ, D], D contiguous */
+  int64_t stride_out_tok, stride_out_head;
+  void* workspace;
+  int64_t workspace_bytes;
+  float scale;
+  int32_t HQ;
+  int32_t dtype;          /* of q and out */
+  int32_t* status;
+} CarryGdnKvAttentionArgs;
+
+int carry_gdn_kv_attention(const CarryGdnKvAttentionArgs* args, void* stream);
+
+/* Bytes of workspace that a call with these arguments needs (0 for none), or a
+ * negative CARRY_GDN_ERR_*.  Looks at sizes only: no pointer is read. */
+int64_t carry_gdn_kv_attention_workspace(const CarryGdnKvAttentionArgs* args);
+
+/*
+ * The entry of a layer: h = x + residual (fp32), residual_out = h rounded to its
+ * type, y = h * rsqrt(mean(h^2) + eps) * weight, and y in e4m3 codes with a
+ * scale per row (group == 0: scale [N]) or per 128 columns (group == 128: scale
+ * [N, ceil(W / 128)], contiguous): scale = max(amax|y|, 1e-12) / 448.  A row
+ * with a number that is not finite gets NaN codes and scales throughout.
+ * residual may be NULL (h = x); residual_out may be NULL, or alias residual or
+ * x.  W is at most 32768.
+ */
+typedef struct CarryGdnNormArgs {
+  const void* x;          /* [N, W], W contiguous */
+  const void* residual;   /* [N, W] */
+  void* residual_out;     /* [N, W] */
+  const void* weight;     /* [W] */
+  uint8_t* codes;         /* [N, W] */
+  float* scale;
+  int64_t stride_x, stride_residual, stride_residual_out, stride_codes;
+  float eps;
+  int32_t N, W, group;
+  int32_t x_dtype, residual_dtype, weight_dtype; /* residual_dtype: of residual and residual_out */
+} CarryGdnNormArgs;
+
+int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* args, void* stream);
+
 /* Human-readable text for a CARRY_GDN_ERR_* code (static storage). */
 const char* carry_gdn_strerror(int code);
 
@@ -331,7 +448,8 @@ int carry_gdn_abi_version(void);
  * 3 = multi-token kernel, 4 = a pool store / load / copy kernel,
  * 5 = 128x128 streaming kernel, step without error feedback,
  * 6 = slot-indexed kernel for 64x64 heads, 7 = kernel of chained steps,
- * 8 = statequant-layout kernel for 64x64 heads.
+ * 8 = statequant-layout kernel for 64x64 heads, 9 = key/value append, 10 = attention over the
+ * key/value cache, 11 = layer norm with 8-bit output.
  * Diagnostic only (tests use it to prove which path ran).
  */
 int carry_gdn_last_kernel(void);
