@@ -1,71 +1,753 @@
-// Attention over the 8-bit key/value cache: one warp for each (row, query head), a token at a time.
+// Attention over the 8-bit key/value cache.
+//
+// Scores s = scale * q . k and outputs sum_j softmax_j(s) v_j in one pass over the cache, with the running maximum and
+// sum of an online softmax.  Keys and values stay e4m3 until they are in registers: tiles of 64 tokens come into a ring of
+// shared-memory stages by 16-byte asynchronous copies, and a warp turns the codes into the fp16 operands of the
+// matrix instructions as it needs them (e4m3 is a subset of fp16).  What each rounding to 16 bits costs:
+//  * a query row is scaled by a power of two until its largest number is in [2^14, 2^15): bf16 and fp16 numbers fit fp16
+//    exactly down to 2^-29 of the largest, fp32 ones go in two parts (22 bits);
+//  * the weights p of the softmax are fp16 (2^-12 of each, against 2^-9 for the rounding of a bf16 output), with fp32
+//    queries in two parts.  They carry the value scale of their block relative to the largest one seen, and 2^15, so
+//    that weights down to 2^-29 of the largest have all their bits.
+// Scores, maxima, sums and outputs are fp32.
+//
+// What a call reads is the cache, once; one matrix tile of 16 rows holds the query heads of a key/value head, so that
+// the tokens are read once for all of them.
+#include <cuda_pipeline_primitives.h>
+
 #include "carry_hybrid.cuh"
 
 namespace carry {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kTile = 64, kGranule = 16, kWarps = 4, kThreads = kWarps * 32;
+constexpr int kRowsPerWarp = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kWeightUp = 15.0f;                // weights are formed times 2^15
+constexpr float kNoTokens = -1.0f;                // in a key scale's place: a padding page, or past the end
 
-// sum = sum * keep + x, with the rounding error carried on
-__device__ __forceinline__ void add(float& sum, float& low, float keep, float x) {
-  const float y = x - low * keep, before = sum * keep, after = before + y;
-  low = (after - before) - y;
-  sum = after;
+struct AttnParams {
+  CarryGdnKvAttentionArgs a;
+  int group;                      // query heads per key/value head
+  int page_granules, page_shift;  // granules in a page, and its logarithm or -1
+  int block_granules;
+  int rows;                       // rows of a row tile that may be in use (decode kernel)
+};
+
+__device__ __forceinline__ void mma_fp16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two e4m3 codes as two fp16 numbers
+__device__ __forceinline__ uint32_t halves_of(uint32_t codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
+  return h.x | static_cast<uint32_t>(h.y) << 16;
+}
+__device__ __forceinline__ uint32_t pack_half2(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+  return fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  x += __shfl_xor_sync(~0u, x, 1);
+  return x + __shfl_xor_sync(~0u, x, 2);
+}
+
+// Where the 16-byte chunk `chunk` of token `row` lies in a tile.  The lanes that read together then fall into different
+// banks both ways: a quad of lanes reads one token's chunks (keys), or the same chunk of every second token (values).
+template <int D>
+__device__ __forceinline__ int tile_at(int row, int chunk) {
+  if constexpr (D == 128) return (row * 8 + (chunk ^ (row & 6) ^ (row & 1) << 2)) * 16;
+  const int line = row >> 1;
+  return (line * 8 + (((row & 1) << 2 | chunk) ^ (line & 3) << 1)) * 16;
 }
 
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) kv_attention_kernel(const __grid_constant__ CarryGdnKvAttentionArgs a) {
-  constexpr int E = D / 32;                       // columns per lane
-  depend_release();
-  depend_wait();
-  const CarryGdnKvCache& c = a.cache;
-  const int b = blockIdx.y, lane = threadIdx.x % 32;
-  const long long task = (long long)blockIdx.x * kWarps + threadIdx.x / 32;
-  const int i = (int)(task / a.HQ), hq = (int)(task % a.HQ), h = hq / (a.HQ / c.HKV);
-  const KvRequest r = kv_request(c, a.rows, b, task == 0 && lane == 0 ? a.status : nullptr);
-  if (i >= r.todo) return;
-  const int seen = max(min(r.length - r.count + i + 1, r.length), 0);
-  const long long row = r.first + i;
-  float q[E], o[E] = {}, top = -INFINITY, total = 0.0f;
-  float o_low[E] = {}, total_low = 0.0f;          // what the sums have lost to rounding
+struct Stage {
+  alignas(128) uint8_t k[kTile * D];
+  uint8_t v[kTile * D];
+  float ks[kTile / kGranule], vs[kTile / kGranule];
+};
+
+// ---- tiles into shared memory ----------------------------------------------------------------------------------------
+
+// The page ids that this thread's copies of a tile need, fetched a tile ahead of the copies.
+template <int D>
+struct Pages {
+  int chunk[D / 32], scale;
+};
+template <int D>
+__device__ __forceinline__ int granule_of(int i) {       // of this thread's i-th chunk of a tile
+  return D == 128 ? i : 2 * i + (threadIdx.x >> 6);
+}
+__device__ __forceinline__ int page_index(const AttnParams& p, int granule) {
+  return p.page_shift >= 0 ? granule >> p.page_shift : granule / p.page_granules;
+}
+__device__ __forceinline__ int page_id(const AttnParams& p, int b, int granule, int length) {
+  if (granule * kGranule >= length) return 0;
+  return kv_page(p.a.cache, b, page_index(p, granule), p.a.status);
+}
+template <int D>
+__device__ __forceinline__ void fetch_pages(const AttnParams& p, int b, int tile, int length, Pages<D>& ids) {
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    q[e] = load_as_float(a.q, row * a.stride_q_tok + hq * a.stride_q_head + lane * E + e, a.dtype) * a.scale;
-  int page = 0;
-  for (int j = 0; j < seen; ++j) {
-    if (j % c.page == 0) page = kv_page(c, b, j / c.page, lane == 0 ? a.status : nullptr);
-    if (page == 0) continue;
-    const long long at = ((long long)h * c.page + j % c.page) * D + lane * E;
-    const long long s_at = h * (c.page / c.block) + j % c.page / c.block;
-    const uint8_t *kc = c.k_codes + page * c.stride_k_page + at, *vc = c.v_codes + page * c.stride_v_page + at;
-    float s = 0.0f;
+  for (int i = 0; i < D / 32; ++i) ids.chunk[i] = page_id(p, b, tile * 4 + granule_of<D>(i), length);
+  ids.scale = threadIdx.x < 8 ? page_id(p, b, tile * 4 + threadIdx.x % 4, length) : 0;
+}
+
+// Tokens at or beyond `length` and tokens of padding pages are filled with zeros, whatever memory holds there.
+template <int D>
+__device__ __forceinline__ void load_tile(const AttnParams& p, Stage<D>& s, int h, int tile, int length, const Pages<D>& ids) {
+  const CarryGdnKvCache& c = p.a.cache;
+  constexpr int kChunks = D / 16, kStep = kThreads / kChunks;
+  const int chunk = threadIdx.x % kChunks;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], __half2float(__half(__nv_cvt_fp8_to_halfraw(kc[e], __NV_E4M3))), s);
+  for (int i = 0; i < D / 32; ++i) {
+    const int row = threadIdx.x / kChunks + i * kStep, granule = tile * 4 + granule_of<D>(i), id = ids.chunk[i];
+    const int in_page = (granule - page_index(p, granule) * p.page_granules) * kGranule + row % kGranule;
+    const long long at = ((long long)h * c.page + in_page) * D + chunk * 16;
+    const size_t zero = id > 0 && tile * kTile + row < length ? 0 : 16;
+    const int to = tile_at<D>(row, chunk);
+    __pipeline_memcpy_async(s.k + to, zero ? c.k_codes : c.k_codes + id * c.stride_k_page + at, 16, zero);
+    __pipeline_memcpy_async(s.v + to, zero ? c.v_codes : c.v_codes + id * c.stride_v_page + at, 16, zero);
+  }
+  if (threadIdx.x < 8) {
+    const int i = threadIdx.x % 4, granule = tile * 4 + i, id = ids.scale;
+    const int at = h * (p.page_granules / p.block_granules) + (granule - page_index(p, granule) * p.page_granules) / p.block_granules;
+    float* to = threadIdx.x < 4 ? &s.ks[i] : &s.vs[i];
+    if (id > 0) __pipeline_memcpy_async(to, threadIdx.x < 4 ? c.k_scale + id * c.stride_ks_page + at : c.v_scale + id * c.stride_vs_page + at, 4);
+    else *to = threadIdx.x < 4 ? kNoTokens : 0.0f;
+  }
+}
+
+// ---- one warp's rows -------------------------------------------------------------------------------------------------
+
+// 16 query rows of a warp as operands of the matrix instructions.  Lane (g, c) = (lane / 4, lane % 4) has rows g and
+// g + 8; the product sums over the columns in an order of its own, in which the lane's share of every 64 columns is 16
+// neighbouring ones from 16 c on: those that one 16-byte load of key codes brings.
+template <int D, int PARTS>
+struct Query {
+  uint32_t x[PARTS][D / 16][4];
+  float unit[2];                  // scale * log2(e) over the power of two that the row was multiplied by
+};
+
+template <int D, int PARTS>
+__device__ __forceinline__ void load_query(const AttnParams& p, const KvRequest& r, int h, int row0, Query<D, PARTS>& q) {
+  const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
 #pragma unroll
-    for (int x = 16; x > 0; x /= 2) s += __shfl_xor_sync(~0u, s, x);
-    s *= c.k_scale[page * c.stride_ks_page + s_at];
-    const float now = fmaxf(top, s), base = now == -INFINITY ? 0.0f : now;
-    const float keep = expf(top - base), p = expf(s - base), pv = p * c.v_scale[page * c.stride_vs_page + s_at];
-    top = now;
-    add(total, total_low, keep, p);
+  for (int half = 0; half < 2; ++half) {
+    const int row = row0 + g + half * 8, i = row / p.group;
+    const bool there = i < r.todo;
+    const long long at = there ? (r.first + i) * p.a.stride_q_tok + (h * p.group + row % p.group) * p.a.stride_q_head : 0;
+    float x[D / 4];
+    uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) add(o[e], o_low[e], keep, pv * __half2float(__half(__nv_cvt_fp8_to_halfraw(vc[e], __NV_E4M3))));
+    for (int e = 0; e < D / 4; ++e) {
+      x[e] = there ? load_as_float(p.a.q, at + e / 16 * 64 + c * 16 + e % 16, p.a.dtype) : 0.0f;
+      top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+    top = max(top, __shfl_xor_sync(~0u, top, 1));
+    top = max(top, __shfl_xor_sync(~0u, top, 2));
+    const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 127) - 14;   // x * 2^-e is below 2^15
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    q.unit[half] = p.a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int pair = 0; pair < 2; ++pair) {
+        float u = x[k * 4 + pair * 2] * up, v = x[k * 4 + pair * 2 + 1] * up;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const uint32_t w = pack_half2(u, v);
+          q.x[part][k][pair * 2 + half] = w;
+          const float2 kept = unpack_half2(w);
+          u -= kept.x;
+          v -= kept.y;
+        }
+      }
+  }
+}
+
+// Running softmax of a warp's rows over the tokens that it has seen.
+template <int D>
+struct Rows {
+  float o[D / 8][4];              // lane (g, c): row g columns 2c (D/8) + n and (2c + 1) D/8 + n, then row g + 8's
+  float top[2], sum[2];           // of rows g and g + 8; the sums are this lane's share
+  float unit;                     // largest value scale so far: o counts in it, times 2^15
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    top[0] = top[1] = -INFINITY;
+    sum[0] = sum[1] = 0.0f;
+    unit = 0x1p-100f;             // the smallest scale
+  }
+};
+
+// TOK tokens of a tile from token `tok0` of the tile on.  `limit` says how many of the tile's tokens rows g and g + 8 see.
+template <int D, int PARTS, int TOK>
+__device__ __forceinline__ void attend(const Stage<D>& s, int tok0, const Query<D, PARTS>& q, const int (&limit)[2], Rows<D>& r) {
+  const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+  float score[TOK / 8][4];
+#pragma unroll
+  for (int n = 0; n < TOK / 8; ++n) {
+    float acc[4] = {};
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const uint4 w = *reinterpret_cast<const uint4*>(s.k + tile_at<D>(tok0 + n * 8 + g, j * 4 + c));
+      const uint32_t codes[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t b0 = halves_of(codes[k] & 0xffffu), b1 = halves_of(codes[k] >> 16);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) mma_fp16(acc, q.x[part][j * 4 + k], b0, b1);
+      }
+    }
+    const float ks = s.ks[(tok0 + n * 8) / kGranule];
+    const int t = ks == kNoTokens ? 1 << 30 : tok0 + n * 8 + 2 * c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) score[n][i] = t + i % 2 < limit[i / 2] ? acc[i] * (q.unit[i / 2] * ks) : -INFINITY;
+  }
+
+  float now[2], unit = r.unit;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < TOK / 8; ++n) m = fmaxf(m, fmaxf(score[n][2 * half], score[n][2 * half + 1]));
+    now[half] = fmaxf(r.top[half], quad_max(m));
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    store_from_float(a.out, row * a.stride_out_tok + hq * a.stride_out_head + lane * E + e, a.dtype,
-                     total == 0.0f ? 0.0f : o[e] / total);
+  for (int n = 0; n < TOK / kGranule; ++n) unit = fmaxf(unit, s.vs[tok0 / kGranule + n]);
+  if (__any_sync(~0u, now[0] > r.top[0] || now[1] > r.top[1]) || unit > r.unit) {
+    const float less = r.unit == unit ? 1.0f : __fdividef(r.unit, unit);
+    float keep[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      keep[half] = now[half] == -INFINITY ? 1.0f : exp2_fast(r.top[half] - now[half]);
+      r.sum[half] *= keep[half];
+      r.top[half] = now[half];
+      keep[half] *= less;
+    }
+    r.unit = unit;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.o[n][i] *= keep[i / 2];
+  }
+  const float base[2] = {now[0] == -INFINITY ? 0.0f : now[0], now[1] == -INFINITY ? 0.0f : now[1]};
+  const float up = __fdividef(exp2f(kWeightUp), unit);
+
+#pragma unroll
+  for (int b = 0; b < TOK / kGranule; ++b) {
+    const float vs = s.vs[tok0 / kGranule + b] * up;
+    uint32_t w[PARTS][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {                  // rows g, g + 8 of the first eight tokens, then of the other eight
+      const int half = x % 2, n = 2 * b + x / 2;
+      float p0 = exp2_fast(score[n][2 * half] - base[half]), p1 = exp2_fast(score[n][2 * half + 1] - base[half]);
+      r.sum[half] += p0 + p1;
+      p0 *= vs;
+      p1 *= vs;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        w[part][x] = pack_half2(p0, p1);
+        const float2 kept = unpack_half2(w[part][x]);
+        p0 -= kept.x;
+        p1 -= kept.y;
+      }
+    }
+    // values: this lane's columns of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+    const int t = tok0 + b * kGranule + 2 * c;
+    constexpr int kWords = D / 32;                // words of D / 8 codes
+    uint32_t v[4][kWords];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = t + i % 2 + i / 2 * 8;
+      if constexpr (D == 128) {
+        const uint4 u = *reinterpret_cast<const uint4*>(s.v + tile_at<D>(row, g));
+        v[i][0] = u.x; v[i][1] = u.y; v[i][2] = u.z; v[i][3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(s.v + tile_at<D>(row, g / 2) + g % 2 * 8);
+        v[i][0] = u.x; v[i][1] = u.y;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kWords; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t first = __byte_perm(v[0][k], v[1][k], e ? 0x7362 : 0x5140);
+        const uint32_t second = __byte_perm(v[2][k], v[3][k], e ? 0x7362 : 0x5140);
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const uint32_t b0 = halves_of(f ? first >> 16 : first & 0xffffu), b1 = halves_of(f ? second >> 16 : second & 0xffffu);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) mma_fp16(r.o[k * 4 + e * 2 + f], w[part], b0, b1);
+        }
+      }
+  }
+}
+
+// eight neighbouring fp32 results to out's type
+__device__ __forceinline__ void store8(void* out, long long at, int dtype, const float* x) {
+  const long long byte = at * (dtype == CARRY_F32 ? 4 : 2);
+  if ((reinterpret_cast<uintptr_t>(out) + byte) % 16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) store_from_float(out, at + i, dtype, x[i]);
+    return;
+  }
+  uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + byte);
+  if (dtype == CARRY_F32) {
+    to[0] = *reinterpret_cast<const uint4*>(x);
+    to[1] = *reinterpret_cast<const uint4*>(x + 4);
+    return;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (dtype == CARRY_BF16) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      w[i] = pack_half2(x[2 * i], x[2 * i + 1]);
+    }
+  }
+  *to = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A finished row's columns of this lane, normalised, to the output.
+template <int D>
+__device__ __forceinline__ void store_rows(const AttnParams& p, const KvRequest& q, int h, int row0, const Rows<D>& r) {
+  const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = row0 + g + half * 8, i = row / p.group;
+    if (i >= q.todo) continue;
+    const long long at = (q.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + c * (D / 4);
+#pragma unroll
+    for (int e = 0; e < D / 4; e += 8) {
+      alignas(16) float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = r.o[(e + k) % (D / 8)][2 * half + (e + k) / (D / 8)];
+      store8(p.a.out, at + e, p.a.dtype, x);
+    }
+  }
+}
+
+// How many of a tile's tokens the lane's rows see.
+__device__ __forceinline__ void row_limits(const AttnParams& p, const KvRequest& q, int row0, int tile, int (&limit)[2]) {
+  const int g = threadIdx.x % 32 / 4;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int i = (row0 + g + half * 8) / p.group;
+    limit[half] = i < q.todo ? q.length - q.count + i + 1 - tile * kTile : 0;
+  }
+}
+
+// ---- few rows per request: the tokens of all requests and heads as one line of tiles, cut evenly over the CTAs ------------
+
+constexpr int kDecodeStages = 3;
+
+// What a CTA leaves for the joining kernel: at most one piece of a (request, head) that began in an earlier CTA (slot 0)
+// and one that goes on in later ones (slot 1).
+struct Piece {
+  int request, head, last;        // last CTA with a piece of the same; last < 0: none began here
+};
+
+template <int D, int MT>
+struct DecodeShared {
+  Stage<D> stage[kDecodeStages];
+  float merge[MT * kRowsPerWarp][D];
+  float top[kWarps / MT][MT * kRowsPerWarp], sum[kWarps / MT][MT * kRowsPerWarp];
+  int scan[kWarps];
+};
+
+__host__ __device__ constexpr long long slot_floats(int rows, int D) { return (long long)rows * (D + 2); }
+
+__device__ __forceinline__ int tiles_of(const AttnParams& p, int b) {
+  const long long cap = min((long long)p.a.cache.max_pages * p.a.cache.page, kMaxTokens);
+  const int length = (int)min((long long)max(p.a.cache.lengths[b], 0), cap);
+  return (length + kTile - 1) / kTile;
+}
+
+// Sum of x over the CTA, and over the threads before this one.
+__device__ __forceinline__ long long block_scan(long long x, long long* scratch, long long& before) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  long long up = x;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long y = __shfl_up_sync(~0u, up, d);
+    if (lane >= d) up += y;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = up;
+  __syncthreads();
+  long long total = 0;
+  before = up - x;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += scratch[w];
+    total += scratch[w];
+  }
+  return total;
+}
+
+// A place on the line of tiles.
+struct Cursor {
+  int b, h, tile, tiles, length;
+};
+__device__ __forceinline__ void open_request(const AttnParams& p, Cursor& at) {
+  while (at.b < p.a.rows.B && (at.tiles = tiles_of(p, at.b)) == 0) ++at.b;
+  if (at.b < p.a.rows.B) at.length = kv_request(p.a.cache, p.a.rows, at.b, nullptr).length;
+}
+__device__ __forceinline__ void advance(const AttnParams& p, Cursor& at) {
+  if (++at.tile < at.tiles) return;
+  at.tile = 0;
+  if (++at.h < p.a.cache.HKV) return;
+  at.h = 0;
+  ++at.b;
+  open_request(p, at);
+}
+
+// CTAs of the decode kernel that an SM holds: what their registers leave room for.
+__host__ __device__ constexpr int resident(int D, int MT, int PARTS) {
+  return D == 64 ? (MT == 4 ? 3 : 4) : MT == 1 && PARTS == 1 ? 3 : 2;
+}
+
+template <int D, int MT, int PARTS>
+__global__ void __launch_bounds__(kThreads, resident(D, MT, PARTS)) kv_decode_kernel(const __grid_constant__ AttnParams p) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  DecodeShared<D, MT>& sh = *reinterpret_cast<DecodeShared<D, MT>*>(raw);
+  __shared__ long long scratch[kWarps];
+  __shared__ int found[2];
+  constexpr int kGroups = kWarps / MT, kTok = kTile / kGroups, kRows = MT * kRowsPerWarp;
+  depend_release();
+  depend_wait();
+  const CarryGdnKvCache& c = p.a.cache;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, cc = lane % 4;
+  const int row0 = warp % MT * kRowsPerWarp, part = warp / MT;
+  Piece* pieces = reinterpret_cast<Piece*>(p.a.workspace);
+  float* slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + (sizeof(Piece) * gridDim.x + 15) / 16 * 16);
+
+  // the line's length, and where on it this CTA begins
+  long long total = 0, before;
+  for (int b0 = 0; b0 < p.a.rows.B; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    total += block_scan(b < p.a.rows.B ? (long long)tiles_of(p, b) * c.HKV : 0, scratch, before);
+  }
+  const long long share = (total + gridDim.x - 1) / gridDim.x;
+  const long long from = min(share * blockIdx.x, total), to = min(from + share, total);
+  // requests without tokens have no tiles: their rows are zero
+  for (int b = blockIdx.x; b < p.a.rows.B; b += gridDim.x) {
+    const KvRequest q = kv_request(c, p.a.rows, b, threadIdx.x == 0 ? p.a.status : nullptr);
+    if (q.length > 0) continue;
+    for (int i = threadIdx.x; i < q.todo * p.a.HQ * D; i += kThreads)
+      store_from_float(p.a.out, (q.first + i / (p.a.HQ * D)) * p.a.stride_out_tok + i / D % p.a.HQ * p.a.stride_out_head + i % D, p.a.dtype, 0.0f);
+  }
+  if (threadIdx.x == 0) pieces[blockIdx.x].last = -1;
+  if (from == to) return;
+  long long seen = 0;
+  for (int b0 = 0; b0 < p.a.rows.B; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    const long long mine = b < p.a.rows.B ? (long long)tiles_of(p, b) * c.HKV : 0;
+    const long long all = block_scan(mine, scratch, before);
+    if (mine > 0 && from >= seen + before && from < seen + before + mine) {
+      found[0] = b;
+      found[1] = (int)(from - seen - before);
+    }
+    seen += all;
+    if (from < seen) break;
+  }
+  __syncthreads();
+  Cursor use;
+  use.b = found[0];
+  use.tiles = 1;
+  open_request(p, use);
+  use.h = found[1] / use.tiles;
+  use.tile = found[1] % use.tiles;
+  Cursor load = use;
+  long long to_load = to - from;
+  Pages<D> ids;
+  fetch_pages<D>(p, load.b, load.tile, load.length, ids);
+  auto next_load = [&](int stage) {
+    if (to_load > 0) {
+      load_tile<D>(p, sh.stage[stage], load.h, load.tile, load.length, ids);
+      advance(p, load);
+      if (--to_load > 0) fetch_pages<D>(p, load.b, load.tile, load.length, ids);
+    }
+    __pipeline_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kDecodeStages - 1; ++s) next_load(s);
+
+  Query<D, PARTS> q;
+  Rows<D> r;
+  KvRequest request;
+  bool begin = true;
+  int first_tile = 0, stage = 0;
+  for (long long at = from; at < to; ++at) {
+    if (begin) {
+      request = kv_request(c, p.a.rows, use.b, nullptr);
+      load_query<D, PARTS>(p, request, use.h, row0, q);
+      r.clear();
+      first_tile = use.tile;
+      begin = false;
+    }
+    __pipeline_wait_prior(kDecodeStages - 2);
+    __syncthreads();                              // this tile has landed, and everybody is done with the one before
+    next_load(stage == 0 ? kDecodeStages - 1 : stage - 1);
+    int limit[2];
+    row_limits(p, request, row0, use.tile, limit);
+    attend<D, PARTS, kTok>(sh.stage[stage], part * kTok, q, limit, r);
+    stage = stage + 1 == kDecodeStages ? 0 : stage + 1;
+    const bool ends = use.tile + 1 == use.tiles;
+    if (ends || at + 1 == to) {
+      // the warps of a row tile join: weights first, then the outputs in turn
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float sum = quad_sum(r.sum[half]);
+        if (cc == 0) {
+          sh.top[part][row0 + g + half * 8] = r.top[half];
+          sh.sum[part][row0 + g + half * 8] = sum;
+        }
+      }
+      __syncthreads();
+      float top[2], sum[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = row0 + g + half * 8;
+        top[half] = -INFINITY;
+        sum[half] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kGroups; ++x) top[half] = fmaxf(top[half], sh.top[x][row]);
+        const float base = top[half] == -INFINITY ? 0.0f : top[half];
+#pragma unroll
+        for (int x = 0; x < kGroups; ++x) sum[half] += sh.sum[x][row] * exp2_fast(sh.top[x][row] - base);
+        const float w = sum[half] == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[half] - base), sum[half]) * exp2f(-kWeightUp);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          r.o[n][2 * half] = r.o[n][2 * half] * w * r.unit;
+          r.o[n][2 * half + 1] = r.o[n][2 * half + 1] * w * r.unit;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kGroups; ++x) {
+        if (x > 0) __syncthreads();
+        if (x != part) continue;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float& cell = sh.merge[row0 + g + half * 8][(2 * cc + i) * (D / 8) + n];
+              float& mine = r.o[n][2 * half + i];
+              if (x > 0) mine += cell;
+              if (x + 1 < kGroups) cell = mine;
+            }
+      }
+      if (part == kGroups - 1) {
+        if (ends && first_tile == 0) {
+          store_rows<D>(p, request, use.h, row0, r);
+        } else {
+          float* slot = slots + (2 * blockIdx.x + (first_tile == 0)) * slot_floats(kRows, D);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int row = row0 + g + half * 8;
+            if (row >= p.rows) continue;
+            if (cc == 0) {
+              slot[row] = top[half];
+              slot[kRows + row] = sum[half];
+            }
+            float4* o = reinterpret_cast<float4*>(slot + 2 * kRows + row * D + cc * (D / 4));
+#pragma unroll
+            for (int e = 0; e < D / 4; e += 4) {
+              const int i = 2 * half + e / (D / 8), n = e % (D / 8);
+              o[e / 4] = make_float4(r.o[n][i], r.o[n + 1][i], r.o[n + 2][i], r.o[n + 3][i]);
+            }
+          }
+        }
+      }
+      if (!ends && first_tile == 0 && threadIdx.x == 0) {
+        // the rest of its tiles: the CTAs up to the one with its last tile
+        const long long last = at + (use.tiles - 1 - use.tile);
+        pieces[blockIdx.x] = {use.b, use.h, (int)(last / share)};
+      }
+      begin = true;
+    }
+    advance(p, use);
+  }
+}
+
+// Joins the pieces of the (request, head) that began in CTA blockIdx.x of the kernel above: one warp per row.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_join_kernel(const __grid_constant__ AttnParams p, const int kRows) {
+  __shared__ float part_o[kWarps][D];
+  depend_release();
+  depend_wait();
+  const Piece piece = reinterpret_cast<const Piece*>(p.a.workspace)[blockIdx.x];
+  if (piece.last < 0) return;
+  const float* slots = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.a.workspace) + (sizeof(Piece) * gridDim.x + 15) / 16 * 16);
+  const KvRequest q = kv_request(p.a.cache, p.a.rows, piece.request, nullptr);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, count = piece.last - blockIdx.x + 1;
+  auto slot = [&](int i) { return slots + (2 * (blockIdx.x + i) + (i == 0)) * slot_floats(kRows, D); };
+  for (int row = blockIdx.y; row < q.todo * p.group; row += gridDim.y) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, slot(i)[row]);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    const float base = top == -INFINITY ? 0.0f : top;
+    for (int i = lane; i < count; i += 32) sum += slot(i)[kRows + row] * exp2_fast(slot(i)[row] - base);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    float o[D / 32] = {};
+#pragma unroll 4
+    for (int i = warp; i < count; i += kWarps) {
+      const float* s = slot(i);
+      const float w = s[kRows + row] * exp2_fast(s[row] - base);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) o[e] = fmaf(w, s[2 * kRows + row * D + e * 32 + lane], o[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) part_o[warp][e * 32 + lane] = o[e];
+    __syncthreads();
+    const int i = row / p.group;
+    for (int d = threadIdx.x; d < D; d += kThreads) {
+      float x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) x += part_o[w][d];
+      store_from_float(p.a.out, (q.first + i) * p.a.stride_out_tok + (piece.head * p.group + row % p.group) * p.a.stride_out_head + d,
+                       p.a.dtype, sum == 0.0f ? 0.0f : __fdiv_rn(x, sum));
+    }
+    __syncthreads();
+  }
+}
+
+// ---- many rows per request: one CTA for each 64 rows of a (request, head) -----------------------------------------------
+
+constexpr int kChunkStages = 3, kChunkRows = kWarps * kRowsPerWarp;
+
+template <int D, int PARTS>
+__global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constant__ AttnParams p) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  Stage<D>* stages = reinterpret_cast<Stage<D>*>(raw);
+  depend_release();
+  depend_wait();
+  const CarryGdnKvCache& c = p.a.cache;
+  const int b = blockIdx.z, h = blockIdx.y, first_row = (gridDim.x - 1 - blockIdx.x) * kChunkRows;   // the longest go first
+  const KvRequest q = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
+  if (first_row >= q.todo * p.group) return;
+  const int row0 = first_row + threadIdx.x / 32 * kRowsPerWarp;
+  const int last = min((first_row + kChunkRows - 1) / p.group, q.todo - 1);
+  const int length = max(min(q.length, q.length - q.count + last + 1), 0), tiles = (length + kTile - 1) / kTile;
+  Pages<D> ids;
+  fetch_pages<D>(p, b, 0, length, ids);
+  auto next_load = [&](int tile) {
+    if (tile < tiles) {
+      load_tile<D>(p, stages[tile % kChunkStages], h, tile, length, ids);
+      if (tile + 1 < tiles) fetch_pages<D>(p, b, tile + 1, length, ids);
+    }
+    __pipeline_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kChunkStages - 1; ++s) next_load(s);
+  Query<D, PARTS> query;
+  Rows<D> r;
+  load_query<D, PARTS>(p, q, h, row0, query);
+  r.clear();
+  for (int tile = 0; tile < tiles; ++tile) {
+    __pipeline_wait_prior(kChunkStages - 2);
+    __syncthreads();
+    next_load(tile + kChunkStages - 1);
+    int limit[2];
+    row_limits(p, q, row0, tile, limit);
+    attend<D, PARTS, kTile>(stages[tile % kChunkStages], 0, query, limit, r);
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const float sum = quad_sum(r.sum[half]);
+    const float w = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kWeightUp), sum);
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      r.o[n][2 * half] = r.o[n][2 * half] * w * r.unit;
+      r.o[n][2 * half + 1] = r.o[n][2 * half + 1] * w * r.unit;
+    }
+  }
+  store_rows<D>(p, q, h, row0, r);
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------------------
+
+int row_tiles(const CarryGdnKvAttentionArgs& a) {   // 1, 2 or 4 for the decode kernel, 0 for the other
+  const long long rows = (long long)a.rows.max_query * (a.HQ / a.cache.HKV);
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 0;
+}
+
+// CTAs of the decode kernel: all that are resident at a time, or one per tile where there cannot be as many.
+long long decode_ctas(const CarryGdnKvAttentionArgs& a, int mt) {
+  const long long tokens = (long long)a.cache.max_pages * a.cache.page;
+  const long long most = (tokens + kTile - 1) / kTile * a.cache.HKV * a.rows.B;
+  const long long fit = (long long)sm_count() * resident(a.cache.D, mt, a.dtype == CARRY_F32 ? 2 : 1);
+  return most < 1 ? 1 : most < fit ? most : fit;
+}
+
+template <class K>
+int prepare(K kernel, size_t smem) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess) return CARRY_GDN_OK;
+  cudaGetLastError();
+  return CARRY_GDN_ERR_LAUNCH;
+}
+
+template <int D, int MT, int PARTS>
+int launch_decode(const AttnParams& p, cudaStream_t stream) {
+  constexpr size_t smem = sizeof(DecodeShared<D, MT>);
+  const unsigned ctas = (unsigned)decode_ctas(p.a, MT);
+  int rc = prepare(kv_decode_kernel<D, MT, PARTS>, smem);
+  if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, MT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
+  if (rc != CARRY_GDN_OK) return rc;
+  return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kThreads, 0, stream, p, MT * kRowsPerWarp);
+}
+
+template <int D, int PARTS>
+int launch_by_rows(const AttnParams& p, int mt, cudaStream_t stream) {
+  if (mt == 1) return launch_decode<D, 1, PARTS>(p, stream);
+  if (mt == 2) return launch_decode<D, 2, PARTS>(p, stream);
+  if (mt == 4) return launch_decode<D, 4, PARTS>(p, stream);
+  constexpr size_t smem = sizeof(Stage<D>) * kChunkStages;
+  const long long rows = (long long)p.a.rows.max_query * p.group;
+  const int rc = prepare(kv_chunk_kernel<D, PARTS>, smem);
+  if (rc != CARRY_GDN_OK) return rc;
+  const dim3 grid((unsigned)((rows + kChunkRows - 1) / kChunkRows), p.a.cache.HKV, p.a.rows.B);
+  return launch_dependent(kv_chunk_kernel<D, PARTS>, grid, kThreads, smem, stream, p);
 }
 
 }  // namespace
 
-int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs&) { return 0; }
+int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a) {
+  const int mt = row_tiles(a);
+  if (mt == 0) return 0;
+  if (sm_count() == 0) return CARRY_GDN_ERR_NO_DEVICE;
+  const long long ctas = decode_ctas(a, mt);
+  return (sizeof(Piece) * ctas + 15) / 16 * 16 + 2 * ctas * slot_floats(mt * kRowsPerWarp, a.cache.D) * 4;
+}
 
 int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream) {
-  const long long tasks = (long long)a.rows.max_query * a.HQ;
-  const dim3 grid((unsigned)((tasks + kWarps - 1) / kWarps), a.rows.B);
-  if (a.cache.D == 64) return launch_dependent(kv_attention_kernel<64>, grid, kWarps * 32, 0, stream, a);
-  return launch_dependent(kv_attention_kernel<128>, grid, kWarps * 32, 0, stream, a);
+  if (sm_count() == 0) return CARRY_GDN_ERR_NO_DEVICE;
+  AttnParams p = {a, a.HQ / a.cache.HKV, a.cache.page / kGranule, -1, a.cache.block / kGranule, 0};
+  for (int s = 0; s < 31; ++s)
+    if (1 << s == p.page_granules) p.page_shift = s;
+  const int mt = row_tiles(a);
+  p.rows = mt ? a.rows.max_query * p.group : 0;
+  if (a.cache.D == 64) return a.dtype == CARRY_F32 ? launch_by_rows<64, 2>(p, mt, stream) : launch_by_rows<64, 1>(p, mt, stream);
+  return a.dtype == CARRY_F32 ? launch_by_rows<128, 2>(p, mt, stream) : launch_by_rows<128, 1>(p, mt, stream);
 }
 
 }  // namespace carry
