@@ -39,10 +39,9 @@ __device__ __forceinline__ void mma_fp16(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two e4m3 codes as two fp16 numbers
-__device__ __forceinline__ uint32_t halves_of(uint32_t codes) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
-  return h.x | static_cast<uint32_t>(h.y) << 16;
+// four e4m3 codes as fp16 numbers, two to a word
+__device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& low, uint32_t& high) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(low), "=r"(high) : "r"(codes));
 }
 __device__ __forceinline__ uint32_t pack_half2(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -131,6 +130,9 @@ __device__ __forceinline__ void load_tile(const AttnParams& p, Stage<D>& s, int 
 
 // ---- one warp's rows -------------------------------------------------------------------------------------------------
 
+// The power of two that a query row is divided by, from the bits of its largest magnitude: what is left is below 2^15.
+__device__ __forceinline__ int up_exponent(uint32_t top) { return min(max(static_cast<int>(top >> 23) - 127, -100), 127) - 14; }
+
 // 16 query rows of a warp as operands of the matrix instructions.  Lane (g, c) = (lane / 4, lane % 4) has rows g and
 // g + 8; the product sums over the columns in an order of its own, in which the lane's share of every 64 columns is 16
 // neighbouring ones from 16 c on: those that one 16-byte load of key codes brings.
@@ -157,7 +159,7 @@ __device__ __forceinline__ void load_query(const AttnParams& p, const KvRequest&
     }
     top = max(top, __shfl_xor_sync(~0u, top, 1));
     top = max(top, __shfl_xor_sync(~0u, top, 2));
-    const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 127) - 14;   // x * 2^-e is below 2^15
+    const int e = up_exponent(top);
     const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
     q.unit[half] = p.a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
@@ -206,7 +208,8 @@ __device__ __forceinline__ void attend(const Stage<D>& s, int tok0, const Query<
       const uint32_t codes[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t b0 = halves_of(codes[k] & 0xffffu), b1 = halves_of(codes[k] >> 16);
+        uint32_t b0, b1;
+        halves_of(codes[k], b0, b1);
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) mma_fp16(acc, q.x[part][j * 4 + k], b0, b1);
       }
@@ -284,14 +287,13 @@ __device__ __forceinline__ void attend(const Stage<D>& s, int tok0, const Query<
     for (int k = 0; k < kWords; ++k)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint32_t first = __byte_perm(v[0][k], v[1][k], e ? 0x7362 : 0x5140);
-        const uint32_t second = __byte_perm(v[2][k], v[3][k], e ? 0x7362 : 0x5140);
+        uint32_t b0[2], b1[2];
+        halves_of(__byte_perm(v[0][k], v[1][k], e ? 0x7362 : 0x5140), b0[0], b0[1]);
+        halves_of(__byte_perm(v[2][k], v[3][k], e ? 0x7362 : 0x5140), b1[0], b1[1]);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const uint32_t b0 = halves_of(f ? first >> 16 : first & 0xffffu), b1 = halves_of(f ? second >> 16 : second & 0xffffu);
+        for (int f = 0; f < 2; ++f)
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part) mma_fp16(r.o[k * 4 + e * 2 + f], w[part], b0, b1);
-        }
+          for (int part = 0; part < PARTS; ++part) mma_fp16(r.o[k * 4 + e * 2 + f], w[part], b0[f], b1[f]);
       }
   }
 }
@@ -353,8 +355,13 @@ __device__ __forceinline__ void row_limits(const AttnParams& p, const KvRequest&
 }
 
 // ---- few rows per request: the tokens of all requests and heads as one line of tiles, cut evenly over the CTAs ------------
+//
+// Here the matrix products are turned round: 16 tokens (keys) or 16 columns (values) are the instruction's rows, and its
+// eight columns are eight query rows, of which there are few.  A warp has all query rows and every fourth run of 32
+// tokens, so that a code is converted once; its copies, its stages and its softmax are its own, and the warps meet only
+// where a request ends.
 
-constexpr int kDecodeStages = 3;
+constexpr int kRun = 32, kLine = kRun * kWarps;   // tokens of a warp's step, and of a tile of the line
 
 // What a CTA leaves for the joining kernel: at most one piece of a (request, head) that began in an earlier CTA (slot 0)
 // and one that goes on in later ones (slot 1).
@@ -362,12 +369,20 @@ struct Piece {
   int request, head, last;        // last CTA with a piece of the same; last < 0: none began here
 };
 
-template <int D, int MT>
+template <int D>
+struct RunStage {
+  alignas(128) uint8_t k[kRun * D];
+  uint8_t v[kRun * D];
+  float ks[kRun / kGranule], vs[kRun / kGranule];
+};
+template <int D>
+constexpr int kRunStages = D == 128 ? 3 : 4;
+
+template <int D, int NT>
 struct DecodeShared {
-  Stage<D> stage[kDecodeStages];
-  float merge[MT * kRowsPerWarp][D];
-  float top[kWarps / MT][MT * kRowsPerWarp], sum[kWarps / MT][MT * kRowsPerWarp];
-  int scan[kWarps];
+  RunStage<D> stage[kWarps][kRunStages<D>];
+  float merge[NT * 8][D + 4];
+  float top[kWarps][NT * 8], sum[kWarps][NT * 8];
 };
 
 __host__ __device__ constexpr long long slot_floats(int rows, int D) { return (long long)rows * (D + 2); }
@@ -375,7 +390,7 @@ __host__ __device__ constexpr long long slot_floats(int rows, int D) { return (l
 __device__ __forceinline__ int tiles_of(const AttnParams& p, int b) {
   const long long cap = min((long long)p.a.cache.max_pages * p.a.cache.page, kMaxTokens);
   const int length = (int)min((long long)max(p.a.cache.lengths[b], 0), cap);
-  return (length + kTile - 1) / kTile;
+  return (length + kLine - 1) / kLine;
 }
 
 // Sum of x over the CTA, and over the threads before this one.
@@ -417,23 +432,244 @@ __device__ __forceinline__ void advance(const AttnParams& p, Cursor& at) {
   open_request(p, at);
 }
 
-// CTAs of the decode kernel that an SM holds: what their registers leave room for.
-__host__ __device__ constexpr int resident(int D, int MT, int PARTS) {
-  return D == 64 ? (MT == 4 ? 3 : 4) : MT == 1 && PARTS == 1 ? 3 : 2;
+// Page ids of a warp's run of tokens, fetched a step ahead of its copies.
+struct RunPages {
+  int id[kRun / kGranule];
+};
+__device__ __forceinline__ RunPages fetch_run(const AttnParams& p, const Cursor& at) {
+  RunPages r;
+#pragma unroll
+  for (int i = 0; i < kRun / kGranule; ++i)
+    r.id[i] = page_id(p, at.b, at.tile * (kLine / kGranule) + threadIdx.x / 32 * (kRun / kGranule) + i, at.length);
+  return r;
 }
 
-template <int D, int MT, int PARTS>
-__global__ void __launch_bounds__(kThreads, resident(D, MT, PARTS)) kv_decode_kernel(const __grid_constant__ AttnParams p) {
+// The copies of a run.  Tokens at or beyond the request's length and tokens of padding pages are filled with zeros,
+// whatever memory holds there.
+template <int D>
+__device__ __forceinline__ void load_run(const AttnParams& p, RunStage<D>& s, const Cursor& at, const RunPages& pages) {
+  const CarryGdnKvCache& c = p.a.cache;
+  constexpr int kChunks = D / 16, kCopies = kGranule * kChunks / 32;   // 16-byte copies of a granule, per lane
+  const int lane = threadIdx.x % 32, first = at.tile * (kLine / kGranule) + threadIdx.x / 32 * (kRun / kGranule);
+#pragma unroll
+  for (int i = 0; i < kRun / kGranule; ++i) {
+    const int granule = first + i, id = pages.id[i], left = id > 0 ? at.length - granule * kGranule : 0;
+    const int in_page = granule - page_index(p, granule) * p.page_granules;
+    const long long off = ((long long)at.h * c.page + in_page * kGranule) * D + lane * 16;
+    const uint8_t *k = c.k_codes + id * c.stride_k_page + off, *v = c.v_codes + id * c.stride_v_page + off;
+#pragma unroll
+    for (int x = 0; x < kCopies; ++x) {
+      const int row = lane / kChunks + x * (32 / kChunks);
+      const int to = tile_at<D>(i * kGranule + row, lane % kChunks);
+      const bool there = row < left;
+      __pipeline_memcpy_async(s.k + to, there ? k + x * 512 : c.k_codes, 16, there ? 0 : 16);
+      __pipeline_memcpy_async(s.v + to, there ? v + x * 512 : c.v_codes, 16, there ? 0 : 16);
+    }
+    if (lane < 2) {
+      const int block = at.h * (p.page_granules / p.block_granules) + in_page / p.block_granules;
+      float* to = lane == 0 ? &s.ks[i] : &s.vs[i];
+      if (id > 0) __pipeline_memcpy_async(to, lane == 0 ? c.k_scale + id * c.stride_ks_page + block : c.v_scale + id * c.stride_vs_page + block, 4);
+      else *to = lane == 0 ? kNoTokens : 0.0f;
+    }
+  }
+}
+
+// Query rows as the second operand: lane (g, c) has row 8 n + g, of every 64 columns the 16 from 16 c on.
+template <int D, int NT, int PARTS>
+struct Columns {
+  uint32_t x[NT][PARTS][D / 16][2];
+  float unit[NT][2];              // of rows 8 n + 2 c and 8 n + 2 c + 1: what a product counts, in log2's scale
+};
+template <int D, int NT, int PARTS>
+__device__ __forceinline__ void load_columns(const AttnParams& p, const KvRequest& r, int h, Columns<D, NT, PARTS>& q) {
+  const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = 8 * n + g, i = row / p.group;
+    const bool there = i < r.todo;
+    const long long at = there ? (r.first + i) * p.a.stride_q_tok + (h * p.group + row % p.group) * p.a.stride_q_head : 0;
+    float x[D / 4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < D / 4; ++e) {
+      x[e] = there ? load_as_float(p.a.q, at + e / 16 * 64 + c * 16 + e % 16, p.a.dtype) : 0.0f;
+      top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+    top = max(top, __shfl_xor_sync(~0u, top, 1));
+    top = max(top, __shfl_xor_sync(~0u, top, 2));
+    const int e = up_exponent(top);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    const float unit = p.a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    q.unit[n][0] = __shfl_sync(~0u, unit, c * 8);
+    q.unit[n][1] = __shfl_sync(~0u, unit, c * 8 + 4);
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int pair = 0; pair < 2; ++pair) {
+        float u = x[k * 4 + pair * 2] * up, v = x[k * 4 + pair * 2 + 1] * up;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const uint32_t w = pack_half2(u, v);
+          q.x[n][part][k][pair] = w;
+          const float2 kept = unpack_half2(w);
+          u -= kept.x;
+          v -= kept.y;
+        }
+      }
+  }
+}
+
+// Running softmax over a warp's tokens.  o: lane (g, c) has columns g D/8 + 2 m and + 1 of rows 8 n + 2 c and + 1.
+template <int D, int NT>
+struct Running {
+  float o[NT][D / 16][4];
+  float top[NT][2], sum[NT][2];   // the sums are this lane's share
+  float unit;                     // largest value scale so far: o counts in it, times 2^15
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.0f;
+      top[n][0] = top[n][1] = -INFINITY;
+      sum[n][0] = sum[n][1] = 0.0f;
+    }
+    unit = 0x1p-100f;             // the smallest scale
+  }
+};
+
+// A run of tokens.  `limit`: how many of the run's tokens rows 8 n + 2 c and + 1 see.
+template <int D, int NT, int PARTS>
+__device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D, NT, PARTS>& q, const int (&limit)[NT][2], Running<D, NT>& r) {
+  const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+  constexpr int kBlocks = kRun / kGranule;
+  float score[kBlocks][NT][4] = {};               // tokens g (0, 1) and g + 8 (2, 3) of a block, rows 2c and 2c + 1
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const uint4 u = *reinterpret_cast<const uint4*>(s.k + tile_at<D>(b * kGranule + g, j * 4 + c));
+      const uint4 v = *reinterpret_cast<const uint4*>(s.k + tile_at<D>(b * kGranule + g + 8, j * 4 + c));
+      const uint32_t near[4] = {u.x, u.y, u.z, u.w}, far[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a[4];
+        halves_of(near[k], a[0], a[2]);
+        halves_of(far[k], a[1], a[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+            mma_fp16(score[b][n], a, q.x[n][part][j * 4 + k][0], q.x[n][part][j * 4 + k][1]);
+      }
+    }
+  float unit = r.unit, now[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) now[n][0] = now[n][1] = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const float ks = s.ks[b];
+    const int t = ks == kNoTokens ? 1 << 30 : b * kGranule + g;
+    unit = fmaxf(unit, s.vs[b]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        score[b][n][i] = t + i / 2 * 8 < limit[n][i % 2] ? score[b][n][i] * (q.unit[n][i % 2] * ks) : -INFINITY;
+        now[n][i % 2] = fmaxf(now[n][i % 2], score[b][n][i]);
+      }
+  }
+  bool more = unit > r.unit;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) now[n][i] = fmaxf(now[n][i], __shfl_xor_sync(~0u, now[n][i], d));
+      now[n][i] = fmaxf(now[n][i], r.top[n][i]);
+      more = more || now[n][i] > r.top[n][i];
+    }
+  if (__any_sync(~0u, more)) {
+    const float less = __fdividef(r.unit, unit);
+    r.unit = unit;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float keep = now[n][i] == -INFINITY ? 1.0f : exp2_fast(r.top[n][i] - now[n][i]);
+        r.sum[n][i] *= keep;
+        r.top[n][i] = now[n][i];
+        keep *= less;
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) {
+          r.o[n][m][i] *= keep;
+          r.o[n][m][i + 2] *= keep;
+        }
+      }
+  }
+  const float up = __fdividef(exp2f(kWeightUp), unit);
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const float vs = s.vs[b] * up;
+    uint32_t w[NT][PARTS][2];     // weights of tokens 2c, 2c + 1 and 2c + 8, 2c + 9, row 8 n + g
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[i] = exp2_fast(score[b][n][half * 2 + i] - (r.top[n][i] == -INFINITY ? 0.0f : r.top[n][i]));
+          r.sum[n][i] += x[i];
+          x[i] *= vs;
+        }
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const uint32_t h = pack_half2(x[0], x[1]);
+          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(w[n][part][half]) : "r"(h));
+          const float2 kept = unpack_half2(h);
+          x[0] -= kept.x;
+          x[1] -= kept.y;
+        }
+      }
+    constexpr int kWords = D / 32;                // this lane's columns of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+    uint32_t v[4][kWords];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = b * kGranule + 2 * c + i % 2 + i / 2 * 8;
+      if constexpr (D == 128) {
+        const uint4 u = *reinterpret_cast<const uint4*>(s.v + tile_at<D>(row, g));
+        v[i][0] = u.x; v[i][1] = u.y; v[i][2] = u.z; v[i][3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(s.v + tile_at<D>(row, g / 2) + g % 2 * 8);
+        v[i][0] = u.x; v[i][1] = u.y;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kWords; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t a[4];
+        halves_of(__byte_perm(v[0][k], v[1][k], e ? 0x7362 : 0x5140), a[0], a[1]);
+        halves_of(__byte_perm(v[2][k], v[3][k], e ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) mma_fp16(r.o[n][k * 2 + e], a, w[n][part][0], w[n][part][1]);
+      }
+  }
+}
+
+template <int D, int NT, int PARTS>
+__global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t raw[];
-  DecodeShared<D, MT>& sh = *reinterpret_cast<DecodeShared<D, MT>*>(raw);
+  DecodeShared<D, NT>& sh = *reinterpret_cast<DecodeShared<D, NT>*>(raw);
   __shared__ long long scratch[kWarps];
   __shared__ int found[2];
-  constexpr int kGroups = kWarps / MT, kTok = kTile / kGroups, kRows = MT * kRowsPerWarp;
+  constexpr int kRows = NT * 8, kStages = kRunStages<D>;
   depend_release();
   depend_wait();
   const CarryGdnKvCache& c = p.a.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, cc = lane % 4;
-  const int row0 = warp % MT * kRowsPerWarp, part = warp / MT;
   Piece* pieces = reinterpret_cast<Piece*>(p.a.workspace);
   float* slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + (sizeof(Piece) * gridDim.x + 15) / 16 * 16);
 
@@ -475,105 +711,125 @@ __global__ void __launch_bounds__(kThreads, resident(D, MT, PARTS)) kv_decode_ke
   use.tile = found[1] % use.tiles;
   Cursor load = use;
   long long to_load = to - from;
-  Pages<D> ids;
-  fetch_pages<D>(p, load.b, load.tile, load.length, ids);
+  RunPages pages = fetch_run(p, load);
   auto next_load = [&](int stage) {
     if (to_load > 0) {
-      load_tile<D>(p, sh.stage[stage], load.h, load.tile, load.length, ids);
+      load_run<D>(p, sh.stage[warp][stage], load, pages);
       advance(p, load);
-      if (--to_load > 0) fetch_pages<D>(p, load.b, load.tile, load.length, ids);
+      if (--to_load > 0) pages = fetch_run(p, load);
     }
     __pipeline_commit();
   };
 #pragma unroll
-  for (int s = 0; s < kDecodeStages - 1; ++s) next_load(s);
+  for (int s = 0; s < kStages - 1; ++s) next_load(s);
 
-  Query<D, PARTS> q;
-  Rows<D> r;
+  Columns<D, NT, PARTS> q;
+  Running<D, NT> r;
   KvRequest request;
   bool begin = true;
   int first_tile = 0, stage = 0;
   for (long long at = from; at < to; ++at) {
     if (begin) {
       request = kv_request(c, p.a.rows, use.b, nullptr);
-      load_query<D, PARTS>(p, request, use.h, row0, q);
+      load_columns<D, NT, PARTS>(p, request, use.h, q);
       r.clear();
       first_tile = use.tile;
       begin = false;
     }
-    __pipeline_wait_prior(kDecodeStages - 2);
-    __syncthreads();                              // this tile has landed, and everybody is done with the one before
-    next_load(stage == 0 ? kDecodeStages - 1 : stage - 1);
-    int limit[2];
-    row_limits(p, request, row0, use.tile, limit);
-    attend<D, PARTS, kTok>(sh.stage[stage], part * kTok, q, limit, r);
-    stage = stage + 1 == kDecodeStages ? 0 : stage + 1;
+    __pipeline_wait_prior(kStages - 2);
+    __syncwarp();                                 // this run has landed, and every lane is done with the one before
+    next_load(stage == 0 ? kStages - 1 : stage - 1);
+    const int start = use.tile * kLine + warp * kRun;
+    if (start < request.length) {
+      int limit[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int x = (8 * n + 2 * cc + i) / p.group;
+          limit[n][i] = x < request.todo ? request.length - request.count + x + 1 - start : 0;
+        }
+      attend_run<D, NT, PARTS>(sh.stage[warp][stage], q, limit, r);
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
     const bool ends = use.tile + 1 == use.tiles;
     if (ends || at + 1 == to) {
-      // the warps of a row tile join: weights first, then the outputs in turn
+      // the warps join: weights first, then the outputs in turn
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float sum = quad_sum(r.sum[half]);
-        if (cc == 0) {
-          sh.top[part][row0 + g + half * 8] = r.top[half];
-          sh.sum[part][row0 + g + half * 8] = sum;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float sum = r.sum[n][i];
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
+          if (g == 0) {
+            sh.top[warp][8 * n + 2 * cc + i] = r.top[n][i];
+            sh.sum[warp][8 * n + 2 * cc + i] = sum;
+          }
         }
+      __syncthreads();
+      float top[NT][2], sum[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 8 * n + 2 * cc + i;
+          float m = -INFINITY, l = 0.0f;
+#pragma unroll
+          for (int x = 0; x < kWarps; ++x) m = fmaxf(m, sh.top[x][row]);
+          const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int x = 0; x < kWarps; ++x) l += sh.sum[x][row] * exp2_fast(sh.top[x][row] - base);
+          const float w = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[n][i] - base), l) * exp2f(-kWeightUp);
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) {
+            r.o[n][x][i] = r.o[n][x][i] * w * r.unit;
+            r.o[n][x][i + 2] = r.o[n][x][i + 2] * w * r.unit;
+          }
+          top[n][i] = m;
+          sum[n][i] = l;
+        }
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        if (x > 0) __syncthreads();
+        if (x != warp) continue;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int m = 0; m < D / 16; m += 2) {
+              float4* cell = reinterpret_cast<float4*>(&sh.merge[8 * n + 2 * cc + i][g * (D / 8) + 2 * m]);
+              float4 mine = make_float4(r.o[n][m][i], r.o[n][m][i + 2], r.o[n][m + 1][i], r.o[n][m + 1][i + 2]);
+              if (x > 0) {
+                const float4 had = *cell;
+                mine.x += had.x; mine.y += had.y; mine.z += had.z; mine.w += had.w;
+              }
+              *cell = mine;
+            }
       }
       __syncthreads();
-      float top[2], sum[2];
+      const bool whole = ends && first_tile == 0;
+      float* slot = slots + (2 * blockIdx.x + (first_tile == 0)) * slot_floats(kRows, D);
+      if (!whole && warp == 0 && g == 0) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = row0 + g + half * 8;
-        top[half] = -INFINITY;
-        sum[half] = 0.0f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int x = 0; x < kGroups; ++x) top[half] = fmaxf(top[half], sh.top[x][row]);
-        const float base = top[half] == -INFINITY ? 0.0f : top[half];
-#pragma unroll
-        for (int x = 0; x < kGroups; ++x) sum[half] += sh.sum[x][row] * exp2_fast(sh.top[x][row] - base);
-        const float w = sum[half] == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[half] - base), sum[half]) * exp2f(-kWeightUp);
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          r.o[n][2 * half] = r.o[n][2 * half] * w * r.unit;
-          r.o[n][2 * half + 1] = r.o[n][2 * half + 1] * w * r.unit;
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < kGroups; ++x) {
-        if (x > 0) __syncthreads();
-        if (x != part) continue;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& cell = sh.merge[row0 + g + half * 8][(2 * cc + i) * (D / 8) + n];
-              float& mine = r.o[n][2 * half + i];
-              if (x > 0) mine += cell;
-              if (x + 1 < kGroups) cell = mine;
-            }
-      }
-      if (part == kGroups - 1) {
-        if (ends && first_tile == 0) {
-          store_rows<D>(p, request, use.h, row0, r);
-        } else {
-          float* slot = slots + (2 * blockIdx.x + (first_tile == 0)) * slot_floats(kRows, D);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int row = row0 + g + half * 8;
-            if (row >= p.rows) continue;
-            if (cc == 0) {
-              slot[row] = top[half];
-              slot[kRows + row] = sum[half];
-            }
-            float4* o = reinterpret_cast<float4*>(slot + 2 * kRows + row * D + cc * (D / 4));
-#pragma unroll
-            for (int e = 0; e < D / 4; e += 4) {
-              const int i = 2 * half + e / (D / 8), n = e % (D / 8);
-              o[e / 4] = make_float4(r.o[n][i], r.o[n + 1][i], r.o[n + 2][i], r.o[n + 3][i]);
-            }
+          for (int i = 0; i < 2; ++i) {
+            slot[8 * n + 2 * cc + i] = top[n][i];
+            slot[kRows + 8 * n + 2 * cc + i] = sum[n][i];
           }
+      }
+      for (int i = threadIdx.x; i < request.todo * p.group * (D / 8); i += kThreads) {
+        const int row = i / (D / 8), col = i % (D / 8) * 8;
+        alignas(16) float x[8];
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(&sh.merge[row][col]);
+        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(&sh.merge[row][col + 4]);
+        if (whole) {
+          store8(p.a.out, (request.first + row / p.group) * p.a.stride_out_tok + (use.h * p.group + row % p.group) * p.a.stride_out_head + col,
+                 p.a.dtype, x);
+        } else {
+          store8(slot, 2 * kRows + row * D + col, CARRY_F32, x);
         }
       }
       if (!ends && first_tile == 0 && threadIdx.x == 0) {
@@ -581,6 +837,7 @@ __global__ void __launch_bounds__(kThreads, resident(D, MT, PARTS)) kv_decode_ke
         const long long last = at + (use.tiles - 1 - use.tile);
         pieces[blockIdx.x] = {use.b, use.h, (int)(last / share)};
       }
+      __syncthreads();
       begin = true;
     }
     advance(p, use);
@@ -686,16 +943,16 @@ __global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constan
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
 
-int row_tiles(const CarryGdnKvAttentionArgs& a) {   // 1, 2 or 4 for the decode kernel, 0 for the other
+// Tiles of eight query rows that a warp of the decode kernel holds, or 0 where the rows are too many for its registers.
+int column_tiles(const CarryGdnKvAttentionArgs& a) {
   const long long rows = (long long)a.rows.max_query * (a.HQ / a.cache.HKV);
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 0;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 && a.dtype != CARRY_F32 ? 4 : 0;
 }
 
 // CTAs of the decode kernel: all that are resident at a time, or one per tile where there cannot be as many.
-long long decode_ctas(const CarryGdnKvAttentionArgs& a, int mt) {
+long long decode_ctas(const CarryGdnKvAttentionArgs& a) {
   const long long tokens = (long long)a.cache.max_pages * a.cache.page;
-  const long long most = (tokens + kTile - 1) / kTile * a.cache.HKV * a.rows.B;
-  const long long fit = (long long)sm_count() * resident(a.cache.D, mt, a.dtype == CARRY_F32 ? 2 : 1);
+  const long long most = (tokens + kLine - 1) / kLine * a.cache.HKV * a.rows.B, fit = 2LL * sm_count();
   return most < 1 ? 1 : most < fit ? most : fit;
 }
 
@@ -706,21 +963,22 @@ int prepare(K kernel, size_t smem) {
   return CARRY_GDN_ERR_LAUNCH;
 }
 
-template <int D, int MT, int PARTS>
+template <int D, int NT, int PARTS>
 int launch_decode(const AttnParams& p, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(DecodeShared<D, MT>);
-  const unsigned ctas = (unsigned)decode_ctas(p.a, MT);
-  int rc = prepare(kv_decode_kernel<D, MT, PARTS>, smem);
-  if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, MT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
+  constexpr size_t smem = sizeof(DecodeShared<D, NT>);
+  const unsigned ctas = (unsigned)decode_ctas(p.a);
+  int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem);
+  if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, NT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
   if (rc != CARRY_GDN_OK) return rc;
-  return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kThreads, 0, stream, p, MT * kRowsPerWarp);
+  return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kThreads, 0, stream, p, NT * 8);
 }
 
 template <int D, int PARTS>
-int launch_by_rows(const AttnParams& p, int mt, cudaStream_t stream) {
-  if (mt == 1) return launch_decode<D, 1, PARTS>(p, stream);
-  if (mt == 2) return launch_decode<D, 2, PARTS>(p, stream);
-  if (mt == 4) return launch_decode<D, 4, PARTS>(p, stream);
+int launch_by_rows(const AttnParams& p, int tiles, cudaStream_t stream) {
+  if (tiles == 1) return launch_decode<D, 1, PARTS>(p, stream);
+  if (tiles == 2) return launch_decode<D, 2, PARTS>(p, stream);
+  if constexpr (PARTS == 1)
+    if (tiles == 4) return launch_decode<D, 4, PARTS>(p, stream);
   constexpr size_t smem = sizeof(Stage<D>) * kChunkStages;
   const long long rows = (long long)p.a.rows.max_query * p.group;
   const int rc = prepare(kv_chunk_kernel<D, PARTS>, smem);
@@ -732,11 +990,11 @@ int launch_by_rows(const AttnParams& p, int mt, cudaStream_t stream) {
 }  // namespace
 
 int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a) {
-  const int mt = row_tiles(a);
-  if (mt == 0) return 0;
+  const int tiles = column_tiles(a);
+  if (tiles == 0) return 0;
   if (sm_count() == 0) return CARRY_GDN_ERR_NO_DEVICE;
-  const long long ctas = decode_ctas(a, mt);
-  return (sizeof(Piece) * ctas + 15) / 16 * 16 + 2 * ctas * slot_floats(mt * kRowsPerWarp, a.cache.D) * 4;
+  const long long ctas = decode_ctas(a);
+  return (sizeof(Piece) * ctas + 15) / 16 * 16 + 2 * ctas * slot_floats(tiles * 8, a.cache.D) * 4;
 }
 
 int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream) {
@@ -744,10 +1002,10 @@ int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream) {
   AttnParams p = {a, a.HQ / a.cache.HKV, a.cache.page / kGranule, -1, a.cache.block / kGranule, 0};
   for (int s = 0; s < 31; ++s)
     if (1 << s == p.page_granules) p.page_shift = s;
-  const int mt = row_tiles(a);
-  p.rows = mt ? a.rows.max_query * p.group : 0;
-  if (a.cache.D == 64) return a.dtype == CARRY_F32 ? launch_by_rows<64, 2>(p, mt, stream) : launch_by_rows<64, 1>(p, mt, stream);
-  return a.dtype == CARRY_F32 ? launch_by_rows<128, 2>(p, mt, stream) : launch_by_rows<128, 1>(p, mt, stream);
+  const int tiles = column_tiles(a);
+  p.rows = tiles ? a.rows.max_query * p.group : 0;
+  if (a.cache.D == 64) return a.dtype == CARRY_F32 ? launch_by_rows<64, 2>(p, tiles, stream) : launch_by_rows<64, 1>(p, tiles, stream);
+  return a.dtype == CARRY_F32 ? launch_by_rows<128, 2>(p, tiles, stream) : launch_by_rows<128, 1>(p, tiles, stream);
 }
 
 }  // namespace carry
