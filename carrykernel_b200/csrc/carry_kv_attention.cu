@@ -130,6 +130,37 @@ __device__ __forceinline__ void load_tile(const AttnParams& p, Stage<D>& s, int 
 
 // ---- one warp's rows -------------------------------------------------------------------------------------------------
 
+// This lane's share of a query row, in one trip to memory: of every 64 columns the 16 from 16 c on.  (One element at a
+// time, with its type asked for each, every load would wait for the conversion of the one before.)
+template <int D, int PARTS>
+__device__ __forceinline__ void load_share(const AttnParams& p, long long at, bool there, float (&x)[D / 4]) {
+  const int c = threadIdx.x % 4;
+  if constexpr (PARTS == 2) {
+    const float* q = reinterpret_cast<const float*>(p.a.q) + at + c * 16;
+#pragma unroll
+    for (int e = 0; e < D / 4; ++e) x[e] = there ? q[e / 16 * 64 + e % 16] : 0.0f;
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p.a.q) + at + c * 16;
+    uint32_t w[D / 8] = {};
+    if (there && reinterpret_cast<uintptr_t>(q) % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(q + i / 2 * 64 + i % 2 * 8);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+      }
+    } else if (there) {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) w[i] = q[i / 8 * 64 + i % 8 * 2] | static_cast<uint32_t>(q[i / 8 * 64 + i % 8 * 2 + 1]) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const float2 f = p.a.dtype == CARRY_BF16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)) : unpack_half2(w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+
 // The power of two that a query row is divided by, from the bits of its largest magnitude: what is left is below 2^15.
 __device__ __forceinline__ int up_exponent(uint32_t top) { return min(max(static_cast<int>(top >> 23) - 127, -100), 127) - 14; }
 
@@ -152,11 +183,9 @@ __device__ __forceinline__ void load_query(const AttnParams& p, const KvRequest&
     const long long at = there ? (r.first + i) * p.a.stride_q_tok + (h * p.group + row % p.group) * p.a.stride_q_head : 0;
     float x[D / 4];
     uint32_t top = 0;
+    load_share<D, PARTS>(p, at, there, x);
 #pragma unroll
-    for (int e = 0; e < D / 4; ++e) {
-      x[e] = there ? load_as_float(p.a.q, at + e / 16 * 64 + c * 16 + e % 16, p.a.dtype) : 0.0f;
-      top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-    }
+    for (int e = 0; e < D / 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     top = max(top, __shfl_xor_sync(~0u, top, 1));
     top = max(top, __shfl_xor_sync(~0u, top, 2));
     const int e = up_exponent(top);
@@ -490,11 +519,9 @@ __device__ __forceinline__ void load_columns(const AttnParams& p, const KvReques
     const long long at = there ? (r.first + i) * p.a.stride_q_tok + (h * p.group + row % p.group) * p.a.stride_q_head : 0;
     float x[D / 4];
     uint32_t top = 0;
+    load_share<D, PARTS>(p, at, there, x);
 #pragma unroll
-    for (int e = 0; e < D / 4; ++e) {
-      x[e] = there ? load_as_float(p.a.q, at + e / 16 * 64 + c * 16 + e % 16, p.a.dtype) : 0.0f;
-      top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-    }
+    for (int e = 0; e < D / 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     top = max(top, __shfl_xor_sync(~0u, top, 1));
     top = max(top, __shfl_xor_sync(~0u, top, 2));
     const int e = up_exponent(top);
@@ -694,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const __grid_con
   for (int b0 = 0; b0 < p.a.rows.B; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
     const long long mine = b < p.a.rows.B ? (long long)tiles_of(p, b) * c.HKV : 0;
-    const long long all = block_scan(mine, scratch, before);
+    const long long all = p.a.rows.B <= kThreads ? total : block_scan(mine, scratch, before);   // else `before` is still right
     if (mine > 0 && from >= seen + before && from < seen + before + mine) {
       found[0] = b;
       found[1] = (int)(from - seen - before);
@@ -844,10 +871,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const __grid_con
   }
 }
 
-// Joins the pieces of the (request, head) that began in CTA blockIdx.x of the kernel above: one warp per row.
+// Joins the pieces of the (request, head) that began in CTA blockIdx.x of the kernel above, row by row: first all
+// weights, then the rows themselves, each in one trip to memory as far as registers go.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinStep = 256;
+
 template <int D>
-__global__ void __launch_bounds__(kThreads) kv_join_kernel(const __grid_constant__ AttnParams p, const int kRows) {
-  __shared__ float part_o[kWarps][D];
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttnParams p, const int kRows) {
+  __shared__ float tops[kJoinWarps], sums[kJoinWarps], weight[kJoinStep], part_o[kJoinWarps][D];
   depend_release();
   depend_wait();
   const Piece piece = reinterpret_cast<const Piece*>(p.a.workspace)[blockIdx.x];
@@ -857,32 +887,52 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(const __grid_constant
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, count = piece.last - blockIdx.x + 1;
   auto slot = [&](int i) { return slots + (2 * (blockIdx.x + i) + (i == 0)) * slot_floats(kRows, D); };
   for (int row = blockIdx.y; row < q.todo * p.group; row += gridDim.y) {
-    float top = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < count; i += 32) top = fmaxf(top, slot(i)[row]);
+    float top = -INFINITY, sum = 0.0f, all = 0.0f, o[D / 32] = {};
+    for (int i = threadIdx.x; i < count; i += kJoinThreads) top = fmaxf(top, slot(i)[row]);
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
     const float base = top == -INFINITY ? 0.0f : top;
-    for (int i = lane; i < count; i += 32) sum += slot(i)[kRows + row] * exp2_fast(slot(i)[row] - base);
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-    float o[D / 32] = {};
-#pragma unroll 4
-    for (int i = warp; i < count; i += kWarps) {
-      const float* s = slot(i);
-      const float w = s[kRows + row] * exp2_fast(s[row] - base);
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) o[e] = fmaf(w, s[2 * kRows + row * D + e * 32 + lane], o[e]);
+    for (int first = 0; first < count; first += kJoinStep) {
+      const int n = min(count - first, kJoinStep);
+      __syncthreads();
+      if (threadIdx.x < n) {
+        const float* s = slot(first + threadIdx.x);
+        const float w = s[kRows + row] * exp2_fast(s[row] - base);
+        weight[threadIdx.x] = w;
+        sum += w;
+      }
+      __syncthreads();
+#pragma unroll 8
+      for (int i = warp; i < n; i += kJoinWarps) {
+        const float* s = slot(first + i) + 2 * kRows + row * D + lane * (D / 32);
+        const float w = weight[i];
+        if constexpr (D == 128) {
+          const float4 x = *reinterpret_cast<const float4*>(s);
+          o[0] = fmaf(w, x.x, o[0]); o[1] = fmaf(w, x.y, o[1]); o[2] = fmaf(w, x.z, o[2]); o[3] = fmaf(w, x.w, o[3]);
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(s);
+          o[0] = fmaf(w, x.x, o[0]); o[1] = fmaf(w, x.y, o[1]);
+        }
+      }
     }
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) part_o[warp][e * 32 + lane] = o[e];
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    if (lane == 0) sums[warp] = sum;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) part_o[warp][lane * (D / 32) + e] = o[e];
     __syncthreads();
-    const int i = row / p.group;
-    for (int d = threadIdx.x; d < D; d += kThreads) {
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) all += sums[w];
+    if (threadIdx.x < D) {
       float x = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) x += part_o[w][d];
-      store_from_float(p.a.out, (q.first + i) * p.a.stride_out_tok + (piece.head * p.group + row % p.group) * p.a.stride_out_head + d,
-                       p.a.dtype, sum == 0.0f ? 0.0f : __fdiv_rn(x, sum));
+      for (int w = 0; w < kJoinWarps; ++w) x += part_o[w][threadIdx.x];
+      store_from_float(p.a.out, (q.first + row / p.group) * p.a.stride_out_tok + (piece.head * p.group + row % p.group) * p.a.stride_out_head + threadIdx.x,
+                       p.a.dtype, all == 0.0f ? 0.0f : __fdiv_rn(x, all));
     }
     __syncthreads();
   }
@@ -970,7 +1020,7 @@ int launch_decode(const AttnParams& p, cudaStream_t stream) {
   int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem);
   if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, NT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
   if (rc != CARRY_GDN_OK) return rc;
-  return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kThreads, 0, stream, p, NT * 8);
+  return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kJoinThreads, 0, stream, p, NT * 8);
 }
 
 template <int D, int PARTS>
