@@ -30,7 +30,7 @@ struct AttnParams {
   CarryGdnKvAttentionArgs a;
   int group;                      // query heads per key/value head
   int page_granules, page_shift;  // granules in a page, and its logarithm or -1
-  int block_granules;
+  int block_granules, block_shift;
   int rows;                       // rows of a row tile that may be in use (decode kernel)
 };
 
@@ -484,21 +484,30 @@ __device__ __forceinline__ void load_run(const AttnParams& p, RunStage<D>& s, co
   for (int i = 0; i < kRun / kGranule; ++i) {
     const int granule = first + i, id = pages.id[i], left = id > 0 ? at.length - granule * kGranule : 0;
     const int in_page = granule - page_index(p, granule) * p.page_granules;
-    const long long off = ((long long)at.h * c.page + in_page * kGranule) * D + lane * 16;
+    const int off = (at.h * c.page + in_page * kGranule) * D + lane * 16;   // a page is below 2^31 bytes
     const uint8_t *k = c.k_codes + id * c.stride_k_page + off, *v = c.v_codes + id * c.stride_v_page + off;
+    int to[kCopies];
 #pragma unroll
-    for (int x = 0; x < kCopies; ++x) {
-      const int row = lane / kChunks + x * (32 / kChunks);
-      const int to = tile_at<D>(i * kGranule + row, lane % kChunks);
-      const bool there = row < left;
-      __pipeline_memcpy_async(s.k + to, there ? k + x * 512 : c.k_codes, 16, there ? 0 : 16);
-      __pipeline_memcpy_async(s.v + to, there ? v + x * 512 : c.v_codes, 16, there ? 0 : 16);
+    for (int x = 0; x < kCopies; ++x) to[x] = tile_at<D>(i * kGranule + lane / kChunks + x * (32 / kChunks), lane % kChunks);
+    if (left >= kGranule) {
+#pragma unroll
+      for (int x = 0; x < kCopies; ++x) {
+        __pipeline_memcpy_async(s.k + to[x], k + x * 512, 16);
+        __pipeline_memcpy_async(s.v + to[x], v + x * 512, 16);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < kCopies; ++x) {
+        const bool there = lane / kChunks + x * (32 / kChunks) < left;
+        __pipeline_memcpy_async(s.k + to[x], there ? k + x * 512 : c.k_codes, 16, there ? 0 : 16);
+        __pipeline_memcpy_async(s.v + to[x], there ? v + x * 512 : c.v_codes, 16, there ? 0 : 16);
+      }
     }
     if (lane < 2) {
-      const int block = at.h * (p.page_granules / p.block_granules) + in_page / p.block_granules;
-      float* to = lane == 0 ? &s.ks[i] : &s.vs[i];
-      if (id > 0) __pipeline_memcpy_async(to, lane == 0 ? c.k_scale + id * c.stride_ks_page + block : c.v_scale + id * c.stride_vs_page + block, 4);
-      else *to = lane == 0 ? kNoTokens : 0.0f;
+      const int block = at.h * (p.page_granules / p.block_granules) + (p.block_shift >= 0 ? in_page >> p.block_shift : in_page / p.block_granules);
+      float* to_scale = lane == 0 ? &s.ks[i] : &s.vs[i];
+      if (id > 0) __pipeline_memcpy_async(to_scale, lane == 0 ? c.k_scale + id * c.stride_ks_page + block : c.v_scale + id * c.stride_vs_page + block, 4);
+      else *to_scale = lane == 0 ? kNoTokens : 0.0f;
     }
   }
 }
@@ -507,7 +516,7 @@ __device__ __forceinline__ void load_run(const AttnParams& p, RunStage<D>& s, co
 template <int D, int NT, int PARTS>
 struct Columns {
   uint32_t x[NT][PARTS][D / 16][2];
-  float unit[NT][2];              // of rows 8 n + 2 c and 8 n + 2 c + 1: what a product counts, in log2's scale
+  float unit[NT][2];              // of rows 8 n + 2 c and 8 n + 2 c + 1: what a product counts in log2's scale; not negative
 };
 template <int D, int NT, int PARTS>
 __device__ __forceinline__ void load_columns(const AttnParams& p, const KvRequest& r, int h, Columns<D, NT, PARTS>& q) {
@@ -525,8 +534,8 @@ __device__ __forceinline__ void load_columns(const AttnParams& p, const KvReques
     top = max(top, __shfl_xor_sync(~0u, top, 1));
     top = max(top, __shfl_xor_sync(~0u, top, 2));
     const int e = up_exponent(top);
-    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    const float unit = p.a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), p.a.scale);
+    const float unit = fabsf(p.a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
     q.unit[n][0] = __shfl_sync(~0u, unit, c * 8);
     q.unit[n][1] = __shfl_sync(~0u, unit, c * 8 + 4);
 #pragma unroll
@@ -564,9 +573,10 @@ struct Running {
   }
 };
 
-// A run of tokens.  `limit`: how many of the run's tokens rows 8 n + 2 c and + 1 see.
+// A run of tokens.  `limit`: how many of the run's tokens rows 8 n + 2 c and + 1 see; `all`: every row of the warp sees
+// every one that is there.
 template <int D, int NT, int PARTS>
-__device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D, NT, PARTS>& q, const int (&limit)[NT][2], Running<D, NT>& r) {
+__device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D, NT, PARTS>& q, const int (&limit)[NT][2], bool all, Running<D, NT>& r) {
   const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
   constexpr int kBlocks = kRun / kGranule;
   float score[kBlocks][NT][4] = {};               // tokens g (0, 1) and g + 8 (2, 3) of a block, rows 2c and 2c + 1
@@ -589,20 +599,26 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
             mma_fp16(score[b][n], a, q.x[n][part][j * 4 + k][0], q.x[n][part][j * 4 + k][1]);
       }
     }
-  float unit = r.unit, now[NT][2];
+  float unit = r.unit, now[NT][2], count[kBlocks][NT][2];     // count: what a product of the block counts
 #pragma unroll
   for (int n = 0; n < NT; ++n) now[n][0] = now[n][1] = -INFINITY;
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
     const float ks = s.ks[b];
-    const int t = ks == kNoTokens ? 1 << 30 : b * kGranule + g;
     unit = fmaxf(unit, s.vs[b]);
+    if (!all || ks == kNoTokens) {
+      const int t = ks == kNoTokens ? 1 << 30 : b * kGranule + g;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) score[b][n][i] = t + i / 2 * 8 < limit[n][i % 2] ? score[b][n][i] : -INFINITY;
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        score[b][n][i] = t + i / 2 * 8 < limit[n][i % 2] ? score[b][n][i] * (q.unit[n][i % 2] * ks) : -INFINITY;
-        now[n][i % 2] = fmaxf(now[n][i % 2], score[b][n][i]);
+      for (int i = 0; i < 2; ++i) {
+        count[b][n][i] = fmaxf(q.unit[n][i] * ks, 0x1p-126f);
+        now[n][i] = fmaxf(now[n][i], fmaxf(score[b][n][i], score[b][n][i + 2]) * count[b][n][i]);
       }
   }
   bool more = unit > r.unit;
@@ -612,8 +628,8 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) now[n][i] = fmaxf(now[n][i], __shfl_xor_sync(~0u, now[n][i], d));
-      now[n][i] = fmaxf(now[n][i], r.top[n][i]);
       more = more || now[n][i] > r.top[n][i];
+      now[n][i] = fmaxf(now[n][i], r.top[n][i]);
     }
   if (__any_sync(~0u, more)) {
     const float less = __fdividef(r.unit, unit);
@@ -634,6 +650,11 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
       }
   }
   const float up = __fdividef(exp2f(kWeightUp), unit);
+  float base[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) base[n][i] = now[n][i] == -INFINITY ? 0.0f : now[n][i];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
     const float vs = s.vs[b] * up;
@@ -645,7 +666,7 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
         float x[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          x[i] = exp2_fast(score[b][n][half * 2 + i] - (r.top[n][i] == -INFINITY ? 0.0f : r.top[n][i]));
+          x[i] = exp2_fast(fmaf(score[b][n][half * 2 + i], count[b][n][i], -base[n][i]));
           r.sum[n][i] += x[i];
           x[i] *= vs;
         }
@@ -754,12 +775,19 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const __grid_con
   Running<D, NT> r;
   KvRequest request;
   bool begin = true;
-  int first_tile = 0, stage = 0;
+  int first_tile = 0, stage = 0, sees[NT][2];     // tokens that rows 8 n + 2 c and + 1 see
   for (long long at = from; at < to; ++at) {
     if (begin) {
       request = kv_request(c, p.a.rows, use.b, nullptr);
       load_columns<D, NT, PARTS>(p, request, use.h, q);
       r.clear();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int x = (8 * n + 2 * cc + i) / p.group;
+          sees[n][i] = x < request.todo ? request.length - request.count + x + 1 : 0;
+        }
       first_tile = use.tile;
       begin = false;
     }
@@ -770,13 +798,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const __grid_con
     if (start < request.length) {
       int limit[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int x = (8 * n + 2 * cc + i) / p.group;
-          limit[n][i] = x < request.todo ? request.length - request.count + x + 1 - start : 0;
-        }
-      attend_run<D, NT, PARTS>(sh.stage[warp][stage], q, limit, r);
+      for (int n = 0; n < NT; ++n) {
+        limit[n][0] = sees[n][0] - start;
+        limit[n][1] = sees[n][1] - start;
+      }
+      attend_run<D, NT, PARTS>(sh.stage[warp][stage], q, limit, start + kRun <= request.length - request.count + 1, r);
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
     const bool ends = use.tile + 1 == use.tiles;
@@ -1049,9 +1075,11 @@ int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a) {
 
 int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream) {
   if (sm_count() == 0) return CARRY_GDN_ERR_NO_DEVICE;
-  AttnParams p = {a, a.HQ / a.cache.HKV, a.cache.page / kGranule, -1, a.cache.block / kGranule, 0};
-  for (int s = 0; s < 31; ++s)
+  AttnParams p = {a, a.HQ / a.cache.HKV, a.cache.page / kGranule, -1, a.cache.block / kGranule, -1, 0};
+  for (int s = 0; s < 31; ++s) {
     if (1 << s == p.page_granules) p.page_shift = s;
+    if (1 << s == p.block_granules) p.block_shift = s;
+  }
   const int tiles = column_tiles(a);
   p.rows = tiles ? a.rows.max_query * p.group : 0;
   if (a.cache.D == 64) return a.dtype == CARRY_F32 ? launch_by_rows<64, 2>(p, tiles, stream) : launch_by_rows<64, 1>(p, tiles, stream);
