@@ -404,12 +404,13 @@ struct RunStage {
   uint8_t v[kRun * D];
   float ks[kRun / kGranule], vs[kRun / kGranule];
 };
-template <int D>
-constexpr int kRunStages = D == 128 ? 3 : 4;
+// CTAs of the decode kernel on an SM, by their registers, and stages of a warp, by the memory that this leaves.
+__host__ __device__ constexpr int resident(int D, int NT, int PARTS) { return NT == 1 && PARTS == 1 ? (D == 128 ? 3 : 4) : 2; }
+__host__ __device__ constexpr int stages(int D, int NT, int PARTS) { return D == 128 ? (resident(D, NT, PARTS) == 3 ? 2 : 3) : 3; }
 
-template <int D, int NT>
+template <int D, int NT, int PARTS>
 struct DecodeShared {
-  RunStage<D> stage[kWarps][kRunStages<D>];
+  RunStage<D> stage[kWarps][stages(D, NT, PARTS)];
   float merge[NT * 8][D + 4];
   float top[kWarps][NT * 8], sum[kWarps][NT * 8];
 };
@@ -708,12 +709,12 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
 }
 
 template <int D, int NT, int PARTS>
-__global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t raw[];
-  DecodeShared<D, NT>& sh = *reinterpret_cast<DecodeShared<D, NT>*>(raw);
+  DecodeShared<D, NT, PARTS>& sh = *reinterpret_cast<DecodeShared<D, NT, PARTS>*>(raw);
   __shared__ long long scratch[kWarps];
   __shared__ int found[2];
-  constexpr int kRows = NT * 8, kStages = kRunStages<D>;
+  constexpr int kRows = NT * 8, kStages = stages(D, NT, PARTS);
   depend_release();
   depend_wait();
   const CarryGdnKvCache& c = p.a.cache;
@@ -1028,7 +1029,8 @@ int column_tiles(const CarryGdnKvAttentionArgs& a) {
 // CTAs of the decode kernel: all that are resident at a time, or one per tile where there cannot be as many.
 long long decode_ctas(const CarryGdnKvAttentionArgs& a) {
   const long long tokens = (long long)a.cache.max_pages * a.cache.page;
-  const long long most = (tokens + kLine - 1) / kLine * a.cache.HKV * a.rows.B, fit = 2LL * sm_count();
+  const long long most = (tokens + kLine - 1) / kLine * a.cache.HKV * a.rows.B;
+  const long long fit = (long long)sm_count() * resident(a.cache.D, column_tiles(a), a.dtype == CARRY_F32 ? 2 : 1);
   return most < 1 ? 1 : most < fit ? most : fit;
 }
 
@@ -1041,7 +1043,7 @@ int prepare(K kernel, size_t smem) {
 
 template <int D, int NT, int PARTS>
 int launch_decode(const AttnParams& p, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(DecodeShared<D, NT>);
+  constexpr size_t smem = sizeof(DecodeShared<D, NT, PARTS>);
   const unsigned ctas = (unsigned)decode_ctas(p.a);
   int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem);
   if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, NT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
