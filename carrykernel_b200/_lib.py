@@ -184,7 +184,8 @@ EXPORTS = ("carry_gdn_quant_step", "carry_gdn_quant_decode", "carry_gdn_fp32_ste
 # what the native call path is given the addresses of, in the order it expects them (csrc/host_native.cpp, Table)
 _NATIVE_ENTRIES = ("carry_gdn_quant_step", "carry_gdn_fp32_step", "carry_gdn_packed_decode",
                    "carry_gdn_packed_decode_multi", "carry_gdn_pool_store", "carry_gdn_pool_load",
-                   "carry_gdn_pool_copy", "carry_gdn_pool_copy_layers", "carry_gdn_quant_decode")
+                   "carry_gdn_pool_copy", "carry_gdn_pool_copy_layers", "carry_gdn_quant_decode", "carry_gdn_kv_append",
+                   "carry_gdn_kv_attention", "carry_gdn_kv_attention_workspace", "carry_gdn_add_rms_norm_quant")
 
 _lib = None
 _lock = threading.Lock()

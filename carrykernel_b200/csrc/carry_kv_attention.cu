@@ -1034,18 +1034,25 @@ long long decode_ctas(const CarryGdnKvAttentionArgs& a) {
   return most < 1 ? 1 : most < fit ? most : fit;
 }
 
+// Lets a kernel use `smem` bytes of shared memory: asked for once per device and thread.
 template <class K>
-int prepare(K kernel, size_t smem) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess) return CARRY_GDN_OK;
-  cudaGetLastError();
-  return CARRY_GDN_ERR_LAUNCH;
+int prepare(K kernel, size_t smem, bool (&ready)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev < 64 && ready[dev]) return CARRY_GDN_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return CARRY_GDN_ERR_LAUNCH;
+  }
+  if (dev < 64) ready[dev] = true;
+  return CARRY_GDN_OK;
 }
 
 template <int D, int NT, int PARTS>
 int launch_decode(const AttnParams& p, cudaStream_t stream) {
   constexpr size_t smem = sizeof(DecodeShared<D, NT, PARTS>);
   const unsigned ctas = (unsigned)decode_ctas(p.a);
-  int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem);
+  static thread_local bool ready[64];
+  int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem, ready);
   if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, NT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
   if (rc != CARRY_GDN_OK) return rc;
   return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kJoinThreads, 0, stream, p, NT * 8);
@@ -1059,7 +1066,8 @@ int launch_by_rows(const AttnParams& p, int tiles, cudaStream_t stream) {
     if (tiles == 4) return launch_decode<D, 4, PARTS>(p, stream);
   constexpr size_t smem = sizeof(Stage<D>) * kChunkStages;
   const long long rows = (long long)p.a.rows.max_query * p.group;
-  const int rc = prepare(kv_chunk_kernel<D, PARTS>, smem);
+  static thread_local bool ready[64];
+  const int rc = prepare(kv_chunk_kernel<D, PARTS>, smem, ready);
   if (rc != CARRY_GDN_OK) return rc;
   const dim3 grid((unsigned)((rows + kChunkRows - 1) / kChunkRows), p.a.cache.HKV, p.a.rows.B);
   return launch_dependent(kv_chunk_kernel<D, PARTS>, grid, kThreads, smem, stream, p);

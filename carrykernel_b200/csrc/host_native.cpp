@@ -36,8 +36,12 @@ struct Table {
   int (*pool_copy)(const CarryGdnPoolCopyArgs*, void*);
   int (*pool_copy_layers)(const CarryGdnPoolCopyLayersArgs*, void*);
   int (*quant_decode)(const CarryGdnDecodeArgs*, void*);
+  int (*kv_append)(const CarryGdnKvAppendArgs*, void*);
+  int (*kv_attention)(const CarryGdnKvAttentionArgs*, void*);
+  int64_t (*kv_attention_workspace)(const CarryGdnKvAttentionArgs*);
+  int (*add_rms_norm_quant)(const CarryGdnNormArgs*, void*);
 };
-constexpr int kEntries = 9;
+constexpr int kEntries = 13;
 
 const Table* table_of(PyObject* o) { return static_cast<const Table*>(PyLong_AsVoidPtr(o)); }
 
@@ -556,6 +560,156 @@ PyObject* pool_copy_layers(PyObject*, PyObject* const* o, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------------------
+// the key/value cache and the layer norm
+// ---------------------------------------------------------------------------
+
+// The call's rows [N, heads, D] and whose they are; `query_start` may be None.
+bool kv_rows_of(const at::Tensor* x, PyObject* lengths, PyObject* query_start, PyObject* max_query_len, int dev,
+                CarryGdnKvCache& c, CarryGdnKvRows& r) {
+  const at::Tensor* len = plain(lengths);
+  if (!x || x->dim() != 3 || !is(x, x->scalar_type(), dev) || x->stride(2) != 1) return false;
+  if (!is(len, at::kInt, dev) || len->dim() != 1 || !len->is_contiguous()) return false;
+  const int64_t N = x->size(0), B = len->size(0);
+  if (!fits32(N) || !fits32(B)) return false;
+  long most = 0;
+  const bool bounded = max_query_len != Py_None;
+  if (bounded && !as_int(max_query_len, most)) return false;
+  if (query_start == Py_None) {
+    if (N % B || (bounded && most != N / B)) return false;
+    r.max_query = static_cast<int32_t>(N / B);
+  } else {
+    const at::Tensor* start = plain(query_start);
+    if (!bounded || most < 1 || !is(start, at::kInt, dev) || !start->is_contiguous() || !shaped(*start, {B + 1})) return false;
+    r.query_start = static_cast<const int32_t*>(start->data_ptr());
+    r.max_query = static_cast<int32_t>(most < N ? most : N);
+  }
+  r.B = static_cast<int32_t>(B);
+  r.N = static_cast<int32_t>(N);
+  c.lengths = static_cast<const int32_t*>(len->data_ptr());
+  return true;
+}
+
+// o: k_codes, k_scale, v_codes, v_scale; everything that the C entry does not look at itself
+bool kv_cache_of(PyObject* const* o, PyObject* table, int64_t B, int& dev, CarryGdnKvCache& c) {
+  const at::Tensor *kc = plain(o[0]), *ks = plain(o[1]), *vc = plain(o[2]), *vs = plain(o[3]), *t = plain(table);
+  if (!kc || !ks || !vc || !vs || !t || kc->dim() != 4 || !kc->is_cuda()) return false;
+  dev = kc->get_device();
+  const int64_t pages = kc->size(0), HKV = kc->size(1), page = kc->size(2), D = kc->size(3);
+  if (!fits32(pages) || !fits32(HKV) || !fits32(page) || ks->dim() != 3) return false;
+  const int64_t per = ks->size(2);
+  if (per < 1 || page % per) return false;
+  if (!is(kc, at::kFloat8_e4m3fn, dev) || !is(vc, at::kFloat8_e4m3fn, dev) || !is(ks, at::kFloat, dev) || !is(vs, at::kFloat, dev)) return false;
+  if (!shaped(*vc, {pages, HKV, page, D}) || !shaped(*ks, {pages, HKV, per}) || !shaped(*vs, {pages, HKV, per})) return false;
+  if (!dense_inside(*kc, {page * D, D, 1}) || !dense_inside(*vc, {page * D, D, 1}) || !dense_inside(*ks, {per, 1}) || !dense_inside(*vs, {per, 1})) return false;
+  if (!is(t, at::kInt, dev) || t->dim() != 2 || t->size(0) != B || !fits32(t->size(1)) || t->stride(1) != 1) return false;
+  c.k_codes = static_cast<uint8_t*>(kc->data_ptr()); c.k_scale = static_cast<float*>(ks->data_ptr());
+  c.v_codes = static_cast<uint8_t*>(vc->data_ptr()); c.v_scale = static_cast<float*>(vs->data_ptr());
+  c.stride_k_page = kc->stride(0); c.stride_ks_page = ks->stride(0);
+  c.stride_v_page = vc->stride(0); c.stride_vs_page = vs->stride(0);
+  c.block_table = static_cast<const int32_t*>(t->data_ptr()); c.stride_table = t->stride(0);
+  c.num_pages = static_cast<int32_t>(pages); c.HKV = static_cast<int32_t>(HKV); c.page = static_cast<int32_t>(page);
+  c.block = static_cast<int32_t>(page / per); c.D = static_cast<int32_t>(D); c.max_pages = static_cast<int32_t>(t->size(1));
+  return true;
+}
+int device_of(PyObject* o) {
+  const at::Tensor* t = plain(o);
+  return t && t->is_cuda() ? t->get_device() : -1;
+}
+
+// (table, k, v, k_codes, k_scale, v_codes, v_scale, block_table, lengths, query_start, max_query_len, status) -> True
+PyObject* kv_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 12) return nullptr;
+    const Table* tab = table_of(o[0]);
+    const at::Tensor *k = plain(o[1]), *v = plain(o[2]);
+    int dev = device_of(o[3]);
+    CarryGdnKvAppendArgs a = {};
+    if (!tab || dev < 0 || !kv_rows_of(k, o[8], o[9], o[10], dev, a.cache, a.rows) || !kv_cache_of(o + 3, o[7], a.rows.B, dev, a.cache)) return nullptr;
+    if (!is(v, k->scalar_type(), dev) || v->dim() != 3 || v->stride(2) != 1) return nullptr;
+    for (const at::Tensor* t : {k, v})
+      if (!shaped(*t, {a.rows.N, a.cache.HKV, a.cache.D})) return nullptr;
+    a.dtype = dtype_id(k->scalar_type());
+    if (a.dtype < 0 || !status_of(o[11], dev, &a.status)) return nullptr;
+    a.k = k->data_ptr(); a.stride_k_tok = k->stride(0); a.stride_k_head = k->stride(1);
+    a.v = v->data_ptr(); a.stride_v_tok = v->stride(0); a.stride_v_head = v->stride(1);
+    return launch(dev, [&](void* s) { return tab->kv_append(&a, s); }) ? Py_NewRef(Py_True) : nullptr;
+  });
+}
+
+// (table, q, scale, k_codes, k_scale, v_codes, v_scale, out, block_table, lengths, query_start, max_query_len, workspace,
+//  status) -> True
+PyObject* kv_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 14) return nullptr;
+    const Table* tab = table_of(o[0]);
+    const at::Tensor *q = plain(o[1]), *out = plain(o[7]);
+    int dev = device_of(o[3]);
+    CarryGdnKvAttentionArgs a = {};
+    if (!tab || dev < 0 || !kv_rows_of(q, o[9], o[10], o[11], dev, a.cache, a.rows) || !kv_cache_of(o + 3, o[8], a.rows.B, dev, a.cache)) return nullptr;
+    if (!is(out, q->scalar_type(), dev) || out->dim() != 3 || out->stride(2) != 1 || out->sizes() != q->sizes() || q->size(2) != a.cache.D) return nullptr;
+    if (!fits32(q->size(1))) return nullptr;
+    a.HQ = static_cast<int32_t>(q->size(1));
+    a.dtype = dtype_id(q->scalar_type());
+    const double scale = PyFloat_AsDouble(o[2]);
+    if ((scale == -1.0 && PyErr_Occurred()) || a.dtype < 0 || !status_of(o[13], dev, &a.status)) return nullptr;
+    a.scale = static_cast<float>(scale);
+    a.q = q->data_ptr(); a.stride_q_tok = q->stride(0); a.stride_q_head = q->stride(1);
+    a.out = out->data_ptr(); a.stride_out_tok = out->stride(0); a.stride_out_head = out->stride(1);
+    c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const int64_t need = tab->kv_attention_workspace(&a);
+    if (need < 0) return nullptr;
+    at::Tensor work;
+    if (o[12] != Py_None) {
+      const at::Tensor* w = plain(o[12]);
+      if (!w || !w->is_cuda() || w->get_device() != dev || !w->is_contiguous()) return nullptr;
+      work = *w;
+    } else if (need > 0) {
+      work = fresh({need}, at::kByte, dev);
+    }
+    if (work.defined()) {
+      a.workspace = work.data_ptr();
+      a.workspace_bytes = static_cast<int64_t>(work.nbytes());
+    }
+    return launch(dev, [&](void* s) { return tab->kv_attention(&a, s); }) ? Py_NewRef(Py_True) : nullptr;
+  });
+}
+
+// (table, x, residual, weight, codes, scale, eps, residual_out) -> True
+PyObject* add_rms_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 8) return nullptr;
+    const Table* tab = table_of(o[0]);
+    const at::Tensor *x = plain(o[1]), *w = plain(o[3]), *codes = plain(o[4]), *scale = plain(o[5]);
+    const at::Tensor *res = o[2] == Py_None ? nullptr : plain(o[2]), *res_out = o[7] == Py_None ? res : plain(o[7]);
+    if (!tab || !x || !w || !codes || !scale || x->dim() != 2 || !x->is_cuda() || (o[2] != Py_None && !res) || (o[7] != Py_None && !res_out)) return nullptr;
+    const int dev = x->get_device();
+    const int64_t N = x->size(0), W = x->size(1), groups = (W + 127) / 128;
+    if (!fits32(N) || !fits32(W)) return nullptr;
+    CarryGdnNormArgs a = {};
+    for (const at::Tensor* t : {x, res, res_out, codes})
+      if (t && (!is(t, t->scalar_type(), dev) || !shaped(*t, {N, W}) || t->stride(1) != 1)) return nullptr;
+    if (res && res->scalar_type() != res_out->scalar_type()) return nullptr;
+    if (!is(w, w->scalar_type(), dev) || !shaped(*w, {W}) || !w->is_contiguous() || codes->scalar_type() != at::kFloat8_e4m3fn) return nullptr;
+    if (!is(scale, at::kFloat, dev) || !scale->is_contiguous() || !(scale->dim() == 1 ? shaped(*scale, {N}) : shaped(*scale, {N, groups}))) return nullptr;
+    a.x = x->data_ptr(); a.stride_x = x->stride(0); a.x_dtype = dtype_id(x->scalar_type());
+    a.residual_dtype = a.x_dtype;
+    if (res) { a.residual = res->data_ptr(); a.stride_residual = res->stride(0); }
+    if (res_out) {
+      a.residual_out = res_out->data_ptr(); a.stride_residual_out = res_out->stride(0);
+      a.residual_dtype = dtype_id(res_out->scalar_type());
+    }
+    a.weight = w->data_ptr(); a.weight_dtype = dtype_id(w->scalar_type());
+    a.codes = static_cast<uint8_t*>(codes->data_ptr()); a.stride_codes = codes->stride(0);
+    a.scale = static_cast<float*>(scale->data_ptr());
+    const double eps = PyFloat_AsDouble(o[6]);
+    if ((eps == -1.0 && PyErr_Occurred()) || a.x_dtype < 0 || a.residual_dtype < 0 || a.weight_dtype < 0) return nullptr;
+    a.eps = static_cast<float>(eps);
+    a.N = static_cast<int32_t>(N); a.W = static_cast<int32_t>(W); a.group = scale->dim() == 2 ? 128 : 0;
+    return launch(dev, [&](void* s) { return tab->add_rms_norm_quant(&a, s); }) ? Py_NewRef(Py_True) : nullptr;
+  });
+}
+
 // (address of each entry point, in the order of Table) -> the table's address; it lives as long as the process
 PyObject* make_table(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (n != kEntries) {
@@ -579,6 +733,7 @@ PyObject* make_table(PyObject*, PyObject* const* o, Py_ssize_t n) {
 #define CARRY_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CARRY_FAST(make_table), CARRY_FAST(packed_decode), CARRY_FAST(quant_step), CARRY_FAST(quant_decode), CARRY_FAST(quant_chain),
                          CARRY_FAST(fp32_step), CARRY_FAST(pool_move), CARRY_FAST(pool_copy), CARRY_FAST(pool_copy_layers),
+                         CARRY_FAST(kv_append), CARRY_FAST(kv_attention), CARRY_FAST(add_rms_norm),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the Python surfaces.", -1, methods};
 

@@ -120,6 +120,10 @@ def quantized_kv_append(k, v, k_codes, k_scale, v_codes, v_scale, block_table, l
     block with earlier tokens the scale only grows.  A token with a number that is not finite gets a NaN key: the
     queries that see it become NaN, and no others.  Two requests must not append to one page."""
     lib = _lib._lib or _lib.load_library()
+    if lib.native.kv_append(lib.native_table, k, v, k_codes, k_scale, v_codes, v_scale, block_table, lengths, query_start,
+                            max_query_len, status):
+        return
+    # not a call the native path takes as it stands: the checks below say what is wrong with it, if anything
     args = _lib.KvAppendArgs()
     dev = k_codes.device
     _rows(args.cache, args.rows, k, lengths, query_start, max_query_len, "k", dev)
@@ -170,6 +174,9 @@ def quantized_paged_attention(q, scale, k_codes, k_scale, v_codes, v_scale, out,
     token (a request of length 0, a padding page) is zero.  ``workspace`` (uint8, at least
     :func:`attention_workspace_bytes`) is allocated by the call when it is not given."""
     lib = _lib._lib or _lib.load_library()
+    if lib.native.kv_attention(lib.native_table, q, scale, k_codes, k_scale, v_codes, v_scale, out, block_table, lengths,
+                               query_start, max_query_len, workspace, status):
+        return out
     args = _attention_args(q, scale, k_codes, k_scale, v_codes, v_scale, out, block_table, lengths, query_start,
                            max_query_len, status)
     dev = k_codes.device

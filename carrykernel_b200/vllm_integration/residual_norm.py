@@ -33,6 +33,8 @@ def add_rms_norm_quant(x, residual, weight, codes, scale, eps: float = 1e-6, res
     given; with ``residual=None`` (a model's first layer) ``h = x``, stored only where ``residual_out`` is given.  A row
     with a number that is not finite gets NaN codes and scales."""
     lib = _lib._lib or _lib.load_library()
+    if lib.native.add_rms_norm(lib.native_table, x, residual, weight, codes, scale, eps, residual_out):
+        return codes, scale
     if x.dim() != 2:
         raise ValueError(f"x must be 2-D [N, W], got {tuple(x.shape)}")
     N, W = x.shape
