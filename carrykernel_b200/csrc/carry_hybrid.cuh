@@ -18,6 +18,54 @@ __device__ __forceinline__ float power_of_two_scale(float amax) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+// Eight neighbouring numbers of a type: as they lie in memory, and as fp32.
+template <int DTYPE>
+struct Raw {
+  uint4 w[DTYPE == CARRY_F32 ? 2 : 1];
+};
+struct Eight {
+  float2 x[4];
+};
+template <int DTYPE>
+__device__ __forceinline__ Raw<DTYPE> load_raw(const void* p, long long at) {
+  Raw<DTYPE> r;
+  if constexpr (DTYPE == CARRY_F32) {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at);
+    r.w[0] = q[0];
+    r.w[1] = q[1];
+  } else {
+    r.w[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at);
+  }
+  return r;
+}
+template <int DTYPE>
+__device__ __forceinline__ Eight unpack(const Raw<DTYPE>& r) {
+  Eight e;
+  const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+  if constexpr (DTYPE == CARRY_F32) {
+    const uint32_t v[4] = {r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      e.x[i] = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+      e.x[i + 2] = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      e.x[i] = DTYPE == CARRY_BF16 ? make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u))
+                                   : __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+  }
+  return e;
+}
+
+// Shift that stands for a division by x, or -1.
+inline int shift_of(int x) {
+  for (int s = 0; s < 31; ++s)
+    if (1 << s == x) return s;
+  return -1;
+}
+__device__ __forceinline__ int divide(int x, int by, int shift) { return shift >= 0 ? x >> shift : x / by; }
+
 // A request's share of a call, with everything that comes from device memory brought into bounds.
 struct KvRequest {
   int first, count;   // its rows: first .. first + count - 1

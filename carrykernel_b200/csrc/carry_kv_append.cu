@@ -13,72 +13,91 @@ namespace {
 constexpr int kThreads = 256, kHalf = kThreads / 2, kMaxBlock = 128;
 constexpr uint32_t kNotFinite = 0x7f800000u;      // bits of |x| from here on: infinities and NaNs
 
-// eight consecutive elements as floats
-template <class T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
-  alignas(16) T raw[8];
-  if (vec) {
-    constexpr int n = sizeof(raw) / 16;
+struct AppendParams {
+  CarryGdnKvAppendArgs a;
+  int page_shift, block_shift;
+  bool vec;                       // every row of k and v starts on a 16-byte boundary
+};
+
+// bits of the largest magnitude among eight numbers
+template <int DTYPE>
+__device__ __forceinline__ uint32_t top_bits(const Raw<DTYPE>& r) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+  uint32_t t = 0;
+  if constexpr (DTYPE == CARRY_F32) {
 #pragma unroll
-    for (int i = 0; i < n; ++i) reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < 8; ++i) t = max(t, w[i] & 0x7fffffffu);
+    return t;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = p[i];
+    for (int i = 0; i < 4; ++i) t = __vmaxu2(t, w[i] & 0x7fff7fffu);
+    t = max(t >> 16, t & 0xffffu);
+    if constexpr (DTYPE == CARRY_BF16) return t << 16;
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(t))));
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(raw[i]);
 }
 
-__device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
-  uint32_t w[2];
+__device__ __forceinline__ uint2 codes8(const Eight& e, float inv) {
+  uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i] * inv, x[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2] * inv, x[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-    w[i] = lo | hi << 16;
-  }
-  return make_uint2(w[0], w[1]);
+  for (int i = 0; i < 4; ++i) c[i] = __nv_cvt_float2_to_fp8x2(make_float2(e.x[i].x * inv, e.x[i].y * inv), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ CarryGdnKvAppendArgs a, const bool vec) {
+// ITEMS: a thread's share of a block's new tokens, eight numbers each, held in registers from the maximum to the codes.
+template <int D, int DTYPE, int ITEMS>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ uint32_t token_top[2][kMaxBlock];    // bits of each new token's largest magnitude
   __shared__ uint32_t top[2][kHalf / 32];
+  constexpr int kPer = D / 8;                     // that many neighbouring lanes have a token
   depend_release();
   depend_wait();
+  const CarryGdnKvAppendArgs& a = p.a;
   const CarryGdnKvCache& c = a.cache;
   const int b = blockIdx.z, h = blockIdx.y;
   const KvRequest r = kv_request(c, a.rows, b, blockIdx.x == 0 && h == 0 && threadIdx.x == 0 ? a.status : nullptr);
   const int origin = r.length - r.count;          // position of the request's row 0
   const int from = max(origin, 0), to = min(r.length, origin + r.todo);
-  const int blk = from / c.block + blockIdx.x;
-  const int start = blk * c.block, t0 = max(start, from), t1 = min(start + c.block, to);
+  const int start = (divide(from, c.block, p.block_shift) + blockIdx.x) * c.block;
+  const int t0 = max(start, from), t1 = min(start + c.block, to);
   if (t0 >= t1) return;
-  const int page = kv_page(c, b, start / c.page, h == 0 && threadIdx.x == 0 ? a.status : nullptr);
+  const int index = divide(start, c.page, p.page_shift), offset = start - index * c.page;
+  const int page = kv_page(c, b, index, h == 0 && threadIdx.x == 0 ? a.status : nullptr);
   if (page == 0) return;
 
   const bool is_v = threadIdx.x >= kHalf;
-  const int tid = threadIdx.x % kHalf, offset = start % c.page;
-  const int per_token = c.D / 8, items = (t1 - t0) * per_token;   // 8 or 16 neighbouring lanes have one token
+  const int tid = threadIdx.x % kHalf, items = (t1 - t0) * kPer;
   const long long stride_tok = is_v ? a.stride_v_tok : a.stride_k_tok;
-  const T* x = reinterpret_cast<const T*>(is_v ? a.v : a.k) + (r.first + (t0 - origin)) * stride_tok +
-               h * (is_v ? a.stride_v_head : a.stride_k_head);
+  const long long row = (r.first + (t0 - origin) + tid / kPer) * stride_tok + h * (is_v ? a.stride_v_head : a.stride_k_head) + tid % kPer * 8;
+  const void* x = is_v ? a.v : a.k;
   uint8_t* codes = (is_v ? c.v_codes + page * c.stride_v_page : c.k_codes + page * c.stride_k_page) +
-                   ((long long)h * c.page + offset) * c.D;
+                   ((long long)h * c.page + offset) * D;
   float* scale = (is_v ? c.v_scale + page * c.stride_vs_page : c.k_scale + page * c.stride_ks_page) +
-                 h * (c.page / c.block) + offset / c.block;
+                 h * divide(c.page, c.block, p.block_shift) + divide(offset, c.block, p.block_shift);
 
-  for (int base = 0; base < items; base += kHalf) {
-    const int i = base + tid;
-    uint32_t t = 0;
-    if (i < items) {
-      float e[8];
-      load8(x + (i / per_token) * stride_tok + i % per_token * 8, vec, e);
+  Raw<DTYPE> e[ITEMS];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t = max(t, __float_as_uint(e[j]) & 0x7fffffffu);
+  for (int n = 0; n < ITEMS; ++n) {
+    if (n * kHalf + tid >= items) continue;
+    const long long at = row + n * (kHalf / kPer) * stride_tok;
+    if (p.vec) {
+      e[n] = load_raw<DTYPE>(x, at);
+    } else if constexpr (DTYPE == CARRY_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) reinterpret_cast<uint32_t*>(&e[n])[i] = reinterpret_cast<const uint32_t*>(x)[at + i];
+    } else {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(x) + at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(&e[n])[i] = q[2 * i] | static_cast<uint32_t>(q[2 * i + 1]) << 16;
     }
-    for (int s = per_token / 2; s > 0; s /= 2) t = max(t, __shfl_xor_sync(~0u, t, s));
-    if (i < items && i % per_token == 0) token_top[is_v][i / per_token] = t;
+  }
+  const float old = t0 > start ? *scale : 0.0f;
+#pragma unroll
+  for (int n = 0; n < ITEMS; ++n) {
+    uint32_t t = n * kHalf + tid < items ? top_bits<DTYPE>(e[n]) : 0;
+#pragma unroll
+    for (int s = kPer / 2; s > 0; s /= 2) t = max(t, __shfl_xor_sync(~0u, t, s));
+    if (n * kHalf + tid < items && tid % kPer == 0) token_top[is_v][(n * kHalf + tid) / kPer] = t;
   }
   __syncthreads();
   uint32_t t = 0;
@@ -91,39 +110,41 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
 
   float now = power_of_two_scale(__uint_as_float(t));
   if (t0 > start) {
-    const float old = *scale;
     if (old < now) {
       const float shift = __fdiv_rn(old, now);
-      uint8_t* early = codes;
-      for (int i = tid; i < (t0 - start) * per_token; i += kHalf) {
-        const uint2 w = reinterpret_cast<const uint2*>(early)[i];
-        float e[8];
+      for (int i = tid; i < (t0 - start) * kPer; i += kHalf) {
+        const uint2 w = reinterpret_cast<const uint2*>(codes)[i];
+        Eight early;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t half = j < 2 ? w.x : w.y;
-          const __half2 v(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(half >> (j % 2 * 16)), __NV_E4M3));
-          e[2 * j] = __low2float(v);
-          e[2 * j + 1] = __high2float(v);
-        }
-        reinterpret_cast<uint2*>(early)[i] = codes8(e, shift);
+        for (int j = 0; j < 4; ++j)
+          early.x[j] = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((j < 2 ? w.x : w.y) >> (j % 2 * 16)), __NV_E4M3)));
+        reinterpret_cast<uint2*>(codes)[i] = codes8(early, shift);
       }
     } else {
       now = old;
     }
   }
-  const float inv = __fdiv_rn(1.0f, now);
-  uint8_t* to_codes = codes + (long long)(t0 - start) * c.D;
-  for (int i = tid; i < items; i += kHalf) {
-    const int token = i / per_token;
-    float e[8];
-    load8(x + token * stride_tok + i % per_token * 8, vec, e);
-    uint2 w = codes8(e, inv);
-    if (token_top[0][token] >= kNotFinite || token_top[1][token] >= kNotFinite)
+  const float inv = __uint_as_float((254u << 23) - __float_as_uint(now));        // of a power of two: exact
+  uint2* to_codes = reinterpret_cast<uint2*>(codes + (long long)(t0 - start) * D);
+#pragma unroll
+  for (int n = 0; n < ITEMS; ++n) {
+    const int i = n * kHalf + tid;
+    if (i >= items) continue;
+    uint2 w = codes8(unpack<DTYPE>(e[n]), inv);
+    if (max(token_top[0][i / kPer], token_top[1][i / kPer]) >= kNotFinite)
       w = is_v ? make_uint2(0, 0) : make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-    reinterpret_cast<uint2*>(to_codes)[i] = w;
+    to_codes[i] = w;
   }
-  __syncthreads();                                // every thread has read the old scale
-  if (tid == 0) *scale = now;
+  if (tid == 0 && now != old) *scale = now;       // every thread read the old one before the first barrier
+}
+
+template <int D, int DTYPE>
+int launch_items(const AppendParams& p, dim3 grid, cudaStream_t stream) {
+  const int tokens = p.a.rows.max_query < p.a.cache.block ? p.a.rows.max_query : p.a.cache.block;
+  const int items = (tokens * D / 8 + kHalf - 1) / kHalf;               // 16 at most
+  if (items <= 1) return launch_dependent(kv_append_kernel<D, DTYPE, 1>, grid, kThreads, 0, stream, p);
+  if (items <= 4) return launch_dependent(kv_append_kernel<D, DTYPE, 4>, grid, kThreads, 0, stream, p);
+  return launch_dependent(kv_append_kernel<D, DTYPE, 16>, grid, kThreads, 0, stream, p);
 }
 
 }  // namespace
@@ -137,10 +158,11 @@ int launch_kv_append(const CarryGdnKvAppendArgs& a, cudaStream_t stream) {
                       (long long)a.stride_k_tok * size, (long long)a.stride_k_head * size,
                       (long long)a.stride_v_tok * size, (long long)a.stride_v_head * size})
     vec = vec && v % 16 == 0;
+  const AppendParams p = {a, shift_of(c.page), shift_of(c.block), vec};
   const dim3 grid(blocks, c.HKV, a.rows.B);
-  if (a.dtype == CARRY_F32) return launch_dependent(kv_append_kernel<float>, grid, kThreads, 0, stream, a, vec);
-  if (a.dtype == CARRY_BF16) return launch_dependent(kv_append_kernel<__nv_bfloat16>, grid, kThreads, 0, stream, a, vec);
-  return launch_dependent(kv_append_kernel<__half>, grid, kThreads, 0, stream, a, vec);
+  if (a.dtype == CARRY_F32) return c.D == 64 ? launch_items<64, CARRY_F32>(p, grid, stream) : launch_items<128, CARRY_F32>(p, grid, stream);
+  if (a.dtype == CARRY_BF16) return c.D == 64 ? launch_items<64, CARRY_BF16>(p, grid, stream) : launch_items<128, CARRY_BF16>(p, grid, stream);
+  return c.D == 64 ? launch_items<64, CARRY_F16>(p, grid, stream) : launch_items<128, CARRY_F16>(p, grid, stream);
 }
 
 }  // namespace carry

@@ -90,7 +90,7 @@ __device__ __forceinline__ int granule_of(int i) {       // of this thread's i-t
   return D == 128 ? i : 2 * i + (threadIdx.x >> 6);
 }
 __device__ __forceinline__ int page_index(const AttnParams& p, int granule) {
-  return p.page_shift >= 0 ? granule >> p.page_shift : granule / p.page_granules;
+  return divide(granule, p.page_granules, p.page_shift);
 }
 __device__ __forceinline__ int page_id(const AttnParams& p, int b, int granule, int length) {
   if (granule * kGranule >= length) return 0;
@@ -505,7 +505,7 @@ __device__ __forceinline__ void load_run(const AttnParams& p, RunStage<D>& s, co
       }
     }
     if (lane < 2) {
-      const int block = at.h * (p.page_granules / p.block_granules) + (p.block_shift >= 0 ? in_page >> p.block_shift : in_page / p.block_granules);
+      const int block = at.h * (p.page_granules / p.block_granules) + divide(in_page, p.block_granules, p.block_shift);
       float* to_scale = lane == 0 ? &s.ks[i] : &s.vs[i];
       if (id > 0) __pipeline_memcpy_async(to_scale, lane == 0 ? c.k_scale + id * c.stride_ks_page + block : c.v_scale + id * c.stride_vs_page + block, 4);
       else *to_scale = lane == 0 ? kNoTokens : 0.0f;
@@ -1086,10 +1086,8 @@ int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a) {
 int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream) {
   if (sm_count() == 0) return CARRY_GDN_ERR_NO_DEVICE;
   AttnParams p = {a, a.HQ / a.cache.HKV, a.cache.page / kGranule, -1, a.cache.block / kGranule, -1, 0};
-  for (int s = 0; s < 31; ++s) {
-    if (1 << s == p.page_granules) p.page_shift = s;
-    if (1 << s == p.block_granules) p.block_shift = s;
-  }
+  p.page_shift = shift_of(p.page_granules);
+  p.block_shift = shift_of(p.block_granules);
   const int tiles = column_tiles(a);
   p.rows = tiles ? a.rows.max_query * p.group : 0;
   if (a.cache.D == 64) return a.dtype == CARRY_F32 ? launch_by_rows<64, 2>(p, tiles, stream) : launch_by_rows<64, 1>(p, tiles, stream);

@@ -35,45 +35,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
-// Eight columns: as they lie in memory (the row after the one being worked on waits in this form), and as numbers.
-template <int DTYPE>
-struct Raw {
-  uint4 w[DTYPE == CARRY_F32 ? 2 : 1];
-};
-struct Eight {
-  float2 x[4];
-};
-template <int DTYPE>
-__device__ __forceinline__ Raw<DTYPE> load_raw(const void* p, long long at) {
-  Raw<DTYPE> r;
-  if constexpr (DTYPE == CARRY_F32) {
-    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at);
-    r.w[0] = q[0];
-    r.w[1] = q[1];
-  } else {
-    r.w[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at);
-  }
-  return r;
-}
-template <int DTYPE>
-__device__ __forceinline__ Eight unpack(const Raw<DTYPE>& r) {
-  Eight e;
-  const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
-  if constexpr (DTYPE == CARRY_F32) {
-    const uint32_t v[4] = {r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      e.x[i] = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-      e.x[i + 2] = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      e.x[i] = DTYPE == CARRY_BF16 ? make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u))
-                                   : __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-  }
-  return e;
-}
 template <int DTYPE>
 __device__ __forceinline__ void store(void* p, long long at, const Eight& e) {
   if constexpr (DTYPE == CARRY_F32) {
