@@ -15,43 +15,19 @@
 // the tokens are read once for all of them.
 #include <cuda_pipeline_primitives.h>
 
-#include "carry_hybrid.cuh"
+#include "carry_kv_attention.cuh"
 
 namespace carry {
 namespace {
 
-constexpr int kTile = 64, kGranule = 16, kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTile = 64, kWarps = 4, kThreads = kWarps * 32;
 constexpr int kRowsPerWarp = 16;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kWeightUp = 15.0f;                // weights are formed times 2^15
-constexpr float kNoTokens = -1.0f;                // in a key scale's place: a padding page, or past the end
-
-struct AttnParams {
-  CarryGdnKvAttentionArgs a;
-  int group;                      // query heads per key/value head
-  int page_granules, page_shift;  // granules in a page, and its logarithm or -1
-  int block_granules, block_shift;
-  int rows;                       // rows of a row tile that may be in use (decode kernel)
-};
 
 __device__ __forceinline__ void mma_fp16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// four e4m3 codes as fp16 numbers, two to a word
-__device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& low, uint32_t& high) {
-  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(low), "=r"(high) : "r"(codes));
-}
-__device__ __forceinline__ uint32_t pack_half2(float x, float y) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_half2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
@@ -88,13 +64,6 @@ struct Pages {
 template <int D>
 __device__ __forceinline__ int granule_of(int i) {       // of this thread's i-th chunk of a tile
   return D == 128 ? i : 2 * i + (threadIdx.x >> 6);
-}
-__device__ __forceinline__ int page_index(const AttnParams& p, int granule) {
-  return divide(granule, p.page_granules, p.page_shift);
-}
-__device__ __forceinline__ int page_id(const AttnParams& p, int b, int granule, int length) {
-  if (granule * kGranule >= length) return 0;
-  return kv_page(p.a.cache, b, page_index(p, granule), p.a.status);
 }
 template <int D>
 __device__ __forceinline__ void fetch_pages(const AttnParams& p, int b, int tile, int length, Pages<D>& ids) {
@@ -160,9 +129,6 @@ __device__ __forceinline__ void load_share(const AttnParams& p, long long at, bo
     }
   }
 }
-
-// The power of two that a query row is divided by, from the bits of its largest magnitude: what is left is below 2^15.
-__device__ __forceinline__ int up_exponent(uint32_t top) { return min(max(static_cast<int>(top >> 23) - 127, -100), 127) - 14; }
 
 // 16 query rows of a warp as operands of the matrix instructions.  Lane (g, c) = (lane / 4, lane % 4) has rows g and
 // g + 8; the product sums over the columns in an order of its own, in which the lane's share of every 64 columns is 16
@@ -325,33 +291,6 @@ __device__ __forceinline__ void attend(const Stage<D>& s, int tok0, const Query<
           for (int part = 0; part < PARTS; ++part) mma_fp16(r.o[k * 4 + e * 2 + f], w[part], b0[f], b1[f]);
       }
   }
-}
-
-// eight neighbouring fp32 results to out's type
-__device__ __forceinline__ void store8(void* out, long long at, int dtype, const float* x) {
-  const long long byte = at * (dtype == CARRY_F32 ? 4 : 2);
-  if ((reinterpret_cast<uintptr_t>(out) + byte) % 16) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) store_from_float(out, at + i, dtype, x[i]);
-    return;
-  }
-  uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + byte);
-  if (dtype == CARRY_F32) {
-    to[0] = *reinterpret_cast<const uint4*>(x);
-    to[1] = *reinterpret_cast<const uint4*>(x + 4);
-    return;
-  }
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (dtype == CARRY_BF16) {
-      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&v);
-    } else {
-      w[i] = pack_half2(x[2 * i], x[2 * i + 1]);
-    }
-  }
-  *to = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // A finished row's columns of this lane, normalised, to the output.
@@ -1062,8 +1001,10 @@ template <int D, int PARTS>
 int launch_by_rows(const AttnParams& p, int tiles, cudaStream_t stream) {
   if (tiles == 1) return launch_decode<D, 1, PARTS>(p, stream);
   if (tiles == 2) return launch_decode<D, 2, PARTS>(p, stream);
-  if constexpr (PARTS == 1)
+  if constexpr (PARTS == 1) {
     if (tiles == 4) return launch_decode<D, 4, PARTS>(p, stream);
+    return launch_kv_prefill(p, stream);
+  }
   constexpr size_t smem = sizeof(Stage<D>) * kChunkStages;
   const long long rows = (long long)p.a.rows.max_query * p.group;
   static thread_local bool ready[64];

@@ -1,0 +1,73 @@
+// What the kernels of the key/value attention share: parameters, pages, rows to memory.
+#pragma once
+
+#include "carry_hybrid.cuh"
+
+namespace carry {
+
+constexpr int kGranule = 16;                      // tokens: no page and no block of a scale begins or ends inside
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoTokens = -1.0f;                // in a key scale's place: a padding page, or past the end
+
+struct AttnParams {
+  CarryGdnKvAttentionArgs a;
+  int group;                      // query heads per key/value head
+  int page_granules, page_shift;  // granules in a page, and its logarithm or -1
+  int block_granules, block_shift;
+  int rows;                       // rows of a request that may be in use (decode kernel)
+};
+
+__device__ __forceinline__ uint32_t pack_half2(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+// four e4m3 codes as fp16 numbers, two to a word
+__device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& low, uint32_t& high) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(low), "=r"(high) : "r"(codes));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ int page_index(const AttnParams& p, int granule) { return divide(granule, p.page_granules, p.page_shift); }
+__device__ __forceinline__ int page_id(const AttnParams& p, int b, int granule, int length) {
+  if (granule * kGranule >= length) return 0;
+  return kv_page(p.a.cache, b, page_index(p, granule), p.a.status);
+}
+
+// The power of two that a query row is divided by, from the bits of its largest magnitude: what is left is below 2^15.
+__device__ __forceinline__ int up_exponent(uint32_t top) { return min(max(static_cast<int>(top >> 23) - 127, -100), 127) - 14; }
+
+// eight neighbouring fp32 results to out's type
+__device__ __forceinline__ void store8(void* out, long long at, int dtype, const float* x) {
+  const long long byte = at * (dtype == CARRY_F32 ? 4 : 2);
+  if ((reinterpret_cast<uintptr_t>(out) + byte) % 16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) store_from_float(out, at + i, dtype, x[i]);
+    return;
+  }
+  uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + byte);
+  if (dtype == CARRY_F32) {
+    to[0] = *reinterpret_cast<const uint4*>(x);
+    to[1] = *reinterpret_cast<const uint4*>(x + 4);
+    return;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (dtype == CARRY_BF16) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      w[i] = pack_half2(x[2 * i], x[2 * i + 1]);
+    }
+  }
+  *to = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+int launch_kv_prefill(const AttnParams& p, cudaStream_t stream);
+
+}  // namespace carry
