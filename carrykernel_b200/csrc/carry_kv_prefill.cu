@@ -168,25 +168,33 @@ __device__ __forceinline__ float stage_query(const AttnParams& p, const KvReques
   return fabsf(p.a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
-// Codes of a step, as a converting thread holds them: chunk tid % (D / 16) of tokens tid / (D / 16) + i * kStride.
-template <int D>
-struct Codes {
-  uint4 k[D / 16], v[D / 16];
+// Pages of a step's granules, as the converting warps hold them: lane l < 8 has granule l's page id (0: no tokens) and
+// first token within it.  They are fetched a step before the codes that they lead to.
+struct StepPages {
+  int id, in_page;
 };
+__device__ __forceinline__ StepPages fetch_pages(const AttnParams& p, int b, int step, int length) {
+  const int granule = step * kBlocks + threadIdx.x % 32;
+  StepPages x = {0, 0};
+  if (threadIdx.x % 32 < kBlocks) {
+    x.id = page_id(p, b, granule, length);
+    x.in_page = (granule - page_index(p, granule) * p.page_granules) * kGranule;
+  }
+  return x;
+}
+// A converting thread's codes of a step: chunk tid % (D / 16) of tokens tid / (D / 16) + i * kStride.  Tokens at or beyond
+// the length and those of padding pages are zeros, whatever memory holds there.
 template <int D>
-__device__ __forceinline__ void fetch_codes(const AttnParams& p, int b, int h, int step, int length, int tid, Codes<D>& x) {
-  const CarryGdnKvCache& c = p.a.cache;
+__device__ __forceinline__ void fetch_codes(const CarryGdnKvCache& c, const uint8_t* codes, long long stride_page, const StepPages& pages, int h,
+                                            int left, int tid, uint4 (&x)[D / 16]) {
   constexpr int kChunks = D / 16, kStride = kConvertThreads / kChunks;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    const int token = step * kTokens + i * kStride + tid / kChunks, granule = token / kGranule;
-    const int id = token < length ? page_id(p, b, granule, length) : 0;
-    x.k[i] = x.v[i] = make_uint4(0, 0, 0, 0);
-    if (id == 0) continue;                        // zeros, whatever memory holds there
-    const int in_page = (granule - page_index(p, granule) * p.page_granules) * kGranule + token % kGranule;
-    const int at = (h * c.page + in_page) * D + tid % kChunks * 16;
-    x.k[i] = *reinterpret_cast<const uint4*>(c.k_codes + id * c.stride_k_page + at);
-    x.v[i] = *reinterpret_cast<const uint4*>(c.v_codes + id * c.stride_v_page + at);
+    const int token = i * kStride + tid / kChunks;
+    const int id = __shfl_sync(~0u, pages.id, token / kGranule), in_page = __shfl_sync(~0u, pages.in_page, token / kGranule);
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (id > 0 && token < left)
+      x[i] = *reinterpret_cast<const uint4*>(codes + id * stride_page + ((h * c.page + in_page + token % kGranule) * D + tid % kChunks * 16));
   }
 }
 template <int D>
@@ -266,23 +274,21 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       const int limit = sees - step * kTokens;
       const bool all = __all_sync(~0u, limit >= kTokens);
       float x[32], now = top;
-#pragma unroll
+#pragma unroll 1
       for (int part = 0; part < 4; ++part) {
         tmem_load(s_at + part * 32, x);
         wait_loads();
+        if (!all) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = part * 32 + e < limit ? x[e] : -INFINITY;
+        }
 #pragma unroll
         for (int block = 0; block < 2; ++block) {
           const float ks = sh.ks[stage][part * 2 + block];
-          if (ks == kNoTokens) continue;
           float m = -INFINITY;
-          if (all) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) m = fmaxf(m, x[block * 16 + e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) m = fmaxf(m, part * 32 + block * 16 + e < limit ? x[block * 16 + e] : -INFINITY);
-          }
-          now = fmaxf(now, m * fmaxf(unit_q * ks, 0x1p-126f));
+          for (int e = 0; e < 16; e += 2) m = fmaxf(m, fmaxf(x[block * 16 + e], x[block * 16 + e + 1]));
+          if (ks != kNoTokens) now = fmaxf(now, m * fmaxf(unit_q * ks, 0x1p-126f));
         }
       }
       const float values = sh.rescale[stage];
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           healthy = barrier_wait(&sh.o_done[tile], (step - 1) & 1, poison, p.a.status);
           if (!healthy) break;
           fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int part = 0; part < D / 32; ++part) {
             tmem_load(o_at + part * 32, x);
             wait_loads();
@@ -306,7 +312,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         }
       }
       const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
+#pragma unroll 1
       for (int part = 0; part < 4; ++part) {
         tmem_load(s_at + part * 32, x);
         wait_loads();
@@ -315,19 +321,24 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         for (int block = 0; block < 2; ++block) {
           const int at = part * 2 + block;
           const float ks = sh.ks[stage][at], by = fmaxf(unit_q * ks, 0x1p-126f), bias = sh.bias[stage][at] - base;
-          float total = 0.0f;
+          float2 total = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
-            float u = exp2_fast(fmaf(x[block * 16 + e], by, bias)), v = exp2_fast(fmaf(x[block * 16 + e + 1], by, bias));
-            if (!all || ks == kNoTokens) {
-              const int t = ks == kNoTokens ? 1 << 30 : part * 32 + block * 16 + e;
-              u = t < limit ? u : 0.0f;
-              v = t + 1 < limit ? v : 0.0f;
-            }
-            total += u + v;
-            w[block * 8 + e / 2] = pack_half2(u, v);
+            float2 y = fma2(make_float2(x[block * 16 + e], x[block * 16 + e + 1]), make_float2(by, by), make_float2(bias, bias));
+            x[block * 16 + e] = exp2_fast(y.x);
+            x[block * 16 + e + 1] = exp2_fast(y.y);
           }
-          sum = fmaf(total, sh.counts[stage][at], sum);
+          if (!all || ks == kNoTokens) {
+            const int t = ks == kNoTokens ? 1 << 30 : at * 16;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[block * 16 + e] = t + e < limit ? x[block * 16 + e] : 0.0f;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            total = add2(total, make_float2(x[block * 16 + e], x[block * 16 + e + 1]));
+            w[block * 8 + e / 2] = pack_half2(x[block * 16 + e], x[block * 16 + e + 1]);
+          }
+          sum = fmaf(total.x + total.y, sh.counts[stage][at], sum);
         }
         tmem_store16(s_at + part * 16, w);        // over scores that this warp has read
       }
@@ -364,21 +375,24 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   } else if (threadIdx.x < kSoftmaxThreads + kConvertThreads) {
     // ---- codes to operands ----
     const int tid = threadIdx.x - kSoftmaxThreads;
-    float unit = 0.0f;
-    Codes<D> x;
-    if (steps > 0) fetch_codes<D>(p, b, h, 0, length, tid, x);
-    for (int step = 0; step < steps; ++step) {
-      const int stage = step & 1, parity = step / 2 & 1;
-      float ks = kNoTokens, vs = 0.0f;
-      if (tid < kBlocks) {
-        const int granule = step * kBlocks + tid, id = page_id(p, b, granule, length);
-        if (id > 0) {
-          const int in_page = granule - page_index(p, granule) * p.page_granules;
-          const int block = h * (p.page_granules / p.block_granules) + divide(in_page, p.block_granules, p.block_shift);
-          ks = c.k_scale[id * c.stride_ks_page + block];
-          vs = c.v_scale[id * c.stride_vs_page + block];
-        }
+    float unit = 0.0f, ks = kNoTokens, vs = 0.0f;
+    uint4 k[D / 16], v[D / 16];
+    StepPages pages = fetch_pages(p, b, 0, length);
+    auto fetch_scales = [&]() {
+      ks = kNoTokens;
+      vs = 0.0f;
+      if (pages.id > 0) {
+        const int block = h * (p.page_granules / p.block_granules) + divide(pages.in_page / kGranule, p.block_granules, p.block_shift);
+        ks = c.k_scale[pages.id * c.stride_ks_page + block];
+        vs = c.v_scale[pages.id * c.stride_vs_page + block];
       }
+    };
+    fetch_codes<D>(c, c.k_codes, c.stride_k_page, pages, h, length, tid, k);
+    fetch_codes<D>(c, c.v_codes, c.stride_v_page, pages, h, length, tid, v);
+    fetch_scales();
+    pages = fetch_pages(p, b, 1, length);
+    for (int step = 0; step < steps; ++step) {
+      const int stage = step & 1, parity = step / 2 & 1, left = length - (step + 1) * kTokens;
       if (step >= 2 && !barrier_wait(&sh.free[stage], parity ^ 1, poison, p.a.status)) break;
       if (tid < 32) {
         float most = vs;
@@ -402,13 +416,16 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           sh.unit = unit;
         }
       }
-      store_codes<D>(x.k, sh.k[stage], tid);
+      store_codes<D>(k, sh.k[stage], tid);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       barrier_arrive(&sh.k_full[stage]);
-      store_codes<D>(x.v, sh.v[stage], tid);
+      fetch_codes<D>(c, c.k_codes, c.stride_k_page, pages, h, left, tid, k);
+      fetch_scales();
+      store_codes<D>(v, sh.v[stage], tid);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       barrier_arrive(&sh.v_full[stage]);
-      if (step + 1 < steps) fetch_codes<D>(p, b, h, step + 1, length, tid, x);
+      fetch_codes<D>(c, c.v_codes, c.stride_v_page, pages, h, left, tid, v);
+      pages = fetch_pages(p, b, step + 2, length);
     }
   } else if (lane == 0) {
     // ---- products ----
