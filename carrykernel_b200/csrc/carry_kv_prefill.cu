@@ -20,7 +20,7 @@ namespace carry {
 namespace {
 
 constexpr int kTokens = 128, kTileRows = 128, kCtaRows = 2 * kTileRows, kPlane = 128 * 128;   // a plane: 128 rows of 64 columns
-constexpr int kSoftmaxThreads = 256, kConvertThreads = 128, kAllThreads = kSoftmaxThreads + kConvertThreads + 32;
+constexpr int kSoftmaxThreads = 256, kConvertThreads = 256, kAllThreads = kSoftmaxThreads + kConvertThreads + 32;
 constexpr int kBlocks = kTokens / kGranule;
 constexpr float kUp = 7.0f, kSlack = 4.0f;
 
@@ -168,51 +168,63 @@ __device__ __forceinline__ float stage_query(const AttnParams& p, const KvReques
   return fabsf(p.a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
-// Pages of a step's granules, as the converting warps hold them: lane l < 8 has granule l's page id (0: no tokens) and
-// first token within it.  They are fetched a step before the codes that they lead to.
+// A step's granules, as the converting warps hold them: lane l < 8 has granule l's place in the codes (-1: no tokens) and
+// in the scales.  They are fetched a step before the codes that they lead to.
 struct StepPages {
-  int id, in_page;
+  long long k, v;
+  int id, block;
 };
-__device__ __forceinline__ StepPages fetch_pages(const AttnParams& p, int b, int step, int length) {
+template <int D>
+__device__ __forceinline__ StepPages fetch_pages(const AttnParams& p, int b, int h, int step, int length) {
+  const CarryGdnKvCache& c = p.a.cache;
   const int granule = step * kBlocks + threadIdx.x % 32;
-  StepPages x = {0, 0};
-  if (threadIdx.x % 32 < kBlocks) {
-    x.id = page_id(p, b, granule, length);
-    x.in_page = (granule - page_index(p, granule) * p.page_granules) * kGranule;
+  StepPages x = {-1, -1, 0, 0};
+  if (threadIdx.x % 32 < kBlocks) x.id = page_id(p, b, granule, length);
+  if (x.id > 0) {
+    const int in_page = granule - page_index(p, granule) * p.page_granules, at = (h * c.page + in_page * kGranule) * D;
+    x.k = x.id * c.stride_k_page + at;
+    x.v = x.id * c.stride_v_page + at;
+    x.block = h * (p.page_granules / p.block_granules) + divide(in_page, p.block_granules, p.block_shift);
   }
   return x;
 }
 // A converting thread's codes of a step: chunk tid % (D / 16) of tokens tid / (D / 16) + i * kStride.  Tokens at or beyond
 // the length and those of padding pages are zeros, whatever memory holds there.
 template <int D>
-__device__ __forceinline__ void fetch_codes(const CarryGdnKvCache& c, const uint8_t* codes, long long stride_page, const StepPages& pages, int h,
-                                            int left, int tid, uint4 (&x)[D / 16]) {
+constexpr int kCodes = kTokens * (D / 16) / kConvertThreads;
+template <int D>
+__device__ __forceinline__ void fetch_codes(const uint8_t* codes, long long place, int left, int tid, uint4 (&x)[kCodes<D>]) {
   constexpr int kChunks = D / 16, kStride = kConvertThreads / kChunks;
+  const uint8_t* mine = codes + tid / kChunks % kGranule * D + tid % kChunks * 16;
+  const int first = tid / kChunks;
+  const bool whole = left >= kTokens && __all_sync(~0u, place >= 0 || threadIdx.x % 32 >= kBlocks);
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const int token = i * kStride + tid / kChunks;
-    const int id = __shfl_sync(~0u, pages.id, token / kGranule), in_page = __shfl_sync(~0u, pages.in_page, token / kGranule);
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (id > 0 && token < left)
-      x[i] = *reinterpret_cast<const uint4*>(codes + id * stride_page + ((h * c.page + in_page + token % kGranule) * D + tid % kChunks * 16));
+  for (int i = 0; i < kCodes<D>; ++i) {
+    const long long at = __shfl_sync(~0u, place, (first + i * kStride) / kGranule);
+    if (whole) {
+      x[i] = *reinterpret_cast<const uint4*>(mine + at);
+    } else {
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (at >= 0 && first + i * kStride < left) x[i] = *reinterpret_cast<const uint4*>(mine + at);
+    }
   }
 }
 template <int D>
-__device__ __forceinline__ void store_codes(const uint4 (&x)[D / 16], uint8_t (*tile)[kPlane], int tid) {
+__device__ __forceinline__ void store_codes(const uint4 (&x)[kCodes<D>], uint8_t (*tile)[kPlane], int tid) {
   constexpr int kChunks = D / 16, kStride = kConvertThreads / kChunks;
-  const int chunk = tid % kChunks;
+  const int chunk = tid % kChunks, turn = chunk / 4;         // the planes' stores take turns, or they would meet in the banks
+  // rows differ by a multiple of eight, so they lie alike in their groups
+  uint8_t* first = tile[chunk / 4] + plane_at(tid / kChunks, chunk % 4 * 2 + turn);
+  uint8_t* second = tile[chunk / 4] + plane_at(tid / kChunks, chunk % 4 * 2 + 1 - turn);
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const int row = i * kStride + tid / kChunks;
+  for (int i = 0; i < kCodes<D>; ++i) {
     uint4 lo, hi;
     halves_of(x[i].x, lo.x, lo.y);
     halves_of(x[i].y, lo.z, lo.w);
     halves_of(x[i].z, hi.x, hi.y);
     halves_of(x[i].w, hi.z, hi.w);
-    uint8_t* plane = tile[chunk / 4];
-    const int first = chunk % 4 * 2, turn = chunk / 4;       // the planes' stores take turns, or they would meet in the banks
-    *reinterpret_cast<uint4*>(plane + plane_at(row, first + turn)) = turn ? hi : lo;
-    *reinterpret_cast<uint4*>(plane + plane_at(row, first + 1 - turn)) = turn ? lo : hi;
+    *reinterpret_cast<uint4*>(first + i * kStride * 128) = turn ? hi : lo;
+    *reinterpret_cast<uint4*>(second + i * kStride * 128) = turn ? lo : hi;
   }
 }
 
@@ -376,21 +388,16 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     // ---- codes to operands ----
     const int tid = threadIdx.x - kSoftmaxThreads;
     float unit = 0.0f, ks = kNoTokens, vs = 0.0f;
-    uint4 k[D / 16], v[D / 16];
-    StepPages pages = fetch_pages(p, b, 0, length);
+    uint4 k[kCodes<D>], v[kCodes<D>];
+    StepPages pages = fetch_pages<D>(p, b, h, 0, length);
     auto fetch_scales = [&]() {
-      ks = kNoTokens;
-      vs = 0.0f;
-      if (pages.id > 0) {
-        const int block = h * (p.page_granules / p.block_granules) + divide(pages.in_page / kGranule, p.block_granules, p.block_shift);
-        ks = c.k_scale[pages.id * c.stride_ks_page + block];
-        vs = c.v_scale[pages.id * c.stride_vs_page + block];
-      }
+      ks = pages.id > 0 ? c.k_scale[pages.id * c.stride_ks_page + pages.block] : kNoTokens;
+      vs = pages.id > 0 ? c.v_scale[pages.id * c.stride_vs_page + pages.block] : 0.0f;
     };
-    fetch_codes<D>(c, c.k_codes, c.stride_k_page, pages, h, length, tid, k);
-    fetch_codes<D>(c, c.v_codes, c.stride_v_page, pages, h, length, tid, v);
-    fetch_scales();
-    pages = fetch_pages(p, b, 1, length);
+    fetch_codes<D>(c.k_codes, pages.k, length, tid, k);
+    fetch_codes<D>(c.v_codes, pages.v, length, tid, v);
+    if (tid < 32) fetch_scales();
+    pages = fetch_pages<D>(p, b, h, 1, length);
     for (int step = 0; step < steps; ++step) {
       const int stage = step & 1, parity = step / 2 & 1, left = length - (step + 1) * kTokens;
       if (step >= 2 && !barrier_wait(&sh.free[stage], parity ^ 1, poison, p.a.status)) break;
@@ -419,13 +426,13 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       store_codes<D>(k, sh.k[stage], tid);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       barrier_arrive(&sh.k_full[stage]);
-      fetch_codes<D>(c, c.k_codes, c.stride_k_page, pages, h, left, tid, k);
-      fetch_scales();
+      fetch_codes<D>(c.k_codes, pages.k, left, tid, k);
+      if (tid < 32) fetch_scales();
       store_codes<D>(v, sh.v[stage], tid);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       barrier_arrive(&sh.v_full[stage]);
-      fetch_codes<D>(c, c.v_codes, c.stride_v_page, pages, h, left, tid, v);
-      pages = fetch_pages(p, b, step + 2, length);
+      fetch_codes<D>(c.v_codes, pages.v, left, tid, v);
+      pages = fetch_pages<D>(p, b, h, step + 2, length);
     }
   } else if (lane == 0) {
     // ---- products ----
