@@ -2,12 +2,12 @@
 //
 // A CTA has 256 rows (query tokens times the query heads of one key/value head) as two tiles of 128, and walks the
 // request's tokens 128 at a time.  The work is in four places that run side by side:
-//  * four warps turn a tile's codes into fp16, keys and values, into shared memory (e4m3 is a subset of fp16; codes of
+//  * eight warps turn a tile's codes into fp16, keys and values, into shared memory (e4m3 is a subset of fp16; codes of
 //    the tile after it wait in registers);
 //  * one thread issues the matrix products on the fifth-generation tensor cores: S = Q K^T, operands in shared memory,
 //    and O += P V with the weights P in tensor memory;
-//  * four warps for each row tile take its scores out of tensor memory, a row to a thread, and put the weights back in
-//    their place.  While one tile's weights are formed, the other's products run.
+//  * eight warps for each row tile take its scores out of tensor memory, half a row to a thread, and put the weights back
+//    in their place.  While one tile's weights are formed, the other's products run.
 // What bounds it: 2 x 128 x 128 exponentials a step take 2048 cycles of the special function units, and the products as
 // many of the tensor cores.
 //
@@ -20,7 +20,7 @@ namespace carry {
 namespace {
 
 constexpr int kTokens = 128, kTileRows = 128, kCtaRows = 2 * kTileRows, kPlane = 128 * 128;   // a plane: 128 rows of 64 columns
-constexpr int kSoftmaxThreads = 256, kConvertThreads = 256, kAllThreads = kSoftmaxThreads + kConvertThreads + 32;
+constexpr int kTileThreads = 256, kSoftmaxThreads = 2 * kTileThreads, kConvertThreads = 256, kAllThreads = kSoftmaxThreads + kConvertThreads + 32;
 constexpr int kBlocks = kTokens / kGranule;
 constexpr float kUp = 7.0f, kSlack = 4.0f;
 
@@ -31,7 +31,9 @@ struct Shared {
   // counts in the row's sum
   float ks[2][kBlocks], bias[2][kBlocks], counts[2][kBlocks];
   float rescale[2], unit;
-  uint64_t k_full[2], v_full[2], free[2], s_full[2], p_full[2], o_done[2];
+  float top[2][2][2][kTileRows];                  // by step, tile and half of a step: largest score of a row
+  float unit_q[2][kTileRows];
+  uint64_t k_full[2], v_full[2], free[2], s_full[2], top_full[2], p_full[2], o_done[2];
   uint32_t tmem;
   int poison;
 };
@@ -250,7 +252,8 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       barrier_init(&sh.v_full[i], kConvertThreads);
       barrier_init(&sh.free[i], 1);
       barrier_init(&sh.s_full[i], 1);
-      barrier_init(&sh.p_full[i], kTileRows);
+      barrier_init(&sh.top_full[i], kTileThreads);
+      barrier_init(&sh.p_full[i], kTileThreads);
       barrier_init(&sh.o_done[i], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -259,9 +262,9 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  float unit_q = 0.0f;
-  if (threadIdx.x < kSoftmaxThreads) {
-    unit_q = stage_query<D>(p, r, h, first_row + threadIdx.x, sh.q[threadIdx.x / kTileRows], threadIdx.x % kTileRows);
+  if (threadIdx.x < kCtaRows) {
+    const int tile = threadIdx.x / kTileRows, row = threadIdx.x % kTileRows;
+    sh.unit_q[tile][row] = stage_query<D>(p, r, h, first_row + threadIdx.x, sh.q[tile], row);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   fence_before();
@@ -271,11 +274,13 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   volatile int* poison = &sh.poison;
 
   if (threadIdx.x < kSoftmaxThreads) {
-    // ---- a row to a thread ----
-    const int tile = threadIdx.x / kTileRows, row = first_row + threadIdx.x, i = row / p.group;
-    const int sees = i < r.todo ? r.length - r.count + i + 1 : 0;
+    // ---- half a row's scores to a thread ----
+    const int tile = threadIdx.x / kTileThreads, part = threadIdx.x / kTileRows % 2, tile_row = threadIdx.x % kTileRows;
+    const int row = first_row + tile * kTileRows + tile_row, i = row / p.group;
+    const int sees = (i < r.todo ? r.length - r.count + i + 1 : 0) - part * 64;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-    const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem + lanes + 256 + tile * 128;
+    const uint32_t s_at = tmem + lanes + tile * 128 + part * 64, o_at = tmem + lanes + 256 + tile * 128 + part * (D / 2);
+    const float unit_q = sh.unit_q[tile][tile_row];
     float top = -INFINITY, sum = 0.0f;
     bool healthy = true;
     for (int step = 0; step < steps; ++step) {
@@ -284,27 +289,32 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       if (!healthy) break;
       fence_after();
       const int limit = sees - step * kTokens;
-      const bool all = __all_sync(~0u, limit >= kTokens);
+      const bool all = __all_sync(~0u, limit >= 64);
       float x[32], now = top;
 #pragma unroll 1
-      for (int part = 0; part < 4; ++part) {
-        tmem_load(s_at + part * 32, x);
+      for (int n = 0; n < 2; ++n) {
+        tmem_load(s_at + n * 32, x);
         wait_loads();
         if (!all) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = part * 32 + e < limit ? x[e] : -INFINITY;
+          for (int e = 0; e < 32; ++e) x[e] = n * 32 + e < limit ? x[e] : -INFINITY;
         }
 #pragma unroll
         for (int block = 0; block < 2; ++block) {
-          const float ks = sh.ks[stage][part * 2 + block];
+          const float ks = sh.ks[stage][part * 4 + n * 2 + block];
           float m = -INFINITY;
 #pragma unroll
           for (int e = 0; e < 16; e += 2) m = fmaxf(m, fmaxf(x[block * 16 + e], x[block * 16 + e + 1]));
           if (ks != kNoTokens) now = fmaxf(now, m * fmaxf(unit_q * ks, 0x1p-126f));
         }
       }
+      sh.top[stage][tile][part][tile_row] = now;
+      barrier_arrive(&sh.top_full[tile]);
+      healthy = barrier_wait(&sh.top_full[tile], step & 1, poison, p.a.status);
+      if (!healthy) break;
+      now = fmaxf(now, sh.top[stage][tile][part ^ 1][tile_row]);
       const float values = sh.rescale[stage];
-      if (__any_sync(~0u, now > top + kSlack) || values != 1.0f) {
+      if (__any_sync(~0u, now > top + kSlack) || values != 1.0f) {   // alike in both halves of a row
         const float keep = now == -INFINITY ? 1.0f : exp2_fast(top - now);
         sum *= keep;
         top = now;
@@ -313,25 +323,25 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           if (!healthy) break;
           fence_after();
 #pragma unroll 1
-          for (int part = 0; part < D / 32; ++part) {
-            tmem_load(o_at + part * 32, x);
+          for (int n = 0; n < D / 64; ++n) {
+            tmem_load(o_at + n * 32, x);
             wait_loads();
 #pragma unroll
             for (int e = 0; e < 32; ++e) x[e] *= keep * values;
-            tmem_store(o_at + part * 32, x);
+            tmem_store(o_at + n * 32, x);
           }
           wait_stores();
         }
       }
       const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 1
-      for (int part = 0; part < 4; ++part) {
-        tmem_load(s_at + part * 32, x);
+      for (int n = 0; n < 2; ++n) {
+        tmem_load(s_at + n * 32, x);
         wait_loads();
         uint32_t w[16];
 #pragma unroll
         for (int block = 0; block < 2; ++block) {
-          const int at = part * 2 + block;
+          const int at = part * 4 + n * 2 + block;
           const float ks = sh.ks[stage][at], by = fmaxf(unit_q * ks, 0x1p-126f), bias = sh.bias[stage][at] - base;
           float2 total = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -341,7 +351,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
             x[block * 16 + e + 1] = exp2_fast(y.y);
           }
           if (!all || ks == kNoTokens) {
-            const int t = ks == kNoTokens ? 1 << 30 : at * 16;
+            const int t = ks == kNoTokens ? 1 << 30 : n * 32 + block * 16;
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[block * 16 + e] = t + e < limit ? x[block * 16 + e] : 0.0f;
           }
@@ -352,7 +362,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           }
           sum = fmaf(total.x + total.y, sh.counts[stage][at], sum);
         }
-        tmem_store16(s_at + part * 16, w);        // over scores that this warp has read
+        tmem_store16(s_at + n * 16, w);           // over scores that this warp has read
       }
       wait_stores();
       fence_before();
@@ -363,14 +373,20 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       fence_after();
     }
     if (healthy) {
+      sh.top[steps & 1][tile][part][tile_row] = sum;             // the halves of a row's sum meet
+      barrier_arrive(&sh.top_full[tile]);
+      healthy = barrier_wait(&sh.top_full[tile], steps & 1, poison, p.a.status);
+    }
+    if (healthy) {
+      sum += sh.top[steps & 1][tile][part ^ 1][tile_row];
       const float by = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kUp), sum);
       const float unit = steps > 0 ? *reinterpret_cast<volatile float*>(&sh.unit) : 1.0f;
-      const long long at = (r.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head;
-#pragma unroll
-      for (int part = 0; part < D / 32; ++part) {
+      const long long at = (r.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + part * (D / 2);
+#pragma unroll 1
+      for (int n = 0; n < D / 64; ++n) {
         alignas(16) float x[32];
         if (steps > 0) {
-          tmem_load(o_at + part * 32, x);
+          tmem_load(o_at + n * 32, x);
           wait_loads();
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = sum == 0.0f ? 0.0f : x[e] * by * unit;
@@ -380,7 +396,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         }
         if (i < r.todo) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) store8(p.a.out, at + part * 32 + e, p.a.dtype, x + e);
+          for (int e = 0; e < 32; e += 8) store8(p.a.out, at + n * 32 + e, p.a.dtype, x + e);
         }
       }
     }
@@ -458,7 +474,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         fence_after();
 #pragma unroll
         for (int k = 0; k < kTokens / 16; ++k)
-          mma_tensor(tmem + 256 + tile * 128, tmem + tile * 128 + k * 8, descriptor(sh.v[stage][0] + k * 2048, kPlane, 1024), instruction(D, true),
+          mma_tensor(tmem + 256 + tile * 128, tmem + tile * 128 + k / 4 * 64 + k % 4 * 8, descriptor(sh.v[stage][0] + k * 2048, kPlane, 1024), instruction(D, true),
                      step > 0 || k > 0);
         mma_commit(&sh.o_done[tile]);
         if (tile == 1) mma_commit(&sh.free[stage]);
