@@ -6,8 +6,8 @@
 //  * eight warps turn a step's codes into fp16, keys and values (e4m3 is a subset of fp16);
 //  * one warp issues the matrix products on the fifth-generation tensor cores: S = Q K^T, operands in shared memory,
 //    and O += P V with the weights P in tensor memory;
-//  * eight warps for each row tile take its scores out of tensor memory, half a row to a thread, and put the weights back
-//    in their place.  While one tile's weights are formed, the other's products run.
+//  * four warps for each row tile take its scores out of tensor memory, a row to a thread, and put the weights back in
+//    their place.  While one tile's weights are formed, the other's products run.
 // What bounds it: 2 x 128 x 64 exponentials a step take 1024 cycles of the special function units, and the products as
 // many of the tensor cores.
 //
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kTokens = 64, kStages = 3, kRawStages = 3, kNotes = 8, kTileRows = 128, kCtaRows = 2 * kTileRows;
 constexpr int kRowPlane = kTileRows * 128, kTokenPlane = kTokens * 128;        // bytes of a plane: 64 columns of all rows, all tokens
-constexpr int kTileThreads = 256, kSoftmaxThreads = 2 * kTileThreads, kConvertThreads = 256;
+constexpr int kSoftmaxThreads = kCtaRows, kConvertThreads = 256;
 constexpr int kFetchWarp = (kSoftmaxThreads + kConvertThreads) / 32, kIssueWarp = kFetchWarp + 1, kAllThreads = (kIssueWarp + 1) * 32;
 constexpr int kBlocks = kTokens / kGranule;
 constexpr float kUp = 7.0f, kSlack = 4.0f;
@@ -33,12 +33,10 @@ struct Shared {
   // of a step's blocks: key scale, log2 of the value scale in the running unit plus kUp, and what a weight so formed
   // counts in the row's sum.  A step's notes are written again kNotes steps later, when everybody is long done with it:
   // kRawStages + kStages steps at most are under way.
-  float ks[kNotes][kBlocks], bias[kNotes][kBlocks], counts[kNotes][kBlocks];
+  alignas(16) float ks[kNotes][kBlocks], bias[kNotes][kBlocks], counts[kNotes][kBlocks];
   float rescale[kNotes], unit;
-  float top[2][2][2][kTileRows];                  // by step, tile and half of a step: largest score of a row
-  float unit_q[2][kTileRows];
   uint64_t raw_full[kRawStages], raw_free[kRawStages], k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages];
-  uint64_t s_full[2][2], p_full[2][2], o_done[2][2], top_full[2];   // by tile, and by step's parity
+  uint64_t s_full[2][2], p_full[2][2], o_done[2][2];   // by tile, and by step's parity
   uint32_t tmem;
   int poison;
 };
@@ -245,20 +243,18 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     }
     for (int i = 0; i < 4; ++i) {
       barrier_init(&sh.s_full[i / 2][i % 2], 1);
-      barrier_init(&sh.p_full[i / 2][i % 2], kTileThreads);
+      barrier_init(&sh.p_full[i / 2][i % 2], kTileRows);
       barrier_init(&sh.o_done[i / 2][i % 2], 1);
     }
-    barrier_init(&sh.top_full[0], kTileThreads);
-    barrier_init(&sh.top_full[1], kTileThreads);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (threadIdx.x < kCtaRows) {
-    const int tile = threadIdx.x / kTileRows, row = threadIdx.x % kTileRows;
-    sh.unit_q[tile][row] = stage_query<D>(p, r, h, first_row + threadIdx.x, sh.q[tile], row);
+  float unit_q = 0.0f;
+  if (threadIdx.x < kSoftmaxThreads) {
+    unit_q = stage_query<D>(p, r, h, first_row + threadIdx.x, sh.q[threadIdx.x / kTileRows], threadIdx.x % kTileRows);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   fence_before();
@@ -268,13 +264,11 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   volatile int* poison = &sh.poison;
 
   if (threadIdx.x < kSoftmaxThreads) {
-    // ---- half a row's scores to a thread ----
-    const int tile = threadIdx.x / kTileThreads, part = threadIdx.x / kTileRows % 2, tile_row = threadIdx.x % kTileRows;
-    const int row = first_row + tile * kTileRows + tile_row, i = row / p.group;
-    const int sees = (i < r.todo ? r.length - r.count + i + 1 : 0) - part * 32;
+    // ---- a row to a thread ----
+    const int tile = threadIdx.x / kTileRows, row = first_row + threadIdx.x, i = row / p.group;
+    const int sees = i < r.todo ? r.length - r.count + i + 1 : 0;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-    const uint32_t s_at = tmem + lanes + tile * 128 + part * 32, o_at = tmem + lanes + 256 + tile * 128 + part * (D / 2);
-    const float unit_q = sh.unit_q[tile][tile_row];
+    const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem + lanes + 256 + tile * 128;
     float top = -INFINITY, sum = 0.0f;
     bool healthy = true;
     for (int step = 0; step < steps; ++step) {
@@ -283,32 +277,36 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
                 barrier_wait(&sh.s_full[tile][turn], step / 2 & 1, poison, p.a.status);
       if (!healthy) break;
       fence_after();
-      float x[32], now = top, by[2];
-      tmem_load(s_at + turn * 64, x);
-      const int limit = sees - step * kTokens;
-      const bool all = __all_sync(~0u, limit >= 32);
-      wait_loads();
-#pragma unroll
-      for (int block = 0; block < 2; ++block) {
-        const float ks = sh.ks[note][part * 2 + block];
-        if (!all || ks == kNoTokens) {
-          const int t = ks == kNoTokens ? 1 << 30 : block * 16;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[block * 16 + e] = t + e < limit ? x[block * 16 + e] : -INFINITY;
-        }
-        float m = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) m = fmaxf(m, fmaxf(x[block * 16 + e], x[block * 16 + e + 1]));
-        by[block] = fmaxf(unit_q * ks, 0x1p-126f);
-        now = fmaxf(now, m * by[block]);
-      }
-      sh.top[turn][tile][part][tile_row] = now;
-      barrier_arrive(&sh.top_full[tile]);
-      healthy = barrier_wait(&sh.top_full[tile], turn, poison, p.a.status);
-      if (!healthy) break;
-      now = fmaxf(now, sh.top[turn][tile][part ^ 1][tile_row]);
+      float x[2][32], now = top, by[kBlocks], ks[kBlocks], bias[kBlocks], counts[kBlocks];
+      tmem_load(s_at + turn * 64, x[0]);
+      tmem_load(s_at + turn * 64 + 32, x[1]);
+      *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(sh.ks[note]);
+      *reinterpret_cast<float4*>(bias) = *reinterpret_cast<const float4*>(sh.bias[note]);
+      *reinterpret_cast<float4*>(counts) = *reinterpret_cast<const float4*>(sh.counts[note]);
       const float values = sh.rescale[note];
-      if (__any_sync(~0u, now > top + kSlack) || values != 1.0f) {   // alike in both halves of a row
+      const int limit = sees - step * kTokens;
+      bool all = limit >= kTokens;
+#pragma unroll
+      for (int block = 0; block < kBlocks; ++block) all = all && ks[block] != kNoTokens;
+      all = __all_sync(~0u, all);
+      wait_loads();
+      if (!all) {
+#pragma unroll
+        for (int e = 0; e < kTokens; ++e) x[e / 32][e % 32] = e < limit && ks[e / 16] != kNoTokens ? x[e / 32][e % 32] : -INFINITY;
+      }
+#pragma unroll
+      for (int block = 0; block < kBlocks; ++block) {
+        const float* y = x[block / 2] + block % 2 * 16;
+        float m = fmaxf(y[0], y[1]), n = fmaxf(y[2], y[3]);
+#pragma unroll
+        for (int e = 4; e < 16; e += 4) {
+          m = fmaxf(m, fmaxf(y[e], y[e + 1]));
+          n = fmaxf(n, fmaxf(y[e + 2], y[e + 3]));
+        }
+        by[block] = fmaxf(unit_q * ks[block], 0x1p-126f);
+        now = fmaxf(now, fmaxf(m, n) * by[block]);
+      }
+      if (__any_sync(~0u, now > top + kSlack) || values != 1.0f) {
         const float keep = now == -INFINITY ? 1.0f : exp2_fast(top - now);
         sum *= keep;
         top = now;
@@ -318,7 +316,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           fence_after();
           const float less = keep * values;
 #pragma unroll 1
-          for (int n = 0; n < D / 32; ++n) {
+          for (int n = 0; n < D / 16; ++n) {
             uint32_t o[16];
             tmem_load16(o_at + n * 16, o);
             wait_loads();
@@ -330,21 +328,25 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         }
       }
       const float base = top == -INFINITY ? 0.0f : top;
-      uint32_t w[16];
 #pragma unroll
-      for (int block = 0; block < 2; ++block) {
-        const float bias = sh.bias[note][part * 2 + block] - base;
-        float2 total = make_float2(0.0f, 0.0f);
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float2 y = fma2(make_float2(x[block * 16 + e], x[block * 16 + e + 1]), make_float2(by[block], by[block]), make_float2(bias, bias));
-          const float2 q = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-          total = add2(total, q);
-          w[block * 8 + e / 2] = pack_half2(q.x, q.y);
+        for (int block = 2 * half; block < 2 * half + 2; ++block) {
+          const float* z = x[half] + block % 2 * 16;
+          const float less = bias[block] - base;
+          float2 total = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float2 y = fma2(make_float2(z[e], z[e + 1]), make_float2(by[block], by[block]), make_float2(less, less));
+            const float2 q = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            total = add2(total, q);
+            w[block % 2 * 8 + e / 2] = pack_half2(q.x, q.y);
+          }
+          sum = fmaf(total.x + total.y, counts[block], sum);
         }
-        sum = fmaf(total.x + total.y, sh.counts[note][part * 2 + block], sum);
+        tmem_store16(s_at + turn * 64 + half * 16, w);           // over scores that this warp has read
       }
-      tmem_store16(s_at + turn * 64, w);          // over scores that this warp has read
       wait_stores();
       fence_before();
       barrier_arrive(&sh.p_full[tile][turn]);
@@ -354,17 +356,11 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       fence_after();
     }
     if (healthy) {
-      sh.top[steps & 1][tile][part][tile_row] = sum;             // the halves of a row's sum meet
-      barrier_arrive(&sh.top_full[tile]);
-      healthy = barrier_wait(&sh.top_full[tile], steps & 1, poison, p.a.status);
-    }
-    if (healthy) {
-      sum += sh.top[steps & 1][tile][part ^ 1][tile_row];
       const float by = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kUp), sum);
       const float unit = steps > 0 ? *reinterpret_cast<volatile float*>(&sh.unit) : 1.0f;
-      const long long at = (r.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + part * (D / 2);
+      const long long at = (r.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head;
 #pragma unroll 1
-      for (int n = 0; n < D / 64; ++n) {
+      for (int n = 0; n < D / 32; ++n) {
         alignas(16) float x[32];
         if (steps > 0) {
           tmem_load(o_at + n * 32, x);
@@ -497,7 +493,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         fence_after();
 #pragma unroll
         for (int k = 0; k < kTokens / 16; ++k)
-          mma_tensor(elected, base + 256 + tile * 128, base + tile * 128 + turn * 64 + k / 2 * 32 + k % 2 * 8,
+          mma_tensor(elected, base + 256 + tile * 128, base + tile * 128 + turn * 64 + k * 8,
                      values + k * 128, instruction(D, true), step > 0 || k > 0);
         mma_commit(elected, &sh.o_done[tile][turn]);
         if (tile == 1) mma_commit(elected, &sh.v_free[stage]);
