@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kTokens = 64, kStages = 3, kRawStages = 3, kNotes = 8, kTileRows = 128, kCtaRows = 2 * kTileRows;
 constexpr int kRowPlane = kTileRows * 128, kTokenPlane = kTokens * 128;        // bytes of a plane: 64 columns of all rows, all tokens
-constexpr int kSoftmaxThreads = kCtaRows, kConvertThreads = 256;
+constexpr int kSoftmaxThreads = kCtaRows, kConvertThreads = 128;
 constexpr int kFetchWarp = (kSoftmaxThreads + kConvertThreads) / 32, kIssueWarp = kFetchWarp + 1, kAllThreads = (kIssueWarp + 1) * 32;
 constexpr int kBlocks = kTokens / kGranule;
 constexpr float kUp = 7.0f, kSlack = 4.0f;
