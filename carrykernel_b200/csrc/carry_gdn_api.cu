@@ -300,7 +300,7 @@ int kv_ok(const CarryGdnKvCache& c, const CarryGdnKvRows& r) {
   if ((c.D != 64 && c.D != 128) || c.block > 128) return CARRY_GDN_ERR_UNSUPPORTED;
   if (r.B < 0 || r.N < 0 || r.max_query < 0) return CARRY_GDN_ERR_SHAPE;
   if (!r.query_start && (long long)r.B * r.max_query != r.N) return CARRY_GDN_ERR_SHAPE;
-  if (r.B > 65535 || c.HKV > 65535 || (long long)c.HKV * c.page * c.D > 0x7fffffff) return CARRY_GDN_ERR_TOO_LARGE;
+  if (r.B > 65535 || c.HKV > 65535 || (long long)r.B * c.HKV > 0x7fffffff || (long long)c.HKV * c.page * c.D > 0x7fffffff) return CARRY_GDN_ERR_TOO_LARGE;
   return CARRY_GDN_OK;
 }
 int kv_pointers_ok(const CarryGdnKvCache& c) {

@@ -915,7 +915,7 @@ __global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constan
   depend_release();
   depend_wait();
   const CarryGdnKvCache& c = p.a.cache;
-  const int b = blockIdx.z, h = blockIdx.y, first_row = (gridDim.x - 1 - blockIdx.x) * kChunkRows;   // the longest go first
+  const int b = blockIdx.x / c.HKV, h = blockIdx.x % c.HKV, first_row = (gridDim.y - 1 - blockIdx.y) * kChunkRows;   // the longest of all go first
   const KvRequest q = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
   if (first_row >= q.todo * p.group) return;
   const int row0 = first_row + threadIdx.x / 32 * kRowsPerWarp;
@@ -1010,7 +1010,8 @@ int launch_by_rows(const AttnParams& p, int tiles, cudaStream_t stream) {
   static thread_local bool ready[64];
   const int rc = prepare(kv_chunk_kernel<D, PARTS>, smem, ready);
   if (rc != CARRY_GDN_OK) return rc;
-  const dim3 grid((unsigned)((rows + kChunkRows - 1) / kChunkRows), p.a.cache.HKV, p.a.rows.B);
+  if ((rows + kChunkRows - 1) / kChunkRows > 65535) return CARRY_GDN_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)((rows + kChunkRows - 1) / kChunkRows));
   return launch_dependent(kv_chunk_kernel<D, PARTS>, grid, kThreads, smem, stream, p);
 }
 

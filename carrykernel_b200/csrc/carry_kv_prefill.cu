@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   depend_release();
   depend_wait();
   const CarryGdnKvCache& c = p.a.cache;
-  const int b = blockIdx.z, h = blockIdx.y, first_row = (gridDim.x - 1 - blockIdx.x) * kCtaRows;     // the longest go first
+  const int b = blockIdx.x / c.HKV, h = blockIdx.x % c.HKV, first_row = (gridDim.y - 1 - blockIdx.y) * kCtaRows;   // the longest of all go first
   const int warp = threadIdx.x / 32;
   const KvRequest r = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
   if (first_row >= r.todo * p.group) return;
@@ -532,7 +532,8 @@ int launch(const AttnParams& p, cudaStream_t stream) {
     if (dev < 64) ready[dev] = true;
   }
   const long long rows = (long long)p.a.rows.max_query * p.group;
-  const dim3 grid((unsigned)((rows + kCtaRows - 1) / kCtaRows), p.a.cache.HKV, p.a.rows.B);
+  if ((rows + kCtaRows - 1) / kCtaRows > 65535) return CARRY_GDN_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)((rows + kCtaRows - 1) / kCtaRows));
   return launch_dependent(kv_prefill_kernel<D>, grid, kAllThreads, smem, stream, p);
 }
 
