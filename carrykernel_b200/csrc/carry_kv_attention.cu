@@ -33,6 +33,11 @@ __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
   return fmaxf(x, __shfl_xor_sync(~0u, x, 2));
 }
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+  return x;
+}
 __device__ __forceinline__ float quad_sum(float x) {
   x += __shfl_xor_sync(~0u, x, 1);
   return x + __shfl_xor_sync(~0u, x, 2);
@@ -920,13 +925,14 @@ __global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constan
   if (first_row >= q.todo * p.group) return;
   const int row0 = first_row + threadIdx.x / 32 * kRowsPerWarp;
   const int last = min((first_row + kChunkRows - 1) / p.group, q.todo - 1);
-  const int length = max(min(q.length, q.length - q.count + last + 1), 0), tiles = (length + kTile - 1) / kTile;
+  const int length = max(min(q.length, q.length - q.count + last + 1), 0), all_tiles = (length + kTile - 1) / kTile;
+  const int share = (all_tiles + p.splits - 1) / p.splits, tile0 = min(share * (int)blockIdx.z, all_tiles), tiles = min(share, all_tiles - tile0);
   Pages<D> ids;
-  fetch_pages<D>(p, b, 0, length, ids);
+  fetch_pages<D>(p, b, tile0, length, ids);
   auto next_load = [&](int tile) {
     if (tile < tiles) {
-      load_tile<D>(p, stages[tile % kChunkStages], h, tile, length, ids);
-      if (tile + 1 < tiles) fetch_pages<D>(p, b, tile + 1, length, ids);
+      load_tile<D>(p, stages[tile % kChunkStages], h, tile0 + tile, length, ids);
+      if (tile + 1 < tiles) fetch_pages<D>(p, b, tile0 + tile + 1, length, ids);
     }
     __pipeline_commit();
   };
@@ -941,20 +947,69 @@ __global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constan
     __syncthreads();
     next_load(tile + kChunkStages - 1);
     int limit[2];
-    row_limits(p, q, row0, tile, limit);
+    row_limits(p, q, row0, tile0 + tile, limit);
     attend<D, PARTS, kTile>(stages[tile % kChunkStages], 0, query, limit, r);
   }
+  float sum[2];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const float sum = quad_sum(r.sum[half]);
-    const float w = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kWeightUp), sum);
+    sum[half] = quad_sum(r.sum[half]);
+    const float w = sum[half] == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kWeightUp), sum[half]);
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
       r.o[n][2 * half] = r.o[n][2 * half] * w * r.unit;
       r.o[n][2 * half + 1] = r.o[n][2 * half + 1] * w * r.unit;
     }
   }
-  store_rows<D>(p, q, h, row0, r);
+  if (p.splits == 1) {
+    store_rows<D>(p, q, h, row0, r);
+    return;
+  }
+  const Parts part = parts_of(p, blockIdx.z, blockIdx.x);
+  const int g = threadIdx.x % 32 / 4, cc = threadIdx.x % 4;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = row0 + g + half * 8;
+    if (cc == 0) {
+      part.top[row] = r.top[half];
+      part.sum[row] = sum[half];
+    }
+    float4* o = reinterpret_cast<float4*>(part.o + (long long)row * D + cc * (D / 4));
+#pragma unroll
+    for (int e = 0; e < D / 4; e += 4) {
+      const int i = 2 * half + e / (D / 8), n = e % (D / 8);
+      o[e / 4] = make_float4(r.o[n][i], r.o[n + 1][i], r.o[n + 2][i], r.o[n + 3][i]);
+    }
+  }
+}
+
+// Joins the parts of a context, a row to a warp: lane s has part s's weight, then the lanes have the columns.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_join_parts_kernel(const __grid_constant__ AttnParams p) {
+  depend_release();
+  depend_wait();
+  const int lane = threadIdx.x % 32, row = blockIdx.y * kWarps + threadIdx.x / 32;
+  const int b = blockIdx.x / p.a.cache.HKV, h = blockIdx.x % p.a.cache.HKV, i = row / p.group;
+  const KvRequest q = kv_request(p.a.cache, p.a.rows, b, nullptr);
+  if (i >= q.todo) return;
+  const Parts mine = parts_of(p, min(lane, p.splits - 1), blockIdx.x);
+  float top = lane < p.splits ? mine.top[row] : -INFINITY, w = lane < p.splits ? mine.sum[row] : 0.0f;
+  const float all_top = warp_max(top), base = all_top == -INFINITY ? 0.0f : all_top;
+  w *= exp2_fast(top - base);
+  float sum = w, o[D / 32] = {};
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+#pragma unroll 8
+  for (int s = 0; s < p.splits; ++s) {
+    const float* x = parts_of(p, s, blockIdx.x).o + (long long)row * D + lane;
+    const float by = __shfl_sync(~0u, w, s);
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) o[e] = fmaf(by, x[e * 32], o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e)
+    store_from_float(p.a.out, (q.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + e * 32 + lane, p.a.dtype,
+                     sum == 0.0f ? 0.0f : __fdiv_rn(o[e], sum));
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
@@ -997,6 +1052,25 @@ int launch_decode(const AttnParams& p, cudaStream_t stream) {
   return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kJoinThreads, 0, stream, p, NT * 8);
 }
 
+// splits and padded rows of the kernel for many fp32 rows
+void lay_out(const CarryGdnKvAttentionArgs& a, int& splits, int& padded) {
+  const long long rows = (long long)a.rows.max_query * (a.HQ / a.cache.HKV), tiles = (rows + kChunkRows - 1) / kChunkRows;
+  padded = tiles > 65535 ? -1 : (int)tiles * kChunkRows;
+  splits = split_count(a, (tiles * a.cache.HKV * a.rows.B + 1) / 2);             // an SM holds two of its CTAs
+}
+
+template <int D, int PARTS>
+int launch_chunk(AttnParams p, cudaStream_t stream) {
+  lay_out(p.a, p.splits, p.padded);
+  constexpr size_t smem = sizeof(Stage<D>) * kChunkStages;
+  static thread_local bool ready[64];
+  int rc = prepare(kv_chunk_kernel<D, PARTS>, smem, ready);
+  if (rc != CARRY_GDN_OK) return rc;
+  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)p.padded / kChunkRows, (unsigned)p.splits);
+  rc = launch_dependent(kv_chunk_kernel<D, PARTS>, grid, kThreads, smem, stream, p);
+  return rc == CARRY_GDN_OK && p.splits > 1 ? launch_join_parts(p, stream) : rc;
+}
+
 template <int D, int PARTS>
 int launch_by_rows(const AttnParams& p, int tiles, cudaStream_t stream) {
   if (tiles == 1) return launch_decode<D, 1, PARTS>(p, stream);
@@ -1005,33 +1079,36 @@ int launch_by_rows(const AttnParams& p, int tiles, cudaStream_t stream) {
     if (tiles == 4) return launch_decode<D, 4, PARTS>(p, stream);
     return launch_kv_prefill(p, stream);
   }
-  constexpr size_t smem = sizeof(Stage<D>) * kChunkStages;
-  const long long rows = (long long)p.a.rows.max_query * p.group;
-  static thread_local bool ready[64];
-  const int rc = prepare(kv_chunk_kernel<D, PARTS>, smem, ready);
-  if (rc != CARRY_GDN_OK) return rc;
-  if ((rows + kChunkRows - 1) / kChunkRows > 65535) return CARRY_GDN_ERR_TOO_LARGE;
-  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)((rows + kChunkRows - 1) / kChunkRows));
-  return launch_dependent(kv_chunk_kernel<D, PARTS>, grid, kThreads, smem, stream, p);
+  if constexpr (PARTS == 2) return launch_chunk<D, PARTS>(p, stream);
 }
 
 }  // namespace
 
 int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a) {
   const int tiles = column_tiles(a);
-  if (tiles == 0) return 0;
   if (sm_count() == 0) return CARRY_GDN_ERR_NO_DEVICE;
+  if (tiles == 0 && a.dtype != CARRY_F32) return kv_prefill_workspace(a);
+  if (tiles == 0) {
+    int splits, padded;
+    lay_out(a, splits, padded);
+    return padded < 0 ? CARRY_GDN_ERR_TOO_LARGE : parts_bytes(a, splits, padded);
+  }
   const long long ctas = decode_ctas(a);
   return (sizeof(Piece) * ctas + 15) / 16 * 16 + 2 * ctas * slot_floats(tiles * 8, a.cache.D) * 4;
 }
 
+int launch_join_parts(const AttnParams& p, cudaStream_t stream) {
+  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)((p.rows + kWarps - 1) / kWarps));
+  return p.a.cache.D == 64 ? launch_dependent(kv_join_parts_kernel<64>, grid, kThreads, 0, stream, p)
+                           : launch_dependent(kv_join_parts_kernel<128>, grid, kThreads, 0, stream, p);
+}
+
 int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream) {
   if (sm_count() == 0) return CARRY_GDN_ERR_NO_DEVICE;
-  AttnParams p = {a, a.HQ / a.cache.HKV, a.cache.page / kGranule, -1, a.cache.block / kGranule, -1, 0};
+  AttnParams p = {a, a.HQ / a.cache.HKV, a.cache.page / kGranule, -1, a.cache.block / kGranule, -1, a.rows.max_query * (a.HQ / a.cache.HKV), 1, 0};
   p.page_shift = shift_of(p.page_granules);
   p.block_shift = shift_of(p.block_granules);
   const int tiles = column_tiles(a);
-  p.rows = tiles ? a.rows.max_query * p.group : 0;
   if (a.cache.D == 64) return a.dtype == CARRY_F32 ? launch_by_rows<64, 2>(p, tiles, stream) : launch_by_rows<64, 1>(p, tiles, stream);
   return a.dtype == CARRY_F32 ? launch_by_rows<128, 2>(p, tiles, stream) : launch_by_rows<128, 1>(p, tiles, stream);
 }

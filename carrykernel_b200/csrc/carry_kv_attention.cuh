@@ -14,8 +14,31 @@ struct AttnParams {
   int group;                      // query heads per key/value head
   int page_granules, page_shift;  // granules in a page, and its logarithm or -1
   int block_granules, block_shift;
-  int rows;                       // rows of a request that may be in use (decode kernel)
+  int rows;                       // rows of a (request, head): most that may be in use
+  int splits, padded;             // parts that a context is cut into where the rows alone are few; rows that a part has room for
 };
+
+// What a part of a context leaves for the joining kernel, by part, (request, head) and row: largest score and sum of
+// weights, then the outputs, normalised.
+struct Parts {
+  float *top, *sum, *o;
+};
+__device__ __forceinline__ Parts parts_of(const AttnParams& p, int part, long long pair) {
+  const long long pairs = (long long)p.a.rows.B * p.a.cache.HKV, all = p.splits * pairs * p.padded, first = (part * pairs + pair) * p.padded;
+  float* base = reinterpret_cast<float*>(p.a.workspace);
+  return {base + first, base + all + first, base + 2 * all + first * p.a.cache.D};
+}
+inline int64_t parts_bytes(const CarryGdnKvAttentionArgs& a, int splits, int padded) {
+  return splits > 1 ? 4LL * splits * a.rows.B * a.cache.HKV * padded * (a.cache.D + 2) : 0;
+}
+// With fewer CTAs than processors a context is cut, into parts of eight steps of 64 tokens or more: a part costs some five
+// microseconds of its own, four steps' worth.
+inline int split_count(const CarryGdnKvAttentionArgs& a, long long ctas) {
+  const long long steps = ((long long)a.cache.max_pages * a.cache.page + 63) / 64;
+  const long long n = sm_count() / (ctas < 1 ? 1 : ctas), most = steps / 8;
+  return (int)(n < most ? (n < 1 ? 1 : n > 32 ? 32 : n) : most < 1 ? 1 : most > 32 ? 32 : most);
+}
+int launch_join_parts(const AttnParams& p, cudaStream_t stream);
 
 __device__ __forceinline__ uint32_t pack_half2(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -69,6 +92,7 @@ __device__ __forceinline__ void store8(void* out, long long at, int dtype, const
   *to = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-int launch_kv_prefill(const AttnParams& p, cudaStream_t stream);
+int launch_kv_prefill(AttnParams p, cudaStream_t stream);
+int64_t kv_prefill_workspace(const CarryGdnKvAttentionArgs& a);
 
 }  // namespace carry

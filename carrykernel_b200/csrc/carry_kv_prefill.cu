@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   const KvRequest r = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
   if (first_row >= r.todo * p.group) return;
   const int last = min((first_row + kCtaRows - 1) / p.group, r.todo - 1);
-  const int length = max(min(r.length, r.length - r.count + last + 1), 0), steps = (length + kTokens - 1) / kTokens;
+  const int length = max(min(r.length, r.length - r.count + last + 1), 0), all_steps = (length + kTokens - 1) / kTokens;
+  const int share = (all_steps + p.splits - 1) / p.splits, step0 = min(share * (int)blockIdx.z, all_steps), steps = min(share, all_steps - step0);
 
   if (threadIdx.x == 0) {
     sh.poison = 0;
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       *reinterpret_cast<float4*>(bias) = *reinterpret_cast<const float4*>(sh.bias[note]);
       *reinterpret_cast<float4*>(counts) = *reinterpret_cast<const float4*>(sh.counts[note]);
       const float values = sh.rescale[note];
-      const int limit = sees - step * kTokens;
+      const int limit = sees - (step0 + step) * kTokens;
       bool all = limit >= kTokens;
 #pragma unroll
       for (int block = 0; block < kBlocks; ++block) all = all && ks[block] != kNoTokens;
@@ -359,6 +360,11 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       const float by = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kUp), sum);
       const float unit = steps > 0 ? *reinterpret_cast<volatile float*>(&sh.unit) : 1.0f;
       const long long at = (r.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head;
+      const Parts part = parts_of(p, blockIdx.z, blockIdx.x);
+      if (p.splits > 1) {
+        part.top[row] = top;
+        part.sum[row] = sum;
+      }
 #pragma unroll 1
       for (int n = 0; n < D / 32; ++n) {
         alignas(16) float x[32];
@@ -371,7 +377,10 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0.0f;
         }
-        if (i < r.todo) {
+        if (p.splits > 1) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) store8(part.o, (long long)row * D + n * 32 + e, CARRY_F32, x + e);
+        } else if (i < r.todo) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) store8(p.a.out, at + n * 32 + e, p.a.dtype, x + e);
         }
@@ -382,7 +391,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     const int tid = threadIdx.x - kSoftmaxThreads;
     int raw = 0, stage = 0, raw_parity = 0, parity = 1;
     for (int step = 0; step < steps; ++step) {
-      const int left = length - step * kTokens;
+      const int left = length - (step0 + step) * kTokens;
       const float* ks = sh.ks[step % kNotes];
       if (!barrier_wait(&sh.raw_full[raw], raw_parity, poison, p.a.status)) break;
       if (step >= kStages && !barrier_wait(&sh.k_free[stage], parity, poison, p.a.status)) break;
@@ -406,7 +415,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       float ks, vs;
     };
     auto find = [&](int step, Granule& g) {
-      const int granule = step * kBlocks + lane;
+      const int granule = (step0 + step) * kBlocks + lane;
       g.id = lane < kBlocks ? page_id(p, b, granule, length) : 0;
       g.in_page = granule - page_index(p, granule) * p.page_granules;
     };
@@ -531,16 +540,29 @@ int launch(const AttnParams& p, cudaStream_t stream) {
     }
     if (dev < 64) ready[dev] = true;
   }
-  const long long rows = (long long)p.a.rows.max_query * p.group;
-  if ((rows + kCtaRows - 1) / kCtaRows > 65535) return CARRY_GDN_ERR_TOO_LARGE;
-  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)((rows + kCtaRows - 1) / kCtaRows));
+  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)p.padded / kCtaRows, (unsigned)p.splits);
   return launch_dependent(kv_prefill_kernel<D>, grid, kAllThreads, smem, stream, p);
+}
+
+// splits and padded rows
+void lay_out(const CarryGdnKvAttentionArgs& a, int& splits, int& padded) {
+  const long long rows = (long long)a.rows.max_query * (a.HQ / a.cache.HKV), tiles = (rows + kCtaRows - 1) / kCtaRows;
+  padded = tiles > 65535 ? -1 : (int)tiles * kCtaRows;
+  splits = split_count(a, tiles * a.cache.HKV * a.rows.B);
 }
 
 }  // namespace
 
-int launch_kv_prefill(const AttnParams& p, cudaStream_t stream) {
-  return p.a.cache.D == 64 ? launch<64>(p, stream) : launch<128>(p, stream);
+int64_t kv_prefill_workspace(const CarryGdnKvAttentionArgs& a) {
+  int splits, padded;
+  lay_out(a, splits, padded);
+  return padded < 0 ? CARRY_GDN_ERR_TOO_LARGE : parts_bytes(a, splits, padded);
+}
+
+int launch_kv_prefill(AttnParams p, cudaStream_t stream) {
+  lay_out(p.a, p.splits, p.padded);
+  const int rc = p.a.cache.D == 64 ? launch<64>(p, stream) : launch<128>(p, stream);
+  return rc == CARRY_GDN_OK && p.splits > 1 ? launch_join_parts(p, stream) : rc;
 }
 
 }  // namespace carry

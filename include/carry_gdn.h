@@ -333,9 +333,8 @@ int carry_gdn_pool_copy_layers(const CarryGdnPoolCopyLayersArgs* args, void* str
  * bound.  Within a page the tensors are contiguous; strides between pages and
  * between the table's rows are in elements.  D is 64 or 128, page and block are
  * multiples of 16, block divides page and is at most 128; code pages start on
- * 16-byte boundaries.  B and HKV are at most 65535 (their
- * product below 2^31), a request's tokens 2^30, and
- * a page of all heads is below 2^31 bytes.
+ * 16-byte boundaries.  B and HKV are at most 65535, their product and a page of
+ * all heads below 2^31, a request's tokens 2^30.
  */
 typedef struct CarryGdnKvCache {
   uint8_t* k_codes;
