@@ -338,8 +338,8 @@ constexpr int kRun = 32, kLine = kRun * kWarps;   // tokens of a warp's step, an
 
 // What a CTA leaves for the joining kernel: at most one piece of a (request, head) that began in an earlier CTA (slot 0)
 // and one that goes on in later ones (slot 1).
-struct Piece {
-  int request, head, last;        // last CTA with a piece of the same; last < 0: none began here
+struct alignas(16) Piece {
+  int first, rows, head, last;    // the request's first row and number of rows; last CTA with a piece of the same, or -1: none began here
 };
 
 template <int D>
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_ke
   const CarryGdnKvCache& c = p.a.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, cc = lane % 4;
   Piece* pieces = reinterpret_cast<Piece*>(p.a.workspace);
-  float* slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + (sizeof(Piece) * gridDim.x + 15) / 16 * 16);
+  float* slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + sizeof(Piece) * gridDim.x);
 
   // the line's length, and where on it this CTA begins
   long long total = 0, before;
@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_ke
       if (!ends && first_tile == 0 && threadIdx.x == 0) {
         // the rest of its tiles: the CTAs up to the one with its last tile
         const long long last = at + (use.tiles - 1 - use.tile);
-        pieces[blockIdx.x] = {use.b, use.h, (int)(last / share)};
+        pieces[blockIdx.x] = {request.first, request.todo * p.group, use.h, (int)(last / share)};
       }
       __syncthreads();
       begin = true;
@@ -842,69 +842,95 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_ke
   }
 }
 
-// Joins the pieces of the (request, head) that began in CTA blockIdx.x of the kernel above, row by row: first all
-// weights, then the rows themselves, each in one trip to memory as far as registers go.
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinStep = 256;
+// Joins the pieces of the (request, head) that began in CTA blockIdx.x of the kernel above.  Eight pieces of a row come in
+// one trip to memory, with their weights.  Where pieces are few a warp has a row; where they are many the warps share one.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kBatch = 8;
+
+template <int D>
+struct Joined {
+  float top, sum, o[D / 32];
+};
+template <int D>
+__device__ __forceinline__ void join_pieces(const float* slots, int rows, int row, int first, int step, int count, Joined<D>& r) {
+  const int lane = threadIdx.x % 32;
+  r.top = -INFINITY;
+  r.sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) r.o[e] = 0.0f;
+  for (int i0 = first; i0 < count; i0 += kBatch * step) {
+    float top[kBatch], sum[kBatch], o[kBatch][D / 32], most = r.top;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * step;
+      top[k] = -INFINITY;
+      sum[k] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) o[k][e] = 0.0f;
+      if (i >= count) continue;
+      const float* s = slots + (2LL * (blockIdx.x + i) + (i == 0)) * slot_floats(rows, D);
+      top[k] = s[row];
+      sum[k] = s[rows + row];
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) o[k][e] = s[2 * rows + row * D + e * 32 + lane];
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) most = fmaxf(most, top[k]);
+    const float base = most == -INFINITY ? 0.0f : most, keep = exp2_fast(r.top - base);
+    r.top = most;
+    r.sum *= keep;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) r.o[e] *= keep;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float w = sum[k] * exp2_fast(top[k] - base);
+      r.sum += w;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) r.o[e] = fmaf(w, o[k][e], r.o[e]);
+    }
+  }
+}
 
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttnParams p, const int kRows) {
-  __shared__ float tops[kJoinWarps], sums[kJoinWarps], weight[kJoinStep], part_o[kJoinWarps][D];
+  __shared__ float tops[kJoinWarps], sums[kJoinWarps], part_o[kJoinWarps][D];
   depend_release();
   depend_wait();
-  const Piece piece = reinterpret_cast<const Piece*>(p.a.workspace)[blockIdx.x];
+  const int4 word = *reinterpret_cast<const int4*>(reinterpret_cast<const Piece*>(p.a.workspace) + blockIdx.x);
+  const Piece piece = {word.x, word.y, word.z, word.w};
   if (piece.last < 0) return;
-  const float* slots = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.a.workspace) + (sizeof(Piece) * gridDim.x + 15) / 16 * 16);
-  const KvRequest q = kv_request(p.a.cache, p.a.rows, piece.request, nullptr);
+  const float* slots = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.a.workspace) + sizeof(Piece) * gridDim.x);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, count = piece.last - blockIdx.x + 1;
-  auto slot = [&](int i) { return slots + (2 * (blockIdx.x + i) + (i == 0)) * slot_floats(kRows, D); };
-  for (int row = blockIdx.y; row < q.todo * p.group; row += gridDim.y) {
-    float top = -INFINITY, sum = 0.0f, all = 0.0f, o[D / 32] = {};
-    for (int i = threadIdx.x; i < count; i += kJoinThreads) top = fmaxf(top, slot(i)[row]);
+  auto place = [&](int row) { return (piece.first + row / p.group) * p.a.stride_out_tok + (piece.head * p.group + row % p.group) * p.a.stride_out_head; };
+  Joined<D> r;
+  if (gridDim.y == 1) {
+    for (int row = warp; row < piece.rows; row += kJoinWarps) {
+      join_pieces<D>(slots, kRows, row, 0, 1, count, r);
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    if (lane == 0) tops[warp] = top;
+      for (int e = 0; e < D / 32; ++e)
+        store_from_float(p.a.out, place(row) + e * 32 + lane, p.a.dtype, r.sum == 0.0f ? 0.0f : __fdiv_rn(r.o[e], r.sum));
+    }
+    return;
+  }
+  for (int row = blockIdx.y; row < piece.rows; row += gridDim.y) {
+    join_pieces<D>(slots, kRows, row, warp, kJoinWarps, count, r);
+    if (lane == 0) {
+      tops[warp] = r.top;
+      sums[warp] = r.sum;
+    }
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) part_o[warp][e * 32 + lane] = r.o[e];
     __syncthreads();
+    float top = -INFINITY, sum = 0.0f, o = 0.0f;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
     const float base = top == -INFINITY ? 0.0f : top;
-    for (int first = 0; first < count; first += kJoinStep) {
-      const int n = min(count - first, kJoinStep);
-      __syncthreads();
-      if (threadIdx.x < n) {
-        const float* s = slot(first + threadIdx.x);
-        const float w = s[kRows + row] * exp2_fast(s[row] - base);
-        weight[threadIdx.x] = w;
-        sum += w;
-      }
-      __syncthreads();
-#pragma unroll 8
-      for (int i = warp; i < n; i += kJoinWarps) {
-        const float* s = slot(first + i) + 2 * kRows + row * D + lane * (D / 32);
-        const float w = weight[i];
-        if constexpr (D == 128) {
-          const float4 x = *reinterpret_cast<const float4*>(s);
-          o[0] = fmaf(w, x.x, o[0]); o[1] = fmaf(w, x.y, o[1]); o[2] = fmaf(w, x.z, o[2]); o[3] = fmaf(w, x.w, o[3]);
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(s);
-          o[0] = fmaf(w, x.x, o[0]); o[1] = fmaf(w, x.y, o[1]);
-        }
-      }
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float by = exp2_fast(tops[w] - base);
+      sum += sums[w] * by;
+      o = fmaf(part_o[w][threadIdx.x % D], by, o);
     }
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-    if (lane == 0) sums[warp] = sum;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) part_o[warp][lane * (D / 32) + e] = o[e];
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) all += sums[w];
-    if (threadIdx.x < D) {
-      float x = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) x += part_o[w][threadIdx.x];
-      store_from_float(p.a.out, (q.first + row / p.group) * p.a.stride_out_tok + (piece.head * p.group + row % p.group) * p.a.stride_out_head + threadIdx.x,
-                       p.a.dtype, all == 0.0f ? 0.0f : __fdiv_rn(x, all));
-    }
+    if (threadIdx.x < D) store_from_float(p.a.out, place(row) + threadIdx.x, p.a.dtype, sum == 0.0f ? 0.0f : __fdiv_rn(o, sum));
     __syncthreads();
   }
 }
@@ -1049,7 +1075,9 @@ int launch_decode(const AttnParams& p, cudaStream_t stream) {
   int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem, ready);
   if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, NT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
   if (rc != CARRY_GDN_OK) return rc;
-  return launch_dependent(kv_join_kernel<D>, dim3(ctas, p.rows < 16 ? p.rows : 16), kJoinThreads, 0, stream, p, NT * 8);
+  // a (request, head) lies in so many pieces: a warp to a row up to eight of them, a CTA to a row beyond
+  const long long pieces = ctas / ((long long)p.a.rows.B * p.a.cache.HKV);
+  return launch_dependent(kv_join_kernel<D>, dim3(ctas, pieces <= kBatch ? 1 : p.rows), kJoinThreads, 0, stream, p, NT * 8);
 }
 
 // splits and padded rows of the kernel for many fp32 rows
@@ -1094,7 +1122,7 @@ int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a) {
     return padded < 0 ? CARRY_GDN_ERR_TOO_LARGE : parts_bytes(a, splits, padded);
   }
   const long long ctas = decode_ctas(a);
-  return (sizeof(Piece) * ctas + 15) / 16 * 16 + 2 * ctas * slot_floats(tiles * 8, a.cache.D) * 4;
+  return sizeof(Piece) * ctas + 2 * ctas * slot_floats(tiles * 8, a.cache.D) * 4;
 }
 
 int launch_join_parts(const AttnParams& p, cudaStream_t stream) {
