@@ -13,6 +13,7 @@
 //
 // What a call reads is the cache, once; one matrix tile of 16 rows holds the query heads of a key/value head, so that
 // the tokens are read once for all of them.
+#include <cooperative_groups.h>
 #include <cuda_pipeline_primitives.h>
 
 #include "carry_kv_attention.cuh"
@@ -357,6 +358,7 @@ struct DecodeShared {
   RunStage<D> stage[kWarps][stages(D, NT, PARTS)];
   float merge[NT * 8][D + 4];
   float top[kWarps][NT * 8], sum[kWarps][NT * 8];
+  float pair_top[NT * 8], pair_sum[NT * 8];
 };
 
 __host__ __device__ constexpr long long slot_floats(int rows, int D) { return (long long)rows * (D + 2); }
@@ -652,6 +654,163 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
   }
 }
 
+// The warps' softmaxes into one: weights first, then the outputs in turn, normalised, in sh.merge.  top and sum are of rows
+// 8 n + 2 c and + 1.
+template <int D, int NT, int PARTS>
+__device__ __forceinline__ void merge_warps(DecodeShared<D, NT, PARTS>& sh, Running<D, NT>& r, float (&top)[NT][2], float (&sum)[NT][2]) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, cc = lane % 4;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float share = r.sum[n][i];
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) share += __shfl_xor_sync(~0u, share, d);
+      if (g == 0) {
+        sh.top[warp][8 * n + 2 * cc + i] = r.top[n][i];
+        sh.sum[warp][8 * n + 2 * cc + i] = share;
+      }
+    }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 8 * n + 2 * cc + i;
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) m = fmaxf(m, sh.top[x][row]);
+      const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) l += sh.sum[x][row] * exp2_fast(sh.top[x][row] - base);
+      const float w = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[n][i] - base), l) * exp2f(-kWeightUp);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        r.o[n][x][i] = r.o[n][x][i] * w * r.unit;
+        r.o[n][x][i + 2] = r.o[n][x][i + 2] * w * r.unit;
+      }
+      top[n][i] = m;
+      sum[n][i] = l;
+    }
+#pragma unroll
+  for (int x = 0; x < kWarps; ++x) {
+    if (x > 0) __syncthreads();
+    if (x != warp) continue;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int m = 0; m < D / 16; m += 2) {
+          float4* cell = reinterpret_cast<float4*>(&sh.merge[8 * n + 2 * cc + i][g * (D / 8) + 2 * m]);
+          float4 mine = make_float4(r.o[n][m][i], r.o[n][m][i + 2], r.o[n][m + 1][i], r.o[n][m + 1][i + 2]);
+          if (x > 0) {
+            const float4 had = *cell;
+            mine.x += had.x; mine.y += had.y; mine.z += had.z; mine.w += had.w;
+          }
+          *cell = mine;
+        }
+  }
+  __syncthreads();
+}
+
+// A (request, head) to a cluster of CTAs, which join through each other's shared memory: one launch, where the line's way
+// takes two.  For short contexts of few (request, head)s.
+constexpr int kCluster = 8;
+
+template <int D, int NT, int PARTS>
+__global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_pair_kernel(const __grid_constant__ AttnParams p) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  DecodeShared<D, NT, PARTS>& sh = *reinterpret_cast<DecodeShared<D, NT, PARTS>*>(raw);
+  constexpr int kStages = stages(D, NT, PARTS);
+  depend_release();
+  depend_wait();
+  const CarryGdnKvCache& c = p.a.cache;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, cc = lane % 4;
+  const int rank = blockIdx.x % kCluster, pair = blockIdx.x / kCluster;
+  Cursor use;
+  use.b = pair / c.HKV;
+  use.h = pair % c.HKV;
+  const KvRequest request = kv_request(c, p.a.rows, use.b, use.h == 0 && rank == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
+  use.length = request.length;
+  use.tiles = (use.length + kLine - 1) / kLine;
+  use.tile = rank;                                // tiles go round the cluster: neighbours read neighbouring pages
+  Cursor load = use;
+  RunPages pages = fetch_run(p, load);
+  auto next_load = [&](int stage) {
+    if (load.tile < load.tiles) {
+      load_run<D>(p, sh.stage[warp][stage], load, pages);
+      load.tile += kCluster;
+      if (load.tile < load.tiles) pages = fetch_run(p, load);
+    }
+    __pipeline_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) next_load(s);
+  Columns<D, NT, PARTS> q;
+  Running<D, NT> r;
+  load_columns<D, NT, PARTS>(p, request, use.h, q);
+  r.clear();
+  int stage = 0;
+  for (; use.tile < use.tiles; use.tile += kCluster) {
+    __pipeline_wait_prior(kStages - 2);
+    __syncwarp();
+    next_load(stage == 0 ? kStages - 1 : stage - 1);
+    const int start = use.tile * kLine + warp * kRun;
+    if (start < request.length) {
+      int limit[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int x = (8 * n + 2 * cc + i) / p.group;
+          limit[n][i] = (x < request.todo ? request.length - request.count + x + 1 : 0) - start;
+        }
+      attend_run<D, NT, PARTS>(sh.stage[warp][stage], q, limit, start + kRun <= request.length - request.count + 1, r);
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  float top[NT][2], sum[NT][2];
+  merge_warps(sh, r, top, sum);
+  if (warp == 0 && g == 0) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sh.pair_top[8 * n + 2 * cc + i] = top[n][i];
+        sh.pair_sum[8 * n + 2 * cc + i] = sum[n][i];
+      }
+  }
+  const auto cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  // the CTAs share out the output, eight columns of a row to a thread
+  for (int i = rank * kThreads + threadIdx.x; i < request.todo * p.group * (D / 8); i += kCluster * kThreads) {
+    const int row = i / (D / 8), col = i % (D / 8) * 8;
+    float tops[kCluster], sums[kCluster], most = -INFINITY, total = 0.0f;
+    alignas(16) float x[8] = {};
+#pragma unroll
+    for (int n = 0; n < kCluster; ++n) {
+      tops[n] = *cluster.map_shared_rank(&sh.pair_top[row], n);
+      sums[n] = *cluster.map_shared_rank(&sh.pair_sum[row], n);
+      most = fmaxf(most, tops[n]);
+    }
+    const float base = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+    for (int n = 0; n < kCluster; ++n) {
+      const float w = sums[n] * exp2_fast(tops[n] - base);
+      const float4* o = reinterpret_cast<const float4*>(cluster.map_shared_rank(&sh.merge[row][col], n));
+      const float4 u = o[0], v = o[1];
+      total += w;
+      x[0] = fmaf(w, u.x, x[0]); x[1] = fmaf(w, u.y, x[1]); x[2] = fmaf(w, u.z, x[2]); x[3] = fmaf(w, u.w, x[3]);
+      x[4] = fmaf(w, v.x, x[4]); x[5] = fmaf(w, v.y, x[5]); x[6] = fmaf(w, v.z, x[6]); x[7] = fmaf(w, v.w, x[7]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = total == 0.0f ? 0.0f : __fdiv_rn(x[e], total);
+    store8(p.a.out, (request.first + row / p.group) * p.a.stride_out_tok + (use.h * p.group + row % p.group) * p.a.stride_out_head + col, p.a.dtype, x);
+  }
+  cluster.sync();                                 // nobody leaves while its memory is read
+}
+
 template <int D, int NT, int PARTS>
 __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t raw[];
@@ -752,61 +911,8 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_ke
     stage = stage + 1 == kStages ? 0 : stage + 1;
     const bool ends = use.tile + 1 == use.tiles;
     if (ends || at + 1 == to) {
-      // the warps join: weights first, then the outputs in turn
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float sum = r.sum[n][i];
-#pragma unroll
-          for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
-          if (g == 0) {
-            sh.top[warp][8 * n + 2 * cc + i] = r.top[n][i];
-            sh.sum[warp][8 * n + 2 * cc + i] = sum;
-          }
-        }
-      __syncthreads();
       float top[NT][2], sum[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = 8 * n + 2 * cc + i;
-          float m = -INFINITY, l = 0.0f;
-#pragma unroll
-          for (int x = 0; x < kWarps; ++x) m = fmaxf(m, sh.top[x][row]);
-          const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-          for (int x = 0; x < kWarps; ++x) l += sh.sum[x][row] * exp2_fast(sh.top[x][row] - base);
-          const float w = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[n][i] - base), l) * exp2f(-kWeightUp);
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            r.o[n][x][i] = r.o[n][x][i] * w * r.unit;
-            r.o[n][x][i + 2] = r.o[n][x][i + 2] * w * r.unit;
-          }
-          top[n][i] = m;
-          sum[n][i] = l;
-        }
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        if (x > 0) __syncthreads();
-        if (x != warp) continue;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int m = 0; m < D / 16; m += 2) {
-              float4* cell = reinterpret_cast<float4*>(&sh.merge[8 * n + 2 * cc + i][g * (D / 8) + 2 * m]);
-              float4 mine = make_float4(r.o[n][m][i], r.o[n][m][i + 2], r.o[n][m + 1][i], r.o[n][m + 1][i + 2]);
-              if (x > 0) {
-                const float4 had = *cell;
-                mine.x += had.x; mine.y += had.y; mine.z += had.z; mine.w += had.w;
-              }
-              *cell = mine;
-            }
-      }
-      __syncthreads();
+      merge_warps(sh, r, top, sum);
       const bool whole = ends && first_tile == 0;
       float* slot = slots + (2 * blockIdx.x + (first_tile == 0)) * slot_floats(kRows, D);
       if (!whole && warp == 0 && g == 0) {
@@ -842,8 +948,8 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_ke
   }
 }
 
-// Joins the pieces of the (request, head) that began in CTA blockIdx.x of the kernel above.  Eight pieces of a row come in
-// one trip to memory, with their weights.  Where pieces are few a warp has a row; where they are many the warps share one.
+// Pieces first, first + step, ... of the `count` of a (request, head) that began in CTA `cta` of the kernel above, for one
+// row, by one warp.  Eight of them come in one trip to memory, with their weights.
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kBatch = 8;
 
 template <int D>
@@ -851,7 +957,7 @@ struct Joined {
   float top, sum, o[D / 32];
 };
 template <int D>
-__device__ __forceinline__ void join_pieces(const float* slots, int rows, int row, int first, int step, int count, Joined<D>& r) {
+__device__ __forceinline__ void join_pieces(const float* slots, int rows, int row, int cta, int first, int step, int count, Joined<D>& r) {
   const int lane = threadIdx.x % 32;
   r.top = -INFINITY;
   r.sum = 0.0f;
@@ -867,7 +973,7 @@ __device__ __forceinline__ void join_pieces(const float* slots, int rows, int ro
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) o[k][e] = 0.0f;
       if (i >= count) continue;
-      const float* s = slots + (2LL * (blockIdx.x + i) + (i == 0)) * slot_floats(rows, D);
+      const float* s = slots + (2LL * (cta + i) + (i == 0)) * slot_floats(rows, D);
       top[k] = s[row];
       sum[k] = s[rows + row];
 #pragma unroll
@@ -890,49 +996,78 @@ __device__ __forceinline__ void join_pieces(const float* slots, int rows, int ro
   }
 }
 
+// One warp to a row, for (request, head)s in few pieces: CTA by CTA of the kernel above, those where one began.
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttnParams p, const int kRows) {
-  __shared__ float tops[kJoinWarps], sums[kJoinWarps], part_o[kJoinWarps][D];
+__global__ void __launch_bounds__(kJoinThreads) kv_join_few_kernel(const __grid_constant__ AttnParams p, const int kRows) {
   depend_release();
   depend_wait();
   const int4 word = *reinterpret_cast<const int4*>(reinterpret_cast<const Piece*>(p.a.workspace) + blockIdx.x);
   const Piece piece = {word.x, word.y, word.z, word.w};
   if (piece.last < 0) return;
   const float* slots = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.a.workspace) + sizeof(Piece) * gridDim.x);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, count = piece.last - blockIdx.x + 1;
-  auto place = [&](int row) { return (piece.first + row / p.group) * p.a.stride_out_tok + (piece.head * p.group + row % p.group) * p.a.stride_out_head; };
+  const int lane = threadIdx.x % 32;
   Joined<D> r;
-  if (gridDim.y == 1) {
-    for (int row = warp; row < piece.rows; row += kJoinWarps) {
-      join_pieces<D>(slots, kRows, row, 0, 1, count, r);
+  for (int row = threadIdx.x / 32; row < piece.rows; row += kJoinWarps) {
+    join_pieces<D>(slots, kRows, row, blockIdx.x, 0, 1, piece.last - blockIdx.x + 1, r);
+    const long long at = (piece.first + row / p.group) * p.a.stride_out_tok + (piece.head * p.group + row % p.group) * p.a.stride_out_head;
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e)
-        store_from_float(p.a.out, place(row) + e * 32 + lane, p.a.dtype, r.sum == 0.0f ? 0.0f : __fdiv_rn(r.o[e], r.sum));
-    }
-    return;
+    for (int e = 0; e < D / 32; ++e)
+      store_from_float(p.a.out, at + e * 32 + lane, p.a.dtype, r.sum == 0.0f ? 0.0f : __fdiv_rn(r.o[e], r.sum));
   }
-  for (int row = blockIdx.y; row < piece.rows; row += gridDim.y) {
-    join_pieces<D>(slots, kRows, row, warp, kJoinWarps, count, r);
-    if (lane == 0) {
-      tops[warp] = r.top;
-      sums[warp] = r.sum;
-    }
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) part_o[warp][e * 32 + lane] = r.o[e];
-    __syncthreads();
-    float top = -INFINITY, sum = 0.0f, o = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float by = exp2_fast(tops[w] - base);
-      sum += sums[w] * by;
-      o = fmaf(part_o[w][threadIdx.x % D], by, o);
-    }
-    if (threadIdx.x < D) store_from_float(p.a.out, place(row) + threadIdx.x, p.a.dtype, sum == 0.0f ? 0.0f : __fdiv_rn(o, sum));
-    __syncthreads();
+}
+
+// One CTA to a row, for (request, head)s in many pieces: there are few of them then, so each finds its CTAs by counting
+// the tiles ahead of it on the line.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const __grid_constant__ AttnParams p, const int kRows, const int ctas) {
+  __shared__ float tops[kJoinWarps], sums[kJoinWarps], part_o[kJoinWarps][D];
+  depend_release();
+  depend_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, HKV = p.a.cache.HKV, b = blockIdx.x / HKV, h = blockIdx.x % HKV;
+  long long total = 0, ahead = 0;
+  int mine = 0;
+  for (int x = lane; x < p.a.rows.B; x += 32) {
+    const int tiles = tiles_of(p, x);
+    total += tiles;
+    if (x < b) ahead += tiles;
+    if (x == b) mine = tiles;
   }
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) {
+    total += __shfl_xor_sync(~0u, total, d);
+    ahead += __shfl_xor_sync(~0u, ahead, d);
+    mine += __shfl_xor_sync(~0u, mine, d);
+  }
+  if (mine == 0) return;
+  const long long share = (total * HKV + ctas - 1) / ctas, from = ahead * HKV + (long long)h * mine;
+  const int first = (int)(from / share), count = (int)((from + mine - 1) / share) - first + 1;
+  if (count == 1) return;                         // one CTA had all of it, and has written the output
+  const KvRequest q = kv_request(p.a.cache, p.a.rows, b, nullptr);
+  const int row = blockIdx.y;
+  if (row >= q.todo * p.group) return;
+  const float* slots = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.a.workspace) + sizeof(Piece) * ctas);
+  Joined<D> r;
+  join_pieces<D>(slots, kRows, row, first, warp, kJoinWarps, count, r);
+  if (lane == 0) {
+    tops[warp] = r.top;
+    sums[warp] = r.sum;
+  }
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) part_o[warp][e * 32 + lane] = r.o[e];
+  __syncthreads();
+  float top = -INFINITY, sum = 0.0f, o = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
+  const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float by = exp2_fast(tops[w] - base);
+    sum += sums[w] * by;
+    o = fmaf(part_o[w][threadIdx.x % D], by, o);
+  }
+  if (threadIdx.x < D)
+    store_from_float(p.a.out, (q.first + row / p.group) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + threadIdx.x, p.a.dtype,
+                     sum == 0.0f ? 0.0f : __fdiv_rn(o, sum));
 }
 
 // ---- many rows per request: one CTA for each 64 rows of a (request, head) -----------------------------------------------
@@ -1054,6 +1189,27 @@ long long decode_ctas(const CarryGdnKvAttentionArgs& a) {
   return most < 1 ? 1 : most < fit ? most : fit;
 }
 
+// launch_dependent() with clusters of kCluster CTAs, so many of them.
+template <class K, class... A>
+int launch_clusters(K kernel, int clusters, size_t smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)clusters * kCluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kCluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return CARRY_GDN_OK;
+  cudaGetLastError();
+  return CARRY_GDN_ERR_LAUNCH;
+}
+
 // Lets a kernel use `smem` bytes of shared memory: asked for once per device and thread.
 template <class K>
 int prepare(K kernel, size_t smem, bool (&ready)[64]) {
@@ -1067,17 +1223,28 @@ int prepare(K kernel, size_t smem, bool (&ready)[64]) {
   return CARRY_GDN_OK;
 }
 
+// Whether clusters take a call: all of them have to be resident, and a context be short enough for eight CTAs.  One
+// request of 1500 tokens and 8 heads takes 8.1 us so, 11.4 by the line; 4 x 4096 tokens PAIRTIME.
+bool by_pairs(const CarryGdnKvAttentionArgs& a) {
+  const long long tokens = (long long)a.cache.max_pages * a.cache.page, pairs = (long long)a.rows.B * a.cache.HKV;
+  return pairs * kCluster <= 2LL * sm_count() && tokens <= 4LL * kCluster * kLine;
+}
+
 template <int D, int NT, int PARTS>
 int launch_decode(const AttnParams& p, cudaStream_t stream) {
   constexpr size_t smem = sizeof(DecodeShared<D, NT, PARTS>);
+  static thread_local bool ready[2][64];
+  if (by_pairs(p.a)) {
+    const int rc = prepare(kv_pair_kernel<D, NT, PARTS>, smem, ready[0]);
+    return rc == CARRY_GDN_OK ? launch_clusters(kv_pair_kernel<D, NT, PARTS>, p.a.rows.B * p.a.cache.HKV, smem, stream, p) : rc;
+  }
   const unsigned ctas = (unsigned)decode_ctas(p.a);
-  static thread_local bool ready[64];
-  int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem, ready);
+  int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem, ready[1]);
   if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, NT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
   if (rc != CARRY_GDN_OK) return rc;
-  // a (request, head) lies in so many pieces: a warp to a row up to eight of them, a CTA to a row beyond
-  const long long pieces = ctas / ((long long)p.a.rows.B * p.a.cache.HKV);
-  return launch_dependent(kv_join_kernel<D>, dim3(ctas, pieces <= kBatch ? 1 : p.rows), kJoinThreads, 0, stream, p, NT * 8);
+  const long long pairs = (long long)p.a.rows.B * p.a.cache.HKV;
+  if (ctas <= kBatch * pairs) return launch_dependent(kv_join_few_kernel<D>, dim3(ctas), kJoinThreads, 0, stream, p, NT * 8);
+  return launch_dependent(kv_join_many_kernel<D>, dim3((unsigned)pairs, p.rows), kJoinThreads, 0, stream, p, NT * 8, (int)ctas);
 }
 
 // splits and padded rows of the kernel for many fp32 rows
@@ -1121,6 +1288,7 @@ int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a) {
     lay_out(a, splits, padded);
     return padded < 0 ? CARRY_GDN_ERR_TOO_LARGE : parts_bytes(a, splits, padded);
   }
+  if (by_pairs(a)) return 0;
   const long long ctas = decode_ctas(a);
   return sizeof(Piece) * ctas + 2 * ctas * slot_floats(tiles * 8, a.cache.D) * 4;
 }
