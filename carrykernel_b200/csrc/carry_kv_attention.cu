@@ -1178,7 +1178,7 @@ __global__ void __launch_bounds__(kThreads) kv_join_parts_kernel(const __grid_co
 // Tiles of eight query rows that a warp of the decode kernel holds, or 0 where the rows are too many for its registers.
 int column_tiles(const CarryGdnKvAttentionArgs& a) {
   const long long rows = (long long)a.rows.max_query * (a.HQ / a.cache.HKV);
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 && a.dtype != CARRY_F32 ? 4 : 0;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
 }
 
 // CTAs of the decode kernel: all that are resident at a time, or one per tile where there cannot be as many.
@@ -1270,10 +1270,7 @@ template <int D, int PARTS>
 int launch_by_rows(const AttnParams& p, int tiles, cudaStream_t stream) {
   if (tiles == 1) return launch_decode<D, 1, PARTS>(p, stream);
   if (tiles == 2) return launch_decode<D, 2, PARTS>(p, stream);
-  if constexpr (PARTS == 1) {
-    if (tiles == 4) return launch_decode<D, 4, PARTS>(p, stream);
-    return launch_kv_prefill(p, stream);
-  }
+  if constexpr (PARTS == 1) return launch_kv_prefill(p, stream);
   if constexpr (PARTS == 2) return launch_chunk<D, PARTS>(p, stream);
 }
 
