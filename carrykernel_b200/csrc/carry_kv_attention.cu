@@ -358,7 +358,6 @@ struct DecodeShared {
   RunStage<D> stage[kWarps][stages(D, NT, PARTS)];
   float merge[NT * 8][D + 4];
   float top[kWarps][NT * 8], sum[kWarps][NT * 8];
-  float pair_top[NT * 8], pair_sum[NT * 8];
 };
 
 __host__ __device__ constexpr long long slot_floats(int rows, int D) { return (long long)rows * (D + 2); }
@@ -714,15 +713,25 @@ __device__ __forceinline__ void merge_warps(DecodeShared<D, NT, PARTS>& sh, Runn
   __syncthreads();
 }
 
-// A (request, head) to a cluster of CTAs, which join through each other's shared memory: one launch, where the line's way
-// takes two.  For short contexts of few (request, head)s.
-constexpr int kCluster = 8;
+// A (request, head) to a cluster of eight CTAs: one launch, where the line's way takes two.  For short contexts of few
+// (request, head)s.  An eighth of the columns is each CTA's to join: all 32 warps of the cluster put what they have of it,
+// normalised, into its shared memory, and one barrier later it is done.  (Joining the warps of a CTA first and reading the
+// others' results afterwards took 2 us longer, of 7.6 for one token over 16.)
+constexpr int kCluster = 8, kSources = kCluster * kWarps;
 
 template <int D, int NT, int PARTS>
-__global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_pair_kernel(const __grid_constant__ AttnParams p) {
+struct PairShared {
+  RunStage<D> stage[kWarps][stages(D, NT, PARTS)];
+  alignas(16) float o[kSources][NT * 8][D / 8];
+  float top[kSources][NT * 8], sum[kSources][NT * 8];
+};
+
+template <int D, int NT, int PARTS>
+__global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t raw[];
-  DecodeShared<D, NT, PARTS>& sh = *reinterpret_cast<DecodeShared<D, NT, PARTS>*>(raw);
+  PairShared<D, NT, PARTS>& sh = *reinterpret_cast<PairShared<D, NT, PARTS>*>(raw);
   constexpr int kStages = stages(D, NT, PARTS);
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   depend_release();
   depend_wait();
   const CarryGdnKvCache& c = p.a.cache;
@@ -737,6 +746,8 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_pair_kern
   use.tile = rank;                                // tiles go round the cluster: neighbours read neighbouring pages
   Cursor load = use;
   RunPages pages = fetch_run(p, load);
+  Columns<D, NT, PARTS> q;                        // while the page ids are on their way
+  load_columns<D, NT, PARTS>(p, request, use.h, q);
   auto next_load = [&](int stage) {
     if (load.tile < load.tiles) {
       load_run<D>(p, sh.stage[warp][stage], load, pages);
@@ -747,9 +758,7 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_pair_kern
   };
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) next_load(s);
-  Columns<D, NT, PARTS> q;
   Running<D, NT> r;
-  load_columns<D, NT, PARTS>(p, request, use.h, q);
   r.clear();
   int stage = 0;
   for (; use.tile < use.tiles; use.tile += kCluster) {
@@ -770,45 +779,43 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_pair_kern
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
-  float top[NT][2], sum[NT][2];
-  merge_warps(sh, r, top, sum);
-  if (warp == 0 && g == 0) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sh.pair_top[8 * n + 2 * cc + i] = top[n][i];
-        sh.pair_sum[8 * n + 2 * cc + i] = sum[n][i];
-      }
-  }
+  // lane (g, c) has the columns that are CTA g's, of rows 8 n + 2 c and + 1
   const auto cluster = cooperative_groups::this_cluster();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // every CTA has started
+  PairShared<D, NT, PARTS>& theirs = *cluster.map_shared_rank(&sh, g);
+  const int source = rank * kWarps + warp;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 8 * n + 2 * cc + i;
+      float sum = r.sum[n][i];
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
+      theirs.top[source][row] = r.top[n][i];
+      theirs.sum[source][row] = sum;
+      const float w = sum == 0.0f ? 0.0f : __fdiv_rn(r.unit * exp2f(-kWeightUp), sum);
+      float4* to = reinterpret_cast<float4*>(theirs.o[source][row]);
+#pragma unroll
+      for (int m = 0; m < D / 16; m += 2)
+        to[m / 2] = make_float4(r.o[n][m][i] * w, r.o[n][m][i + 2] * w, r.o[n][m + 1][i] * w, r.o[n][m + 1][i + 2] * w);
+    }
   cluster.sync();
-  // the CTAs share out the output, eight columns of a row to a thread
-  for (int i = rank * kThreads + threadIdx.x; i < request.todo * p.group * (D / 8); i += kCluster * kThreads) {
-    const int row = i / (D / 8), col = i % (D / 8) * 8;
-    float tops[kCluster], sums[kCluster], most = -INFINITY, total = 0.0f;
-    alignas(16) float x[8] = {};
+  for (int i = threadIdx.x; i < request.todo * p.group * (D / 8); i += kThreads) {
+    const int row = i / (D / 8), col = i % (D / 8);
+    float top = -INFINITY, total = 0.0f, x = 0.0f;
 #pragma unroll
-    for (int n = 0; n < kCluster; ++n) {
-      tops[n] = *cluster.map_shared_rank(&sh.pair_top[row], n);
-      sums[n] = *cluster.map_shared_rank(&sh.pair_sum[row], n);
-      most = fmaxf(most, tops[n]);
-    }
-    const float base = most == -INFINITY ? 0.0f : most;
-#pragma unroll
-    for (int n = 0; n < kCluster; ++n) {
-      const float w = sums[n] * exp2_fast(tops[n] - base);
-      const float4* o = reinterpret_cast<const float4*>(cluster.map_shared_rank(&sh.merge[row][col], n));
-      const float4 u = o[0], v = o[1];
+    for (int n = 0; n < kSources; ++n) top = fmaxf(top, sh.top[n][row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll 8
+    for (int n = 0; n < kSources; ++n) {
+      const float w = sh.sum[n][row] * exp2_fast(sh.top[n][row] - base);
       total += w;
-      x[0] = fmaf(w, u.x, x[0]); x[1] = fmaf(w, u.y, x[1]); x[2] = fmaf(w, u.z, x[2]); x[3] = fmaf(w, u.w, x[3]);
-      x[4] = fmaf(w, v.x, x[4]); x[5] = fmaf(w, v.y, x[5]); x[6] = fmaf(w, v.z, x[6]); x[7] = fmaf(w, v.w, x[7]);
+      x = fmaf(w, sh.o[n][row][col], x);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = total == 0.0f ? 0.0f : __fdiv_rn(x[e], total);
-    store8(p.a.out, (request.first + row / p.group) * p.a.stride_out_tok + (use.h * p.group + row % p.group) * p.a.stride_out_head + col, p.a.dtype, x);
+    store_from_float(p.a.out, (request.first + row / p.group) * p.a.stride_out_tok + (use.h * p.group + row % p.group) * p.a.stride_out_head + rank * (D / 8) + col,
+                     p.a.dtype, total == 0.0f ? 0.0f : __fdiv_rn(x, total));
   }
-  cluster.sync();                                 // nobody leaves while its memory is read
 }
 
 template <int D, int NT, int PARTS>
@@ -1232,11 +1239,11 @@ bool by_pairs(const CarryGdnKvAttentionArgs& a) {
 
 template <int D, int NT, int PARTS>
 int launch_decode(const AttnParams& p, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(DecodeShared<D, NT, PARTS>);
+  constexpr size_t smem = sizeof(DecodeShared<D, NT, PARTS>), pair_smem = sizeof(PairShared<D, NT, PARTS>);
   static thread_local bool ready[2][64];
   if (by_pairs(p.a)) {
-    const int rc = prepare(kv_pair_kernel<D, NT, PARTS>, smem, ready[0]);
-    return rc == CARRY_GDN_OK ? launch_clusters(kv_pair_kernel<D, NT, PARTS>, p.a.rows.B * p.a.cache.HKV, smem, stream, p) : rc;
+    const int rc = prepare(kv_pair_kernel<D, NT, PARTS>, pair_smem, ready[0]);
+    return rc == CARRY_GDN_OK ? launch_clusters(kv_pair_kernel<D, NT, PARTS>, p.a.rows.B * p.a.cache.HKV, pair_smem, stream, p) : rc;
   }
   const unsigned ctas = (unsigned)decode_ctas(p.a);
   int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem, ready[1]);
