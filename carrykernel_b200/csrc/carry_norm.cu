@@ -57,146 +57,245 @@ __device__ __forceinline__ Eight load_slow(const void* p, long long at, int n, i
 __host__ __device__ constexpr int max_threads(int C) { return C == 1 ? 128 : 512; }
 __host__ __device__ constexpr int min_ctas(int C) { return C == 1 ? 8 : C == 2 ? 2 : 1; }
 
-// C chunks of 8 columns per thread, chunk j of thread t being number j * blockDim + t of the row.  VEC: x is of type X,
-// the residual of type R, every row starts on a 16-byte boundary and W is a multiple of 8; otherwise X and R say nothing.
-template <int C, bool VEC, int X, int R>
+// The reduction of a row across its warps, and what comes of it.
+struct RowSums {
+  float2 part[2][kMaxWarps];      // sum of squares and largest |t| of a warp; the sum is NaN where squares left its range
+  float sum[2][kMaxWarps], large[2][kMaxWarps];
+};
+struct RowScale {
+  float rstd, top;                // rstd is NaN where a number of the row is not finite
+};
+__device__ __forceinline__ RowScale reduce_row(const NormParams& p, RowSums& sh, int turn, float sum, float large, float top) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+#pragma unroll
+  for (int s = 16; s > 0; s /= 2) sum += __shfl_xor_sync(~0u, sum, s);
+  top = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top)));  // no NaNs, not negative: ordered as whole numbers
+  const bool out = __any_sync(~0u, large != 0.0f);
+  if (out) {
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) large += __shfl_xor_sync(~0u, large, s);
+  }
+  if (lane == 0) {
+    sh.part[turn][warp] = make_float2(out ? NAN : sum, top);
+    sh.sum[turn][warp] = sum;
+    sh.large[turn][warp] = large;
+  }
+  __syncthreads();                // the next row has the other half: one barrier a row
+  sum = 0.0f;
+  for (int i = 0; i < warps; ++i) {
+    const float2 x = sh.part[turn][i];
+    sum += x.x;
+    top = fmaxf(top, x.y);
+  }
+  float rstd = rsqrtf(fmaf(sum, p.inv_width, p.a.eps));
+  if (sum != sum) {
+    sum = large = 0.0f;
+    for (int i = 0; i < warps; ++i) {
+      sum += sh.sum[turn][i];
+      large += sh.large[turn][i];
+    }
+    rstd = large < INFINITY ? rsqrtf(fmaf(sum, 0x1p-128f, large) * p.inv_width) * 0x1p-64f : NAN;
+  }
+  return {top < INFINITY ? rstd : NAN, top};
+}
+
+// Sum of the squares of eight numbers; from kLarge on it counts in `large`, times 2^-128 (NaNs do, too).
+__device__ __forceinline__ void add_squares(const Eight& t, float2& ss, float& large) {
+  float2 part = mul2(t.x[0], t.x[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) part = fma2(t.x[i], t.x[i], part);
+  if (part.x + part.y < kLarge) {
+    ss = add2(ss, part);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float u = t.x[i].x * 0x1p-64f, v = t.x[i].y * 0x1p-64f;
+      large += u * u + v * v;
+    }
+  }
+}
+// t * weight, and its largest magnitude
+__device__ __forceinline__ float weigh(Eight& t, const Eight& w) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t.x[i] = mul2(t.x[i], w.x[i]);
+    top = fmaxf(top, fmaxf(fabsf(t.x[i].x), fabsf(t.x[i].y)));
+  }
+  return top;
+}
+__device__ __forceinline__ uint2 codes_of(const Eight& t, float by) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = __nv_cvt_float2_to_fp8x2(mul2(t.x[i], make_float2(by, by)), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+}
+// The scale of a row or a group, whose largest |t| is `top`, and what t is multiplied by.
+__device__ __forceinline__ float scale_of(const RowScale& r, float top, float& by) {
+  const float scale = fmaxf(top * r.rstd, kAmaxFloor) * (1.0f / kF8Max);      // fmaxf drops a NaN
+  by = r.rstd == r.rstd ? __fdividef(r.rstd, scale) : NAN;
+  return r.rstd == r.rstd ? scale : NAN;
+}
+__device__ __forceinline__ float group_max(float top) {                       // 16 neighbouring lanes have a group
+#pragma unroll
+  for (int s = 8; s > 0; s /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+  return top;
+}
+
+// C chunks of 8 columns per thread, chunk j of thread t being number j * blockDim + t of the row; x is of type X, the
+// residual of type R, every row starts on a 16-byte boundary and W is a multiple of 8.
+template <int C, int X, int R>
 __global__ void __launch_bounds__(max_threads(C), min_ctas(C)) norm_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float sums[2][kMaxWarps], larges[2][kMaxWarps], tops[2][kMaxWarps];
+  __shared__ RowSums sums;
   constexpr bool kAhead = C <= 4;                 // more would not fit the registers
+  constexpr int kX = X == CARRY_F32 ? 4 : 2, kR = R == CARRY_F32 ? 4 : 2;
   depend_release();
   depend_wait();
   const CarryGdnNormArgs& a = p.a;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, groups = (a.W + kGroup - 1) / kGroup;
+  const int lane = threadIdx.x % 32, groups = (a.W + kGroup - 1) / kGroup, first = threadIdx.x * 8, jump = blockDim.x * 8;
   const bool has_residual = a.residual != nullptr;
+  // this thread's first chunk of the CTA's next row to load, and of the present one
+  const long long row0 = blockIdx.x, rows = gridDim.x;
+  const char* x = static_cast<const char*>(a.x) + (row0 * a.stride_x + first) * kX;
+  const char* r = static_cast<const char*>(a.residual) + (row0 * a.stride_residual + first) * kR;
+  char* out = static_cast<char*>(a.residual_out) + (row0 * a.stride_residual_out + first) * kR;
+  uint8_t* codes = a.codes + row0 * a.stride_codes + first;
+  float* scales = a.scale + row0 * (a.group ? groups : 1);
   Raw<X> next_x[C];
   Raw<R> next_r[C];
-  auto fetch = [&](long long row) {
-    if (!VEC || row >= a.N) return;
-    const long long x_row = row * a.stride_x, r_row = row * a.stride_residual;
+  auto fetch = [&](bool there) {
+    if (there) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        if (first + j * jump >= a.W) continue;
+        next_x[j] = load_raw<X>(x, j * jump);
+        if (has_residual) next_r[j] = load_raw<R>(r, j * jump);
+      }
+    }
+    x += rows * a.stride_x * kX;
+    r += rows * a.stride_residual * kR;
+  };
+  if (kAhead) fetch(row0 < a.N);
+  int turn = 0;
+  for (long long row = row0; row < a.N; row += rows, turn ^= 1) {
+    Eight t[C];
+    float2 ss = make_float2(0.0f, 0.0f);
+    float large = 0.0f, top[C], all = 0.0f;
+    if (!kAhead) fetch(true);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      const int at = (j * blockDim.x + threadIdx.x) * 8;
-      if (at >= a.W) continue;
-      next_x[j] = load_raw<X>(a.x, x_row + at);
-      if (has_residual) next_r[j] = load_raw<R>(a.residual, r_row + at);
+      t[j] = unpack<X>(next_x[j]);
+      if (has_residual) {
+        const Eight add = unpack<R>(next_r[j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[j].x[i] = add2(t[j].x[i], add.x[i]);
+      }
     }
-  };
-  if (kAhead) fetch(blockIdx.x);
+    if (kAhead) fetch(row + rows < a.N);          // in flight while this row is reduced
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int at = first + j * jump;
+      top[j] = 0.0f;
+      if (at >= a.W) continue;
+      if (a.residual_out) store<R>(out, j * jump, t[j]);
+      add_squares(t[j], ss, large);
+      if (a.weight_dtype == X) top[j] = weigh(t[j], unpack<X>(load_raw<X>(a.weight, at)));
+      else if (a.weight_dtype == CARRY_F32) top[j] = weigh(t[j], unpack<CARRY_F32>(load_raw<CARRY_F32>(a.weight, at)));
+      else top[j] = weigh(t[j], load_slow(a.weight, at, 8, a.weight_dtype));
+      all = fmaxf(all, top[j]);
+    }
+    const RowScale s = reduce_row(p, sums, turn, ss.x + ss.y, large, all);
+    if (a.group == 0) {
+      float by;
+      const float scale = scale_of(s, s.top, by);
+      if (threadIdx.x == 0) *scales = scale;
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if (first + j * jump < a.W) *reinterpret_cast<uint2*>(codes + j * jump) = codes_of(t[j], by);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int at = first + j * jump;
+        float by;
+        const float scale = scale_of(s, group_max(top[j]), by);
+        if (at >= a.W) continue;
+        if (lane % 16 == 0) scales[at / kGroup] = scale;
+        *reinterpret_cast<uint2*>(codes + j * jump) = codes_of(t[j], by);
+      }
+    }
+    out += rows * a.stride_residual_out * kR;
+    codes += rows * a.stride_codes;
+    scales += rows * (a.group ? groups : 1);
+  }
+}
+
+// The same a number at a time, for rows that are not aligned and for types that have no kernel of their own.
+template <int C>
+__global__ void __launch_bounds__(512) norm_slow_kernel(const __grid_constant__ NormParams p) {
+  __shared__ RowSums sums;
+  depend_release();
+  depend_wait();
+  const CarryGdnNormArgs& a = p.a;
+  const int lane = threadIdx.x % 32, groups = (a.W + kGroup - 1) / kGroup;
   int turn = 0;
   for (long long row = blockIdx.x; row < a.N; row += gridDim.x, turn ^= 1) {
     Eight t[C];
     float2 ss = make_float2(0.0f, 0.0f);
     float large = 0.0f, top[C], all = 0.0f;
-    if (!kAhead) fetch(row);
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int at = (j * blockDim.x + threadIdx.x) * 8, n = min(a.W - at, 8);
-      if (n <= 0) continue;
-      if constexpr (VEC) t[j] = unpack<X>(next_x[j]);
-      else t[j] = load_slow(a.x, row * a.stride_x + at, n, a.x_dtype);
-      if (has_residual) {
-        Eight r;
-        if constexpr (VEC) r = unpack<R>(next_r[j]);
-        else r = load_slow(a.residual, row * a.stride_residual + at, n, a.residual_dtype);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[j].x[i] = add2(t[j].x[i], r.x[i]);
-      }
-    }
-    if (kAhead) fetch(row + gridDim.x);           // in flight while this row is reduced
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int at = (j * blockDim.x + threadIdx.x) * 8, n = min(a.W - at, 8);
       top[j] = 0.0f;
       if (n <= 0) continue;
-      Eight w;
-      if constexpr (VEC) {
-        if (a.residual_out) store<R>(a.residual_out, row * a.stride_residual_out + at, t[j]);
-        if (a.weight_dtype == X) w = unpack<X>(load_raw<X>(a.weight, at));
-        else if (a.weight_dtype == CARRY_F32) w = unpack<CARRY_F32>(load_raw<CARRY_F32>(a.weight, at));
-        else w = load_slow(a.weight, at, 8, a.weight_dtype);
-      } else {
-        w = load_slow(a.weight, at, n, a.weight_dtype);
-        if (a.residual_out) {
+      t[j] = load_slow(a.x, row * a.stride_x + at, n, a.x_dtype);
+      if (a.residual) {
+        const Eight add = load_slow(a.residual, row * a.stride_residual + at, n, a.residual_dtype);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < n) store_from_float(a.residual_out, row * a.stride_residual_out + at + i, a.residual_dtype, i % 2 ? t[j].x[i / 2].y : t[j].x[i / 2].x);
-        }
+        for (int i = 0; i < 4; ++i) t[j].x[i] = add2(t[j].x[i], add.x[i]);
       }
-      float2 part = mul2(t[j].x[0], t[j].x[0]);
+      if (a.residual_out) {
 #pragma unroll
-      for (int i = 1; i < 4; ++i) part = fma2(t[j].x[i], t[j].x[i], part);
-      if (part.x + part.y < kLarge) {
-        ss = add2(ss, part);
-      } else {                                    // NaNs come here too
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = t[j].x[i].x * 0x1p-64f, v = t[j].x[i].y * 0x1p-64f;
-          large += u * u + v * v;
-        }
+        for (int i = 0; i < 8; ++i)
+          if (i < n) store_from_float(a.residual_out, row * a.stride_residual_out + at + i, a.residual_dtype, i % 2 ? t[j].x[i / 2].y : t[j].x[i / 2].x);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        t[j].x[i] = mul2(t[j].x[i], w.x[i]);
-        top[j] = fmaxf(top[j], fmaxf(fabsf(t[j].x[i].x), fabsf(t[j].x[i].y)));
-      }
+      add_squares(t[j], ss, large);
+      top[j] = weigh(t[j], load_slow(a.weight, at, n, a.weight_dtype));
       all = fmaxf(all, top[j]);
     }
-    float sum = ss.x + ss.y;
-#pragma unroll
-    for (int s = 16; s > 0; s /= 2) sum += __shfl_xor_sync(~0u, sum, s);
-    all = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(all)));   // no NaNs, not negative: ordered as whole numbers
-    if (__any_sync(~0u, large != 0.0f)) {
-#pragma unroll
-      for (int s = 16; s > 0; s /= 2) large += __shfl_xor_sync(~0u, large, s);
-    }
-    if (lane == 0) { sums[turn][warp] = sum; larges[turn][warp] = large; tops[turn][warp] = all; }
-    __syncthreads();              // the next row has the other half: one barrier a row
-    sum = large = 0.0f;
-    for (int i = 0; i < warps; ++i) { sum += sums[turn][i]; large += larges[turn][i]; all = fmaxf(all, tops[turn][i]); }
-    const bool finite = large < INFINITY && all < INFINITY;
-    float rstd = large == 0.0f ? rsqrtf(fmaf(sum, p.inv_width, a.eps)) : rsqrtf(fmaf(sum, 0x1p-128f, large) * p.inv_width) * 0x1p-64f;
-    if (!finite) rstd = __uint_as_float(0x7fffffffu);
-    float scale = fmaxf(all * rstd, kAmaxFloor) * (1.0f / kF8Max), mul = __fdividef(rstd, scale);
-    if (a.group == 0 && threadIdx.x == 0) a.scale[row] = finite ? scale : rstd;
+    const RowScale s = reduce_row(p, sums, turn, ss.x + ss.y, large, all);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int at = (j * blockDim.x + threadIdx.x) * 8, n = min(a.W - at, 8);
-      if (a.group) {              // 16 neighbouring lanes have a group
-#pragma unroll
-        for (int s = 8; s > 0; s /= 2) top[j] = fmaxf(top[j], __shfl_xor_sync(~0u, top[j], s));
-        scale = fmaxf(top[j] * rstd, kAmaxFloor) * (1.0f / kF8Max);
-        mul = __fdividef(rstd, scale);
-        if (n > 0 && lane % 16 == 0) a.scale[row * groups + at / kGroup] = finite ? scale : rstd;
-      }
+      float by;
+      const float scale = scale_of(s, a.group ? group_max(top[j]) : s.top, by);
       if (n <= 0) continue;
-      const float2 by = finite ? make_float2(mul, mul) : make_float2(rstd, rstd);
-      uint32_t c[4];
+      if (a.group && lane % 16 == 0) a.scale[row * groups + at / kGroup] = scale;
+      if (!a.group && at == 0) a.scale[row] = scale;
+      const uint2 c = codes_of(t[j], by);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = __nv_cvt_float2_to_fp8x2(mul2(t[j].x[i], by), __NV_SATFINITE, __NV_E4M3);
-      uint8_t* to = a.codes + row * a.stride_codes + at;
-      if constexpr (VEC) {
-        *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n) to[i] = static_cast<uint8_t>(c[i / 2] >> (i % 2 * 8));
-      }
+      for (int i = 0; i < 8; ++i)
+        if (i < n) a.codes[row * a.stride_codes + at + i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (i % 4 * 8));
     }
   }
 }
 
-template <bool VEC, int X, int R>
-int launch_typed(const NormParams& p, cudaStream_t stream) {
+template <class K>
+int launch_rows(K kernel, const NormParams& p, int c, cudaStream_t stream) {
   const int chunks = (p.a.W + 7) / 8;
-  auto launch = [&](auto kernel, int c) {
-    const unsigned threads = (chunks + 32 * c - 1) / (32 * c) * 32;
-    const long long resident = (long long)sm_count() * (max_threads(c) * min_ctas(c) / threads);
-    return launch_dependent(kernel, dim3((unsigned)(p.a.N < resident ? p.a.N : resident)), threads, 0, stream, p);
-  };
-  if (chunks <= 128) return launch(norm_kernel<1, VEC, X, R>, 1);
-  if (chunks <= 1024) return launch(norm_kernel<2, VEC, X, R>, 2);
-  if (chunks <= 2048) return launch(norm_kernel<4, VEC, X, R>, 4);
-  return launch(norm_kernel<8, VEC, X, R>, 8);
+  const unsigned threads = (chunks + 32 * c - 1) / (32 * c) * 32;
+  const long long resident = (long long)sm_count() * (max_threads(c) * min_ctas(c) / threads);
+  return launch_dependent(kernel, dim3((unsigned)(p.a.N < resident ? p.a.N : resident)), threads, 0, stream, p);
+}
+template <int X, int R>
+int launch_typed(const NormParams& p, cudaStream_t stream) {
+  if (p.a.W <= 1024) return launch_rows(norm_kernel<1, X, R>, p, 1, stream);
+  if (p.a.W <= 8192) return launch_rows(norm_kernel<2, X, R>, p, 2, stream);
+  if (p.a.W <= 16384) return launch_rows(norm_kernel<4, X, R>, p, 4, stream);
+  return launch_rows(norm_kernel<8, X, R>, p, 8, stream);
+}
+int launch_slow(const NormParams& p, cudaStream_t stream) {
+  if (p.a.W <= 1024) return launch_rows(norm_slow_kernel<1>, p, 1, stream);
+  return p.a.W <= 8192 ? launch_rows(norm_slow_kernel<2>, p, 2, stream) : launch_rows(norm_slow_kernel<8>, p, 8, stream);
 }
 
 }  // namespace
@@ -216,12 +315,12 @@ int launch_norm(const CarryGdnNormArgs& a, cudaStream_t stream) {
   rows(a.codes, a.stride_codes, 1, 8);
   // the residual stream has x's type or is fp32; other pairs go an element at a time
   const int xd = a.x_dtype, rd = a.residual_dtype;
-  if (vec && xd == CARRY_BF16 && rd == CARRY_BF16) return launch_typed<true, CARRY_BF16, CARRY_BF16>(p, stream);
-  if (vec && xd == CARRY_F16 && rd == CARRY_F16) return launch_typed<true, CARRY_F16, CARRY_F16>(p, stream);
-  if (vec && xd == CARRY_F32 && rd == CARRY_F32) return launch_typed<true, CARRY_F32, CARRY_F32>(p, stream);
-  if (vec && xd == CARRY_BF16 && rd == CARRY_F32) return launch_typed<true, CARRY_BF16, CARRY_F32>(p, stream);
-  if (vec && xd == CARRY_F16 && rd == CARRY_F32) return launch_typed<true, CARRY_F16, CARRY_F32>(p, stream);
-  return launch_typed<false, CARRY_F32, CARRY_F32>(p, stream);
+  if (vec && xd == CARRY_BF16 && rd == CARRY_BF16) return launch_typed<CARRY_BF16, CARRY_BF16>(p, stream);
+  if (vec && xd == CARRY_F16 && rd == CARRY_F16) return launch_typed<CARRY_F16, CARRY_F16>(p, stream);
+  if (vec && xd == CARRY_F32 && rd == CARRY_F32) return launch_typed<CARRY_F32, CARRY_F32>(p, stream);
+  if (vec && xd == CARRY_BF16 && rd == CARRY_F32) return launch_typed<CARRY_BF16, CARRY_F32>(p, stream);
+  if (vec && xd == CARRY_F16 && rd == CARRY_F32) return launch_typed<CARRY_F16, CARRY_F32>(p, stream);
+  return launch_slow(p, stream);
 }
 
 }  // namespace carry
