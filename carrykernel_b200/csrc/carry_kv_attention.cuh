@@ -1,10 +1,13 @@
 // What the kernels of the key/value attention share: parameters, pages, rows to memory.
 #pragma once
 
+#include <cuda_pipeline_primitives.h>
+
 #include "carry_hybrid.cuh"
 
 namespace carry {
 
+constexpr float kWeightUp = 15.0f;                // where products are formed in registers, weights are formed times 2^15
 constexpr int kGranule = 16;                      // tokens: no page and no block of a scale begins or ends inside
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoTokens = -1.0f;                // in a key scale's place: a padding page, or past the end
@@ -92,6 +95,84 @@ __device__ __forceinline__ void store8(void* out, long long at, int dtype, const
   *to = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+__device__ __forceinline__ void mma_fp16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+  return fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+  return x;
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  x += __shfl_xor_sync(~0u, x, 1);
+  return x + __shfl_xor_sync(~0u, x, 2);
+}
+
+// Where the 16-byte chunk `chunk` of token `row` lies in a tile.  The lanes that read together then fall into different
+// banks both ways: a quad of lanes reads one token's chunks (keys), or the same chunk of every second token (values).
+template <int D>
+__device__ __forceinline__ int tile_at(int row, int chunk) {
+  if constexpr (D == 128) return (row * 8 + (chunk ^ (row & 6) ^ (row & 1) << 2)) * 16;
+  const int line = row >> 1;
+  return (line * 8 + (((row & 1) << 2 | chunk) ^ (line & 3) << 1)) * 16;
+}
+
+// This lane's share of a query row, in one trip to memory: of every 64 columns the 16 from 16 c on.  (One element at a
+// time, with its type asked for each, every load would wait for the conversion of the one before.)
+template <int D, int PARTS>
+__device__ __forceinline__ void load_share(const AttnParams& p, long long at, bool there, float (&x)[D / 4]) {
+  const int c = threadIdx.x % 4;
+  if constexpr (PARTS == 2) {
+    const float* q = reinterpret_cast<const float*>(p.a.q) + at + c * 16;
+#pragma unroll
+    for (int e = 0; e < D / 4; ++e) x[e] = there ? q[e / 16 * 64 + e % 16] : 0.0f;
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p.a.q) + at + c * 16;
+    uint32_t w[D / 8] = {};
+    if (there && reinterpret_cast<uintptr_t>(q) % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(q + i / 2 * 64 + i % 2 * 8);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+      }
+    } else if (there) {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) w[i] = q[i / 8 * 64 + i % 8 * 2] | static_cast<uint32_t>(q[i / 8 * 64 + i % 8 * 2 + 1]) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const float2 f = p.a.dtype == CARRY_BF16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)) : unpack_half2(w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// Lets a kernel use `smem` bytes of shared memory: asked for once per device and thread.
+template <class K>
+int prepare(K kernel, size_t smem, bool (&ready)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev < 64 && ready[dev]) return CARRY_GDN_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return CARRY_GDN_ERR_LAUNCH;
+  }
+  if (dev < 64) ready[dev] = true;
+  return CARRY_GDN_OK;
+}
+
+// few rows of a request; many; many fp32 rows
+bool few_rows(const CarryGdnKvAttentionArgs& a);
+int launch_kv_decode(const AttnParams& p, cudaStream_t stream);
+int64_t kv_decode_workspace(const CarryGdnKvAttentionArgs& a);
+int launch_kv_chunk(AttnParams p, cudaStream_t stream);
+int64_t kv_chunk_workspace(const CarryGdnKvAttentionArgs& a);
 int launch_kv_prefill(AttnParams p, cudaStream_t stream);
 int64_t kv_prefill_workspace(const CarryGdnKvAttentionArgs& a);
 
