@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_parts_kernel(const __gri
   depend_release();
   depend_wait();
   const int lane = threadIdx.x % 32, row = blockIdx.y * kJoinWarps + threadIdx.x / 32;
-  const int b = blockIdx.x / p.a.cache.HKV, h = blockIdx.x % p.a.cache.HKV, i = row / p.group;
+  const int b = blockIdx.x / p.a.cache.HKV, h = blockIdx.x % p.a.cache.HKV, i = token_of(p, row);
   const KvRequest q = kv_request(p.a.cache, p.a.rows, b, nullptr);
   if (i >= q.todo) return;
   const Parts mine = parts_of(p, min(lane, p.splits - 1), blockIdx.x);
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_parts_kernel(const __gri
   }
 #pragma unroll
   for (int e = 0; e < D / 32; ++e)
-    store_from_float(p.a.out, (q.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + e * 32 + lane, p.a.dtype,
+    store_from_float(p.a.out, row_place(p, q, h, row, i, p.a.stride_out_tok, p.a.stride_out_head) + e * 32 + lane, p.a.dtype,
                      sum == 0.0f ? 0.0f : __fdiv_rn(o[e], sum));
 }
 
@@ -69,6 +69,7 @@ int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream) {
   p.group = a.HQ / a.cache.HKV;
   p.page_granules = a.cache.page / kGranule;
   p.block_granules = a.cache.block / kGranule;
+  p.group_shift = shift_of(p.group);
   p.page_shift = shift_of(p.page_granules);
   p.block_shift = shift_of(p.block_granules);
   p.rows = a.rows.max_query * p.group;

@@ -14,7 +14,7 @@ constexpr float kNoTokens = -1.0f;                // in a key scale's place: a p
 
 struct AttnParams {
   CarryGdnKvAttentionArgs a;
-  int group;                      // query heads per key/value head
+  int group, group_shift;         // query heads per key/value head, and its logarithm or -1
   int page_granules, page_shift;  // granules in a page, and its logarithm or -1
   int block_granules, block_shift;
   int rows;                       // rows of a (request, head): most that may be in use
@@ -59,6 +59,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// a (request, head)'s row: number of its query token, and where it lies in q or out
+__device__ __forceinline__ int token_of(const AttnParams& p, int row) { return divide(row, p.group, p.group_shift); }
+__device__ __forceinline__ long long row_place(const AttnParams& p, const KvRequest& r, int h, int row, int token, long long stride_tok, long long stride_head) {
+  return (r.first + token) * stride_tok + (h * p.group + row - token * p.group) * stride_head;
+}
 __device__ __forceinline__ int page_index(const AttnParams& p, int granule) { return divide(granule, p.page_granules, p.page_shift); }
 __device__ __forceinline__ int page_id(const AttnParams& p, int b, int granule, int length) {
   if (granule * kGranule >= length) return 0;

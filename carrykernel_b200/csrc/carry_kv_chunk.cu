@@ -79,9 +79,9 @@ __device__ __forceinline__ void load_query(const AttnParams& p, const KvRequest&
   const int lane = threadIdx.x % 32, g = lane / 4;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int row = row0 + g + half * 8, i = row / p.group;
+    const int row = row0 + g + half * 8, i = token_of(p, row);
     const bool there = i < r.todo;
-    const long long at = there ? (r.first + i) * p.a.stride_q_tok + (h * p.group + row % p.group) * p.a.stride_q_head : 0;
+    const long long at = there ? row_place(p, r, h, row, i, p.a.stride_q_tok, p.a.stride_q_head) : 0;
     float x[D / 4];
     uint32_t top = 0;
     load_share<D, PARTS>(p, at, there, x);
@@ -234,9 +234,9 @@ __device__ __forceinline__ void store_rows(const AttnParams& p, const KvRequest&
   const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int row = row0 + g + half * 8, i = row / p.group;
+    const int row = row0 + g + half * 8, i = token_of(p, row);
     if (i >= q.todo) continue;
-    const long long at = (q.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + c * (D / 4);
+    const long long at = row_place(p, q, h, row, i, p.a.stride_out_tok, p.a.stride_out_head) + c * (D / 4);
 #pragma unroll
     for (int e = 0; e < D / 4; e += 8) {
       alignas(16) float x[8];
@@ -252,7 +252,7 @@ __device__ __forceinline__ void row_limits(const AttnParams& p, const KvRequest&
   const int g = threadIdx.x % 32 / 4;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int i = (row0 + g + half * 8) / p.group;
+    const int i = token_of(p, row0 + g + half * 8);
     limit[half] = i < q.todo ? q.length - q.count + i + 1 - tile * kTile : 0;
   }
 }
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constan
   const KvRequest q = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
   if (first_row >= q.todo * p.group) return;
   const int row0 = first_row + threadIdx.x / 32 * kRowsPerWarp;
-  const int last = min((first_row + kChunkRows - 1) / p.group, q.todo - 1);
+  const int last = min(token_of(p, first_row + kChunkRows - 1), q.todo - 1);
   const int length = max(min(q.length, q.length - q.count + last + 1), 0), all_tiles = (length + kTile - 1) / kTile;
   const int share = (all_tiles + p.splits - 1) / p.splits, tile0 = min(share * (int)blockIdx.z, all_tiles), tiles = min(share, all_tiles - tile0);
   Pages<D> ids;

@@ -156,9 +156,9 @@ __device__ __forceinline__ void load_columns(const AttnParams& p, const KvReques
   const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int row = 8 * n + g, i = row / p.group;
+    const int row = 8 * n + g, i = token_of(p, row);
     const bool there = i < r.todo;
-    const long long at = there ? (r.first + i) * p.a.stride_q_tok + (h * p.group + row % p.group) * p.a.stride_q_head : 0;
+    const long long at = there ? row_place(p, r, h, row, i, p.a.stride_q_tok, p.a.stride_q_head) : 0;
     float x[D / 4];
     uint32_t top = 0;
     load_share<D, PARTS>(p, at, there, x);
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int x = (8 * n + 2 * cc + i) / p.group;
+          const int x = token_of(p, 8 * n + 2 * cc + i);
           limit[n][i] = (x < request.todo ? request.length - request.count + x + 1 : 0) - start;
         }
       attend_run<D, NT, PARTS>(sh.stage[warp][stage], q, limit, start + kRun <= request.length - request.count + 1, r);
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
       total += w;
       x = fmaf(w, sh.o[n][row][col], x);
     }
-    store_from_float(p.a.out, (request.first + row / p.group) * p.a.stride_out_tok + (use.h * p.group + row % p.group) * p.a.stride_out_head + rank * (D / 8) + col,
+    store_from_float(p.a.out, row_place(p, request, use.h, row, token_of(p, row), p.a.stride_out_tok, p.a.stride_out_head) + rank * (D / 8) + col,
                      p.a.dtype, total == 0.0f ? 0.0f : __fdiv_rn(x, total));
   }
 }
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_ke
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int x = (8 * n + 2 * cc + i) / p.group;
+          const int x = token_of(p, 8 * n + 2 * cc + i);
           sees[n][i] = x < request.todo ? request.length - request.count + x + 1 : 0;
         }
       first_tile = use.tile;
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, resident(D, NT, PARTS)) kv_decode_ke
         *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(&sh.merge[row][col]);
         *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(&sh.merge[row][col + 4]);
         if (whole) {
-          store8(p.a.out, (request.first + row / p.group) * p.a.stride_out_tok + (use.h * p.group + row % p.group) * p.a.stride_out_head + col,
+          store8(p.a.out, row_place(p, request, use.h, row, token_of(p, row), p.a.stride_out_tok, p.a.stride_out_head) + col,
                  p.a.dtype, x);
         } else {
           store8(slot, 2 * kRows + row * D + col, CARRY_F32, x);
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const __grid
     o = fmaf(part_o[w][threadIdx.x % D], by, o);
   }
   if (threadIdx.x < D)
-    store_from_float(p.a.out, (q.first + row / p.group) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head + threadIdx.x, p.a.dtype,
+    store_from_float(p.a.out, row_place(p, q, h, row, token_of(p, row), p.a.stride_out_tok, p.a.stride_out_head) + threadIdx.x, p.a.dtype,
                      sum == 0.0f ? 0.0f : __fdiv_rn(o, sum));
 }
 

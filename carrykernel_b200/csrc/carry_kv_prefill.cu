@@ -118,6 +118,11 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // 32 columns of a warp's 32 rows, a row to a lane
 __device__ __forceinline__ void tmem_load(uint32_t at, float (&x)[32]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(x);
@@ -148,44 +153,86 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16
 // where the 16-byte chunk `chunk` (eight numbers) of a row of a plane lies
 __device__ __forceinline__ int plane_at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
-// A query row as fp16, scaled by a power of two, into its tile; what a product of it counts, in log2's scale.
+// Where a row lies, or null for one that is not there.  Each lane works out its own row's place (that takes some forty
+// instructions), and D / 8 or eight lanes that have a row between them get it from there.
+template <class T>
+__device__ __forceinline__ T* place_of(T* mine, int row) {
+  return reinterpret_cast<T*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(mine), row));
+}
+
+// A warp's 32 query rows as fp16, scaled by powers of two, into their tile; returns what a product of this lane's row
+// counts, in log2's scale.  Rows come in whole lines of memory, and each lane then has a row, in place.
 template <int D>
-__device__ __forceinline__ float stage_query(const AttnParams& p, const KvRequest& r, int h, int row, uint8_t (*tile)[kRowPlane], int tile_row) {
-  const int i = row / p.group;
-  const bool there = i < r.todo;
-  const uint16_t* q = reinterpret_cast<const uint16_t*>(p.a.q) +
-                      (there ? (r.first + i) * p.a.stride_q_tok + (h * p.group + row % p.group) * p.a.stride_q_head : 0);
-  const bool vec = reinterpret_cast<uintptr_t>(q) % 16 == 0;
-  const bool bf16 = p.a.dtype == CARRY_BF16;
-  uint32_t top = 0, w[D / 2];
-#pragma unroll
-  for (int c = 0; c < D / 8; ++c) {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (there && vec) {
-      u = *reinterpret_cast<const uint4*>(q + c * 8);
-    } else if (there) {
-      auto two = [&](int e) { return q[c * 8 + e] | static_cast<uint32_t>(q[c * 8 + e + 1]) << 16; };
-      u = make_uint4(two(0), two(2), two(4), two(6));
+__device__ __forceinline__ float stage_queries(const AttnParams& p, const KvRequest& r, int h, int first_row, uint8_t (*tile)[kRowPlane], int tile_row) {
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;      // lanes to a row, rows at a time
+  const int lane = threadIdx.x % 32, chunk = lane % kLanes, row = first_row + lane, token = token_of(p, row);
+  const uint16_t* mine = token < r.todo ? reinterpret_cast<const uint16_t*>(p.a.q) + row_place(p, r, h, row, token, p.a.stride_q_tok, p.a.stride_q_head) : nullptr;
+#pragma unroll 4
+  for (int n = 0; n < 32; n += kRows) {
+    const uint16_t* q = place_of(mine, n + lane / kLanes);
+    uint8_t* to = tile[chunk / 8] + plane_at(tile_row + n + lane / kLanes, chunk % 8);
+    if (!q) {
+      *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+    } else if (reinterpret_cast<uintptr_t>(q) % 16 == 0) {
+      __pipeline_memcpy_async(to, q + chunk * 8, 16);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(to)[e] = q[chunk * 8 + e];
     }
-    w[4 * c] = u.x; w[4 * c + 1] = u.y; w[4 * c + 2] = u.z; w[4 * c + 3] = u.w;
   }
-  auto numbers = [&](uint32_t u) { return bf16 ? make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)) : unpack_half2(u); };
-#pragma unroll
-  for (int c = 0; c < D / 2; ++c) {
-    const float2 x = numbers(w[c]);
-    top = max(top, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
+  __pipeline_commit();
+  __pipeline_wait_prior(0);
+  __syncwarp();
+  const bool bf16 = p.a.dtype == CARRY_BF16;
+  uint32_t top = 0;
+#pragma unroll 4
+  for (int c = 0; c < kLanes; ++c) {
+    const uint4 u = *reinterpret_cast<const uint4*>(tile[c / 8] + plane_at(tile_row + lane, c % 8));
+    top = __vmaxu2(__vmaxu2(top, __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu)), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
   }
+  top = max(top >> 16, top & 0xffffu);
+  top = bf16 ? top << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(top))));
   const int e = up_exponent(top);
   const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), p.a.scale);
+#pragma unroll 4
+  for (int c = 0; c < kLanes; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(tile[c / 8] + plane_at(tile_row + lane, c % 8));
+    const uint4 u = *at;
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int c = 0; c < D / 2; ++c) {
-    const float2 x = numbers(w[c]);
-    w[c] = pack_half2(x.x * up, x.y * up);
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = bf16 ? make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)) : unpack_half2(w[k]);
+      w[k] = pack_half2(x.x * up, x.y * up);
+    }
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
   }
-#pragma unroll
-  for (int c = 0; c < D / 8; ++c)
-    *reinterpret_cast<uint4*>(tile[c / 8] + plane_at(tile_row, c % 8)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
   return fabsf(p.a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// 128 bytes of each of a warp's 32 rows, which lane l has of row l, to memory by way of shared memory: eight lanes then
+// write a row's.  `mine` is where this lane's go, or null; SIZE: of a number.
+template <int SIZE>
+__device__ __forceinline__ void store_lines(uint8_t* scratch, const uint4 (&x)[8], uint8_t* mine) {
+  const int lane = threadIdx.x % 32;
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(scratch + plane_at(lane, c)) = x[c];
+  __syncwarp();
+#pragma unroll 2
+  for (int n = 0; n < 8; ++n) {
+    const int row = n * 4 + lane / 8, chunk = lane % 8;
+    uint8_t* to = place_of(mine, row);
+    const uint4 u = *reinterpret_cast<const uint4*>(scratch + plane_at(row, chunk));
+    if (!to) continue;
+    to += chunk * 16;
+    if (reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+      *reinterpret_cast<uint4*>(to) = u;
+    } else if constexpr (SIZE == 2) {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(to)[e] = static_cast<uint16_t>(w[e / 2] >> (e % 2 * 16));
+    }
+  }
 }
 
 // A converting thread's codes of a step: chunk tid % (D / 16) of tokens tid / (D / 16) + i * kStride.  Tokens at or beyond
@@ -214,6 +261,44 @@ __device__ __forceinline__ void convert(const uint8_t* raw, uint8_t (*tile)[kTok
   }
 }
 
+// What the fetching warp knows of the steps to come: lane l has granule l of each.  What a step waits for has been asked for
+// before: its scales a step, the page ids behind them two steps ago.
+template <int D>
+struct Fetch {
+  struct Granule {
+    int id, in_page;
+    float ks, vs;
+  };
+  const AttnParams& p;
+  const int b, h, step0, length;
+  Granule now, next, after;
+  __device__ __forceinline__ Fetch(const AttnParams& p, int b, int h, int step0, int length) : p(p), b(b), h(h), step0(step0), length(length) {}
+  __device__ __forceinline__ void find(int step, Granule& g) const {
+    const int lane = threadIdx.x % 32, granule = (step0 + step) * kBlocks + lane;
+    g.id = lane < kBlocks ? page_id(p, b, granule, length) : 0;
+    g.in_page = granule - page_index(p, granule) * p.page_granules;
+  }
+  __device__ __forceinline__ void scales(Granule& g) const {
+    const CarryGdnKvCache& c = p.a.cache;
+    const int block = h * divide(p.page_granules, p.block_granules, p.block_shift) + divide(g.in_page, p.block_granules, p.block_shift);
+    g.ks = g.id > 0 ? c.k_scale[g.id * c.stride_ks_page + block] : kNoTokens;
+    g.vs = g.id > 0 ? c.v_scale[g.id * c.stride_vs_page + block] : 0.0f;
+  }
+  __device__ __forceinline__ void begin() {
+    find(0, now);
+    find(1, next);
+    scales(now);
+  }
+  __device__ __forceinline__ void ahead(int step) {
+    find(step + 2, after);
+    scales(next);
+  }
+  __device__ __forceinline__ void advance() {
+    now = next;
+    next = after;
+  }
+};
+
 template <int D>
 __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ uint8_t raw[];
@@ -225,7 +310,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   const int warp = threadIdx.x / 32;
   const KvRequest r = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
   if (first_row >= r.todo * p.group) return;
-  const int last = min((first_row + kCtaRows - 1) / p.group, r.todo - 1);
+  const int last = min(token_of(p, first_row + kCtaRows - 1), r.todo - 1);
   const int length = max(min(r.length, r.length - r.count + last + 1), 0), all_steps = (length + kTokens - 1) / kTokens;
   const int share = (all_steps + p.splits - 1) / p.splits, step0 = min(share * (int)blockIdx.z, all_steps), steps = min(share, all_steps - step0);
 
@@ -253,9 +338,12 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // the fetching warp's first trips to memory run while the queries are staged
+  Fetch<D> fetch(p, b, h, step0, length);
+  if (warp == kFetchWarp) fetch.begin();
   float unit_q = 0.0f;
   if (threadIdx.x < kSoftmaxThreads) {
-    unit_q = stage_query<D>(p, r, h, first_row + threadIdx.x, sh.q[threadIdx.x / kTileRows], threadIdx.x % kTileRows);
+    unit_q = stage_queries<D>(p, r, h, first_row + warp * 32, sh.q[warp / 4], warp % 4 * 32);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   fence_before();
@@ -266,7 +354,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
 
   if (threadIdx.x < kSoftmaxThreads) {
     // ---- a row to a thread ----
-    const int tile = threadIdx.x / kTileRows, row = first_row + threadIdx.x, i = row / p.group;
+    const int tile = threadIdx.x / kTileRows, row = first_row + threadIdx.x, i = token_of(p, row);
     const int sees = i < r.todo ? r.length - r.count + i + 1 : 0;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem + lanes + 256 + tile * 128;
@@ -356,33 +444,47 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       healthy = barrier_wait(&sh.o_done[tile][(steps - 1) & 1], (steps - 1) / 2 & 1, poison, p.a.status);
       fence_after();
     }
-    if (healthy) {
+    if (healthy && first_row + warp * 32 < r.todo * p.group) {       // a warp without rows has nothing to leave
       const float by = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kUp), sum);
       const float unit = steps > 0 ? *reinterpret_cast<volatile float*>(&sh.unit) : 1.0f;
-      const long long at = (r.first + i) * p.a.stride_out_tok + (h * p.group + row % p.group) * p.a.stride_out_head;
       const Parts part = parts_of(p, blockIdx.z, blockIdx.x);
-      if (p.splits > 1) {
+      if (p.splits > 1 && i < r.todo) {
         part.top[row] = top;
         part.sum[row] = sum;
       }
+      // every score has been formed by now, so the queries' memory is free: 4 KB to a warp
+      uint8_t* scratch = sh.q[0][0] + warp * 4096;
+      uint16_t* mine = i < r.todo ? reinterpret_cast<uint16_t*>(p.a.out) + row_place(p, r, h, row, i, p.a.stride_out_tok, p.a.stride_out_head) : nullptr;
+      auto numbers = [&](int n, float (&x)[32]) {  // columns 32 n and on
+        if (steps > 0) tmem_load(o_at + n * 32, x);
+        wait_loads();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = sum == 0.0f ? 0.0f : x[e] * by * unit;
+      };
+      float x[32];
+      uint4 line[8];
+      if (p.splits > 1) {
 #pragma unroll 1
-      for (int n = 0; n < D / 32; ++n) {
-        alignas(16) float x[32];
-        if (steps > 0) {
-          tmem_load(o_at + n * 32, x);
-          wait_loads();
+        for (int n = 0; n < D / 32; ++n) {
+          numbers(n, x);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = sum == 0.0f ? 0.0f : x[e] * by * unit;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+          for (int e = 0; e < 8; ++e)
+            line[e] = make_uint4(__float_as_uint(x[4 * e]), __float_as_uint(x[4 * e + 1]), __float_as_uint(x[4 * e + 2]), __float_as_uint(x[4 * e + 3]));
+          store_lines<4>(scratch, line, i < r.todo ? reinterpret_cast<uint8_t*>(part.o + (long long)row * D + n * 32) : nullptr);
         }
-        if (p.splits > 1) {
+      } else {
+#pragma unroll 1
+        for (int n = 0; n < D / 64; ++n) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) store8(part.o, (long long)row * D + n * 32 + e, CARRY_F32, x + e);
-        } else if (i < r.todo) {
+          for (int half = 0; half < 2; ++half) {
+            numbers(n * 2 + half, x);
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) store8(p.a.out, at + n * 32 + e, p.a.dtype, x + e);
+            for (int e = 0; e < 4; ++e) {
+              auto two = [&](int k) { return p.a.dtype == CARRY_BF16 ? pack_bf16(x[8 * e + k], x[8 * e + k + 1]) : pack_half2(x[8 * e + k], x[8 * e + k + 1]); };
+              line[half * 4 + e] = make_uint4(two(0), two(2), two(4), two(6));
+            }
+          }
+          store_lines<2>(scratch, line, mine ? reinterpret_cast<uint8_t*>(mine + n * 64) : nullptr);
         }
       }
     }
@@ -407,32 +509,13 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       if (++stage == kStages) { stage = 0; parity ^= 1; }
     }
   } else if (warp == kFetchWarp) {
-    // ---- codes and scales out of the cache: lane l has granule l of a step.  What a step waits for has been asked for
-    // before: its scales a step, the page ids behind them two steps ago ----
-    const int lane = threadIdx.x % 32, heads_blocks = p.page_granules / p.block_granules;
-    struct Granule {
-      int id, in_page;
-      float ks, vs;
-    };
-    auto find = [&](int step, Granule& g) {
-      const int granule = (step0 + step) * kBlocks + lane;
-      g.id = lane < kBlocks ? page_id(p, b, granule, length) : 0;
-      g.in_page = granule - page_index(p, granule) * p.page_granules;
-    };
-    auto fetch = [&](Granule& g) {
-      const int block = h * heads_blocks + divide(g.in_page, p.block_granules, p.block_shift);
-      g.ks = g.id > 0 ? c.k_scale[g.id * c.stride_ks_page + block] : kNoTokens;
-      g.vs = g.id > 0 ? c.v_scale[g.id * c.stride_vs_page + block] : 0.0f;
-    };
-    Granule now, next, after;
-    find(0, now);
-    find(1, next);
-    fetch(now);
+    // ---- codes and scales out of the cache ----
+    const int lane = threadIdx.x % 32;
     float unit = 0.0f;
     int raw = 0, parity = 1;
     for (int step = 0; step < steps; ++step) {
-      find(step + 2, after);
-      fetch(next);
+      fetch.ahead(step);
+      const typename Fetch<D>::Granule& now = fetch.now;
       if (step >= kRawStages && !__all_sync(~0u, barrier_wait(&sh.raw_free[raw], parity, poison, p.a.status))) break;
       const uint32_t there = __ballot_sync(~0u, now.id > 0);
       float most = now.vs;
@@ -465,8 +548,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         bulk_copy(sh.raw_k[raw] + to, c.k_codes + now.id * c.stride_k_page + at, kGranule * D, &sh.raw_full[raw]);
         bulk_copy(sh.raw_v[raw] + to, c.v_codes + now.id * c.stride_v_page + at, kGranule * D, &sh.raw_full[raw]);
       }
-      now = next;
-      next = after;
+      fetch.advance();
       if (++raw == kRawStages) { raw = 0; parity ^= 1; }
     }
   } else {
