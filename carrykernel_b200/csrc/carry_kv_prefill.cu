@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   const int warp = threadIdx.x / 32;
   const KvRequest r = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
   if (first_row >= r.todo * p.group) return;
+  const int tiles = first_row + kTileRows < r.todo * p.group ? 2 : 1;      // a second tile without rows takes no part
   const int last = min(token_of(p, first_row + kCtaRows - 1), r.todo - 1);
   const int length = max(min(r.length, r.length - r.count + last + 1), 0), all_steps = (length + kTokens - 1) / kTokens;
   const int share = (all_steps + p.splits - 1) / p.splits, step0 = min(share * (int)blockIdx.z, all_steps), steps = min(share, all_steps - step0);
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem + lanes + 256 + tile * 128;
     float top = -INFINITY, sum = 0.0f;
     bool healthy = true;
-    for (int step = 0; step < steps; ++step) {
+    for (int step = 0; step < steps && tile < tiles; ++step) {
       const int stage = step % kStages, note = step % kNotes, turn = step & 1;
       healthy = barrier_wait(&sh.k_full[stage], step / kStages & 1, poison, p.a.status) &&
                 barrier_wait(&sh.s_full[tile][turn], step / 2 & 1, poison, p.a.status);
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       fence_before();
       barrier_arrive(&sh.p_full[tile][turn]);
     }
-    if (healthy && steps > 0) {
+    if (healthy && steps > 0 && tile < tiles) {
       healthy = barrier_wait(&sh.o_done[tile][(steps - 1) & 1], (steps - 1) / 2 & 1, poison, p.a.status);
       fence_after();
     }
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       for (int k = 0; k < D / 16; ++k)
         mma_shared(elected, to, q + k / 4 * kRowStep + k % 4 * 2, keys + k / 4 * kTokenStep + k % 4 * 2, instruction(kTokens, false), k > 0);
       mma_commit(elected, &sh.s_full[tile][step & 1]);
-      if (tile == 1) mma_commit(elected, &sh.k_free[step % kStages]);
+      if (tile + 1 == tiles) mma_commit(elected, &sh.k_free[step % kStages]);
     };
     bool healthy = true;
     for (int step = 0; step < 2 && step < steps && healthy; ++step) {
@@ -571,13 +572,14 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       if (!healthy) break;
       fence_after();
       scores(0, step);
-      scores(1, step);
+      if (tiles == 2) scores(1, step);
     }
     for (int step = 0; healthy && step < steps; ++step) {
       const int stage = step % kStages, turn = step & 1, parity = step / kStages & 1;
       const uint32_t values = v0 + stage * kStageStep;
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
+        if (tile >= tiles) break;
         healthy = (tile > 0 || wait(&sh.v_full[stage], parity)) &&
                   wait(&sh.p_full[tile][turn], step / 2 & 1);
         if (!healthy) break;
@@ -587,7 +589,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           mma_tensor(elected, base + 256 + tile * 128, base + tile * 128 + turn * 64 + k * 8,
                      values + k * 128, instruction(D, true), step > 0 || k > 0);
         mma_commit(elected, &sh.o_done[tile][turn]);
-        if (tile == 1) mma_commit(elected, &sh.v_free[stage]);
+        if (tile + 1 == tiles) mma_commit(elected, &sh.v_free[stage]);
         if (step + 2 < steps) {
           healthy = tile > 0 || wait(&sh.k_full[(step + 2) % kStages], (step + 2) / kStages & 1);
           if (!healthy) break;
