@@ -1,9 +1,9 @@
 // Attention over the 8-bit key/value cache.
 //
 // Scores s = scale * q . k and outputs sum_j softmax_j(s) v_j in one pass over the cache, with the running maximum and
-// sum of an online softmax.  Keys and values stay e4m3 until they are in registers: tiles of 64 tokens come into a ring of
-// shared-memory stages by 16-byte asynchronous copies, and a warp turns the codes into the fp16 operands of the
-// matrix instructions as it needs them (e4m3 is a subset of fp16).  What each rounding to 16 bits costs:
+// sum of an online softmax.  Keys and values stay e4m3 until they are on the processor: tiles come into a ring of
+// shared-memory stages by asynchronous copies, and the codes become the fp16 operands of the matrix instructions there
+// (e4m3 is a subset of fp16).  What each rounding to 16 bits costs:
 //  * a query row is scaled by a power of two until its largest number is in [2^14, 2^15): bf16 and fp16 numbers fit fp16
 //    exactly down to 2^-29 of the largest, fp32 ones go in two parts (22 bits);
 //  * the weights p of the softmax are fp16 (2^-12 of each, against 2^-9 for the rounding of a bf16 output), with fp32
@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_parts_kernel(const __gri
   const int lane = threadIdx.x % 32, row = blockIdx.y * kJoinWarps + threadIdx.x / 32;
   const int b = blockIdx.x / p.a.cache.HKV, h = blockIdx.x % p.a.cache.HKV, i = token_of(p, row);
   const KvRequest q = kv_request(p.a.cache, p.a.rows, b, nullptr);
-  if (i >= q.todo) return;
+  if (i >= q.todo || row >= p.padded) return;
   const Parts mine = parts_of(p, min(lane, p.splits - 1), blockIdx.x);
   float top = lane < p.splits ? mine.top[row] : -INFINITY, w = lane < p.splits ? mine.sum[row] : 0.0f;
   const float all_top = warp_max(top), base = all_top == -INFINITY ? 0.0f : all_top;
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_parts_kernel(const __gri
 }  // namespace
 
 int launch_join_parts(const AttnParams& p, cudaStream_t stream) {
-  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)((p.rows + kJoinWarps - 1) / kJoinWarps));
+  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)((min(p.rows, p.padded) + kJoinWarps - 1) / kJoinWarps));
   return p.a.cache.D == 64 ? launch_dependent(kv_join_parts_kernel<64>, grid, kJoinThreads, 0, stream, p)
                            : launch_dependent(kv_join_parts_kernel<128>, grid, kJoinThreads, 0, stream, p);
 }

@@ -18,7 +18,7 @@ struct AttnParams {
   int page_granules, page_shift;  // granules in a page, and its logarithm or -1
   int block_granules, block_shift;
   int rows;                       // rows of a (request, head): most that may be in use
-  int splits, padded;             // parts that a context is cut into where the rows alone are few; rows that a part has room for
+  int splits, padded;             // parts that a context is cut into where the rows alone are few; rows from the first that are cut
 };
 
 // What a part of a context leaves for the joining kernel, by part, (request, head) and row: largest score and sum of

@@ -9,7 +9,7 @@
 // the lengths are; where a cut falls inside a (request, head), pieces are joined by a second kernel.  Short contexts of few
 // (request, head)s have a cluster each and no second kernel.
 //
-// What bounds it: 128 requests of 8192 tokens (8 heads of 128, 2.15 GB) take 396 us, 5.4 TB/s, 83 % of the copy rate; 64 of 1 to
+// What bounds it: 128 requests of 8192 tokens (8 heads of 128, 2.15 GB) take 394 us, 5.5 TB/s, 83 % of the copy rate; 64 of 1 to
 // 8192 tokens 120 us, 4.6 TB/s, some 15 us of it the way in and out.  A run is about 700 instructions of a warp, half of them
 // conversions and byte permutations at two cycles each; twelve warps an SM issue two instructions a cycle.  Tried and slower:
 // e4m3 matrix instructions on unconverted keys (131 us for the 64 requests: twice the registers), runs of 64 tokens, two CTAs
@@ -800,7 +800,7 @@ int launch_clusters(K kernel, int clusters, size_t smem, cudaStream_t stream, co
 }
 
 // Whether clusters take a call: all of them have to be resident, and a context be short enough for eight CTAs.  One
-// request of 1500 tokens and 8 heads takes 8.1 us so, 11.4 by the line; 4 x 4096 tokens PAIRTIME.
+// request of 1500 tokens and 8 heads takes 8.2 us so, 11.4 by the line; four of 4096 15.7 and 18.2.
 bool by_pairs(const CarryGdnKvAttentionArgs& a) {
   const long long tokens = (long long)a.cache.max_pages * a.cache.page, pairs = (long long)a.rows.B * a.cache.HKV;
   return pairs * kCluster <= 2LL * sm_count() && tokens <= 4LL * kCluster * kLine;

@@ -3,13 +3,16 @@
 // A CTA has 256 rows (query tokens times the query heads of one key/value head) as two tiles of 128, and walks the
 // request's tokens 64 at a time.  The work is in five places that run side by side:
 //  * one warp brings codes in (bulk copies, three steps ahead) and notes their scales;
-//  * eight warps turn a step's codes into fp16, keys and values (e4m3 is a subset of fp16);
+//  * four warps turn a step's codes into fp16, keys and values (e4m3 is a subset of fp16);
 //  * one warp issues the matrix products on the fifth-generation tensor cores: S = Q K^T, operands in shared memory,
 //    and O += P V with the weights P in tensor memory;
 //  * four warps for each row tile take its scores out of tensor memory, a row to a thread, and put the weights back in
 //    their place.  While one tile's weights are formed, the other's products run.
-// What bounds it: 2 x 128 x 64 exponentials a step take 1024 cycles of the special function units, and the products as
-// many of the tensor cores.
+// What bounds it: 2 x 128 x 64 exponentials a step take 1024 cycles of the special function units, and the products 1330 of
+// the tensor cores (64 columns of scores come at two thirds of the rate of 128, which tensor memory has no room for beside
+// the outputs and a second step's scores); a step takes 1750.  A chunk of 2048 tokens at 16384, 32 heads over 8 of 128: 600 us,
+// 870 TFLOP/s, 53 % of the burst rate of a large matrix product, at a clock that the GPU's power brings down to some 1.5 GHz.
+// A CTA's way in and out is some 7 us: six prompts of up to 2000 tokens and 16 heads take 95 us, 415 TFLOP/s, half of it that.
 //
 // A row's weights are relative to a maximum that is replaced, and O rescaled, only when it is outgrown by 2^4; values
 // likewise count in the largest value scale until one is 2^4 larger.  A weight is formed times 2^7, so it stays below
@@ -306,14 +309,17 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   depend_release();
   depend_wait();
   const CarryGdnKvCache& c = p.a.cache;
-  const int b = blockIdx.x / c.HKV, h = blockIdx.x % c.HKV, first_row = (gridDim.y - 1 - blockIdx.y) * kCtaRows;   // the longest of all go first
+  // The longest contexts go first.  Those of the first `cut` row tiles are cut into parts, and come last.
+  const int cut = p.padded / kCtaRows, whole = gridDim.y - cut * p.splits, late = (int)blockIdx.y - whole;
+  const int splits = late < 0 ? 1 : p.splits, part_number = late < 0 ? 0 : late % splits;
+  const int b = blockIdx.x / c.HKV, h = blockIdx.x % c.HKV, first_row = cut * kCtaRows + (late < 0 ? -1 - late : -1 - late / splits) * kCtaRows;
   const int warp = threadIdx.x / 32;
   const KvRequest r = kv_request(c, p.a.rows, b, first_row == 0 && h == 0 && threadIdx.x == 0 ? p.a.status : nullptr);
   if (first_row >= r.todo * p.group) return;
   const int tiles = first_row + kTileRows < r.todo * p.group ? 2 : 1;      // a second tile without rows takes no part
   const int last = min(token_of(p, first_row + kCtaRows - 1), r.todo - 1);
   const int length = max(min(r.length, r.length - r.count + last + 1), 0), all_steps = (length + kTokens - 1) / kTokens;
-  const int share = (all_steps + p.splits - 1) / p.splits, step0 = min(share * (int)blockIdx.z, all_steps), steps = min(share, all_steps - step0);
+  const int share = (all_steps + splits - 1) / splits, step0 = min(share * part_number, all_steps), steps = min(share, all_steps - step0);
 
   if (threadIdx.x == 0) {
     sh.poison = 0;
@@ -363,8 +369,8 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     bool healthy = true;
     for (int step = 0; step < steps && tile < tiles; ++step) {
       const int stage = step % kStages, note = step % kNotes, turn = step & 1;
-      healthy = barrier_wait(&sh.k_full[stage], step / kStages & 1, poison, p.a.status) &&
-                barrier_wait(&sh.s_full[tile][turn], step / 2 & 1, poison, p.a.status);
+      healthy = __all_sync(~0u, barrier_wait(&sh.k_full[stage], step / kStages & 1, poison, p.a.status) &&
+                                    barrier_wait(&sh.s_full[tile][turn], step / 2 & 1, poison, p.a.status));
       if (!healthy) break;
       fence_after();
       float x[2][32], now = top, by[kBlocks], ks[kBlocks], bias[kBlocks], counts[kBlocks];
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         sum *= keep;
         top = now;
         if (step > 0) {
-          healthy = barrier_wait(&sh.o_done[tile][turn ^ 1], (step - 1) / 2 & 1, poison, p.a.status);
+          healthy = __all_sync(~0u, barrier_wait(&sh.o_done[tile][turn ^ 1], (step - 1) / 2 & 1, poison, p.a.status));
           if (!healthy) break;
           fence_after();
           const float less = keep * values;
@@ -442,14 +448,14 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       barrier_arrive(&sh.p_full[tile][turn]);
     }
     if (healthy && steps > 0 && tile < tiles) {
-      healthy = barrier_wait(&sh.o_done[tile][(steps - 1) & 1], (steps - 1) / 2 & 1, poison, p.a.status);
+      healthy = __all_sync(~0u, barrier_wait(&sh.o_done[tile][(steps - 1) & 1], (steps - 1) / 2 & 1, poison, p.a.status));
       fence_after();
     }
     if (healthy && first_row + warp * 32 < r.todo * p.group) {       // a warp without rows has nothing to leave
       const float by = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kUp), sum);
       const float unit = steps > 0 ? *reinterpret_cast<volatile float*>(&sh.unit) : 1.0f;
-      const Parts part = parts_of(p, blockIdx.z, blockIdx.x);
-      if (p.splits > 1 && i < r.todo) {
+      const Parts part = parts_of(p, part_number, blockIdx.x);
+      if (splits > 1 && i < r.todo) {
         part.top[row] = top;
         part.sum[row] = sum;
       }
@@ -464,7 +470,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       };
       float x[32];
       uint4 line[8];
-      if (p.splits > 1) {
+      if (splits > 1) {
 #pragma unroll 1
         for (int n = 0; n < D / 32; ++n) {
           numbers(n, x);
@@ -612,6 +618,35 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   }
 }
 
+long long row_tiles(const CarryGdnKvAttentionArgs& a) {
+  return ((long long)a.rows.max_query * (a.HQ / a.cache.HKV) + kCtaRows - 1) / kCtaRows;
+}
+
+// What does not fill the processors is cut: the CTAs beyond the last full round of one to a processor (all of them, where
+// they are few), which are the first row tiles' of every (request, head).  Into as many parts as bring the end nearest,
+// counted in steps of 64 tokens: a part costs some four of its own, and its outputs, written and read, a twentieth; the
+// join four.  A chunk of 2048 tokens, 32 heads over 8, at 16384 tokens has 256 CTAs, and
+// takes 600 us either way, for the processors that stay idle leave the others their power; one of 1280 has 160, and takes 379 us,
+// 592 uncut.
+void lay_out(const CarryGdnKvAttentionArgs& a, int& splits, int& padded) {
+  const long long tiles = row_tiles(a), pairs = (long long)a.cache.HKV * a.rows.B, sms = sm_count();
+  splits = 1;
+  padded = tiles > 65535 ? -1 : 0;
+  const long long late = tiles * pairs % sms, cut = tiles - (tiles * pairs - late) / pairs;
+  if (cut == 0 || cut > 1024 || tiles > 30000) return;
+  const long long cached = max((long long)a.cache.max_pages * a.cache.page - a.rows.max_query, 0LL);
+  const long long steps = (cached + min(cut * kCtaRows / (a.HQ / a.cache.HKV), (long long)a.rows.max_query) + 63) / 64;
+  long long least = (late + sms - 1) / sms * (steps + 4);
+  for (int n = 2; n <= 32 && n * 8 <= steps; ++n) {
+    const long long cost = (late * n + sms - 1) / sms * ((steps + n - 1) / n + 4) + cut * pairs * n * a.cache.D / (20 * 128) + 4;
+    if (cost < least) {
+      least = cost;
+      splits = n;
+      padded = (int)cut * kCtaRows;
+    }
+  }
+}
+
 template <int D>
 int launch(const AttnParams& p, cudaStream_t stream) {
   constexpr size_t smem = sizeof(Shared<D>) + 1024;
@@ -624,15 +659,9 @@ int launch(const AttnParams& p, cudaStream_t stream) {
     }
     if (dev < 64) ready[dev] = true;
   }
-  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)p.padded / kCtaRows, (unsigned)p.splits);
+  const long long tiles = row_tiles(p.a), cut = p.padded / kCtaRows;
+  const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)(tiles - cut + cut * p.splits));
   return launch_dependent(kv_prefill_kernel<D>, grid, kAllThreads, smem, stream, p);
-}
-
-// splits and padded rows
-void lay_out(const CarryGdnKvAttentionArgs& a, int& splits, int& padded) {
-  const long long rows = (long long)a.rows.max_query * (a.HQ / a.cache.HKV), tiles = (rows + kCtaRows - 1) / kCtaRows;
-  padded = tiles > 65535 ? -1 : (int)tiles * kCtaRows;
-  splits = split_count(a, tiles * a.cache.HKV * a.rows.B);
 }
 
 }  // namespace

@@ -418,9 +418,9 @@ int64_t carry_gdn_kv_attention_workspace(const CarryGdnKvAttentionArgs* args);
  * type, y = h * rsqrt(mean(h^2) + eps) * weight, and y in e4m3 codes with a
  * scale per row (group == 0: scale [N]) or per 128 columns (group == 128: scale
  * [N, ceil(W / 128)], contiguous): scale = max(amax|y|, 1e-12) / 448.  A row
- * with a number that is not finite gets NaN codes and scales throughout.
- * residual may be NULL (h = x); residual_out may be NULL, or alias residual or
- * x.  W is at most 32768.
+ * of h with a number that is not finite gets NaN codes and scales throughout;
+ * weights are taken to be finite.  residual may be NULL (h = x); residual_out
+ * may be NULL, or alias residual or x.  W is at most 32768.
  */
 typedef struct CarryGdnNormArgs {
   const void* x;          /* [N, W], W contiguous */
