@@ -6,6 +6,8 @@
 //
 // What bounds it: 16384 rows of 4096 in bf16 take 83 us, 5.7 TB/s, 87 % of the copy rate; 256 rows take 3.8 us, of which the
 // launch and one trip to memory are most.  A row's instructions are 440 a warp; with 533 they were the bound (92 us).
+#include <type_traits>
+
 #include "carry_hybrid.cuh"
 
 namespace carry {
@@ -102,17 +104,18 @@ __device__ __forceinline__ RowScale reduce_row(const NormParams& p, RowSums& sh,
   return {top < INFINITY ? rstd : NAN, top};
 }
 
-// Sum of the squares of eight numbers; from kLarge on it counts in `large`, times 2^-128 (NaNs do, too).
-__device__ __forceinline__ void add_squares(const Eight& t, float2& ss, float& large) {
-  float2 part = mul2(t.x[0], t.x[0]);
+// Sum of the squares of 2 N numbers; from kLarge on it counts in `large`, times 2^-128 (NaNs do, too).
+template <int N>
+__device__ __forceinline__ void add_squares(const float2 (&t)[N], float2& ss, float& large) {
+  float2 part = mul2(t[0], t[0]);
 #pragma unroll
-  for (int i = 1; i < 4; ++i) part = fma2(t.x[i], t.x[i], part);
+  for (int i = 1; i < N; ++i) part = fma2(t[i], t[i], part);
   if (part.x + part.y < kLarge) {
     ss = add2(ss, part);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float u = t.x[i].x * 0x1p-64f, v = t.x[i].y * 0x1p-64f;
+    for (int i = 0; i < N; ++i) {
+      const float u = t[i].x * 0x1p-64f, v = t[i].y * 0x1p-64f;
       large += u * u + v * v;
     }
   }
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(max_threads(C), min_ctas(C)) norm_kernel(const
       top[j] = 0.0f;
       if (at >= a.W) continue;
       if (a.residual_out) store<R>(out, j * jump, t[j]);
-      add_squares(t[j], ss, large);
+      add_squares(t[j].x, ss, large);
       if (a.weight_dtype == X) top[j] = weigh(t[j], unpack<X>(load_raw<X>(a.weight, at)));
       else if (a.weight_dtype == CARRY_F32) top[j] = weigh(t[j], unpack<CARRY_F32>(load_raw<CARRY_F32>(a.weight, at)));
       else top[j] = weigh(t[j], load_slow(a.weight, at, 8, a.weight_dtype));
@@ -232,52 +235,138 @@ __global__ void __launch_bounds__(max_threads(C), min_ctas(C)) norm_kernel(const
   }
 }
 
-// The same a number at a time, for rows that are not aligned and for types that have no kernel of their own.
-template <int C>
-__global__ void __launch_bounds__(512) norm_slow_kernel(const __grid_constant__ NormParams p) {
+// ---- any rows: odd widths, rows off the 16-byte grid, other pairs of types ---------------------------------------------
+
+template <int DTYPE>
+struct Number {
+  using type = uint16_t;
+};
+template <>
+struct Number<CARRY_F32> {
+  using type = float;
+};
+template <int DTYPE>
+__device__ __forceinline__ float value_of(typename Number<DTYPE>::type u) {
+  if constexpr (DTYPE == CARRY_F32) return u;
+  else if constexpr (DTYPE == CARRY_BF16) return __uint_as_float(static_cast<uint32_t>(u) << 16);
+  else return __half2float(__ushort_as_half(u));
+}
+template <int DTYPE>
+__device__ __forceinline__ void round_two(float2 v, typename Number<DTYPE>::type& low, typename Number<DTYPE>::type& high) {
+  if constexpr (DTYPE == CARRY_F32) {
+    low = v.x;
+    high = v.y;
+  } else {
+    uint32_t u;
+    if constexpr (DTYPE == CARRY_BF16) {
+      const __nv_bfloat162 h = __float22bfloat162_rn(v);
+      u = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = __float22half2_rn(v);
+      u = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    low = static_cast<uint16_t>(u);
+    high = static_cast<uint16_t>(u >> 16);
+  }
+}
+
+// A warp takes 128 columns at a time, lane l the numbers l, 32 + l, 64 + l and 96 + l of them: neighbouring lanes have
+// neighbouring numbers, so a warp's access is one or two lines wherever the row begins, and a group's maximum is a
+// warp's.  C of these runs to a warp, run j of warp w being number j * warps + w of the row.
+__host__ __device__ constexpr int any_ctas(int C) { return C <= 4 ? 2 : 1; }
+template <int C, int X, int R>
+__global__ void __launch_bounds__(512, any_ctas(C)) norm_any_kernel(const __grid_constant__ NormParams p) {
   __shared__ RowSums sums;
   depend_release();
   depend_wait();
+  using XT = typename Number<X>::type;
+  using RT = typename Number<R>::type;
   const CarryGdnNormArgs& a = p.a;
-  const int lane = threadIdx.x % 32, groups = (a.W + kGroup - 1) / kGroup;
+  const int lane = threadIdx.x % 32, groups = (a.W + kGroup - 1) / kGroup, warps = blockDim.x / 32;
+  const int first = threadIdx.x / 32 * kGroup + lane, jump = warps * kGroup;
+  const bool has_residual = a.residual != nullptr;
   int turn = 0;
   for (long long row = blockIdx.x; row < a.N; row += gridDim.x, turn ^= 1) {
-    Eight t[C];
-    float2 ss = make_float2(0.0f, 0.0f);
+    const XT* x = static_cast<const XT*>(a.x) + row * a.stride_x + first;
+    const RT* r = static_cast<const RT*>(a.residual) + row * a.stride_residual + first;
+    RT* out = static_cast<RT*>(a.residual_out) + row * a.stride_residual_out + first;
+    uint8_t* codes = a.codes + row * a.stride_codes + first;
+    float2 t[C][2], ss = make_float2(0.0f, 0.0f);
     float large = 0.0f, top[C], all = 0.0f;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      const int at = (j * blockDim.x + threadIdx.x) * 8, n = min(a.W - at, 8);
-      top[j] = 0.0f;
-      if (n <= 0) continue;
-      t[j] = load_slow(a.x, row * a.stride_x + at, n, a.x_dtype);
-      if (a.residual) {
-        const Eight add = load_slow(a.residual, row * a.stride_residual + at, n, a.residual_dtype);
+      const int left = a.W - first - j * jump;    // numbers from this lane's first of the run on
+      XT u[4] = {};
+      RT v[4] = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[j].x[i] = add2(t[j].x[i], add.x[i]);
+      for (int i = 0; i < 4; ++i)
+        if (i * 32 < left) u[i] = x[j * jump + i * 32];
+      if (has_residual) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i * 32 < left) v[i] = r[j * jump + i * 32];
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        t[j][i] = make_float2(value_of<X>(u[2 * i]), value_of<X>(u[2 * i + 1]));
+        if (has_residual) t[j][i] = add2(t[j][i], make_float2(value_of<R>(v[2 * i]), value_of<R>(v[2 * i + 1])));
+      }
+    }
+    auto weigh_all = [&](auto tag) {
+      using T = typename Number<decltype(tag)::value>::type;
+      const T* w = static_cast<const T*>(a.weight) + first;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int left = a.W - first - j * jump;
+        T u[4] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i * 32 < left) u[i] = w[j * jump + i * 32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) t[j][i] = mul2(t[j][i], make_float2(value_of<decltype(tag)::value>(u[2 * i]), value_of<decltype(tag)::value>(u[2 * i + 1])));
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int left = a.W - first - j * jump;
       if (a.residual_out) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n) store_from_float(a.residual_out, row * a.stride_residual_out + at + i, a.residual_dtype, i % 2 ? t[j].x[i / 2].y : t[j].x[i / 2].x);
+        for (int i = 0; i < 2; ++i) {
+          RT low, high;
+          round_two<R>(t[j][i], low, high);
+          if (i * 64 < left) out[j * jump + i * 64] = low;
+          if (i * 64 + 32 < left) out[j * jump + i * 64 + 32] = high;
+        }
       }
       add_squares(t[j], ss, large);
-      top[j] = weigh(t[j], load_slow(a.weight, at, n, a.weight_dtype));
+    }
+    if (a.weight_dtype == CARRY_BF16) weigh_all(std::integral_constant<int, CARRY_BF16>());
+    else if (a.weight_dtype == CARRY_F16) weigh_all(std::integral_constant<int, CARRY_F16>());
+    else weigh_all(std::integral_constant<int, CARRY_F32>());
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      top[j] = fmaxf(fmaxf(fabsf(t[j][0].x), fabsf(t[j][0].y)), fmaxf(fabsf(t[j][1].x), fabsf(t[j][1].y)));
       all = fmaxf(all, top[j]);
     }
     const RowScale s = reduce_row(p, sums, turn, ss.x + ss.y, large, all);
+    float by = 0.0f;
+    if (a.group == 0) {
+      const float scale = scale_of(s, s.top, by);
+      if (threadIdx.x == 0) a.scale[row] = scale;
+    }
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      const int at = (j * blockDim.x + threadIdx.x) * 8, n = min(a.W - at, 8);
-      float by;
-      const float scale = scale_of(s, a.group ? group_max(top[j]) : s.top, by);
-      if (n <= 0) continue;
-      if (a.group && lane % 16 == 0) a.scale[row * groups + at / kGroup] = scale;
-      if (!a.group && at == 0) a.scale[row] = scale;
-      const uint2 c = codes_of(t[j], by);
+      const int left = a.W - first - j * jump;
+      if (a.group) {
+        const float scale = scale_of(s, __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top[j]))), by);
+        if (lane == 0 && left > 0) a.scale[row * groups + (first + j * jump) / kGroup] = scale;
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) a.codes[row * a.stride_codes + at + i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (i % 4 * 8));
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t c = __nv_cvt_float2_to_fp8x2(mul2(t[j][i], make_float2(by, by)), __NV_SATFINITE, __NV_E4M3);
+        if (i * 64 < left) codes[j * jump + i * 64] = static_cast<uint8_t>(c);
+        if (i * 64 + 32 < left) codes[j * jump + i * 64 + 32] = static_cast<uint8_t>(c >> 8);
+      }
     }
   }
 }
@@ -296,9 +385,26 @@ int launch_typed(const NormParams& p, cudaStream_t stream) {
   if (p.a.W <= 16384) return launch_rows(norm_kernel<4, X, R>, p, 4, stream);
   return launch_rows(norm_kernel<8, X, R>, p, 8, stream);
 }
-int launch_slow(const NormParams& p, cudaStream_t stream) {
-  if (p.a.W <= 1024) return launch_rows(norm_slow_kernel<1>, p, 1, stream);
-  return p.a.W <= 8192 ? launch_rows(norm_slow_kernel<2>, p, 2, stream) : launch_rows(norm_slow_kernel<8>, p, 8, stream);
+template <int C, int X, int R>
+int launch_any(const NormParams& p, cudaStream_t stream) {
+  const int runs = (p.a.W + kGroup - 1) / kGroup, warps = (runs + C - 1) / C;
+  const long long resident = (long long)sm_count() * (16 * any_ctas(C) / warps);
+  return launch_dependent(norm_any_kernel<C, X, R>, dim3((unsigned)(p.a.N < resident ? p.a.N : resident)), warps * 32, 0, stream, p);
+}
+template <int X, int R>
+int launch_any(const NormParams& p, cudaStream_t stream) {
+  if (p.a.W <= 2048 && p.a.N <= sm_count()) return launch_any<1, X, R>(p, stream);
+  if (p.a.W <= 8192) return launch_any<4, X, R>(p, stream);
+  return p.a.W <= 16384 ? launch_any<8, X, R>(p, stream) : launch_any<16, X, R>(p, stream);
+}
+template <int X>
+int launch_any(const NormParams& p, cudaStream_t stream) {
+  if (p.a.residual_dtype == CARRY_F32) return launch_any<X, CARRY_F32>(p, stream);
+  return p.a.residual_dtype == CARRY_BF16 ? launch_any<X, CARRY_BF16>(p, stream) : launch_any<X, CARRY_F16>(p, stream);
+}
+int launch_any(const NormParams& p, cudaStream_t stream) {
+  if (p.a.x_dtype == CARRY_F32) return launch_any<CARRY_F32>(p, stream);
+  return p.a.x_dtype == CARRY_BF16 ? launch_any<CARRY_BF16>(p, stream) : launch_any<CARRY_F16>(p, stream);
 }
 
 }  // namespace
@@ -323,7 +429,7 @@ int launch_norm(const CarryGdnNormArgs& a, cudaStream_t stream) {
   if (vec && xd == CARRY_F32 && rd == CARRY_F32) return launch_typed<CARRY_F32, CARRY_F32>(p, stream);
   if (vec && xd == CARRY_BF16 && rd == CARRY_F32) return launch_typed<CARRY_BF16, CARRY_F32>(p, stream);
   if (vec && xd == CARRY_F16 && rd == CARRY_F32) return launch_typed<CARRY_F16, CARRY_F32>(p, stream);
-  return launch_slow(p, stream);
+  return launch_any(p, stream);
 }
 
 }  // namespace carry
