@@ -5,7 +5,8 @@
 // the maximum come out of one pass and one reduction.
 //
 // What bounds it: 16384 rows of 4096 in bf16 take 83 us, 5.7 TB/s, 87 % of the copy rate; 256 rows take 3.8 us, of which the
-// launch and one trip to memory are most.  A row's instructions are 440 a warp; with 533 they were the bound (92 us).
+// launch and one trip to memory are most.  A row is 440 instructions of a warp; with
+// 533 they were the bound (92 us).
 #include <type_traits>
 
 #include "carry_hybrid.cuh"
@@ -45,14 +46,11 @@ __device__ __forceinline__ void store(void* p, long long at, const Eight& e) {
     *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-// the same an element at a time, for rows that are not aligned, or of types that have no kernel of their own
-__device__ __forceinline__ Eight load_slow(const void* p, long long at, int n, int dtype) {
+// an element at a time: weights of another type than x
+__device__ __forceinline__ Eight load_slow(const void* p, long long at, int dtype) {
   Eight e;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    e.x[i].x = 2 * i < n ? load_as_float(p, at + 2 * i, dtype) : 0.0f;
-    e.x[i].y = 2 * i + 1 < n ? load_as_float(p, at + 2 * i + 1, dtype) : 0.0f;
-  }
+  for (int i = 0; i < 4; ++i) e.x[i] = make_float2(load_as_float(p, at + 2 * i, dtype), load_as_float(p, at + 2 * i + 1, dtype));
   return e;
 }
 
@@ -207,7 +205,7 @@ __global__ void __launch_bounds__(max_threads(C), min_ctas(C)) norm_kernel(const
       add_squares(t[j].x, ss, large);
       if (a.weight_dtype == X) top[j] = weigh(t[j], unpack<X>(load_raw<X>(a.weight, at)));
       else if (a.weight_dtype == CARRY_F32) top[j] = weigh(t[j], unpack<CARRY_F32>(load_raw<CARRY_F32>(a.weight, at)));
-      else top[j] = weigh(t[j], load_slow(a.weight, at, 8, a.weight_dtype));
+      else top[j] = weigh(t[j], load_slow(a.weight, at, a.weight_dtype));
       all = fmaxf(all, top[j]);
     }
     const RowScale s = reduce_row(p, sums, turn, ss.x + ss.y, large, all);
@@ -270,9 +268,11 @@ __device__ __forceinline__ void round_two(float2 v, typename Number<DTYPE>::type
   }
 }
 
-// A warp takes 128 columns at a time, lane l the numbers l, 32 + l, 64 + l and 96 + l of them: neighbouring lanes have
+// A warp takes C runs of 128 columns, lane l the numbers l, 32 + l, 64 + l and 96 + l of each: neighbouring lanes have
 // neighbouring numbers, so a warp's access is one or two lines wherever the row begins, and a group's maximum is a
-// warp's.  C of these runs to a warp, run j of warp w being number j * warps + w of the row.
+// warp's.  Only a row's last warp asks of its numbers whether they are there.  16384 rows of 4095 in bf16 take 128 us, 3.7 TB/s, bound
+// by instructions for lanes of 2 bytes (a lane with eight neighbouring numbers 351; four, from the boundary that its
+// tensors share, with edges by themselves, 170), in fp32 144 us, 92 % of the copy rate.
 __host__ __device__ constexpr int any_ctas(int C) { return C <= 4 ? 2 : 1; }
 template <int C, int X, int R>
 __global__ void __launch_bounds__(512, any_ctas(C)) norm_any_kernel(const __grid_constant__ NormParams p) {
@@ -282,67 +282,94 @@ __global__ void __launch_bounds__(512, any_ctas(C)) norm_any_kernel(const __grid
   using XT = typename Number<X>::type;
   using RT = typename Number<R>::type;
   const CarryGdnNormArgs& a = p.a;
-  const int lane = threadIdx.x % 32, groups = (a.W + kGroup - 1) / kGroup, warps = blockDim.x / 32;
-  const int first = threadIdx.x / 32 * kGroup + lane, jump = warps * kGroup;
-  const bool has_residual = a.residual != nullptr;
-  int turn = 0;
-  for (long long row = blockIdx.x; row < a.N; row += gridDim.x, turn ^= 1) {
-    const XT* x = static_cast<const XT*>(a.x) + row * a.stride_x + first;
-    const RT* r = static_cast<const RT*>(a.residual) + row * a.stride_residual + first;
-    RT* out = static_cast<RT*>(a.residual_out) + row * a.stride_residual_out + first;
-    uint8_t* codes = a.codes + row * a.stride_codes + first;
-    float2 t[C][2], ss = make_float2(0.0f, 0.0f);
-    float large = 0.0f, top[C], all = 0.0f;
+  const int lane = threadIdx.x % 32, groups = (a.W + kGroup - 1) / kGroup, run0 = threadIdx.x / 32 * C;
+  const int first = run0 * kGroup + lane, left = a.W - first;      // columns from this lane's first on
+  const bool whole = (run0 + C) * kGroup <= a.W;
+  // Where a row's numbers leave the registers for it, the next row's are asked for while it is reduced, and the weights stay.
+  constexpr bool kAhead = C <= 2;
+  XT u[C][4];
+  RT v[C][4];
+  float weights[kAhead ? C : 1][4];
+  auto fetch = [&](long long row) {
+    auto get = [&](auto w) {
+      constexpr bool kWhole = decltype(w)::value;
+      const XT* x = static_cast<const XT*>(a.x) + row * a.stride_x + first;
+      const RT* r = static_cast<const RT*>(a.residual) + row * a.stride_residual + first;
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int left = a.W - first - j * jump;    // numbers from this lane's first of the run on
-      XT u[4] = {};
-      RT v[4] = {};
+      for (int i = 0; i < 4 * C; ++i) u[i / 4][i % 4] = kWhole || i * 32 < left ? x[i * 32] : XT(0);
+      if (a.residual) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i * 32 < left) u[i] = x[j * jump + i * 32];
-      if (has_residual) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i * 32 < left) v[i] = r[j * jump + i * 32];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        t[j][i] = make_float2(value_of<X>(u[2 * i]), value_of<X>(u[2 * i + 1]));
-        if (has_residual) t[j][i] = add2(t[j][i], make_float2(value_of<R>(v[2 * i]), value_of<R>(v[2 * i + 1])));
-      }
-    }
-    auto weigh_all = [&](auto tag) {
-      using T = typename Number<decltype(tag)::value>::type;
-      const T* w = static_cast<const T*>(a.weight) + first;
-#pragma unroll
-      for (int j = 0; j < C; ++j) {
-        const int left = a.W - first - j * jump;
-        T u[4] = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i * 32 < left) u[i] = w[j * jump + i * 32];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) t[j][i] = mul2(t[j][i], make_float2(value_of<decltype(tag)::value>(u[2 * i]), value_of<decltype(tag)::value>(u[2 * i + 1])));
+        for (int i = 0; i < 4 * C; ++i) v[i / 4][i % 4] = kWhole || i * 32 < left ? r[i * 32] : RT(0);
       }
     };
+    if (row >= a.N) return;
+    if (whole) get(std::true_type());
+    else get(std::false_type());
+  };
+  if constexpr (kAhead) {
+    fetch(blockIdx.x);
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int left = a.W - first - j * jump;
+    for (int i = 0; i < 4 * C; ++i) weights[i / 4][i % 4] = i * 32 < left ? load_as_float(a.weight, first + i * 32, a.weight_dtype) : 0.0f;
+  }
+  int turn = 0;
+  for (long long row = blockIdx.x; row < a.N; row += gridDim.x, turn ^= 1) {
+    float2 t[C][2], ss = make_float2(0.0f, 0.0f);
+    float large = 0.0f, top[C], all = 0.0f;
+    auto sum_up = [&] {
+#pragma unroll
+      for (int i = 0; i < 2 * C; ++i) {
+        t[i / 2][i % 2] = make_float2(value_of<X>(u[i / 2][i % 2 * 2]), value_of<X>(u[i / 2][i % 2 * 2 + 1]));
+        if (a.residual)
+          t[i / 2][i % 2] = add2(t[i / 2][i % 2], make_float2(value_of<R>(v[i / 2][i % 2 * 2]), value_of<R>(v[i / 2][i % 2 * 2 + 1])));
+      }
+    };
+    if constexpr (kAhead) {
+      sum_up();
+      fetch(row + gridDim.x);
+    }
+    auto enter = [&](auto w) {
+      constexpr bool kWhole = decltype(w)::value;
+      RT* out = static_cast<RT*>(a.residual_out) + row * a.stride_residual_out + first;
+      auto there = [&](int at) { return kWhole || at < left; };
+      if constexpr (!kAhead) {
+        const XT* x = static_cast<const XT*>(a.x) + row * a.stride_x + first;
+        const RT* r = static_cast<const RT*>(a.residual) + row * a.stride_residual + first;
+#pragma unroll
+        for (int i = 0; i < 4 * C; ++i) u[i / 4][i % 4] = there(i * 32) ? x[i * 32] : XT(0);
+        if (a.residual) {
+#pragma unroll
+          for (int i = 0; i < 4 * C; ++i) v[i / 4][i % 4] = there(i * 32) ? r[i * 32] : RT(0);
+        }
+        sum_up();
+      }
       if (a.residual_out) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2 * C; ++i) {
           RT low, high;
-          round_two<R>(t[j][i], low, high);
-          if (i * 64 < left) out[j * jump + i * 64] = low;
-          if (i * 64 + 32 < left) out[j * jump + i * 64 + 32] = high;
+          round_two<R>(t[i / 2][i % 2], low, high);
+          if (there(i * 64)) out[i * 64] = low;
+          if (there(i * 64 + 32)) out[i * 64 + 32] = high;
         }
       }
-      add_squares(t[j], ss, large);
-    }
-    if (a.weight_dtype == CARRY_BF16) weigh_all(std::integral_constant<int, CARRY_BF16>());
-    else if (a.weight_dtype == CARRY_F16) weigh_all(std::integral_constant<int, CARRY_F16>());
-    else weigh_all(std::integral_constant<int, CARRY_F32>());
+#pragma unroll
+      for (int j = 0; j < C; ++j) add_squares(t[j], ss, large);
+      auto weigh_all = [&](auto tag) {
+        constexpr int T = decltype(tag)::value;
+        const typename Number<T>::type* weight = static_cast<const typename Number<T>::type*>(a.weight) + first;
+#pragma unroll
+        for (int i = 0; i < 2 * C; ++i)
+          t[i / 2][i % 2] = mul2(t[i / 2][i % 2], make_float2(there(i * 64) ? value_of<T>(weight[i * 64]) : 0.0f,
+                                                              there(i * 64 + 32) ? value_of<T>(weight[i * 64 + 32]) : 0.0f));
+      };
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int i = 0; i < 2 * C; ++i) t[i / 2][i % 2] = mul2(t[i / 2][i % 2], make_float2(weights[i / 2][i % 2 * 2], weights[i / 2][i % 2 * 2 + 1]));
+      } else if (a.weight_dtype == CARRY_BF16) weigh_all(std::integral_constant<int, CARRY_BF16>());
+      else if (a.weight_dtype == CARRY_F16) weigh_all(std::integral_constant<int, CARRY_F16>());
+      else weigh_all(std::integral_constant<int, CARRY_F32>());
+    };
+    if (whole) enter(std::true_type());
+    else enter(std::false_type());
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       top[j] = fmaxf(fmaxf(fabsf(t[j][0].x), fabsf(t[j][0].y)), fmaxf(fabsf(t[j][1].x), fabsf(t[j][1].y)));
@@ -354,20 +381,23 @@ __global__ void __launch_bounds__(512, any_ctas(C)) norm_any_kernel(const __grid
       const float scale = scale_of(s, s.top, by);
       if (threadIdx.x == 0) a.scale[row] = scale;
     }
+    auto leave = [&](auto w) {
+      constexpr bool kWhole = decltype(w)::value;
+      uint8_t* codes = a.codes + row * a.stride_codes + first;
+      auto there = [&](int at) { return kWhole || at < left; };
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int left = a.W - first - j * jump;
-      if (a.group) {
-        const float scale = scale_of(s, __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top[j]))), by);
-        if (lane == 0 && left > 0) a.scale[row * groups + (first + j * jump) / kGroup] = scale;
+      for (int i = 0; i < 2 * C; ++i) {
+        if (a.group && i % 2 == 0) {
+          const float scale = scale_of(s, __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top[i / 2]))), by);
+          if (lane == 0 && there(i * 64)) a.scale[row * groups + run0 + i / 2] = scale;
+        }
+        const uint32_t c = __nv_cvt_float2_to_fp8x2(mul2(t[i / 2][i % 2], make_float2(by, by)), __NV_SATFINITE, __NV_E4M3);
+        if (there(i * 64)) codes[i * 64] = static_cast<uint8_t>(c);
+        if (there(i * 64 + 32)) codes[i * 64 + 32] = static_cast<uint8_t>(c >> 8);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t c = __nv_cvt_float2_to_fp8x2(mul2(t[j][i], make_float2(by, by)), __NV_SATFINITE, __NV_E4M3);
-        if (i * 64 < left) codes[j * jump + i * 64] = static_cast<uint8_t>(c);
-        if (i * 64 + 32 < left) codes[j * jump + i * 64 + 32] = static_cast<uint8_t>(c >> 8);
-      }
-    }
+    };
+    if (whole) leave(std::true_type());
+    else leave(std::false_type());
   }
 }
 
@@ -393,7 +423,10 @@ int launch_any(const NormParams& p, cudaStream_t stream) {
 }
 template <int X, int R>
 int launch_any(const NormParams& p, cudaStream_t stream) {
-  if (p.a.W <= 2048 && p.a.N <= sm_count()) return launch_any<1, X, R>(p, stream);
+  // A row of 256 is a warp or two, which would wait for memory row by row (220 us for 2^26 numbers; 175 ahead of it); few rows
+  // have all warps at work, and the weights on their way with the rest (one of 4097 3.4 us, 4.2 the other way).
+  if (p.a.W <= 256 || (p.a.W <= 2048 && p.a.N <= sm_count())) return launch_any<1, X, R>(p, stream);
+  if (p.a.W <= 4096 && p.a.N <= sm_count()) return launch_any<2, X, R>(p, stream);
   if (p.a.W <= 8192) return launch_any<4, X, R>(p, stream);
   return p.a.W <= 16384 ? launch_any<8, X, R>(p, stream) : launch_any<16, X, R>(p, stream);
 }
@@ -422,11 +455,13 @@ int launch_norm(const CarryGdnNormArgs& a, cudaStream_t stream) {
   rows(a.residual_out, a.stride_residual_out, size(a.residual_dtype), 16);
   rows(a.weight, 0, size(a.weight_dtype), 16);
   rows(a.codes, a.stride_codes, 1, 8);
-  // the residual stream has x's type or is fp32; other pairs go an element at a time
+  // the residual stream has x's type or is fp32; other pairs go a number at a time
   const int xd = a.x_dtype, rd = a.residual_dtype;
   if (vec && xd == CARRY_BF16 && rd == CARRY_BF16) return launch_typed<CARRY_BF16, CARRY_BF16>(p, stream);
   if (vec && xd == CARRY_F16 && rd == CARRY_F16) return launch_typed<CARRY_F16, CARRY_F16>(p, stream);
-  if (vec && xd == CARRY_F32 && rd == CARRY_F32) return launch_typed<CARRY_F32, CARRY_F32>(p, stream);
+  // fp32 rows fill whole lines a number to a lane as well, and hold fewer registers so: 16384 rows of 4096 144 us, eight
+  // numbers to a lane 172.  Few rows wait for one trip to memory less the other way (200 of 4096 3.5 us, 5.0).
+  if (vec && xd == CARRY_F32 && rd == CARRY_F32 && (a.W <= 256 || a.N <= 4 * sm_count())) return launch_typed<CARRY_F32, CARRY_F32>(p, stream);
   if (vec && xd == CARRY_BF16 && rd == CARRY_F32) return launch_typed<CARRY_BF16, CARRY_F32>(p, stream);
   if (vec && xd == CARRY_F16 && rd == CARRY_F32) return launch_typed<CARRY_F16, CARRY_F32>(p, stream);
   return launch_any(p, stream);
