@@ -400,30 +400,29 @@ __device__ __forceinline__ void merge_warps(DecodeShared<D, NT, PARTS>& sh, Runn
   __syncthreads();
 }
 
-// A (request, head) to a cluster of eight CTAs: one launch, where the line's way takes two.  For short contexts of few
-// (request, head)s.  An eighth of the columns is each CTA's to join: all 32 warps of the cluster put what they have of it,
-// normalised, into its shared memory, and one barrier later it is done.  (Joining the warps of a CTA first and reading the
-// others' results afterwards took 2 us longer, of 7.6 for one token over 16.)
-constexpr int kCluster = 8, kSources = kCluster * kWarps;
-
-template <int D, int NT, int PARTS>
+// A (request, head) to a cluster of CL CTAs: one launch, where the line's way takes two.  For short contexts.  A CL-th of
+// the columns is each CTA's to join: all warps of the cluster put what they have of it, normalised, into its shared memory, and
+// one barrier later it is done.  (Joining the warps of a CTA first and reading the others' results afterwards took 2 us longer,
+// of 7.6 for one token over 16.)
+__host__ __device__ constexpr int pair_stages(int D) { return D == 128 ? 2 : 3; }       // two CTAs to an SM
+template <int D, int NT, int PARTS, int CL>
 struct PairShared {
-  RunStage<D> stage[kWarps][stages(D, NT, PARTS)];
-  alignas(16) float o[kSources][NT * 8][D / 8];
-  float top[kSources][NT * 8], sum[kSources][NT * 8];
+  RunStage<D> stage[kWarps][pair_stages(D)];
+  alignas(16) float o[CL * kWarps][NT * 8][D / CL];
+  float top[CL * kWarps][NT * 8], sum[CL * kWarps][NT * 8];
 };
 
-template <int D, int NT, int PARTS>
+template <int D, int NT, int PARTS, int CL>
 __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t raw[];
-  PairShared<D, NT, PARTS>& sh = *reinterpret_cast<PairShared<D, NT, PARTS>*>(raw);
-  constexpr int kStages = stages(D, NT, PARTS);
+  PairShared<D, NT, PARTS, CL>& sh = *reinterpret_cast<PairShared<D, NT, PARTS, CL>*>(raw);
+  constexpr int kStages = pair_stages(D), kSources = CL * kWarps, kColumns = D / CL;
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   depend_release();
   depend_wait();
   const CarryGdnKvCache& c = p.a.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, cc = lane % 4;
-  const int rank = blockIdx.x % kCluster, pair = blockIdx.x / kCluster;
+  const int rank = blockIdx.x % CL, pair = blockIdx.x / CL;
   Cursor use;
   use.b = pair / c.HKV;
   use.h = pair % c.HKV;
@@ -438,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
   auto next_load = [&](int stage) {
     if (load.tile < load.tiles) {
       load_run<D>(p, sh.stage[warp][stage], load, pages);
-      load.tile += kCluster;
+      load.tile += CL;
       if (load.tile < load.tiles) pages = fetch_run(p, load);
     }
     __pipeline_commit();
@@ -448,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
   Running<D, NT> r;
   r.clear();
   int stage = 0;
-  for (; use.tile < use.tiles; use.tile += kCluster) {
+  for (; use.tile < use.tiles; use.tile += CL) {
     __pipeline_wait_prior(kStages - 2);
     __syncwarp();
     next_load(stage == 0 ? kStages - 1 : stage - 1);
@@ -466,10 +465,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
-  // lane (g, c) has the columns that are CTA g's, of rows 8 n + 2 c and + 1
+  // lane (g, c) has the g-th eighth of the columns, of rows 8 n + 2 c and + 1
   const auto cluster = cooperative_groups::this_cluster();
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // every CTA has started
-  PairShared<D, NT, PARTS>& theirs = *cluster.map_shared_rank(&sh, g);
+  PairShared<D, NT, PARTS, CL>& theirs = *cluster.map_shared_rank(&sh, g * CL / 8);
   const int source = rank * kWarps + warp;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -482,14 +481,14 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
       theirs.top[source][row] = r.top[n][i];
       theirs.sum[source][row] = sum;
       const float w = sum == 0.0f ? 0.0f : __fdiv_rn(r.unit * exp2f(-kWeightUp), sum);
-      float4* to = reinterpret_cast<float4*>(theirs.o[source][row]);
+      float4* to = reinterpret_cast<float4*>(theirs.o[source][row] + g % (8 / CL) * (D / 8));
 #pragma unroll
       for (int m = 0; m < D / 16; m += 2)
         to[m / 2] = make_float4(r.o[n][m][i] * w, r.o[n][m][i + 2] * w, r.o[n][m + 1][i] * w, r.o[n][m + 1][i + 2] * w);
     }
   cluster.sync();
-  for (int i = threadIdx.x; i < request.todo * p.group * (D / 8); i += kThreads) {
-    const int row = i / (D / 8), col = i % (D / 8);
+  for (int i = threadIdx.x; i < request.todo * p.group * kColumns; i += kThreads) {
+    const int row = i / kColumns, col = i % kColumns;
     float top = -INFINITY, total = 0.0f, x = 0.0f;
 #pragma unroll
     for (int n = 0; n < kSources; ++n) top = fmaxf(top, sh.top[n][row]);
@@ -500,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
       total += w;
       x = fmaf(w, sh.o[n][row][col], x);
     }
-    store_from_float(p.a.out, row_place(p, request, use.h, row, token_of(p, row), p.a.stride_out_tok, p.a.stride_out_head) + rank * (D / 8) + col,
+    store_from_float(p.a.out, row_place(p, request, use.h, row, token_of(p, row), p.a.stride_out_tok, p.a.stride_out_head) + rank * kColumns + col,
                      p.a.dtype, total == 0.0f ? 0.0f : __fdiv_rn(x, total));
   }
 }
@@ -778,11 +777,11 @@ long long decode_ctas(const CarryGdnKvAttentionArgs& a) {
   return most < 1 ? 1 : most < fit ? most : fit;
 }
 
-// launch_dependent() with clusters of kCluster CTAs, so many of them.
+// launch_dependent() with clusters of so many CTAs.
 template <class K, class... A>
-int launch_clusters(K kernel, int clusters, size_t smem, cudaStream_t stream, const A&... args) {
+int launch_clusters(K kernel, int clusters, int size, size_t smem, cudaStream_t stream, const A&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)clusters * kCluster);
+  cfg.gridDim = dim3((unsigned)clusters * size);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -790,7 +789,7 @@ int launch_clusters(K kernel, int clusters, size_t smem, cudaStream_t stream, co
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kCluster;
+  attr[1].val.clusterDim.x = size;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
@@ -799,23 +798,38 @@ int launch_clusters(K kernel, int clusters, size_t smem, cudaStream_t stream, co
   return CARRY_GDN_ERR_LAUNCH;
 }
 
-// Whether clusters take a call: all of them have to be resident, and a context be short enough for eight CTAs.  One
-// request of 1500 tokens and 8 heads takes 8.2 us so, 11.4 by the line; four of 4096 15.7 and 18.2.
-bool by_pairs(const CarryGdnKvAttentionArgs& a) {
+// CTAs of the clusters that take a call, or 0: as many as leave all clusters resident, two CTAs to an SM but for what the
+// groups of SMs that a cluster has to fit in leave over; and where a context is four tiles for each CTA at most.  One request of
+// 1500 tokens and 8 heads takes 8.2 us so (clusters of eight), 11.4 by the line, four of 4096 15.7 and 18.2; 16 of 128 (two)
+// 6.1 and 11.8, 32 of 300 (one) 9.5 and 14.7.  With more than are resident at a time the line is as good: 56 of 120 18.1 and 19.5,
+// of 500 38.6 and 35.8.
+int cluster_size(const CarryGdnKvAttentionArgs& a) {
   const long long tokens = (long long)a.cache.max_pages * a.cache.page, pairs = (long long)a.rows.B * a.cache.HKV;
-  return pairs * kCluster <= 2LL * sm_count() && tokens <= 4LL * kCluster * kLine;
+  for (int size = 8; size > 0; size /= 2)
+    if (4 * pairs * size <= 7LL * sm_count()) return tokens <= 4LL * size * kLine ? size : 0;
+  return 0;
+}
+
+template <int D, int NT, int PARTS, int CL>
+int launch_pairs(const AttnParams& p, cudaStream_t stream) {
+  constexpr size_t smem = sizeof(PairShared<D, NT, PARTS, CL>);
+  static thread_local bool ready[64];
+  const int rc = prepare(kv_pair_kernel<D, NT, PARTS, CL>, smem, ready);
+  return rc == CARRY_GDN_OK ? launch_clusters(kv_pair_kernel<D, NT, PARTS, CL>, p.a.rows.B * p.a.cache.HKV, CL, smem, stream, p) : rc;
 }
 
 template <int D, int NT, int PARTS>
 int launch_decode(const AttnParams& p, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(DecodeShared<D, NT, PARTS>), pair_smem = sizeof(PairShared<D, NT, PARTS>);
-  static thread_local bool ready[2][64];
-  if (by_pairs(p.a)) {
-    const int rc = prepare(kv_pair_kernel<D, NT, PARTS>, pair_smem, ready[0]);
-    return rc == CARRY_GDN_OK ? launch_clusters(kv_pair_kernel<D, NT, PARTS>, p.a.rows.B * p.a.cache.HKV, pair_smem, stream, p) : rc;
+  constexpr size_t smem = sizeof(DecodeShared<D, NT, PARTS>);
+  static thread_local bool ready[64];
+  switch (cluster_size(p.a)) {
+    case 8: return launch_pairs<D, NT, PARTS, 8>(p, stream);
+    case 4: return launch_pairs<D, NT, PARTS, 4>(p, stream);
+    case 2: return launch_pairs<D, NT, PARTS, 2>(p, stream);
+    case 1: return launch_pairs<D, NT, PARTS, 1>(p, stream);
   }
   const unsigned ctas = (unsigned)decode_ctas(p.a);
-  int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem, ready[1]);
+  int rc = prepare(kv_decode_kernel<D, NT, PARTS>, smem, ready);
   if (rc == CARRY_GDN_OK) rc = launch_dependent(kv_decode_kernel<D, NT, PARTS>, dim3(ctas), kThreads, smem, stream, p);
   if (rc != CARRY_GDN_OK) return rc;
   const long long pairs = (long long)p.a.rows.B * p.a.cache.HKV;
@@ -833,7 +847,7 @@ int launch_tiles(const AttnParams& p, cudaStream_t stream) {
 bool few_rows(const CarryGdnKvAttentionArgs& a) { return column_tiles(a) > 0; }
 
 int64_t kv_decode_workspace(const CarryGdnKvAttentionArgs& a) {
-  if (by_pairs(a)) return 0;
+  if (cluster_size(a)) return 0;
   const long long ctas = decode_ctas(a);
   return sizeof(Piece) * ctas + 2 * ctas * slot_floats(column_tiles(a) * 8, a.cache.D) * 4;
 }
