@@ -799,11 +799,10 @@ int launch_clusters(K kernel, int clusters, int size, size_t smem, cudaStream_t 
 }
 
 // CTAs of the clusters that take a call, or 0: as many as leave all clusters resident, two CTAs to an SM but for what the
-// groups of SMs that a cluster has to fit in leave over; no more than a context has tiles, and
-// four tiles for each CTA at most.  One request of
-// 1500 tokens and 8 heads takes 8.2 us so (clusters of eight), 11.4 by the line, four of 4096 15.7 and 18.2; 16 of 128 (two)
-// 6.1 and 11.8, 32 of 300 (one) 9.5 and 14.7.  With more than are resident at a time the line is as good: 56 of 120 18.1 and 19.5,
-// of 500 38.6 and 35.8.
+// groups of SMs that a cluster has to fit in leave over; no more than a context has tiles, and four tiles for each CTA at most.
+// One request of 1500 tokens and 8 heads takes 8.2 us so (clusters of eight), 11.4 by the line, four of 4096 15.7 and 18.2; 16 of
+// 128 6.1 and 11.8, 32 of 300 (one CTA each) 9.5 and 14.7.  With more than are resident at a time the line is as good: 56 requests
+// of 120 and 16 heads 18.1 and 19.5, of 500 38.6 and 35.8.
 int cluster_size(const CarryGdnKvAttentionArgs& a) {
   const long long tokens = (long long)a.cache.max_pages * a.cache.page, pairs = (long long)a.rows.B * a.cache.HKV;
   for (int size = 8; size > 0; size /= 2)
