@@ -632,6 +632,7 @@ void lay_out(const CarryGdnKvAttentionArgs& a, int& splits, int& padded) {
   const long long tiles = row_tiles(a), pairs = (long long)a.cache.HKV * a.rows.B, sms = sm_count();
   splits = 1;
   padded = tiles > 65535 ? -1 : 0;
+  if (pairs == 0 || sms == 0) return;
   const long long late = tiles * pairs % sms, cut = tiles - (tiles * pairs - late) / pairs;
   if (cut == 0 || cut > 1024 || tiles > 30000) return;
   const long long cached = max((long long)a.cache.max_pages * a.cache.page - a.rows.max_query, 0LL);

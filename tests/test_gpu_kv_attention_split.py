@@ -35,3 +35,15 @@ def test_the_first_rows_of_a_prompt_are_cut(length, tokens):
     for first in (0, 127, 253, 511, 767, 1279, tokens - 3):
         rows = slice(first, first + 3)
         check(out[rows], q[rows], 0.125, cache, table, [length - tokens + first + 3], "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_rows_of_no_request(rows, dtype):
+    """Rows that no request claims are left as they are."""
+    g = torch.Generator().manual_seed(9)
+    cache = make_cache(3, 2, 32, 64, 32, g)
+    q = torch.randn(rows, 4, 64, generator=g).to(TYPES[dtype])
+    table = torch.zeros(0, 4, dtype=torch.int32)
+    out = attend(q, 0.125, cache, table, [], query_start=[0], max_query_len=rows)
+    assert (out == 7).all()
