@@ -20,7 +20,8 @@ LIB = os.path.join(PKG, "libcarry_gdn.so")
 # Test-only twin of the library, built with CARRY_TEST_WAIT_EXPIRY: one tile's copies never complete and the
 # wait limit is short, so that tests/test_gpu_wait_expiry.py can watch a bounded wait run out; it also
 # forces, reports and (with an extra kernel that writes a buffer late) provokes the path of set-up inputs
-# that changed under the streaming kernel's feet.  Nothing in the package loads it.
+# that changed under the streaming kernel's feet.  The many-row attention's warps come late there
+# (tests/test_gpu_kv_attention_waits.py).  Nothing in the package loads it.
 WAIT_TEST_LIB = os.path.join(PKG, "libcarry_gdn_waittest.so")
 # Native call path of the Python surfaces (CPython extension over torch's C++ tensors; no device code)
 NATIVE_SOURCE = "host_native.cpp"
@@ -86,7 +87,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(obj_dir, exist_ok=True)
 
     # the sources whose code differs in the test-only twin (the kernels that wait for bulk copies)
-    twin_sources = ("carry_gdn_tile128_vk.cu", "carry_gdn_tile128_kv.cu", "carry_gdn_multi.cu", "carry_gdn_dense128.cu")
+    twin_sources = ("carry_gdn_tile128_vk.cu", "carry_gdn_tile128_kv.cu", "carry_gdn_multi.cu", "carry_gdn_dense128.cu",
+                    "carry_kv_prefill.cu")
 
     def compile_one(job):
         src, twin = job

@@ -39,6 +39,10 @@ struct Shared {
   alignas(16) float ks[kNotes][kBlocks], bias[kNotes][kBlocks], counts[kNotes][kBlocks];
   float rescale[kNotes], unit;
   uint64_t raw_full[kRawStages], raw_free[kRawStages], k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages];
+  // The rows' threads wait here for a step's notes, and not at k_full, which runs up to three steps ahead of them: once
+  // everybody has left the weights of step - 1, the keys of step + 3 can be there before a late warp asks for those of `step`,
+  // and a phase that is two behind is not seen.  The notes of step + 8 wait for the weights of step + 2.
+  uint64_t noted[kNotes];
   uint64_t s_full[2][2], p_full[2][2], o_done[2][2];   // by tile, and by step's parity
   uint32_t tmem;
   int poison;
@@ -47,7 +51,17 @@ static_assert(kRawStages + kStages < kNotes, "notes outlive their step");
 
 // ---- waiting ---------------------------------------------------------------------------------------------------------
 
-constexpr int kSpinLimit = 1 << 20;               // polls of a barrier, each of which the hardware may hold for a while
+// Polls of a barrier, each of which the hardware may hold for a while.  The test-only build has a warp of every row tile
+// come late to each of its steps, by more than the other warps' work on three: results must not depend on it.
+#ifdef CARRY_TEST_WAIT_EXPIRY
+constexpr int kSpinLimit = 1 << 14;
+__device__ __forceinline__ void test_come_late(int warp, int step) {
+  if (warp % 4 == step % 4) __nanosleep(4000);
+}
+#else
+constexpr int kSpinLimit = 1 << 20;
+__device__ __forceinline__ void test_come_late(int, int) {}
+#endif
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void barrier_init(uint64_t* bar, uint32_t count) {
@@ -334,6 +348,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
       barrier_init(&sh.k_free[i], 1);
       barrier_init(&sh.v_free[i], 1);
     }
+    for (int i = 0; i < kNotes; ++i) barrier_init(&sh.noted[i], 1);
     for (int i = 0; i < 4; ++i) {
       barrier_init(&sh.s_full[i / 2][i % 2], 1);
       barrier_init(&sh.p_full[i / 2][i % 2], kTileRows);
@@ -368,8 +383,9 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     float top = -INFINITY, sum = 0.0f;
     bool healthy = true;
     for (int step = 0; step < steps && tile < tiles; ++step) {
-      const int stage = step % kStages, note = step % kNotes, turn = step & 1;
-      healthy = __all_sync(~0u, barrier_wait(&sh.k_full[stage], step / kStages & 1, poison, p.a.status) &&
+      const int note = step % kNotes, turn = step & 1;
+      test_come_late(warp, step);
+      healthy = __all_sync(~0u, barrier_wait(&sh.noted[note], step / kNotes & 1, poison, p.a.status) &&
                                     barrier_wait(&sh.s_full[tile][turn], step / 2 & 1, poison, p.a.status));
       if (!healthy) break;
       fence_after();
@@ -548,7 +564,10 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         sh.unit = unit;
       }
       __syncwarp();
-      if (lane == 0) barrier_expect(&sh.raw_full[raw], 2 * kGranule * D * __popc(there));     // what was written above goes with it
+      if (lane == 0) {                            // what was written above goes with both
+        barrier_arrive(&sh.noted[note]);
+        barrier_expect(&sh.raw_full[raw], 2 * kGranule * D * __popc(there));
+      }
       __syncwarp();
       if (now.id > 0) {
         const int at = (h * c.page + now.in_page * kGranule) * D, to = lane * kGranule * D;
