@@ -32,6 +32,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_parts_kernel(const __gri
   if (i >= q.todo || row >= p.padded) return;
   const Parts mine = parts_of(p, min(lane, p.splits - 1), blockIdx.x);
   float top = lane < p.splits ? mine.top[row] : -INFINITY, w = lane < p.splits ? mine.sum[row] : 0.0f;
+  if (__any_sync(~0u, w == kNoPart)) return;
   const float all_top = warp_max(top), base = all_top == -INFINITY ? 0.0f : all_top;
   w *= exp2_fast(top - base);
   float sum = w, o[D / 32] = {};

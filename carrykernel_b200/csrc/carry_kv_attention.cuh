@@ -22,7 +22,8 @@ struct AttnParams {
 };
 
 // What a part of a context leaves for the joining kernel, by part, (request, head) and row: largest score and sum of
-// weights, then the outputs, normalised.
+// weights, then the outputs, normalised.  A part whose waits ran out leaves kNoPart as the sum, and the row stays as it was.
+constexpr float kNoPart = -1.0f;
 struct Parts {
   float *top, *sum, *o;
 };

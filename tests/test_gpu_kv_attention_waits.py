@@ -1,5 +1,6 @@
 """The waits of the many-row attention over the 8-bit key/value cache, in the test-only twin of the library, where every
-softmax warp comes microseconds late to a quarter of its steps."""
+softmax warp comes microseconds late to a quarter of its steps, and, in caches of three heads, the first copies of request 0's
+head 1 never complete."""
 
 import pytest
 import torch
@@ -30,3 +31,23 @@ def test_a_late_warp_misses_no_phase(lengths, tokens, HQ, HKV, D):
         got = attend(*call, status=status)
     assert status.item() == 0 and torch.equal(got, want)
     check(got, *call, "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lengths,tokens", [([130, 200], 80), ([1500, 1300, 20], 40), ([3000], 300)])
+def test_rows_of_a_wait_that_runs_out_are_left_as_they_were(lengths, tokens, dtype):
+    """Contexts whole and cut into parts: the other rows come out as they should, nothing is joined from what is missing."""
+    from carrykernel_b200 import _lib
+    call = made(lengths, tokens, 6, 3, 128, dtype, seed=tokens)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    want = attend(*call, status=status)
+    assert status.item() == 0
+    with wait_test_library():
+        got = attend(*call, status=status)
+    assert status.item() == _lib.STATUS_TIMEOUT
+    want[:tokens, 2:4] = 7.0                             # what `attend` fills its output with
+    assert torch.equal(got, want)
+    status.zero_()
+    want = attend(*call, status=status)
+    assert status.item() == 0
+    check(want, *call, dtype)
