@@ -14,9 +14,12 @@
 // 870 TFLOP/s, 53 % of the burst rate of a large matrix product, at a clock that the GPU's power brings down to some 1.5 GHz.
 // A CTA's way in and out is some 7 us: six prompts of up to 2000 tokens and 16 heads take 95 us, 415 TFLOP/s, half of it that.
 //
-// A row's weights are relative to a maximum that is replaced, and O rescaled, only when it is outgrown by 2^4; values
-// likewise count in the largest value scale until one is 2^4 larger.  A weight is formed times 2^7, so it stays below
-// fp16's 2^16, and has all its bits down to 2^-21 of the row's largest.
+// A row's weights are relative to a maximum that is replaced, and O rescaled, only when it is outgrown by 2^4.  With the value
+// scales of their blocks they count in a unit of the row's own, the largest weight times scale that it has met to within a
+// power of two, which is looked at again when the maximum moves or a scale is 2^4 above it: blocks that a row does not see, or hardly
+// weighs, cost it no bits.  A weight is formed times 2^7, so it stays below fp16's 2^16, and has all its bits down to 2^-21 of
+// the row's largest.  The sum takes the scale off again, block by block; scales below 2^-60 of the unit count as 2^-60 in both places, so
+// that neither flushes: their values are lost to fp16 and their weights are not.
 #include "carry_kv_attention.cuh"
 
 namespace carry {
@@ -27,17 +30,17 @@ constexpr int kRowPlane = kTileRows * 128, kTokenPlane = kTokens * 128;        /
 constexpr int kSoftmaxThreads = kCtaRows, kConvertThreads = 128;
 constexpr int kFetchWarp = (kSoftmaxThreads + kConvertThreads) / 32, kIssueWarp = kFetchWarp + 1, kAllThreads = (kIssueWarp + 1) * 32;
 constexpr int kBlocks = kTokens / kGranule;
-constexpr float kUp = 7.0f, kSlack = 4.0f;
+constexpr float kUp = 7.0f, kSlack = 4.0f, kLow = -60.0f, kUnitFloor = -100.0f;
 
 template <int D>
 struct Shared {
   uint8_t q[2][D / 64][kRowPlane], k[kStages][D / 64][kTokenPlane], v[kStages][D / 64][kTokenPlane];
   uint8_t raw_k[kRawStages][kTokens * D], raw_v[kRawStages][kTokens * D];        // codes as the cache has them
-  // of a step's blocks: key scale, log2 of the value scale in the running unit plus kUp, and what a weight so formed
-  // counts in the row's sum.  A step's notes are written again kNotes steps later, when everybody is long done with it:
+  // of a step's blocks: key scale, log2 of the value scale (minus infinity below 2^-100) and one over it, and of the step the
+  // largest of the logarithms.  A step's notes are written again kNotes steps later, when everybody is long done with it:
   // kRawStages + kStages steps at most are under way.
-  alignas(16) float ks[kNotes][kBlocks], bias[kNotes][kBlocks], counts[kNotes][kBlocks];
-  float rescale[kNotes], unit;
+  alignas(16) float ks[kNotes][kBlocks], vs[kNotes][kBlocks], vs_inv[kNotes][kBlocks];
+  float vs_top[kNotes];
   uint64_t raw_full[kRawStages], raw_free[kRawStages], k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages];
   // The rows' threads wait here for a step's notes, and not at k_full, which runs up to three steps ahead of them: once
   // everybody has left the weights of step - 1, the keys of step + 3 can be there before a late warp asks for those of `step`,
@@ -341,7 +344,6 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
 
   if (threadIdx.x == 0) {
     sh.poison = 0;
-    sh.unit = 1.0f;
     for (int i = 0; i < kRawStages; ++i) {
       barrier_init(&sh.raw_full[i], 1);
       barrier_init(&sh.raw_free[i], kConvertThreads);
@@ -384,7 +386,8 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     const int sees = i < r.todo ? r.length - r.count + i + 1 : 0;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem + lanes + 256 + tile * 128;
-    float top = -INFINITY, sum = 0.0f;
+    // outputs count in 2^(unit - kUp), which is `in_unit`, beside 2^top
+    float top = -INFINITY, sum = 0.0f, unit = kUnitFloor, in_unit = exp2f(kUnitFloor - kUp);
     bool healthy = true;
     for (int step = 0; step < steps && tile < tiles; ++step) {
       const int note = step % kNotes, turn = step & 1;
@@ -393,13 +396,13 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
                                     barrier_wait(&sh.s_full[tile][turn], step / 2 & 1, poison, p.a.status));
       if (!healthy) break;
       fence_after();
-      float x[2][32], now = top, by[kBlocks], ks[kBlocks], bias[kBlocks], counts[kBlocks];
+      float x[2][32], now = top, by[kBlocks], peak[kBlocks], ks[kBlocks], vs[kBlocks], vs_inv[kBlocks];
       tmem_load(s_at + turn * 64, x[0]);
       tmem_load(s_at + turn * 64 + 32, x[1]);
       *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(sh.ks[note]);
-      *reinterpret_cast<float4*>(bias) = *reinterpret_cast<const float4*>(sh.bias[note]);
-      *reinterpret_cast<float4*>(counts) = *reinterpret_cast<const float4*>(sh.counts[note]);
-      const float values = sh.rescale[note];
+      *reinterpret_cast<float4*>(vs) = *reinterpret_cast<const float4*>(sh.vs[note]);
+      *reinterpret_cast<float4*>(vs_inv) = *reinterpret_cast<const float4*>(sh.vs_inv[note]);
+      const float vs_top = sh.vs_top[note];
       const int limit = sees - (step0 + step) * kTokens;
       bool all = limit >= kTokens;
 #pragma unroll
@@ -420,17 +423,23 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           n = fmaxf(n, fmaxf(y[e + 2], y[e + 3]));
         }
         by[block] = fmaxf(unit_q * ks[block], 0x1p-126f);
-        now = fmaxf(now, fmaxf(m, n) * by[block]);
+        peak[block] = fmaxf(m, n) * by[block];
+        now = fmaxf(now, peak[block]);
       }
-      if (__any_sync(~0u, now > top + kSlack) || values != 1.0f) {
-        const float keep = now == -INFINITY ? 1.0f : exp2_fast(top - now);
-        sum *= keep;
+      if (__any_sync(~0u, now > top + kSlack || (vs_top > unit + kSlack && now > -INFINITY))) {
+        const float moved = now == -INFINITY ? 0.0f : top - now, zero = now == -INFINITY ? 0.0f : now, had = unit + moved;
+        float then = fmaxf(had, kUnitFloor);
+#pragma unroll
+        for (int block = 0; block < kBlocks; ++block) then = fmaxf(then, peak[block] + vs[block] - zero);
+        unit = ceilf(then);                       // a whole number, so that powers of two are exact in it
+        in_unit = exp2f(unit - kUp);
         top = now;
+        sum *= exp2_fast(moved);
         if (step > 0) {
           healthy = __all_sync(~0u, barrier_wait(&sh.o_done[tile][turn ^ 1], (step - 1) / 2 & 1, poison, p.a.status));
           if (!healthy) break;
           fence_after();
-          const float less = keep * values;
+          const float less = exp2_fast(had - unit);
 #pragma unroll 1
           for (int n = 0; n < D / 16; ++n) {
             uint32_t o[16];
@@ -443,14 +452,14 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
           wait_stores();
         }
       }
-      const float base = top == -INFINITY ? 0.0f : top;
+      const float rest = (top == -INFINITY ? 0.0f : top) - kUp;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t w[16];
 #pragma unroll
         for (int block = 2 * half; block < 2 * half + 2; ++block) {
           const float* z = x[half] + block % 2 * 16;
-          const float less = bias[block] - base;
+          const float less = fmaxf(vs[block] - unit, kLow) - rest;
           float2 total = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
             total = add2(total, q);
             w[block % 2 * 8 + e / 2] = pack_half2(q.x, q.y);
           }
-          sum = fmaf(total.x + total.y, counts[block], sum);
+          sum = fmaf(total.x + total.y, fminf(in_unit * vs_inv[block], exp2f(-kLow - kUp)), sum);
         }
         tmem_store16(s_at + turn * 64 + half * 16, w);           // over scores that this warp has read
       }
@@ -473,8 +482,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     }
     if (!healthy && splits > 1 && i < r.todo) parts_of(p, part_number, blockIdx.x).sum[row] = kNoPart;
     if (healthy && first_row + warp * 32 < r.todo * p.group) {       // a warp without rows has nothing to leave
-      const float by = sum == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kUp), sum);
-      const float unit = steps > 0 ? *reinterpret_cast<volatile float*>(&sh.unit) : 1.0f;
+      const float by = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
       const Parts part = parts_of(p, part_number, blockIdx.x);
       if (splits > 1 && i < r.todo) {
         part.top[row] = top;
@@ -487,7 +495,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
         if (steps > 0) tmem_load(o_at + n * 32, x);
         wait_loads();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = sum == 0.0f ? 0.0f : x[e] * by * unit;
+        for (int e = 0; e < 32; ++e) x[e] = sum == 0.0f ? 0.0f : x[e] * by * in_unit;
       };
       float x[32];
       uint4 line[8];
@@ -539,35 +547,25 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
   } else if (warp == kFetchWarp) {
     // ---- codes and scales out of the cache ----
     const int lane = threadIdx.x % 32;
-    float unit = 0.0f;
     int raw = 0, parity = 1;
     for (int step = 0; step < steps; ++step) {
       fetch.ahead(step);
       const typename Fetch<D>::Granule& now = fetch.now;
       if (step >= kRawStages && !__all_sync(~0u, barrier_wait(&sh.raw_free[raw], parity, poison, p.a.status))) break;
       const uint32_t there = __ballot_sync(~0u, now.id > 0);
-      float most = now.vs;
+      const bool counts = now.vs >= exp2f(kUnitFloor);
+      const uint32_t bits = __float_as_uint(now.vs);
+      const float vs = counts ? static_cast<int>(bits >> 23) - 127 + __log2f(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u)) : -INFINITY;
+      float most = vs;
 #pragma unroll
       for (int d = kBlocks / 2; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-      most = fmaxf(__shfl_sync(~0u, most, 0), 0x1p-100f);
-      float rescale = 1.0f;
-      if (step == 0) {
-        unit = most;
-      } else if (most > unit * exp2f(kSlack)) {
-        rescale = __fdividef(unit, most);
-        unit = most;
-      }
       const int note = step % kNotes;
       if (lane < kBlocks) {
-        const float ratio = now.vs > 0.0f ? __fdividef(now.vs, unit) : 1.0f;
         sh.ks[note][lane] = now.ks;
-        sh.bias[note][lane] = __log2f(ratio) + kUp;
-        sh.counts[note][lane] = __fdividef(exp2f(-kUp), ratio);
+        sh.vs[note][lane] = vs;
+        sh.vs_inv[note][lane] = counts ? __fdiv_rn(1.0f, now.vs) : INFINITY;
       }
-      if (lane == 0) {
-        sh.rescale[note] = rescale;
-        sh.unit = unit;
-      }
+      if (lane == 0) sh.vs_top[note] = most;
       __syncwarp();
       if (lane == 0) {                            // what was written above goes with both
         barrier_arrive(&sh.noted[note]);
