@@ -7,7 +7,6 @@
 
 namespace carry {
 
-constexpr float kWeightUp = 15.0f;                // where products are formed in registers, weights are formed times 2^15
 constexpr int kGranule = 16;                      // tokens: no page and no block of a scale begins or ends inside
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoTokens = -1.0f;                // in a key scale's place: a padding page, or past the end
@@ -49,6 +48,29 @@ __device__ __forceinline__ uint32_t pack_half2(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+// Where products are formed in registers, a row's weights count, with the value scales of their blocks, in a unit of its own, a
+// power of two within 2^5 of the largest weight times scale that it has met: blocks that a row does not see, or hardly weighs,
+// cost it no bits (weights below 2^-126 are none).  Units stay while scales are within 2^4 of them, below as well where a maximum
+// moves, and rows that have met no others have the same.  What is kept is `up`, 2^11 over the unit: a weight stays below 2^15 in fp16
+// and has all its bits down to 2^-20 of the row's largest.
+constexpr float kUpStart = 0x1p-108f;             // of the largest scale
+constexpr float kSlack = 16.0f;
+// 2^11 over a power of two, both ways
+__device__ __forceinline__ float up_of(float unit) { return __uint_as_float((265u << 23) - __float_as_uint(unit)); }
+// 2^11 over the power of two that is not below x
+__device__ __forceinline__ float up_above(float x) { return up_of(__uint_as_float((__float_as_uint(fmaxf(x, 0x1p-100f)) + 0x7fffffu) & 0x7f800000u)); }
+// Value scales that leave all rows' units as they are.
+struct Scales {
+  float most, least;
+  __device__ __forceinline__ void clear() { most = least = 0.0f; }
+  __device__ __forceinline__ bool fresh() const { return most == 0.0f; }        // no value has counted yet
+  __device__ __forceinline__ void set(float up_most, float up_least) {
+    most = kSlack * up_of(up_most);
+    least = up_of(up_least) * (1.0f / kSlack);
+  }
+};
+// two weights with their values' scale, the scale first: a weight is at most 1, and together they are at most kSlack units
+__device__ __forceinline__ float2 scaled(float2 weights, float vs, float2 up) { return mul2(mul2(weights, make_float2(vs, vs)), up); }
 // four e4m3 codes as fp16 numbers, two to a word
 __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& low, uint32_t& high) {
   asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(low), "=r"(high) : "r"(codes));

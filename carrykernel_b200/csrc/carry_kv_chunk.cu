@@ -114,13 +114,15 @@ template <int D>
 struct Rows {
   float o[D / 8][4];              // lane (g, c): row g columns 2c (D/8) + n and (2c + 1) D/8 + n, then row g + 8's
   float top[2], sum[2];           // of rows g and g + 8; the sums are this lane's share
-  float unit;                     // largest value scale so far: o counts in it, times 2^15
+  float up[2];                    // 2^11 over the unit that a row's outputs count in: o is that many times too large
+  Scales scales;
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
     top[0] = top[1] = -INFINITY;
     sum[0] = sum[1] = 0.0f;
-    unit = 0x1p-100f;             // the smallest scale
+    up[0] = up[1] = kUpStart;
+    scales.clear();
   }
 };
 
@@ -150,7 +152,7 @@ __device__ __forceinline__ void attend(const Stage<D>& s, const Query<D>& q, con
     for (int i = 0; i < 4; ++i) score[n][i] = t + i % 2 < limit[i / 2] ? acc[i] * (q.unit[i / 2] * ks) : -INFINITY;
   }
 
-  float now[2], unit = r.unit;
+  float now[2], vs_top = 0.0f;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     float m = -INFINITY;
@@ -159,43 +161,61 @@ __device__ __forceinline__ void attend(const Stage<D>& s, const Query<D>& q, con
     now[half] = fmaxf(r.top[half], quad_max(m));
   }
 #pragma unroll
-  for (int n = 0; n < kTile / kGranule; ++n) unit = fmaxf(unit, s.vs[n]);
-  if (__any_sync(~0u, now[0] > r.top[0] || now[1] > r.top[1]) || unit > r.unit) {
-    const float less = r.unit == unit ? 1.0f : __fdividef(r.unit, unit);
-    float keep[2];
+  for (int b = 0; b < kTile / kGranule; ++b) vs_top = fmaxf(vs_top, s.vs[b]);
+  if (__any_sync(~0u, now[0] > r.top[0] || now[1] > r.top[1]) || vs_top > r.scales.most) {
+    float keep[2], vs_low = vs_top;
+#pragma unroll
+    for (int b = 0; b < kTile / kGranule; ++b) vs_low = fminf(vs_low, s.ks[b] == kNoTokens ? vs_top : s.vs[b]);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       keep[half] = now[half] == -INFINITY ? 1.0f : exp2_fast(r.top[half] - now[half]);
       r.sum[half] *= keep[half];
       r.top[half] = now[half];
-      keep[half] *= less;
     }
-    r.unit = unit;
+    // what follows is the same in every lane
+    if (r.scales.fresh() && vs_top > 0.0f && vs_low * kSlack >= vs_top) {
+      r.up[0] = r.up[1] = up_above(vs_top);
+      r.scales.set(r.up[0], r.up[0]);
+    } else if (__builtin_expect(vs_top > r.scales.most || vs_low < r.scales.least, 0)) {
+      const bool fresh = r.scales.fresh();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // the largest score and the largest scale may be far from one another
+        const float zero = now[half] == -INFINITY ? 0.0f : now[half], had = fresh ? 0.0f : up_of(r.up[half]) * keep[half];
+        float met = 0.0f;
+#pragma unroll
+        for (int b = 0; b < kTile / kGranule; ++b) {
+          const float m = fmaxf(fmaxf(score[2 * b][2 * half], score[2 * b][2 * half + 1]), fmaxf(score[2 * b + 1][2 * half], score[2 * b + 1][2 * half + 1]));
+          met = fmaxf(met, exp2_fast(quad_max(m) - zero) * s.vs[b]);
+        }
+        if (now[half] == -INFINITY) met = vs_top;                // has seen nothing: any unit will do
+        r.up[half] = up_above(fmaxf(had, met));
+        keep[half] = had * r.up[half] * 0x1p-11f;
+      }
+      r.scales.set(warp_max(fmaxf(r.up[0], r.up[1])), -warp_max(-fminf(r.up[0], r.up[1])));
+    }
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) r.o[n][i] *= keep[i / 2];
   }
   const float base[2] = {now[0] == -INFINITY ? 0.0f : now[0], now[1] == -INFINITY ? 0.0f : now[1]};
-  const float up = __fdividef(exp2f(kWeightUp), unit);
 
 #pragma unroll
   for (int b = 0; b < kTile / kGranule; ++b) {
-    const float vs = s.vs[b] * up;
     uint32_t w[PARTS][4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {                  // rows g, g + 8 of the first eight tokens, then of the other eight
       const int half = x % 2, n = 2 * b + x / 2;
-      float p0 = exp2_fast(score[n][2 * half] - base[half]), p1 = exp2_fast(score[n][2 * half + 1] - base[half]);
-      r.sum[half] += p0 + p1;
-      p0 *= vs;
-      p1 *= vs;
+      float2 y = make_float2(exp2_fast(score[n][2 * half] - base[half]), exp2_fast(score[n][2 * half + 1] - base[half]));
+      r.sum[half] += y.x + y.y;
+      y = scaled(y, s.vs[b], make_float2(r.up[half], r.up[half]));
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
-        w[part][x] = pack_half2(p0, p1);
+        w[part][x] = pack_half2(y.x, y.y);
         const float2 kept = unpack_half2(w[part][x]);
-        p0 -= kept.x;
-        p1 -= kept.y;
+        y.x -= kept.x;
+        y.y -= kept.y;
       }
     }
     // values: this lane's columns of tokens 2c, 2c + 1, 2c + 8, 2c + 9
@@ -300,11 +320,11 @@ __global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constan
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     sum[half] = quad_sum(r.sum[half]);
-    const float w = sum[half] == 0.0f ? 0.0f : __fdiv_rn(exp2f(-kWeightUp), sum[half]);
+    const float w = sum[half] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[half]), unit = up_of(r.up[half]) * 0x1p-11f;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
-      r.o[n][2 * half] = r.o[n][2 * half] * w * r.unit;
-      r.o[n][2 * half + 1] = r.o[n][2 * half + 1] * w * r.unit;
+      r.o[n][2 * half] = r.o[n][2 * half] * w * unit;
+      r.o[n][2 * half + 1] = r.o[n][2 * half + 1] * w * unit;
     }
   }
   if (p.splits == 1) {

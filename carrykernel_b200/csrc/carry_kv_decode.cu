@@ -193,7 +193,8 @@ template <int D, int NT>
 struct Running {
   float o[NT][D / 16][4];
   float top[NT][2], sum[NT][2];   // the sums are this lane's share
-  float unit;                     // largest value scale so far: o counts in it, times 2^15
+  float up[NT][2];                // 2^11 over the unit that the row's outputs count in: o is that many times too large
+  Scales scales;
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -201,8 +202,9 @@ struct Running {
       for (int m = 0; m < D / 16; ++m) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.0f;
       top[n][0] = top[n][1] = -INFINITY;
       sum[n][0] = sum[n][1] = 0.0f;
+      up[n][0] = up[n][1] = kUpStart;
     }
-    unit = 0x1p-100f;             // the smallest scale
+    scales.clear();
   }
 };
 
@@ -232,13 +234,14 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
             mma_fp16(score[b][n], a, q.x[n][part][j * 4 + k][0], q.x[n][part][j * 4 + k][1]);
       }
     }
-  float unit = r.unit, now[NT][2], count[kBlocks][NT][2];     // count: what a product of the block counts
+  float now[NT][2], count[kBlocks][NT][2];     // count: what a product of the block counts
+  float vs_top = 0.0f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) now[n][0] = now[n][1] = -INFINITY;
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
     const float ks = s.ks[b];
-    unit = fmaxf(unit, s.vs[b]);
+    vs_top = fmaxf(vs_top, s.vs[b]);
     if (!all || ks == kNoTokens) {
       const int t = ks == kNoTokens ? 1 << 30 : b * kGranule + g;
 #pragma unroll
@@ -254,7 +257,7 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
         now[n][i] = fmaxf(now[n][i], fmaxf(score[b][n][i], score[b][n][i + 2]) * count[b][n][i]);
       }
   }
-  bool more = unit > r.unit;
+  bool more = vs_top > r.scales.most;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -262,54 +265,83 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) now[n][i] = fmaxf(now[n][i], __shfl_xor_sync(~0u, now[n][i], d));
       more = more || now[n][i] > r.top[n][i];
-      now[n][i] = fmaxf(now[n][i], r.top[n][i]);
     }
   if (__any_sync(~0u, more)) {
-    const float less = __fdividef(r.unit, unit);
-    r.unit = unit;
+    float vs_low = vs_top, keep[NT][2];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) vs_low = fminf(vs_low, s.ks[b] == kNoTokens ? vs_top : s.vs[b]);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float keep = now[n][i] == -INFINITY ? 1.0f : exp2_fast(r.top[n][i] - now[n][i]);
-        r.sum[n][i] *= keep;
-        r.top[n][i] = now[n][i];
-        keep *= less;
-#pragma unroll
-        for (int m = 0; m < D / 16; ++m) {
-          r.o[n][m][i] *= keep;
-          r.o[n][m][i + 2] *= keep;
-        }
+        const float high = fmaxf(now[n][i], r.top[n][i]);
+        keep[n][i] = high == -INFINITY ? 1.0f : exp2_fast(r.top[n][i] - high);
+        r.sum[n][i] *= keep[n][i];
+        r.top[n][i] = high;
       }
+    // what follows is the same in every lane
+    if (r.scales.fresh() && vs_top > 0.0f && vs_low * kSlack >= vs_top) {
+      const float up = up_above(vs_top);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) r.up[n][0] = r.up[n][1] = up;
+      r.scales.set(up, up);
+    } else if (__builtin_expect(vs_top > r.scales.most || vs_low < r.scales.least, 0)) {
+      const bool fresh = r.scales.fresh();
+      float up_most = 0.0f, up_least = INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // the largest score and the largest scale may be far from one another
+          const float zero = r.top[n][i] == -INFINITY ? 0.0f : r.top[n][i], had = fresh ? 0.0f : up_of(r.up[n][i]) * keep[n][i];
+          float met = 0.0f;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            float m = fmaxf(score[b][n][i], score[b][n][i + 2]) * count[b][n][i];
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+            met = fmaxf(met, exp2_fast(m - zero) * s.vs[b]);
+          }
+          if (r.top[n][i] == -INFINITY) met = vs_top;            // has seen nothing: any unit will do
+          r.up[n][i] = up_above(fmaxf(had, met));
+          keep[n][i] = had * r.up[n][i] * 0x1p-11f;
+          up_most = fmaxf(up_most, r.up[n][i]);
+          up_least = fminf(up_least, r.up[n][i]);
+        }
+      r.scales.set(quad_max(up_most), -quad_max(-up_least));
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.o[n][m][i] *= keep[n][i % 2];
   }
-  const float up = __fdividef(exp2f(kWeightUp), unit);
   float base[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) base[n][i] = now[n][i] == -INFINITY ? 0.0f : now[n][i];
+    for (int i = 0; i < 2; ++i) base[n][i] = r.top[n][i] == -INFINITY ? 0.0f : r.top[n][i];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
-    const float vs = s.vs[b] * up;
+    const float vs = s.vs[b];
     uint32_t w[NT][PARTS][2];     // weights of tokens 2c, 2c + 1 and 2c + 8, 2c + 9, row 8 n + g
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float x[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          x[i] = exp2_fast(fmaf(score[b][n][half * 2 + i], count[b][n][i], -base[n][i]));
-          r.sum[n][i] += x[i];
-          x[i] *= vs;
-        }
+        float2 x = make_float2(exp2_fast(fmaf(score[b][n][half * 2], count[b][n][0], -base[n][0])),
+                               exp2_fast(fmaf(score[b][n][half * 2 + 1], count[b][n][1], -base[n][1])));
+        r.sum[n][0] += x.x;
+        r.sum[n][1] += x.y;
+        x = scaled(x, vs, make_float2(r.up[n][0], r.up[n][1]));
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          const uint32_t h = pack_half2(x[0], x[1]);
+          const uint32_t h = pack_half2(x.x, x.y);
           asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(w[n][part][half]) : "r"(h));
           const float2 kept = unpack_half2(h);
-          x[0] -= kept.x;
-          x[1] -= kept.y;
+          x.x -= kept.x;
+          x.y -= kept.y;
         }
       }
     constexpr int kWords = D / 32;                // this lane's columns of tokens 2c, 2c + 1, 2c + 8, 2c + 9
@@ -369,11 +401,11 @@ __device__ __forceinline__ void merge_warps(DecodeShared<D, NT, PARTS>& sh, Runn
       const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) l += sh.sum[x][row] * exp2_fast(sh.top[x][row] - base);
-      const float w = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[n][i] - base), l) * exp2f(-kWeightUp);
+      const float w = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[n][i] - base), l), unit = up_of(r.up[n][i]) * 0x1p-11f;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
-        r.o[n][x][i] = r.o[n][x][i] * w * r.unit;
-        r.o[n][x][i + 2] = r.o[n][x][i + 2] * w * r.unit;
+        r.o[n][x][i] = r.o[n][x][i] * w * unit;
+        r.o[n][x][i + 2] = r.o[n][x][i + 2] * w * unit;
       }
       top[n][i] = m;
       sum[n][i] = l;
@@ -480,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
       for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
       theirs.top[source][row] = r.top[n][i];
       theirs.sum[source][row] = sum;
-      const float w = sum == 0.0f ? 0.0f : __fdiv_rn(r.unit * exp2f(-kWeightUp), sum);
+      const float w = sum == 0.0f ? 0.0f : __fdiv_rn(up_of(r.up[n][i]), sum) * 0x1p-11f;
       float4* to = reinterpret_cast<float4*>(theirs.o[source][row] + g % (8 / CL) * (D / 8));
 #pragma unroll
       for (int m = 0; m < D / 16; m += 2)

@@ -64,10 +64,10 @@ def hardly_weighed(power, tokens, D, dtype):
     run(q, cache, table, 300, dtype)
 
 
-def of_every_size(seed, tokens, D, dtype):
-    q, cache, table, g = made(700, tokens, D, dtype, seed)
+def of_every_size(seed, tokens, D, dtype, context=700):
+    q, cache, table, g = made(context, tokens, D, dtype, seed)
     cache[3].copy_(2.0 ** torch.randint(-100, 110, cache[3].shape, generator=g).float())
-    run(q, cache, table, 700, dtype)
+    run(q, cache, table, context, dtype)
 
 
 MANY = [(20, 128, "bf16"), (150, 64, "bf16")]
@@ -95,3 +95,32 @@ def test_many_rows_large_values_of_little_weight(power, tokens, D, dtype):
 @pytest.mark.parametrize("seed", range(3))
 def test_many_rows_scales_of_every_size(seed, tokens, D, dtype):
     of_every_size(seed, tokens, D, dtype)
+
+
+# few rows, by clusters (short contexts) and by the line, and many fp32 rows
+FEW = [(1, 128, "bf16"), (4, 64, "bf16"), (8, 128, "bf16"), (4, 128, "fp32"), (8, 64, "fp32"), (40, 128, "fp32"), (70, 64, "fp32")]
+
+
+@pytest.mark.parametrize("tokens,D,dtype", FEW)
+@pytest.mark.parametrize("power", [21, 36, 100])
+def test_few_rows_blocks_of_zeros_beside_large_values(power, tokens, D, dtype):
+    zeros_beside(power, tokens, D, dtype)
+
+
+@pytest.mark.parametrize("tokens,D,dtype", FEW[1:])
+@pytest.mark.parametrize("power", [26, 33, 50, 100])
+def test_few_rows_large_values_that_a_row_does_not_see(power, tokens, D, dtype):
+    unseen(power, tokens, D, dtype)
+
+
+@pytest.mark.parametrize("tokens,D,dtype", FEW)
+@pytest.mark.parametrize("power", [10, 24, 40, 90])
+def test_few_rows_large_values_of_little_weight(power, tokens, D, dtype):
+    hardly_weighed(power, tokens, D, dtype)
+
+
+@pytest.mark.parametrize("tokens,D,dtype", FEW)
+@pytest.mark.parametrize("seed", range(3))
+def test_few_rows_scales_of_every_size(seed, tokens, D, dtype):
+    of_every_size(seed, tokens, D, dtype)
+    of_every_size(seed, tokens, D, dtype, context=9000)
