@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
     float top = -INFINITY, total = 0.0f, x = 0.0f;
 #pragma unroll
     for (int n = 0; n < kSources; ++n) top = fmaxf(top, sh.top[n][row]);
-    const float base = top == -INFINITY ? 0.0f : top;
+    const float base = (top == -INFINITY ? 0.0f : top) + kJoinDown;
 #pragma unroll 8
     for (int n = 0; n < kSources; ++n) {
       const float w = sh.sum[n][row] * exp2_fast(sh.top[n][row] - base);
@@ -713,7 +713,7 @@ __device__ __forceinline__ void join_pieces(const float* slots, int rows, int ro
     for (int e = 0; e < D / 32; ++e) r.o[e] *= keep;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const float w = sum[k] * exp2_fast(top[k] - base);
+      const float w = sum[k] * exp2_fast(top[k] - base - kJoinDown);
       r.sum += w;
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) r.o[e] = fmaf(w, o[k][e], r.o[e]);

@@ -124,3 +124,14 @@ def test_few_rows_large_values_of_little_weight(power, tokens, D, dtype):
 def test_few_rows_scales_of_every_size(seed, tokens, D, dtype):
     of_every_size(seed, tokens, D, dtype)
     of_every_size(seed, tokens, D, dtype, context=9000)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("context,tokens", [(60, 1), (180, 8), (1500, 1), (9000, 2), (9000, 8), (60, 40), (9000, 40)])
+def test_values_at_the_end_of_the_range(context, tokens, dtype):
+    """448 * 2^119 throughout, which is what comes out: no sum on the way leaves fp32.  Contexts in one piece, in a cluster's, in
+    CTAs' and in parts."""
+    q, cache, table, _ = made(context, tokens, 128, dtype, tokens)
+    cache[2].fill_(448.0)
+    cache[3].fill_(2.0 ** 119)
+    run(q, cache, table, context, dtype)
