@@ -48,6 +48,29 @@ __device__ __forceinline__ uint2 codes8(const Eight& e, float inv) {
   return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
 }
 
+// A block that already holds tokens may have them under any scale (a cache that was filled elsewhere), and only of a power of two
+// with one in fp32's normal numbers is the reciprocal exact in fp32.  Of others it is taken in 64 bits, by Newton's iteration, so
+// that a quotient halfway between two codes is found to be that.  (A division would be a call, and take the kernel's registers.)
+__device__ __forceinline__ bool exact_inverse(float scale) {
+  const uint32_t u = __float_as_uint(scale);
+  return (u & 0x7fffffu) == 0 && u - 1 < (254u << 23) - 1;
+}
+__device__ __forceinline__ double inverse64(float scale) {
+  const double d = scale;
+  const long long u = __double_as_longlong(d);
+  const double part = __longlong_as_double((u & 0xfffffffffffffll) | 1023ll << 52);       // of [1, 2)
+  double r = __fdividef(1.0f, static_cast<float>(part));
+  r = r * (2.0 - part * r);
+  r = r * (2.0 - part * r);
+  return r * __longlong_as_double((2046ll << 52) - (u & 0x7ff0000000000000ll));
+}
+__device__ __forceinline__ uint2 codes8(const Eight& e, double inv) {
+  Eight y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y.x[i] = make_float2(static_cast<float>(e.x[i].x * inv), static_cast<float>(e.x[i].y * inv));
+  return codes8(y, 1.0f);
+}
+
 // ITEMS: a thread's share of a block's new tokens, eight numbers each, held in registers from the maximum to the codes.
 template <int D, int DTYPE, int ITEMS>
 __global__ void __launch_bounds__(kThreads, ITEMS <= 4 && DTYPE != CARRY_F32 ? 6 : 1) kv_append_kernel(const __grid_constant__ AppendParams p) {
@@ -128,17 +151,20 @@ __global__ void __launch_bounds__(kThreads, ITEMS <= 4 && DTYPE != CARRY_F32 ? 6
       now = old;
     }
   }
-  const float inv = __uint_as_float((254u << 23) - __float_as_uint(now));        // of a power of two: exact
   uint2* to_codes = reinterpret_cast<uint2*>(codes + (long long)(t0 - start) * D);
+  auto store = [&](auto by) {
 #pragma unroll
-  for (int n = 0; n < ITEMS; ++n) {
-    const int i = n * kHalf + tid;
-    if (i >= items) continue;
-    uint2 w = codes8(unpack<DTYPE>(e[n]), inv);
-    if (max(token_top[0][i / kPer], token_top[1][i / kPer]) >= kNotFinite)
-      w = is_v ? make_uint2(0, 0) : make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-    to_codes[i] = w;
-  }
+    for (int n = 0; n < ITEMS; ++n) {
+      const int i = n * kHalf + tid;
+      if (i >= items) continue;
+      uint2 w = codes8(unpack<DTYPE>(e[n]), by);
+      if (max(token_top[0][i / kPer], token_top[1][i / kPer]) >= kNotFinite)
+        w = is_v ? make_uint2(0, 0) : make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+      to_codes[i] = w;
+    }
+  };
+  if (__builtin_expect(exact_inverse(now), 1)) store(__uint_as_float((254u << 23) - __float_as_uint(now)));
+  else store(inverse64(now));
   if (tid == 0 && now != old) *scale = now;       // every thread read the old one before the first barrier
 }
 

@@ -364,8 +364,9 @@ typedef struct CarryGdnKvRows {
  * Append: the rows' keys and values become codes at their positions.  The scale
  * of a block is the smallest power of two s with amax / s <= 448, amax over the
  * block's tokens so far; where it grows, the codes of the block's earlier
- * tokens are rounded to it (exactly, down to e4m3's subnormals).  A block whose
- * first token is among the new ones is started afresh.  A token whose key or
+ * tokens are rounded to it (exactly, down to e4m3's subnormals).  A larger scale
+ * that earlier tokens have stays, a power of two or not.  A block whose first
+ * token is among the new ones is started afresh.  A token whose key or
  * value has a number that is not finite gets a NaN key and takes no part in the
  * scale: the queries that see it become NaN, no others.  Rows at a negative
  * position or in a padding page are skipped.  No two requests may append to one
