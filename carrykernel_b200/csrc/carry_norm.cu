@@ -17,7 +17,8 @@ namespace {
 constexpr float kAmaxFloor = 1e-12f;
 constexpr int kGroup = 128, kMaxWarps = 16;
 
-// Squares from here on are summed times 2^-128: those of numbers that fp32 holds need not fit it.
+// Squares from here on are summed times 2^-160: those of numbers that fp32 holds need not fit it, and 32768 of the largest, times
+// that, do.
 constexpr float kLarge = 0x1p100f;
 
 struct NormParams {
@@ -97,12 +98,12 @@ __device__ __forceinline__ RowScale reduce_row(const NormParams& p, RowSums& sh,
       sum += sh.sum[turn][i];
       large += sh.large[turn][i];
     }
-    rstd = large < INFINITY ? rsqrtf(fmaf(sum, 0x1p-128f, large) * p.inv_width) * 0x1p-64f : NAN;
+    rstd = large < INFINITY ? rsqrtf(fmaf(sum * 0x1p-80f, 0x1p-80f, large) * p.inv_width) * 0x1p-80f : NAN;
   }
   return {top < INFINITY ? rstd : NAN, top};
 }
 
-// Sum of the squares of 2 N numbers; from kLarge on it counts in `large`, times 2^-128 (NaNs do, too).
+// Sum of the squares of 2 N numbers; from kLarge on it counts in `large`, times 2^-160 (NaNs do, too).
 template <int N>
 __device__ __forceinline__ void add_squares(const float2 (&t)[N], float2& ss, float& large) {
   float2 part = mul2(t[0], t[0]);
@@ -113,7 +114,7 @@ __device__ __forceinline__ void add_squares(const float2 (&t)[N], float2& ss, fl
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float u = t[i].x * 0x1p-64f, v = t[i].y * 0x1p-64f;
+      const float u = t[i].x * 0x1p-80f, v = t[i].y * 0x1p-80f;
       large += u * u + v * v;
     }
   }

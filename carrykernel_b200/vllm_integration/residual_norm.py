@@ -31,7 +31,7 @@ def add_rms_norm_quant(x, residual, weight, codes, scale, eps: float = 1e-6, res
     float8_e4m3fn, ``scale`` fp32: ``[N]`` for one scale per row or ``[N, ceil(W / 128)]`` for one per 128 columns.
     ``scale = max(amax|y|, 1e-12) / 448``.  The sum goes back into ``residual`` unless ``residual_out`` (its dtype) is
     given; with ``residual=None`` (a model's first layer) ``h = x``, stored only where ``residual_out`` is given.  A row
-    of ``h`` with a number that is not finite gets NaN codes and scales; weights are taken to be finite."""
+    of ``h`` with a number that is not finite, or whose product with its weight is not in fp32, gets NaN codes and scales."""
     lib = _lib._lib or _lib.load_library()
     if lib.native.add_rms_norm(lib.native_table, x, residual, weight, codes, scale, eps, residual_out):
         return codes, scale

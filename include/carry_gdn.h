@@ -419,8 +419,8 @@ int64_t carry_gdn_kv_attention_workspace(const CarryGdnKvAttentionArgs* args);
  * type, y = h * rsqrt(mean(h^2) + eps) * weight, and y in e4m3 codes with a
  * scale per row (group == 0: scale [N]) or per 128 columns (group == 128: scale
  * [N, ceil(W / 128)], contiguous): scale = max(amax|y|, 1e-12) / 448.  A row
- * of h with a number that is not finite gets NaN codes and scales throughout;
- * weights are taken to be finite.  residual may be NULL (h = x); residual_out
+ * of h with a number that is not finite, or whose product with its weight is
+ * not in fp32, gets NaN codes and scales throughout.  residual may be NULL (h = x); residual_out
  * may be NULL, or alias residual or x.  W is at most 32768.
  */
 typedef struct CarryGdnNormArgs {
