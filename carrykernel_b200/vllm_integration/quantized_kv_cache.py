@@ -198,12 +198,14 @@ def quantized_paged_attention(q, scale, k_codes, k_scale, v_codes, v_scale, out,
 
 
 def attention_workspace_bytes(q, k_codes, k_scale, block_table, query_start=None, max_query_len=None) -> int:
-    """Bytes of workspace that :func:`quantized_paged_attention` needs for a call of these sizes (on the current device)."""
+    """Bytes of workspace that :func:`quantized_paged_attention` needs for a call of these sizes on the cache's device
+    (on the current one, where the cache is on none)."""
     lib = _lib._lib or _lib.load_library()
     B = block_table.shape[0]
     lengths = torch.empty(B, dtype=torch.int32, device=k_codes.device)
     args = _attention_args(q, 1.0, k_codes, k_scale, k_codes, k_scale, q, block_table, lengths, query_start, max_query_len,
                            None)
-    need = lib.carry_gdn_kv_attention_workspace(args)
+    with torch.cuda.device_of(k_codes):
+        need = lib.carry_gdn_kv_attention_workspace(args)
     _lib.check(min(need, 0), "carry_gdn_kv_attention_workspace")
     return need
