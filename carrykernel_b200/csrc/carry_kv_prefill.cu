@@ -674,14 +674,8 @@ template <int D>
 int launch(const AttnParams& p, cudaStream_t stream) {
   constexpr size_t smem = sizeof(Shared<D>) + 1024;
   static thread_local bool ready[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || !ready[dev]) {
-    if (cudaFuncSetAttribute(kv_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-      cudaGetLastError();
-      return CARRY_GDN_ERR_LAUNCH;
-    }
-    if (dev < 64) ready[dev] = true;
-  }
+  const int rc = prepare(kv_prefill_kernel<D>, smem, ready);
+  if (rc != CARRY_GDN_OK) return rc;
   const long long tiles = row_tiles(p.a), cut = p.padded / kCtaRows;
   const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)(tiles - cut + cut * p.splits));
   return launch_dependent(kv_prefill_kernel<D>, grid, kAllThreads, smem, stream, p);
