@@ -7,9 +7,9 @@
 //  * a query row is scaled by a power of two until its largest number is in [2^14, 2^15): bf16 and fp16 numbers fit fp16
 //    exactly down to 2^-29 of the largest, fp32 ones go in two parts (22 bits);
 //  * the weights p of the softmax are fp16 (2^-12 of each, against 2^-9 for the rounding of a bf16 output), with fp32
-//    queries in two parts.  They carry the value scale of their block relative to the largest weight times scale
-//    that the row has met, and 2^11 (2^7 in the tensor-memory kernel), so that weights down to 2^-20 of the largest have all
-//    their bits.
+//    queries in two parts.  They carry the value scale of their block relative to the largest scale that the warp
+//    has met or, where those lie far apart, to the row's largest weight times scale, and 2^15: weights down to 2^-21 of the
+//    largest have all their bits, and to 2^-29 where scales are the same (in the tensor-memory kernel always to the row's, and 2^7).
 // Scores, maxima, sums and outputs are fp32.
 //
 // Up to 16 rows of a (request, head) go to carry_kv_decode.cu, more to carry_kv_prefill.cu or, where they are fp32, to

@@ -51,28 +51,32 @@ __device__ __forceinline__ uint32_t pack_half2(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
-// Where products are formed in registers, a row's weights count, with the value scales of their blocks, in a unit of its own, a
-// power of two within 2^5 of the largest weight times scale that it has met: blocks that a row does not see, or hardly weighs,
-// cost it no bits (weights below 2^-126 are none).  Units stay while scales are within 2^4 of them, below as well where a maximum
-// moves, and rows that have met no others have the same.  What is kept is `up`, 2^11 over the unit: a weight stays below 2^15 in fp16
-// and has all its bits down to 2^-20 of the row's largest.
-constexpr float kUpStart = 0x1p-108f;             // of the largest scale
-constexpr float kSlack = 16.0f;
-// 2^11 over a power of two, both ways
-__device__ __forceinline__ float up_of(float unit) { return __uint_as_float((265u << 23) - __float_as_uint(unit)); }
-// 2^11 over the power of two that is not below x
+// Where products are formed in registers, weights count with the value scales of their blocks, in a unit that is a power of two;
+// what is kept is `up`, 2^15 over it.  As long as the scales that a warp meets lie within 2^4 of its first ones, the unit is the
+// largest of them, for all rows: a weight then has all its bits down to 2^-21 of the row's largest weight times scale, and to 2^-29
+// where the scales are the same.  From then on every row has a unit of its own, not below its largest weight times scale and looked
+// at again with every step: blocks that a row does not see, or hardly weighs, cost it no bits (weights below 2^-126 are none).
+constexpr float kUpStart = 0x1p-104f;             // of the largest scale
+// 2^15 over a power of two, both ways
+__device__ __forceinline__ float up_of(float unit) { return __uint_as_float((269u << 23) - __float_as_uint(unit)); }
+// 2^15 over the power of two that is not below x
 __device__ __forceinline__ float up_above(float x) { return up_of(__uint_as_float((__float_as_uint(fmaxf(x, 0x1p-100f)) + 0x7fffffu) & 0x7f800000u)); }
-// Value scales that leave all rows' units as they are.
+// what outputs are multiplied by when the unit grows; there are none yet where it would be more than 1
+__device__ __forceinline__ float rescale(float up, float now) { return fminf(now * up_of(up) * 0x1p-15f, 1.0f); }
 struct Scales {
-  float most, least;
-  __device__ __forceinline__ void clear() { most = least = 0.0f; }
-  __device__ __forceinline__ bool fresh() const { return most == 0.0f; }        // no value has counted yet
-  __device__ __forceinline__ void set(float up_most, float up_least) {
-    most = kSlack * up_of(up_most);
-    least = up_of(up_least) * (1.0f / kSlack);
+  float most;                     // 2^4 times the first ones; infinite before them, and -1 once rows have their own units
+  __device__ __forceinline__ bool fresh() const { return most == INFINITY; }
+  // whether a step's scales may stand with the others; the same in every lane
+  __device__ __forceinline__ bool alike(float vs_top, float vs_low) {
+    if (fresh()) most = 16.0f * vs_top;
+    if (most > 0.0f && vs_top <= most && vs_low * 256.0f >= most) return true;
+    most = -1.0f;
+    return false;
   }
+  // larger ones are looked at
+  __device__ __forceinline__ float limit(float up) const { return most < 0.0f ? -1.0f : up_of(up); }
 };
-// two weights with their values' scale, the scale first: a weight is at most 1, and together they are at most kSlack units
+// two weights with their values' scale, the scale first: a weight is at most 1, and together they are at most a unit
 __device__ __forceinline__ float2 scaled(float2 weights, float vs, float2 up) { return mul2(mul2(weights, make_float2(vs, vs)), up); }
 // four e4m3 codes as fp16 numbers, two to a word
 __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& low, uint32_t& high) {

@@ -114,7 +114,7 @@ template <int D>
 struct Rows {
   float o[D / 8][4];              // lane (g, c): row g columns 2c (D/8) + n and (2c + 1) D/8 + n, then row g + 8's
   float top[2], sum[2];           // of rows g and g + 8; the sums are this lane's share
-  float up[2];                    // 2^11 over the unit that a row's outputs count in: o is that many times too large
+  float up[2];                    // 2^15 over the unit that a row's outputs count in: o is that many times too large
   Scales scales;
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -122,7 +122,7 @@ struct Rows {
     top[0] = top[1] = -INFINITY;
     sum[0] = sum[1] = 0.0f;
     up[0] = up[1] = kUpStart;
-    scales.clear();
+    scales.most = INFINITY;
   }
 };
 
@@ -162,7 +162,7 @@ __device__ __forceinline__ void attend(const Stage<D>& s, const Query<D>& q, con
   }
 #pragma unroll
   for (int b = 0; b < kTile / kGranule; ++b) vs_top = fmaxf(vs_top, s.vs[b]);
-  if (__any_sync(~0u, now[0] > r.top[0] || now[1] > r.top[1]) || vs_top > r.scales.most) {
+  if (__any_sync(~0u, now[0] > r.top[0] || now[1] > r.top[1]) || vs_top > r.scales.limit(r.up[0])) {
     float keep[2], vs_low = vs_top;
 #pragma unroll
     for (int b = 0; b < kTile / kGranule; ++b) vs_low = fminf(vs_low, s.ks[b] == kNoTokens ? vs_top : s.vs[b]);
@@ -172,15 +172,17 @@ __device__ __forceinline__ void attend(const Stage<D>& s, const Query<D>& q, con
       r.sum[half] *= keep[half];
       r.top[half] = now[half];
     }
-    // what follows is the same in every lane
-    if (r.scales.fresh() && vs_top > 0.0f && vs_low * kSlack >= vs_top) {
-      r.up[0] = r.up[1] = up_above(vs_top);
-      r.scales.set(r.up[0], r.up[0]);
-    } else if (__builtin_expect(vs_top > r.scales.most || vs_low < r.scales.least, 0)) {
-      const bool fresh = r.scales.fresh();
+    const bool fresh = r.scales.fresh();
+    if (__builtin_expect(r.scales.alike(vs_top, vs_low), 1)) {
+      if (fresh || vs_top > up_of(r.up[0])) {
+        const float up = up_above(vs_top), less = rescale(r.up[0], up);
+        r.up[0] = r.up[1] = up;
+        keep[0] *= less;
+        keep[1] *= less;
+      }
+    } else {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        // the largest score and the largest scale may be far from one another
         const float zero = now[half] == -INFINITY ? 0.0f : now[half], had = fresh ? 0.0f : up_of(r.up[half]) * keep[half];
         float met = 0.0f;
 #pragma unroll
@@ -188,11 +190,9 @@ __device__ __forceinline__ void attend(const Stage<D>& s, const Query<D>& q, con
           const float m = fmaxf(fmaxf(score[2 * b][2 * half], score[2 * b][2 * half + 1]), fmaxf(score[2 * b + 1][2 * half], score[2 * b + 1][2 * half + 1]));
           met = fmaxf(met, exp2_fast(quad_max(m) - zero) * s.vs[b]);
         }
-        if (now[half] == -INFINITY) met = vs_top;                // has seen nothing: any unit will do
         r.up[half] = up_above(fmaxf(had, met));
-        keep[half] = had * r.up[half] * 0x1p-11f;
+        keep[half] = had * r.up[half] * 0x1p-15f;
       }
-      r.scales.set(warp_max(fmaxf(r.up[0], r.up[1])), -warp_max(-fminf(r.up[0], r.up[1])));
     }
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constan
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     sum[half] = quad_sum(r.sum[half]);
-    const float w = sum[half] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[half]), unit = up_of(r.up[half]) * 0x1p-11f;
+    const float w = sum[half] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[half]), unit = up_of(r.up[half]) * 0x1p-15f;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
       r.o[n][2 * half] = r.o[n][2 * half] * w * unit;

@@ -193,8 +193,9 @@ template <int D, int NT>
 struct Running {
   float o[NT][D / 16][4];
   float top[NT][2], sum[NT][2];   // the sums are this lane's share
-  float up[NT][2];                // 2^11 over the unit that the row's outputs count in: o is that many times too large
+  float up[NT][2];                // 2^15 over the unit that the row's outputs count in: o is that many times too large
   Scales scales;
+  float limit;
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -204,7 +205,8 @@ struct Running {
       sum[n][0] = sum[n][1] = 0.0f;
       up[n][0] = up[n][1] = kUpStart;
     }
-    scales.clear();
+    scales.most = INFINITY;
+    limit = scales.limit(kUpStart);
   }
 };
 
@@ -257,7 +259,7 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
         now[n][i] = fmaxf(now[n][i], fmaxf(score[b][n][i], score[b][n][i + 2]) * count[b][n][i]);
       }
   }
-  bool more = vs_top > r.scales.most;
+  bool more = vs_top > r.limit;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -279,20 +281,23 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
         r.sum[n][i] *= keep[n][i];
         r.top[n][i] = high;
       }
-    // what follows is the same in every lane
-    if (r.scales.fresh() && vs_top > 0.0f && vs_low * kSlack >= vs_top) {
-      const float up = up_above(vs_top);
+    const bool fresh = r.scales.fresh();
+    if (__builtin_expect(r.scales.alike(vs_top, vs_low), 1)) {
+      if (fresh || vs_top > r.limit) {
+        const float up = up_above(vs_top), less = rescale(r.up[0][0], up);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) r.up[n][0] = r.up[n][1] = up;
-      r.scales.set(up, up);
-    } else if (__builtin_expect(vs_top > r.scales.most || vs_low < r.scales.least, 0)) {
-      const bool fresh = r.scales.fresh();
-      float up_most = 0.0f, up_least = INFINITY;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            r.up[n][i] = up;
+            keep[n][i] *= less;
+          }
+      }
+    } else {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          // the largest score and the largest scale may be far from one another
           const float zero = r.top[n][i] == -INFINITY ? 0.0f : r.top[n][i], had = fresh ? 0.0f : up_of(r.up[n][i]) * keep[n][i];
           float met = 0.0f;
 #pragma unroll
@@ -302,14 +307,11 @@ __device__ __forceinline__ void attend_run(const RunStage<D>& s, const Columns<D
             for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
             met = fmaxf(met, exp2_fast(m - zero) * s.vs[b]);
           }
-          if (r.top[n][i] == -INFINITY) met = vs_top;            // has seen nothing: any unit will do
           r.up[n][i] = up_above(fmaxf(had, met));
-          keep[n][i] = had * r.up[n][i] * 0x1p-11f;
-          up_most = fmaxf(up_most, r.up[n][i]);
-          up_least = fminf(up_least, r.up[n][i]);
+          keep[n][i] = had * r.up[n][i] * 0x1p-15f;
         }
-      r.scales.set(quad_max(up_most), -quad_max(-up_least));
     }
+    r.limit = r.scales.limit(r.up[0][0]);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -401,7 +403,7 @@ __device__ __forceinline__ void merge_warps(DecodeShared<D, NT, PARTS>& sh, Runn
       const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) l += sh.sum[x][row] * exp2_fast(sh.top[x][row] - base);
-      const float w = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[n][i] - base), l), unit = up_of(r.up[n][i]) * 0x1p-11f;
+      const float w = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(r.top[n][i] - base), l), unit = up_of(r.up[n][i]) * 0x1p-15f;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
         r.o[n][x][i] = r.o[n][x][i] * w * unit;
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_pair_kernel(const __grid_const
       for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
       theirs.top[source][row] = r.top[n][i];
       theirs.sum[source][row] = sum;
-      const float w = sum == 0.0f ? 0.0f : __fdiv_rn(up_of(r.up[n][i]), sum) * 0x1p-11f;
+      const float w = sum == 0.0f ? 0.0f : __fdiv_rn(up_of(r.up[n][i]), sum) * 0x1p-15f;
       float4* to = reinterpret_cast<float4*>(theirs.o[source][row] + g % (8 / CL) * (D / 8));
 #pragma unroll
       for (int m = 0; m < D / 16; m += 2)

@@ -135,3 +135,24 @@ def test_values_at_the_end_of_the_range(context, tokens, dtype):
     cache[2].fill_(448.0)
     cache[3].fill_(2.0 ** 119)
     run(q, cache, table, context, dtype)
+
+
+@pytest.mark.parametrize("zero", [2.0 ** -100, 0.0])
+@pytest.mark.parametrize("power", [15, 24, 40])
+@pytest.mark.parametrize("context,first", [(300, 1), (700, 8), (3000, 64)])
+@pytest.mark.parametrize("tokens,D,dtype", FEW + MANY)
+def test_blocks_of_zeros_that_have_nearly_all_the_weight(tokens, D, dtype, context, first, power, zero):
+    """The `first` blocks and then every fourth have scores that are `power` above the others' in log2, and values that are all
+    zero: the others' small weights are all that comes out."""
+    q, cache, table, _ = made(context, tokens, D, dtype, power)
+    cache[3].fill_(2.0 ** -9)
+    cache[0].view(torch.uint8)[..., 0] = 0
+    cache[1].fill_(2.0 ** -11)
+    q[..., 0] = power * 0.693 * 16 * D ** 0.5
+    for n in range((context + 15) // 16):
+        if n < first or n % 4 == 0:
+            page, at = block_of(table, n)
+            rows = slice(at * 16, at * 16 + 16)
+            cache[3][page, 0, at], cache[2][page, 0, rows] = zero, 0
+            cache[0].view(torch.uint8)[page, 0, rows, 0] = 0x70
+    run(q, cache, table, context, dtype)
