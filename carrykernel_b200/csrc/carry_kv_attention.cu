@@ -35,11 +35,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_parts_kernel(const __gri
   float top = lane < p.splits ? mine.top[row] : -INFINITY, w = lane < p.splits ? mine.sum[row] : 0.0f;
   if (__any_sync(~0u, w == kNoPart)) return;
   const float all_top = warp_max(top), base = all_top == -INFINITY ? 0.0f : all_top;
-  w *= exp2_fast(top - base);
+  w *= exp2_fast(top - base - kJoinDown);
   float sum = w, o[D / 32] = {};
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-  w = sum == 0.0f ? 0.0f : __fdiv_rn(w, sum);     // first: values may be near fp32's end
 #pragma unroll 8
   for (int s = 0; s < p.splits; ++s) {
     const float* x = parts_of(p, s, blockIdx.x).o + (long long)row * D + lane;
@@ -49,7 +48,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_parts_kernel(const __gri
   }
 #pragma unroll
   for (int e = 0; e < D / 32; ++e)
-    store_from_float(p.a.out, row_place(p, q, h, row, i, p.a.stride_out_tok, p.a.stride_out_head) + e * 32 + lane, p.a.dtype, o[e]);
+    store_from_float(p.a.out, row_place(p, q, h, row, i, p.a.stride_out_tok, p.a.stride_out_head) + e * 32 + lane, p.a.dtype,
+                     sum == 0.0f ? 0.0f : __fdiv_rn(o[e], sum));
 }
 
 }  // namespace

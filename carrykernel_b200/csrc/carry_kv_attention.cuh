@@ -41,7 +41,7 @@ inline int split_count(const CarryGdnKvAttentionArgs& a, long long ctas) {
   const long long n = sm_count() / (ctas < 1 ? 1 : ctas), most = steps / 8;
   return (int)(n < most ? (n < 1 ? 1 : n > 32 ? 32 : n) : most < 1 ? 1 : most > 32 ? 32 : most);
 }
-// Pieces of a row are joined by sums of their weights, which count up to a request's tokens: less this in the exponent, so that
+// Parts and pieces of a row are joined by sums of their weights, which count up to a request's tokens: less this in the exponent, so that
 // values at fp32's end times the sums stay within it.
 constexpr float kJoinDown = 30.0f;
 int launch_join_parts(const AttnParams& p, cudaStream_t stream);
