@@ -279,8 +279,11 @@ __device__ __forceinline__ void row_limits(const AttnParams& p, const KvRequest&
 
 constexpr int kChunkStages = 3, kChunkRows = kWarps * kRowsPerWarp;
 
+// Two CTAs to an SM.  At D = 64 the compiler is told so, or it fits the registers of three: few or ragged CTAs come uneven then (four
+// requests of 32 rows over 4096 tokens 49 us, 65 in threes; three prompts of 1 to 1968 tokens and 8 heads 97 and 122; four prompts
+// of 900 tokens, of which six come to an SM, are faster in threes, 122 against 137).
 template <int D>
-__global__ void __launch_bounds__(kThreads) kv_chunk_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 0) kv_chunk_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t raw[];
   Stage<D>* stages = reinterpret_cast<Stage<D>*>(raw);
   depend_release();
@@ -359,16 +362,11 @@ void lay_out(const CarryGdnKvAttentionArgs& a, int& splits, int& padded) {
 template <int D>
 int launch_chunk(AttnParams p, cudaStream_t stream) {
   lay_out(p.a, p.splits, p.padded);
-  // At D = 64 three CTAs fit an SM.  Where two to an SM are all there are, they ask for half of its memory, so that they are spread
-  // over all SMs (four requests of 32 rows over 4096 tokens 49 us, 65 with three here and none there; 900 tokens of four prompts, six
-  // to an SM, 122 us three at a time, 137 in twos).
-  constexpr size_t least = sizeof(Stage<D>) * kChunkStages, half = 100 << 10;
-  static_assert(least <= half, "two CTAs on an SM");
+  constexpr size_t smem = sizeof(Stage<D>) * kChunkStages;
   static thread_local bool ready[64];
-  int rc = prepare(kv_chunk_kernel<D>, half, ready);
+  int rc = prepare(kv_chunk_kernel<D>, smem, ready);
   if (rc != CARRY_GDN_OK) return rc;
   const dim3 grid((unsigned)p.a.cache.HKV * p.a.rows.B, (unsigned)p.padded / kChunkRows, (unsigned)p.splits);
-  const size_t smem = (long long)grid.x * grid.y * grid.z <= 2LL * sm_count() ? half : least;
   rc = launch_dependent(kv_chunk_kernel<D>, grid, kThreads, smem, stream, p);
   return rc == CARRY_GDN_OK && p.splits > 1 ? launch_join_parts(p, stream) : rc;
 }
