@@ -6,9 +6,11 @@
 // codes of the block's earlier tokens move by whole binades, so a block filled token by token ends with the codes of
 // one filled at once, subnormals apart.
 //
-// A CTA lives for three trips to memory (lengths, page id, rows) and one block, so what counts is how many are on an SM:
-// six of 40 registers a thread write 8192 tokens of 8 heads (50 MB) in 11.5 us, 4.4 TB/s; five took 13.2, and reading the
-// rows a second time for the codes 25.
+// A CTA lives for three trips to memory (lengths, page id, rows) and one block, so what counts is how many are on an SM.  With blocks
+// of 32 tokens of 128 numbers and 16-bit rows (four items of eight numbers to a thread) six of 40 registers a thread write 8192
+// tokens of 8 heads (50 MB) in 11.3 us, 4.4 TB/s, where the calls before have left them in L2, and 12.9 where not; five took 13.2, and
+// reading the rows a second time for the codes 25.  Blocks of 64 and 128 take the kernel of 16 items (124 registers, two CTAs): 18.4
+// and 13.0 us.  fp32 rows: 15.1 in blocks of 32 (70 registers, three CTAs), 31.3 and 21.9 in the others (190, one).
 #include "carry_hybrid.cuh"
 
 namespace carry {

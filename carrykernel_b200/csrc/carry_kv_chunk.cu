@@ -3,7 +3,7 @@
 //
 // A CTA has 64 rows, 16 to a warp, and walks the tokens in tiles of 64; every warp converts the tile's codes for itself.
 // Each number of q and each weight is two fp16 numbers, so products cost twice.  512 tokens of a prompt, 32 heads over 8 of 128:
-// 43 us.
+// 41 us.
 #include "carry_kv_attention.cuh"
 
 namespace carry {

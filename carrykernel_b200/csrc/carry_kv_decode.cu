@@ -9,8 +9,8 @@
 // the lengths are; where a cut falls inside a (request, head), pieces are joined by a second kernel.  Short contexts of few
 // (request, head)s have a cluster each and no second kernel.
 //
-// What bounds it: 128 requests of 8192 tokens (8 heads of 128, 2.15 GB) take 394 us, 5.5 TB/s, 83 % of the copy rate; 64 of 1 to
-// 8192 tokens 120 us, 4.6 TB/s, some 15 us of it the way in and out.  A run is about 700 instructions of a warp, half of them
+// What bounds it: 128 requests of 8192 tokens (8 heads of 128, 2.15 GB) take 350 to 400 us from box to box, 82 to 93 % of the copy
+// rate; 64 of 1 to 8192 tokens 120 us, 4.6 TB/s, some 15 us of it the way in and out.  A run is about 700 instructions of a warp, half of them
 // conversions and byte permutations at two cycles each; twelve warps an SM issue two instructions a cycle.  Tried and slower:
 // e4m3 matrix instructions on unconverted keys (131 us for the 64 requests: twice the registers), runs of 64 tokens, two CTAs
 // an SM with more stages (146).
@@ -39,7 +39,7 @@ struct RunStage {
 // CTAs of the decode kernel on an SM, by their registers, and stages of a warp, by the memory that this leaves.
 __host__ __device__ constexpr int resident(int D, int NT, int PARTS) { return NT == 1 && PARTS == 1 ? (D == 128 ? 3 : 4) : 2; }
 // Four leave the joining kernel some registers to wait in beside them: a call behind such a one starts when all its CTAs have
-// (two requests of 8344 tokens, four heads over 32 of 64, one after another 11.5 us, 13.0 with 121 registers a thread).
+// (two requests of 8344 tokens, 32 heads over 4 of 64, one after another 11.5 us, 13.0 with 121 registers a thread).
 __host__ __device__ constexpr int registers(int D, int NT, int PARTS) {
   return resident(D, NT, PARTS) == 4 ? 120 : resident(D, NT, PARTS) == 3 ? 168 : 255;
 }
@@ -839,8 +839,8 @@ int launch_clusters(K kernel, int clusters, int size, size_t smem, cudaStream_t 
 
 // CTAs of the clusters that take a call, or 0: as many as leave all clusters resident, two CTAs to an SM but for what the
 // groups of SMs that a cluster has to fit in leave over; no more than a context has tiles, and four tiles for each CTA at most.
-// One request of 1500 tokens and 8 heads takes 8.2 us so (clusters of eight), 11.4 by the line, four of 4096 15.7 and 18.2; 16 of
-// 128 6.1 and 11.8, 32 of 300 (one CTA each) 9.5 and 14.7.  With more than are resident at a time the line is as good: 56 requests
+// One request of 1500 tokens and 8 heads takes 8.2 us so (clusters of eight), 11.4 by the line, four of 4096 16 and 18.2; 16 of
+// 128 6.4 and 11.8, 32 of 300 (one CTA each) 10.1 and 14.7.  With more than are resident at a time the line is as good: 56 requests
 // of 120 and 16 heads 18.1 and 19.5, of 500 38.6 and 35.8.
 int cluster_size(const CarryGdnKvAttentionArgs& a) {
   const long long tokens = (long long)a.cache.max_pages * a.cache.page, pairs = (long long)a.rows.B * a.cache.HKV;

@@ -8,11 +8,12 @@
 //    and O += P V with the weights P in tensor memory;
 //  * four warps for each row tile take its scores out of tensor memory, a row to a thread, and put the weights back in
 //    their place.  While one tile's weights are formed, the other's products run.
-// What bounds it: 2 x 128 x 64 exponentials a step take 1024 cycles of the special function units, and the products 1330 of
-// the tensor cores (64 columns of scores come at two thirds of the rate of 128, which tensor memory has no room for beside
-// the outputs and a second step's scores); a step takes 1750.  A chunk of 2048 tokens at 16384, 32 heads over 8 of 128: 600 us,
-// 870 TFLOP/s, 53 % of the burst rate of a large matrix product, at a clock that the GPU's power brings down to some 1.5 GHz.
-// A CTA's way in and out is some 7 us: six prompts of up to 2000 tokens and 16 heads take 95 us, 415 TFLOP/s, half of it that.
+// What bounds it: a step takes 2200 cycles.  Its 2 x 128 x 64 exponentials are 1024 of the special function units, and its products some
+// 1330 of the tensor cores (64 columns of scores come at two thirds of the rate of 128, which tensor memory has no room for beside
+// the outputs and a second step's scores); neither is full, at 43 % of the cycles each, and what is left is the chain of a row
+// tile's step, out of tensor memory and back.  A chunk of 2048 tokens at 16384, 32 heads over 8 of 128: 580 to 600 us, 870 to 900 TFLOP/s,
+// 55 % of the burst rate of a large matrix product, at a clock that the GPU's power brings down to 1.5 to 1.6 GHz.
+// A CTA's way in and out is some 7 us: six prompts of up to 2000 tokens and 16 heads take 92 to 95 us, 425 TFLOP/s, half of it that.
 //
 // A row's weights are relative to a maximum that is replaced, and O rescaled, only when it is outgrown by 2^4.  With the value
 // scales of their blocks they count in a unit of the row's own, the largest weight times scale that it has met to within a
