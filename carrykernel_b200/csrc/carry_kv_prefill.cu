@@ -56,13 +56,14 @@ static_assert(kRawStages + kStages < kNotes, "notes outlive their step");
 // ---- waiting ---------------------------------------------------------------------------------------------------------
 
 // Polls of a barrier, each of which the hardware may hold for a while.  The test-only build has a warp of every row tile
-// come late to each of its steps, by more than the other warps' work on three: results must not depend on it.  And there,
+// come late to each of its steps, and the other warps to every third or fifth, by more than the others' work on three: results must
+// not depend on it.  And there,
 // in a cache of three heads, the first copies of request 0's head 1, of the first part where its context is cut, announce 16 bytes
 // more than they bring: a wait runs out, and the rows are left as they were.
 #ifdef CARRY_TEST_WAIT_EXPIRY
 constexpr int kSpinLimit = 1 << 14;
 __device__ __forceinline__ void test_come_late(int warp, int step) {
-  if (warp % 4 == step % 4) __nanosleep(4000);
+  if (warp < kSoftmaxThreads / 32 ? warp % 4 == step % 4 : (warp + step) % (warp % 2 ? 3 : 5) == 0) __nanosleep(4000);
 }
 __device__ __forceinline__ uint32_t test_extra_bytes(int heads, int pair, int part, int step) { return heads == 3 && pair == 1 && part == 0 && step == 0 ? 16 : 0; }
 #else
@@ -532,6 +533,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     for (int step = 0; step < steps; ++step) {
       const int left = length - (step0 + step) * kTokens;
       const float* ks = sh.ks[step % kNotes];
+      test_come_late(warp, step);
       if (!barrier_wait(&sh.raw_full[raw], raw_parity, poison, p.a.status)) break;
       if (step >= kStages && !barrier_wait(&sh.k_free[stage], parity, poison, p.a.status)) break;
       convert<D>(sh.raw_k[raw], sh.k[stage], ks, left, tid);
@@ -551,6 +553,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     int raw = 0, parity = 1;
     for (int step = 0; step < steps; ++step) {
       fetch.ahead(step);
+      test_come_late(warp, step);
       const typename Fetch<D>::Granule& now = fetch.now;
       if (step >= kRawStages && !__all_sync(~0u, barrier_wait(&sh.raw_free[raw], parity, poison, p.a.status))) break;
       const uint32_t there = __ballot_sync(~0u, now.id > 0);
@@ -606,6 +609,7 @@ __global__ void __launch_bounds__(kAllThreads, 1) kv_prefill_kernel(const __grid
     for (int step = 0; healthy && step < steps; ++step) {
       const int stage = step % kStages, turn = step & 1, parity = step / kStages & 1;
       const uint32_t values = v0 + stage * kStageStep;
+      test_come_late(warp, step);
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
         if (tile >= tiles) break;

@@ -51,3 +51,18 @@ def test_rows_of_a_wait_that_runs_out_are_left_as_they_were(lengths, tokens, dty
     want = attend(*call, status=status)
     assert status.item() == 0
     check(want, *call, dtype)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths,tokens,HQ,HKV", [([4000, 900], 300, 2, 2), ([1300] * 40, 40, 8, 4), ([130, 64, 65, 700], 260, 1, 1)])
+def test_warps_of_every_kind_that_come_late(lengths, tokens, HQ, HKV, D):
+    """Those that fetch, convert and issue as well: long rows of steps, several CTAs to an SM's turn, value scales that move the
+    rows' units, contexts that end inside a step."""
+    q, scale, cache, table, lengths = made(lengths, tokens, HQ, HKV, D, "fp16", seed=tokens)
+    g = torch.Generator().manual_seed(D)
+    cache[3].copy_(2.0 ** torch.randint(-20, -4, cache[3].shape, generator=g).float())
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    want = attend(q, scale, cache, table, lengths, status=status)
+    with wait_test_library():
+        got = attend(q, scale, cache, table, lengths, status=status)
+    assert status.item() == 0 and torch.equal(got, want)
