@@ -312,6 +312,11 @@ int kv_pointers_ok(const CarryGdnKvCache& c) {
   if (c.stride_k_page % 16 || c.stride_v_page % 16) return CARRY_GDN_ERR_SHAPE;
   return CARRY_GDN_OK;
 }
+// No request has more rows than the call: a looser bound costs nothing, and no size worked out from it leaves its type.
+CarryGdnKvRows kv_bounded(CarryGdnKvRows r) {
+  if (r.max_query > r.N) r.max_query = r.N;
+  return r;
+}
 int kv_attention_ok(const CarryGdnKvAttentionArgs* a) {
   if (!a) return CARRY_GDN_ERR_NULL;
   const int rc = kv_ok(a->cache, a->rows);
@@ -330,14 +335,20 @@ int carry_gdn_kv_append(const CarryGdnKvAppendArgs* a, void* stream) {
   if (a->rows.N == 0 || a->rows.B == 0 || a->rows.max_query == 0) return CARRY_GDN_OK;
   if (!a->k || !a->v) return CARRY_GDN_ERR_NULL;
   rc = kv_pointers_ok(a->cache);
-  if (rc == CARRY_GDN_OK) rc = carry::launch_kv_append(*a, static_cast<cudaStream_t>(stream));
+  if (rc != CARRY_GDN_OK) return rc;
+  CarryGdnKvAppendArgs bounded = *a;
+  bounded.rows = kv_bounded(a->rows);
+  rc = carry::launch_kv_append(bounded, static_cast<cudaStream_t>(stream));
   if (rc == CARRY_GDN_OK) g_last_kernel = 9;
   return rc;
 }
 
 int64_t carry_gdn_kv_attention_workspace(const CarryGdnKvAttentionArgs* a) {
   const int rc = kv_attention_ok(a);
-  return rc == CARRY_GDN_OK ? carry::kv_attention_workspace(*a) : rc;
+  if (rc != CARRY_GDN_OK) return rc;
+  CarryGdnKvAttentionArgs bounded = *a;
+  bounded.rows = kv_bounded(a->rows);
+  return carry::kv_attention_workspace(bounded);
 }
 
 int carry_gdn_kv_attention(const CarryGdnKvAttentionArgs* a, void* stream) {
@@ -348,11 +359,13 @@ int carry_gdn_kv_attention(const CarryGdnKvAttentionArgs* a, void* stream) {
   if (!a->q || !a->out) return CARRY_GDN_ERR_NULL;
   rc = kv_pointers_ok(a->cache);
   if (rc != CARRY_GDN_OK) return rc;
-  const int64_t need = carry::kv_attention_workspace(*a);
+  CarryGdnKvAttentionArgs bounded = *a;
+  bounded.rows = kv_bounded(a->rows);
+  const int64_t need = carry::kv_attention_workspace(bounded);
   if (need < 0) return static_cast<int>(need);
   if (need > 0 && !a->workspace) return CARRY_GDN_ERR_NULL;
   if (need > 0 && (a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)) return CARRY_GDN_ERR_SHAPE;
-  rc = carry::launch_kv_attention(*a, static_cast<cudaStream_t>(stream));
+  rc = carry::launch_kv_attention(bounded, static_cast<cudaStream_t>(stream));
   if (rc == CARRY_GDN_OK) g_last_kernel = 10;
   return rc;
 }
