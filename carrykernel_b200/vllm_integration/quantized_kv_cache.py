@@ -16,7 +16,8 @@ context.  This is the second kind, held in 8 bits too:
 :func:`quantized_kv_append` writes new tokens, :func:`quantized_paged_attention` attends over what is cached: one
 token a request (decode), a few (speculation), a chunk of a prompt.  Scales are powers of two, so that a block whose
 scale grows while it fills keeps the codes of its earlier tokens exactly (down to e4m3's subnormals); a speculated token
-that is rejected is overwritten by the next append, its scale stays.
+that is rejected is overwritten by the next append, its scale stays.  (A cache that was filled elsewhere may have any scales from
+2^-100 to 2^119, or 0 for blocks whose codes are all 0.)
 
 The calls read nothing back to the host, never synchronise and can be captured in a CUDA graph.  ``status``: as in
 ``quantized_packed_decode``; ids, lengths and query ranges outside of the call's bounds are skipped and flagged there

@@ -325,7 +325,9 @@ int carry_gdn_pool_copy_layers(const CarryGdnPoolCopyLayersArgs* args, void* str
  * The key/value cache of one full-attention layer, in 8 bits: pages of `page`
  * tokens, e4m3 codes [pages, HKV, page, D] and one fp32 scale for every `block`
  * tokens of a head, [pages, HKV, page / block]; a value is code * scale.  The
- * scales that carry_gdn_kv_append writes are powers of two, 2^-100 to 2^119.
+ * scales that carry_gdn_kv_append writes are powers of two, 2^-100 to 2^119;
+ * those of a cache that was filled elsewhere may be any numbers of that range,
+ * or 0 for blocks whose codes are all 0.
  * Request b holds lengths[b] tokens, token j of it in page
  * block_table[b][j / page]; a page id <= 0 is padding, its tokens are not
  * there.  A page id >= num_pages and a length beyond max_pages * page are
@@ -420,7 +422,8 @@ int64_t carry_gdn_kv_attention_workspace(const CarryGdnKvAttentionArgs* args);
  * scale per row (group == 0: scale [N]) or per 128 columns (group == 128: scale
  * [N, ceil(W / 128)], contiguous): scale = max(amax|y|, 1e-12) / 448.  A row
  * of h with a number that is not finite, or whose product with its weight is
- * not in fp32, gets NaN codes and scales throughout.  residual may be NULL (h = x); residual_out
+ * not in fp32, gets NaN codes and scales throughout.  Squares below fp32's
+ * range count as 0: eps stands in for them.  residual may be NULL (h = x); residual_out
  * may be NULL, or alias residual or x.  W is at most 32768.
  */
 typedef struct CarryGdnNormArgs {
