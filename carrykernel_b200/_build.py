@@ -29,8 +29,10 @@ SOURCES = ("carry_gdn_api.cu", "carry_gdn_generic.cu", "carry_gdn_tile128.cu",
            "carry_gdn_tile128_vk.cu", "carry_gdn_tile128_kv.cu", "carry_gdn_multi.cu",
            "carry_gdn_pool.cu", "carry_gdn_narrow.cu", "carry_gdn_chain.cu", "carry_gdn_dense64.cu",
            "carry_gdn_dense128.cu", "carry_kv_append.cu", "carry_kv_attention.cu", "carry_kv_decode.cu",
-           "carry_kv_chunk.cu", "carry_kv_prefill.cu", "carry_norm.cu")
-HEADERS = ("carry_gdn_common.cuh", "carry_gdn_tile128.cuh", "carry_gdn_slot_tile.inc", "carry_hybrid.cuh", "carry_kv_attention.cuh",
+           "carry_kv_chunk.cu", "carry_kv_prefill.cu", "carry_norm.cu", "carry_rotate.cu", "carry_delta_recurrent.cu",
+           "carry_delta_chunk.cu")
+HEADERS = ("carry_gdn_common.cuh", "carry_gdn_tile128.cuh", "carry_gdn_slot_tile.inc", "carry_hybrid.cuh", "carry_kv_attention.cuh", "carry_tensor.cuh",
+           "carry_delta.cuh",
            os.path.join("..", "..", "include", "carry_gdn.h"))
 NVCC_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xptxas", "-v", "-Xcompiler", "-fPIC")

@@ -174,18 +174,52 @@ class NormArgs(C.Structure):
     ]
 
 
+class PrefillArgs(C.Structure):
+    _fields_ = [
+        ("mixed_qkv", C.c_void_p), ("stride_mixed_tok", C.c_int64),
+        ("a", C.c_void_p), ("stride_a_tok", C.c_int64), ("b", C.c_void_p), ("stride_b_tok", C.c_int64),
+        ("A_log", C.c_void_p), ("dt_bias", C.c_void_p),
+        ("initial_state", C.c_void_p), ("stride_initial_req", C.c_int64),
+        ("final_state", C.c_void_p), ("stride_final_req", C.c_int64),
+        ("out", C.c_void_p), ("stride_out_tok", C.c_int64), ("query_start", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p),
+        ("scale", C.c_float), ("B", C.c_int32), ("N", C.c_int32), ("max_query", C.c_int32),
+        ("H", C.c_int32), ("HV", C.c_int32), ("K", C.c_int32), ("V", C.c_int32),
+        ("qkv_dtype", C.c_int32), ("ab_dtype", C.c_int32), ("A_log_dtype", C.c_int32), ("dt_bias_dtype", C.c_int32),
+        ("out_dtype", C.c_int32), ("use_qk_l2norm", C.c_int32),
+    ]
+
+
+class RotateArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("stride_q_tok", C.c_int64), ("stride_q_head", C.c_int64), ("stride_k_tok", C.c_int64), ("stride_k_head", C.c_int64),
+        ("stride_q_out_tok", C.c_int64), ("stride_q_out_head", C.c_int64),
+        ("stride_k_out_tok", C.c_int64), ("stride_k_out_head", C.c_int64),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("cos_sin", C.c_void_p),
+        ("stride_table", C.c_int64), ("table_rows", C.c_int64),
+        ("positions", C.c_void_p), ("stride_positions", C.c_int64), ("status", C.c_void_p),
+        ("eps", C.c_float), ("weight_offset", C.c_float),
+        ("N", C.c_int32), ("HQ", C.c_int32), ("HK", C.c_int32), ("D", C.c_int32), ("rotary", C.c_int32),
+        ("axes", C.c_int32), ("sections", C.c_int32 * 4), ("positions_64", C.c_int32), ("interleaved", C.c_int32),
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("table_dtype", C.c_int32),
+    ]
+
+
 ERR_UNSUPPORTED = -5
 
 EXPORTS = ("carry_gdn_quant_step", "carry_gdn_quant_decode", "carry_gdn_fp32_step", "carry_gdn_packed_decode",
            "carry_gdn_packed_decode_multi", "carry_gdn_pool_store", "carry_gdn_pool_load",
            "carry_gdn_pool_copy", "carry_gdn_pool_copy_layers", "carry_gdn_kv_append", "carry_gdn_kv_attention",
-           "carry_gdn_kv_attention_workspace", "carry_gdn_add_rms_norm_quant", "carry_gdn_strerror",
+           "carry_gdn_kv_attention_workspace", "carry_gdn_add_rms_norm_quant", "carry_gdn_prefill",
+           "carry_gdn_prefill_workspace", "carry_gdn_qk_norm_rope", "carry_gdn_strerror",
            "carry_gdn_abi_version", "carry_gdn_last_kernel")
 # what the native call path is given the addresses of, in the order it expects them (csrc/host_native.cpp, Table)
 _NATIVE_ENTRIES = ("carry_gdn_quant_step", "carry_gdn_fp32_step", "carry_gdn_packed_decode",
                    "carry_gdn_packed_decode_multi", "carry_gdn_pool_store", "carry_gdn_pool_load",
                    "carry_gdn_pool_copy", "carry_gdn_pool_copy_layers", "carry_gdn_quant_decode", "carry_gdn_kv_append",
-                   "carry_gdn_kv_attention", "carry_gdn_kv_attention_workspace", "carry_gdn_add_rms_norm_quant")
+                   "carry_gdn_kv_attention", "carry_gdn_kv_attention_workspace", "carry_gdn_add_rms_norm_quant",
+                   "carry_gdn_prefill", "carry_gdn_prefill_workspace", "carry_gdn_qk_norm_rope")
 
 _lib = None
 _lock = threading.Lock()
@@ -249,10 +283,15 @@ def load_library(path: str | None = None):
         lib.carry_gdn_kv_attention_workspace.argtypes = [C.POINTER(KvAttentionArgs)]
         lib.carry_gdn_kv_attention_workspace.restype = C.c_int64
         lib.carry_gdn_add_rms_norm_quant.argtypes = [C.POINTER(NormArgs), C.c_void_p]
+        lib.carry_gdn_prefill.argtypes = [C.POINTER(PrefillArgs), C.c_void_p]
+        lib.carry_gdn_prefill_workspace.argtypes = [C.POINTER(PrefillArgs)]
+        lib.carry_gdn_prefill_workspace.restype = C.c_int64
+        lib.carry_gdn_qk_norm_rope.argtypes = [C.POINTER(RotateArgs), C.c_void_p]
         for fn in (lib.carry_gdn_quant_step, lib.carry_gdn_fp32_step, lib.carry_gdn_packed_decode,
                    lib.carry_gdn_packed_decode_multi, lib.carry_gdn_pool_store, lib.carry_gdn_pool_load,
                    lib.carry_gdn_pool_copy, lib.carry_gdn_pool_copy_layers, lib.carry_gdn_quant_decode,
-                   lib.carry_gdn_kv_append, lib.carry_gdn_kv_attention, lib.carry_gdn_add_rms_norm_quant):
+                   lib.carry_gdn_kv_append, lib.carry_gdn_kv_attention, lib.carry_gdn_add_rms_norm_quant,
+                   lib.carry_gdn_prefill, lib.carry_gdn_qk_norm_rope):
             fn.restype = C.c_int
         lib.native, lib.native_table = _NoNative(), None
         try:

@@ -1,0 +1,44 @@
+// The gated delta rule over whole sequences: what its kernels share.
+//
+//   alpha = exp(-exp(A_log) softplus(a + dt_bias)),  beta = sigmoid(b)
+//   S <- alpha S;  u = beta (v - S k);  S <- S + u k^T;  o = S (scale q)          S [V, K], for every value head
+#pragma once
+
+#include "carry_hybrid.cuh"
+
+namespace carry {
+
+constexpr float kL2Eps = 1e-6f;
+
+// A request's rows, brought into bounds.
+struct PrefillRequest {
+  int first, count;
+};
+__device__ __forceinline__ PrefillRequest prefill_request(const CarryGdnPrefillArgs& a, int b, int* status) {
+  PrefillRequest r;
+  if (a.query_start) {
+    const int from = a.query_start[b], to = a.query_start[b + 1];
+    r.first = min(max(from, 0), a.N);
+    r.count = min(max(min(to, a.N) - r.first, 0), a.max_query);
+    if (status && (r.first != from || r.first + r.count != to)) atomicOr(status, CARRY_GDN_STATUS_BAD_RANGE);
+  } else {
+    r.first = b * a.max_query;
+    r.count = a.max_query;
+  }
+  return r;
+}
+
+// log alpha and beta of a token.  The softplus of a large negative number is that number's exponential, of which log(1 + x)
+// would leave few bits; steps of 0.001 are where models begin.
+__device__ __forceinline__ void prefill_gates(const CarryGdnPrefillArgs& a, long long row, int hv, float& log_alpha, float& beta) {
+  const float x = load_as_float(a.a, row * a.stride_a_tok + hv, a.ab_dtype) + load_as_float(a.dt_bias, hv, a.dt_bias_dtype);
+  const float softplus = x <= kSoftplusThreshold ? log1pf(expf(x)) : x;
+  log_alpha = -expf(load_as_float(a.A_log, hv, a.A_log_dtype)) * softplus;
+  beta = __fdiv_rn(1.0f, 1.0f + expf(-load_as_float(a.b, row * a.stride_b_tok + hv, a.ab_dtype)));
+}
+
+int64_t delta_workspace(const CarryGdnPrefillArgs& a);
+int launch_delta(const CarryGdnPrefillArgs& a, cudaStream_t stream);
+int launch_delta_recurrent(const CarryGdnPrefillArgs& a, cudaStream_t stream);
+
+}  // namespace carry

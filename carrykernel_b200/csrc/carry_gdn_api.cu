@@ -1,7 +1,7 @@
 // C ABI of libcarry_gdn.so: argument checks and kernel selection.  See
 // include/carry_gdn.h for the contract of every entry point.
 #include "carry_gdn_common.cuh"
-#include "carry_hybrid.cuh"
+#include "carry_delta.cuh"
 
 #include <initializer_list>
 
@@ -380,6 +380,73 @@ int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* a, void* stream) {
   if (!a->x || !a->weight || !a->codes || !a->scale) return CARRY_GDN_ERR_NULL;
   const int rc = carry::launch_norm(*a, static_cast<cudaStream_t>(stream));
   if (rc == CARRY_GDN_OK) g_last_kernel = 11;
+  return rc;
+}
+
+namespace {
+int prefill_ok(const CarryGdnPrefillArgs* a) {
+  if (!a) return CARRY_GDN_ERR_NULL;
+  if (a->B < 0 || a->N < 0 || a->max_query < 0 || a->H <= 0 || a->HV <= 0 || a->HV % a->H) return CARRY_GDN_ERR_SHAPE;
+  if (!a->query_start && (long long)a->B * a->max_query != a->N) return CARRY_GDN_ERR_SHAPE;
+  if (a->K != a->V || (a->K != 64 && a->K != 128)) return CARRY_GDN_ERR_UNSUPPORTED;
+  if (a->B > 65535 || a->HV > 65535) return CARRY_GDN_ERR_TOO_LARGE;
+  for (int t : {a->qkv_dtype, a->ab_dtype, a->A_log_dtype, a->dt_bias_dtype, a->out_dtype})
+    if (!dtype_ok(t)) return CARRY_GDN_ERR_DTYPE;
+  return CARRY_GDN_OK;
+}
+// No request has more rows than the call: a looser bound costs nothing.
+CarryGdnPrefillArgs prefill_bounded(const CarryGdnPrefillArgs& a) {
+  CarryGdnPrefillArgs bounded = a;
+  if (bounded.max_query > bounded.N) bounded.max_query = bounded.N;
+  return bounded;
+}
+}  // namespace
+
+int64_t carry_gdn_prefill_workspace(const CarryGdnPrefillArgs* a) {
+  const int rc = prefill_ok(a);
+  return rc != CARRY_GDN_OK ? rc : carry::delta_workspace(prefill_bounded(*a));
+}
+
+int carry_gdn_prefill(const CarryGdnPrefillArgs* a, void* stream) {
+  clear_stale_error();
+  int rc = prefill_ok(a);
+  if (rc != CARRY_GDN_OK) return rc;
+  if (a->B == 0) return CARRY_GDN_OK;
+  if (!a->final_state || !a->A_log || !a->dt_bias) return CARRY_GDN_ERR_NULL;
+  if (a->N > 0 && (!a->mixed_qkv || !a->a || !a->b || !a->out)) return CARRY_GDN_ERR_NULL;
+  for (const void* p : {(const void*)a->initial_state, (const void*)a->final_state})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return CARRY_GDN_ERR_SHAPE;
+  if (a->stride_final_req % 4 || (a->initial_state && a->stride_initial_req % 4)) return CARRY_GDN_ERR_SHAPE;
+  const CarryGdnPrefillArgs bounded = prefill_bounded(*a);
+  const int64_t need = carry::delta_workspace(bounded);
+  if (need < 0) return static_cast<int>(need);
+  if (need > 0 && !a->workspace) return CARRY_GDN_ERR_NULL;
+  if (need > 0 && (a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)) return CARRY_GDN_ERR_SHAPE;
+  rc = carry::launch_delta(bounded, static_cast<cudaStream_t>(stream));
+  if (rc == CARRY_GDN_OK) g_last_kernel = need > 0 ? 14 : 13;
+  return rc;
+}
+
+int carry_gdn_qk_norm_rope(const CarryGdnRotateArgs* a, void* stream) {
+  clear_stale_error();
+  if (!a) return CARRY_GDN_ERR_NULL;
+  if (a->N < 0 || a->HQ < 0 || a->HK < 0 || a->D <= 0 || a->D % 2 || a->rotary < 0 || a->rotary % 2 || a->rotary > a->D) return CARRY_GDN_ERR_SHAPE;
+  if (a->axes < 1 || a->axes > 4 || a->table_rows < 0) return CARRY_GDN_ERR_SHAPE;
+  long long pairs = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    if (a->sections[i] < 0) return CARRY_GDN_ERR_SHAPE;
+    pairs += a->sections[i];
+  }
+  if (2 * pairs != a->rotary) return CARRY_GDN_ERR_SHAPE;
+  if (a->D > 512) return CARRY_GDN_ERR_UNSUPPORTED;
+  for (int t : {a->dtype, a->weight_dtype, a->table_dtype})
+    if (!dtype_ok(t)) return CARRY_GDN_ERR_DTYPE;
+  if (!(a->eps >= 0.0f)) return CARRY_GDN_ERR_SHAPE;
+  if (a->N == 0 || (a->HQ == 0 && a->HK == 0)) return CARRY_GDN_OK;
+  if (!a->positions || (a->rotary > 0 && a->table_rows > 0 && !a->cos_sin)) return CARRY_GDN_ERR_NULL;
+  if ((a->HQ > 0 && (!a->q || !a->q_out || !a->q_weight)) || (a->HK > 0 && (!a->k || !a->k_out || !a->k_weight))) return CARRY_GDN_ERR_NULL;
+  const int rc = carry::launch_rotate(*a, static_cast<cudaStream_t>(stream));
+  if (rc == CARRY_GDN_OK) g_last_kernel = 12;
   return rc;
 }
 

@@ -119,5 +119,6 @@ int launch_kv_append(const CarryGdnKvAppendArgs& a, cudaStream_t stream);
 int launch_kv_attention(const CarryGdnKvAttentionArgs& a, cudaStream_t stream);
 int64_t kv_attention_workspace(const CarryGdnKvAttentionArgs& a);
 int launch_norm(const CarryGdnNormArgs& a, cudaStream_t stream);
+int launch_rotate(const CarryGdnRotateArgs& a, cudaStream_t stream);
 
 }  // namespace carry

@@ -40,8 +40,11 @@ struct Table {
   int (*kv_attention)(const CarryGdnKvAttentionArgs*, void*);
   int64_t (*kv_attention_workspace)(const CarryGdnKvAttentionArgs*);
   int (*add_rms_norm_quant)(const CarryGdnNormArgs*, void*);
+  int (*prefill)(const CarryGdnPrefillArgs*, void*);
+  int64_t (*prefill_workspace)(const CarryGdnPrefillArgs*);
+  int (*qk_norm_rope)(const CarryGdnRotateArgs*, void*);
 };
-constexpr int kEntries = 13;
+constexpr int kEntries = 16;
 
 const Table* table_of(PyObject* o) { return static_cast<const Table*>(PyLong_AsVoidPtr(o)); }
 
@@ -710,6 +713,141 @@ PyObject* add_rms_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------------------
+// a prompt's way in: the recurrence over sequences, norm and rotation of queries and keys
+// ---------------------------------------------------------------------------
+
+// (table, mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, initial_state, query_start, max_query_len, use_qk_l2norm,
+//  workspace, status) -> True
+PyObject* prefill(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 15) return nullptr;
+    const Table* tab = table_of(o[0]);
+    const at::Tensor *mixed = plain(o[1]), *a = plain(o[2]), *b = plain(o[3]), *A_log = plain(o[4]), *dt_bias = plain(o[5]);
+    const at::Tensor *out = plain(o[7]), *last = plain(o[8]), *first = o[9] == Py_None ? nullptr : plain(o[9]);
+    if (!tab || !mixed || !a || !b || !A_log || !dt_bias || !out || !last || (o[9] != Py_None && !first)) return nullptr;
+    if (!last->is_cuda() || last->dim() != 4 || mixed->dim() != 2) return nullptr;
+    const int dev = last->get_device();
+    const int64_t N = mixed->size(0), B = last->size(0), HV = last->size(1), V = last->size(2), K = last->size(3);
+    if (!fits32(N) || !fits32(B) || !fits32(HV) || K != V || (K != 64 && K != 128)) return nullptr;
+    const int64_t qk = mixed->size(1) - HV * V, H = qk / (2 * K);
+    if (qk <= 0 || H <= 0 || HV % H || 2 * H * K != qk) return nullptr;
+    for (const at::Tensor* t : {last, first})
+      if (t && (!is(t, at::kFloat, dev) || !shaped(*t, {B, HV, V, K}) || !dense_inside(*t, {V * K, K, 1}))) return nullptr;
+    if (!is(mixed, mixed->scalar_type(), dev) || mixed->stride(1) != 1) return nullptr;
+    for (const at::Tensor* t : {a, b})
+      if (!is(t, a->scalar_type(), dev) || !shaped(*t, {N, HV}) || t->stride(1) != 1) return nullptr;
+    for (const at::Tensor* t : {A_log, dt_bias})
+      if (!is(t, t->scalar_type(), dev) || !shaped(*t, {HV}) || !t->is_contiguous()) return nullptr;
+    if (!is(out, out->scalar_type(), dev) || !shaped(*out, {N, HV, V}) || !dense_inside(*out, {V, 1})) return nullptr;
+    CarryGdnPrefillArgs p = {};
+    p.qkv_dtype = dtype_id(mixed->scalar_type()); p.ab_dtype = dtype_id(a->scalar_type());
+    p.A_log_dtype = dtype_id(A_log->scalar_type()); p.dt_bias_dtype = dtype_id(dt_bias->scalar_type()); p.out_dtype = dtype_id(out->scalar_type());
+    for (int t : {p.qkv_dtype, p.ab_dtype, p.A_log_dtype, p.dt_bias_dtype, p.out_dtype})
+      if (t < 0) return nullptr;
+    long most = 0;
+    const bool bounded = o[11] != Py_None;
+    if (bounded && !as_int(o[11], most)) return nullptr;
+    if (o[10] == Py_None) {
+      if (N % B || (bounded && most != N / B)) return nullptr;
+      p.max_query = static_cast<int32_t>(N / B);
+    } else {
+      const at::Tensor* start = plain(o[10]);
+      if (!bounded || most < 1 || !is(start, at::kInt, dev) || !start->is_contiguous() || !shaped(*start, {B + 1})) return nullptr;
+      p.query_start = static_cast<const int32_t*>(start->data_ptr());
+      p.max_query = static_cast<int32_t>(most < N ? most : N);
+    }
+    const double scale = PyFloat_AsDouble(o[6]);
+    if ((scale == -1.0 && PyErr_Occurred()) || !status_of(o[14], dev, &p.status)) return nullptr;
+    if (o[12] != Py_True && o[12] != Py_False) return nullptr;
+    p.scale = static_cast<float>(scale);
+    p.use_qk_l2norm = o[12] == Py_True;
+    p.mixed_qkv = mixed->data_ptr(); p.stride_mixed_tok = mixed->stride(0);
+    p.a = a->data_ptr(); p.stride_a_tok = a->stride(0); p.b = b->data_ptr(); p.stride_b_tok = b->stride(0);
+    p.A_log = A_log->data_ptr(); p.dt_bias = dt_bias->data_ptr();
+    if (first) { p.initial_state = static_cast<const float*>(first->data_ptr()); p.stride_initial_req = first->stride(0); }
+    p.final_state = static_cast<float*>(last->data_ptr()); p.stride_final_req = last->stride(0);
+    p.out = out->data_ptr(); p.stride_out_tok = out->stride(0);
+    p.B = static_cast<int32_t>(B); p.N = static_cast<int32_t>(N); p.H = static_cast<int32_t>(H); p.HV = static_cast<int32_t>(HV);
+    p.K = p.V = static_cast<int32_t>(K);
+    c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const int64_t need = tab->prefill_workspace(&p);
+    if (need < 0) return nullptr;
+    at::Tensor work;
+    if (o[13] != Py_None) {
+      const at::Tensor* w = plain(o[13]);
+      if (!w || !w->is_cuda() || w->get_device() != dev || !w->is_contiguous()) return nullptr;
+      work = *w;
+    } else if (need > 0) {
+      work = fresh({need}, at::kByte, dev);
+    }
+    if (work.defined()) {
+      p.workspace = work.data_ptr();
+      p.workspace_bytes = static_cast<int64_t>(work.nbytes());
+    }
+    return launch(dev, [&](void* s) { return tab->prefill(&p, s); }) ? Py_NewRef(Py_True) : nullptr;
+  });
+}
+
+// (table, q, k, q_weight, k_weight, cos_sin, positions, eps, q_out, k_out, sections, interleaved, weight_offset, status) -> True
+PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 14) return nullptr;
+    const Table* tab = table_of(o[0]);
+    const at::Tensor *q = plain(o[1]), *k = plain(o[2]), *qw = plain(o[3]), *kw = plain(o[4]), *table = plain(o[5]), *pos = plain(o[6]);
+    const at::Tensor *q_out = o[8] == Py_None ? q : plain(o[8]), *k_out = o[9] == Py_None ? k : plain(o[9]);
+    if (!tab || !q || !k || !qw || !kw || !table || !pos || !q_out || !k_out || !q->is_cuda() || q->dim() != 3 || k->dim() != 3) return nullptr;
+    const int dev = q->get_device();
+    const int64_t N = q->size(0), HQ = q->size(1), HK = k->size(1), D = q->size(2);
+    if (!fits32(N) || !fits32(HQ) || !fits32(HK) || !fits32(D)) return nullptr;
+    CarryGdnRotateArgs a = {};
+    a.dtype = dtype_id(q->scalar_type());
+    a.weight_dtype = dtype_id(qw->scalar_type());
+    a.table_dtype = dtype_id(table->scalar_type());
+    if (a.dtype < 0 || a.weight_dtype < 0 || a.table_dtype < 0) return nullptr;
+    for (const at::Tensor* t : {q, q_out})
+      if (!is(t, q->scalar_type(), dev) || !shaped(*t, {N, HQ, D}) || t->stride(2) != 1) return nullptr;
+    for (const at::Tensor* t : {k, k_out})
+      if (!is(t, q->scalar_type(), dev) || !shaped(*t, {N, HK, D}) || t->stride(2) != 1) return nullptr;
+    for (const at::Tensor* t : {qw, kw})
+      if (!is(t, qw->scalar_type(), dev) || !shaped(*t, {D}) || !t->is_contiguous()) return nullptr;
+    if (!is(table, table->scalar_type(), dev) || table->dim() != 2 || table->stride(1) != 1 || table->size(1) > D) return nullptr;
+    const bool wide = pos->scalar_type() == at::kLong;
+    if (!is(pos, wide ? at::kLong : at::kInt, dev) || pos->dim() < 1 || pos->dim() > 2) return nullptr;
+    a.axes = pos->dim() == 1 ? 1 : static_cast<int32_t>(pos->size(0));
+    if (a.axes < 1 || a.axes > 4 || pos->size(pos->dim() - 1) != N || pos->stride(pos->dim() - 1) != 1) return nullptr;
+    a.stride_positions = pos->dim() == 1 ? 0 : pos->stride(0);
+    if (o[10] == Py_None) {
+      if (a.axes != 1) return nullptr;
+      a.sections[0] = static_cast<int32_t>(table->size(1) / 2);
+    } else {
+      if (!PyList_Check(o[10]) && !PyTuple_Check(o[10])) return nullptr;
+      if (PySequence_Fast_GET_SIZE(o[10]) != a.axes) return nullptr;
+      for (int i = 0; i < a.axes; ++i) {
+        long section;
+        if (!as_int(PySequence_Fast_GET_ITEM(o[10], i), section) || section < 0 || section > D) return nullptr;
+        a.sections[i] = static_cast<int32_t>(section);
+      }
+    }
+    const double eps = PyFloat_AsDouble(o[7]);
+    if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+    const double offset = PyFloat_AsDouble(o[12]);
+    if ((offset == -1.0 && PyErr_Occurred()) || !status_of(o[13], dev, &a.status)) return nullptr;
+    if (o[11] != Py_True && o[11] != Py_False) return nullptr;
+    a.q = q->data_ptr(); a.k = k->data_ptr(); a.q_out = q_out->data_ptr(); a.k_out = k_out->data_ptr();
+    a.stride_q_tok = q->stride(0); a.stride_q_head = q->stride(1); a.stride_k_tok = k->stride(0); a.stride_k_head = k->stride(1);
+    a.stride_q_out_tok = q_out->stride(0); a.stride_q_out_head = q_out->stride(1);
+    a.stride_k_out_tok = k_out->stride(0); a.stride_k_out_head = k_out->stride(1);
+    a.q_weight = qw->data_ptr(); a.k_weight = kw->data_ptr();
+    a.cos_sin = table->data_ptr(); a.stride_table = table->stride(0); a.table_rows = table->size(0);
+    a.positions = pos->data_ptr(); a.positions_64 = wide;
+    a.eps = static_cast<float>(eps); a.weight_offset = static_cast<float>(offset); a.interleaved = o[11] == Py_True;
+    a.N = static_cast<int32_t>(N); a.HQ = static_cast<int32_t>(HQ); a.HK = static_cast<int32_t>(HK); a.D = static_cast<int32_t>(D);
+    a.rotary = static_cast<int32_t>(table->size(1));
+    return launch(dev, [&](void* s) { return tab->qk_norm_rope(&a, s); }) ? Py_NewRef(Py_True) : nullptr;
+  });
+}
+
 // (address of each entry point, in the order of Table) -> the table's address; it lives as long as the process
 PyObject* make_table(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (n != kEntries) {
@@ -734,6 +872,7 @@ PyObject* make_table(PyObject*, PyObject* const* o, Py_ssize_t n) {
 PyMethodDef methods[] = {CARRY_FAST(make_table), CARRY_FAST(packed_decode), CARRY_FAST(quant_step), CARRY_FAST(quant_decode), CARRY_FAST(quant_chain),
                          CARRY_FAST(fp32_step), CARRY_FAST(pool_move), CARRY_FAST(pool_copy), CARRY_FAST(pool_copy_layers),
                          CARRY_FAST(kv_append), CARRY_FAST(kv_attention), CARRY_FAST(add_rms_norm),
+                         CARRY_FAST(prefill), CARRY_FAST(qk_norm_rope),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the Python surfaces.", -1, methods};
 

@@ -441,6 +441,91 @@ typedef struct CarryGdnNormArgs {
 
 int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* args, void* stream);
 
+/*
+ * The gated delta rule over whole sequences, from a floating-point state (or
+ * none) to a floating-point state: what goes ahead of carry_gdn_packed_decode for
+ * a prompt, between carry_gdn_pool_load and carry_gdn_pool_store for a further
+ * chunk of one.  The recurrence, gates, head map and L2 norm are those of
+ * carry_gdn_packed_decode with the state left unquantized:
+ *   S <- alpha S;  u = beta (v - S k);  S <- S + u k^T;  o = S (scale q)
+ * for every token of a request in turn, with q and k divided by
+ * sqrt(sum of squares + 1e-6) where use_qk_l2norm is set.  The rows of request
+ * b are query_start[b] .. query_start[b + 1] - 1 (at most max_query; more, and
+ * rows outside 0 .. N - 1, are skipped and flagged with
+ * CARRY_GDN_STATUS_BAD_RANGE), or, with query_start NULL, max_query = N / B
+ * each.  No two requests share a row.  A request without rows hands its state
+ * on.  K and V are 64 or 128 (one width for both), B and HV at most 65535.
+ * final_state may be initial_state.  `workspace` is at least
+ * carry_gdn_prefill_workspace() bytes, 16-byte aligned; nothing is kept in it
+ * between calls.
+ */
+typedef struct CarryGdnPrefillArgs {
+  const void* mixed_qkv;      /* [N, 2*H*K + HV*V] = q | k | v, as in carry_gdn_packed_decode */
+  int64_t stride_mixed_tok;
+  const void* a;              /* [N, HV] */
+  int64_t stride_a_tok;
+  const void* b;              /* [N, HV] */
+  int64_t stride_b_tok;
+  const void* A_log;          /* [HV] */
+  const void* dt_bias;        /* [HV] */
+  const float* initial_state; /* [B, HV, V, K], dense within a request, or NULL for zeros */
+  int64_t stride_initial_req;
+  float* final_state;         /* [B, HV, V, K] */
+  int64_t stride_final_req;
+  void* out;                  /* [N, HV, V], dense within a token */
+  int64_t stride_out_tok;
+  const int32_t* query_start; /* [B + 1], or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;            /* optional device word, may be NULL */
+  float scale;
+  int32_t B, N, max_query, H, HV, K, V;
+  int32_t qkv_dtype, ab_dtype, A_log_dtype, dt_bias_dtype, out_dtype;
+  int32_t use_qk_l2norm;
+} CarryGdnPrefillArgs;
+
+int carry_gdn_prefill(const CarryGdnPrefillArgs* args, void* stream);
+
+/* Bytes of workspace that a call with these arguments needs (0 for none), or a
+ * negative CARRY_GDN_ERR_*.  Looks at sizes only: no pointer is read. */
+int64_t carry_gdn_prefill_workspace(const CarryGdnPrefillArgs* args);
+
+/*
+ * RMS norm of every query and key head and the rotation by the token's
+ * position: y = x * rsqrt(mean(x^2) + eps) * (weight + weight_offset), and of
+ * y's first `rotary` numbers the pairs (y1, y2) -> (y1 cos - y2 sin, y2 cos +
+ * y1 sin).  Pair i < rotary / 2 is (y[i], y[i + rotary / 2]), or (y[2 i],
+ * y[2 i + 1]) where `interleaved` is set; its cos and sin are columns i and
+ * rotary / 2 + i of row p of cos_sin, p the token's position on the pair's axis:
+ * the first sections[0] pairs are axis 0's, the next sections[1] axis 1's, and so
+ * on.  A token with a negative position is left alone (nothing of it is
+ * written), and so is one with a position beyond the table, which is flagged
+ * with CARRY_GDN_STATUS_BAD_RANGE.  A head with a number that is not finite
+ * becomes NaN.  q_out and k_out may be q and k.  D is even and at most 512,
+ * rotary even and at most D, axes 1 to 4.
+ */
+typedef struct CarryGdnRotateArgs {
+  const void* q;          /* [N, HQ, D], D contiguous */
+  const void* k;          /* [N, HK, D] */
+  void* q_out;
+  void* k_out;
+  int64_t stride_q_tok, stride_q_head, stride_k_tok, stride_k_head;
+  int64_t stride_q_out_tok, stride_q_out_head, stride_k_out_tok, stride_k_out_head;
+  const void* q_weight;   /* [D] */
+  const void* k_weight;   /* [D] */
+  const void* cos_sin;    /* [table_rows, rotary] = cos | sin */
+  int64_t stride_table, table_rows;
+  const void* positions;  /* [axes, N], int32 or int64, N contiguous */
+  int64_t stride_positions;
+  int32_t* status;        /* optional device word, may be NULL */
+  float eps, weight_offset;
+  int32_t N, HQ, HK, D, rotary, axes, sections[4];
+  int32_t positions_64, interleaved;
+  int32_t dtype, weight_dtype, table_dtype; /* dtype: of q, k, q_out and k_out */
+} CarryGdnRotateArgs;
+
+int carry_gdn_qk_norm_rope(const CarryGdnRotateArgs* args, void* stream);
+
 /* Human-readable text for a CARRY_GDN_ERR_* code (static storage). */
 const char* carry_gdn_strerror(int code);
 
@@ -454,7 +539,8 @@ int carry_gdn_abi_version(void);
  * 5 = 128x128 streaming kernel, step without error feedback,
  * 6 = slot-indexed kernel for 64x64 heads, 7 = kernel of chained steps,
  * 8 = statequant-layout kernel for 64x64 heads, 9 = key/value append, 10 = attention over the
- * key/value cache, 11 = layer norm with 8-bit output.
+ * key/value cache, 11 = layer norm with 8-bit output, 12 = norm and rotation of queries and keys, 13 = gated
+ * delta rule over sequences, token by token, 14 = the same in chunks.
  * Diagnostic only (tests use it to prove which path ran).
  */
 int carry_gdn_last_kernel(void);

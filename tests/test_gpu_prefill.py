@@ -1,0 +1,306 @@
+"""The gated delta rule over whole sequences against the recurrence in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from carrykernel_b200 import _lib
+from carrykernel_b200.vllm_integration import packed_prefill as pp
+from oracle import prompt_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda"
+TOKEN_BY_TOKEN, IN_CHUNKS = 13, 14
+
+
+def make(lengths, H, HV, D, dtype, initial=False, l2norm=True, seed=0, gates=None):
+    g = torch.Generator().manual_seed(seed)
+    N = sum(lengths)
+    x = torch.nn.functional.silu(torch.randn(N, 2 * H * D + HV * D, generator=g))
+    if not l2norm:
+        qk = x[:, :2 * H * D].view(N, 2 * H, D)
+        qk /= qk.norm(dim=-1, keepdim=True) + 1e-3
+    c = dict(mixed_qkv=x.to(dtype), a=torch.randn(N, HV, generator=g).to(gates or dtype), b=torch.randn(N, HV, generator=g).to(gates or dtype),
+             A_log=torch.log(1 + 15 * torch.rand(HV, generator=g)), dt_bias=torch.randn(HV, generator=g) - 4, scale=D ** -0.5)
+    state = torch.randn(len(lengths), HV, D, D, generator=g) if initial else None
+    return c, state
+
+
+def starts(lengths):
+    return torch.tensor([sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=torch.int32)
+
+
+def run(c, state, lengths, HV, D, l2norm=True, out_dtype=None, most=None, **more):
+    N = sum(lengths)
+    dev = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in c.items()}
+    out = torch.full((N, HV, D), float("nan"), dtype=out_dtype or c["mixed_qkv"].dtype, device=DEV)
+    final = torch.full((len(lengths), HV, D, D), float("nan"), device=DEV)
+    pp.gated_delta_rule_packed_prefill(**dev, out=out, final_state=final, initial_state=None if state is None else state.to(DEV),
+                                       query_start=starts(lengths).to(DEV), max_query_len=max(lengths) if most is None else most,
+                                       use_qk_l2norm_in_kernel=l2norm, **more)
+    return out, final
+
+
+def bounds(out, wanted, in_chunks, fp32_operands):
+    """What outputs and states may be off by.
+
+    A token's own arithmetic is fp32: a product of the state with a key is a sum of 128 numbers (at most 32 roundings one after the
+    other token by token; on the tensor cores 48 steps of sixteen, each of which may lose 2^-23 of the largest), key and query
+    norms, gates (an exponential of an exponential and a logarithm: 8 roundings relative to the log decay) and a few products: 64
+    roundings of 2^-24 token by token, 256 in chunks.  In chunks T comes as two bf16 numbers, 2^-18 off (three, 2^-26, for fp32
+    operands, where what T is solved from counts: 16 roundings of 2^-24), and P T is a sum of products of such, 2^-16.  Then the rounding
+    to the output's type.  Below 2^-126 fp32 has no relative precision, and below 2^-149 nothing (sigmoid(-200) is 2^-288, and a decay
+    by exp(-100) is good to 2^-150): each factor and each number may lose 2^-126 of what it multiplies or is added to."""
+    want_out, want_state, out_weight, weight = wanted
+    floor = 2.0 ** -126
+    own = (256 if in_chunks else 64) * 2.0 ** -24
+    of_t = 0.0 if not in_chunks else 2.0 ** -20 if fp32_operands else 2.0 ** -18 + 2.0 ** -20
+    state = own * weight[..., 0] + of_t * weight[..., 1] + floor * (1 + weight[..., 0])
+    half_step = torch.finfo(out.dtype).eps / 2
+    value = own * out_weight[..., 0] + 4 * of_t * out_weight[..., 1] + floor * (1 + out_weight[..., 0])
+    return (1 + half_step) * value + half_step * want_out.abs() + torch.finfo(out.dtype).smallest_normal * half_step, state
+
+
+def check(got, c, state, lengths, H, D, l2norm=True, in_chunks=None, rows=None, requests=None):
+    out, final = got
+    wanted = orc.delta_rule(**{k: v for k, v in c.items() if k != "mixed_qkv"}, mixed=c["mixed_qkv"], H=H, D=D, lengths=lengths, initial=state,
+                            l2norm=l2norm)
+    out_bound, state_bound = bounds(out, wanted, in_chunks, c["mixed_qkv"].dtype == F32)
+    off, off_state = (out.cpu().double() - wanted[0]).abs(), (final.cpu().double() - wanted[1]).abs()
+    rows, requests = slice(None) if rows is None else rows, slice(None) if requests is None else requests
+    assert (off <= out_bound)[rows].all(), f"outputs off by up to {(off / out_bound)[rows].max():.2f} of the bound"
+    assert (off_state <= state_bound)[requests].all(), f"states off by up to {(off_state / state_bound)[requests].max():.2f} of the bound"
+    # In the mean: a split's error is as good as random, at most 2^-18 of T's entry (2^-22 with what counts for fp32 operands), and
+    # what a token's own arithmetic loses is 16 roundings.
+    weight = wanted[3][requests]
+    mean = 2.0 ** -20 * weight[..., 0] + (2.0 ** -22 if c["mixed_qkv"].dtype == F32 else 2.0 ** -18) * weight[..., 2] + 2.0 ** -126
+    assert off_state[requests].norm() <= mean.expand_as(off_state[requests]).norm() / D ** 0.5
+
+
+FEW = [[1], [3], [1, 1, 1], [5, 0, 2], [33], [64], [1, 64, 17]]
+MANY = [[65], [128], [1, 0, 64, 65, 3], [200, 77], [191, 1]]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", FEW + MANY, ids=str)
+def test_against_recurrence(dtype, D, lengths):
+    H, HV = (2, 4) if D == 64 else (1, 3)
+    initial = len(lengths) % 2 == 1
+    c, state = make(lengths, H, HV, D, dtype, initial)
+    got = run(c, state, lengths, HV, D)
+    in_chunks = max(lengths) > 64
+    assert _lib.load_library().carry_gdn_last_kernel() == (IN_CHUNKS if in_chunks else TOKEN_BY_TOKEN)
+    check(got, c, state, lengths, H, D, in_chunks=in_chunks)
+
+
+@pytest.mark.parametrize("lengths", [[40], [130]], ids=str)
+@pytest.mark.parametrize("H,HV", [(1, 1), (1, 8), (5, 5), (4, 8)])
+def test_head_maps_and_unnormed_keys(lengths, H, HV):
+    for dtype, out_dtype, gates in ((BF16, F32, F32), (F16, BF16, BF16), (F32, F16, F16)):
+        c, state = make(lengths, H, HV, 64, dtype, True, l2norm=False, seed=H, gates=gates)
+        got = run(c, state, lengths, HV, 64, l2norm=False, out_dtype=out_dtype)
+        check(got, c, state, lengths, H, 64, l2norm=False, in_chunks=max(lengths) > 64)
+
+
+@pytest.mark.parametrize("lengths", [[3, 20], [100, 70]], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_strides_and_alignment(lengths, dtype):
+    """Rows of wider tensors that begin off the grid, states apart from one another, in place; what lies beside them stays."""
+    H, HV, D = 1, 2, 64
+    c, state = make(lengths, H, HV, D, dtype, True)
+    plain = run(c, state, lengths, HV, D)
+    N, width = c["mixed_qkv"].shape
+    wide = torch.full((N, width + 3), 9.0, dtype=dtype, device=DEV)
+    wide[:, 1:1 + width] = c["mixed_qkv"].to(DEV)
+    gates = torch.full((N, 2 * HV + 1), 9.0, dtype=dtype, device=DEV)
+    gates[:, :HV], gates[:, HV + 1:] = c["a"].to(DEV), c["b"].to(DEV)
+    outs = torch.full((N + 2, HV * D + 7), 9.0, dtype=dtype, device=DEV)
+    states = torch.full((4, HV, D, D), 9.0, device=DEV)
+    states[::2] = state.to(DEV)
+    out = outs[1:-1, 3:3 + HV * D].unflatten(1, (HV, D))
+    pp.gated_delta_rule_packed_prefill(wide[:, 1:1 + width], gates[:, :HV], gates[:, HV + 1:], c["A_log"].to(DEV), c["dt_bias"].to(DEV), c["scale"],
+                                       out, states[::2], initial_state=states[::2], query_start=starts(lengths).to(DEV),
+                                       max_query_len=max(lengths), use_qk_l2norm_in_kernel=True)
+    assert torch.equal(out, plain[0]) and torch.equal(states[::2], plain[1])
+    assert (states[1::2] == 9).all() and (outs[[0, -1]] == 9).all() and (outs[:, :3] == 9).all() and (outs[:, 3 + HV * D:] == 9).all()
+
+
+@pytest.mark.parametrize("most", [64, 200])
+def test_rows_outside_of_the_requests(most):
+    """Rows ahead of the first request and behind the last one are left as they were, whatever they hold."""
+    H, HV, D, lengths = 1, 2, 128, [40, 90 if most > 64 else 30]
+    c, state = make([7, *lengths, 70], H, HV, D, BF16, True)
+    for x in (c["mixed_qkv"], c["a"], c["b"]):
+        x[:7], x[7 + sum(lengths):] = float("nan"), float("inf")
+    N = c["mixed_qkv"].shape[0]
+    dev = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in c.items()}
+    out, final = torch.full((N, HV, D), 9.0, dtype=BF16, device=DEV), torch.empty(2, HV, D, D, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    pp.gated_delta_rule_packed_prefill(**dev, out=out, final_state=final, initial_state=state[1:3].to(DEV), query_start=7 + starts(lengths).to(DEV),
+                                       max_query_len=most, use_qk_l2norm_in_kernel=True, status=status)
+    assert status.item() == 0 and (out[:7] == 9).all() and (out[7 + sum(lengths):] == 9).all()
+    inner = {k: v[7:7 + sum(lengths)] if k in ("mixed_qkv", "a", "b") else v for k, v in c.items()}
+    check((out[7:7 + sum(lengths)], final), inner, state[1:3], lengths, H, D, in_chunks=most > 64)
+
+
+@pytest.mark.parametrize("n", [20, 150])
+def test_a_request_with_numbers_that_are_not_finite_spoils_no_other(n):
+    H, HV, D, lengths = 2, 2, 64, [n, n, n]
+    c, state = make(lengths, H, HV, D, BF16, True)
+    clean = run(c, state, lengths, HV, D)
+    c["mixed_qkv"][n + 5:n + 9] = float("nan")
+    c["a"][n + 3], state[1, 0, 0, 0] = float("nan"), float("inf")
+    got = run(c, state, lengths, HV, D)
+    for r in (slice(0, n), slice(2 * n, None)):
+        assert torch.equal(got[0][r], clean[0][r])
+    assert torch.equal(got[1][::2], clean[1][::2]) and got[1][1].isnan().any()
+
+
+def test_bad_row_ranges_are_flagged_and_skipped():
+    H, HV, D = 1, 1, 64
+    c, _ = make([100], H, HV, D, BF16)
+    dev = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in c.items()}
+    for start, most in (([0, 70, 250], 90), ([-5, 20, 60], 64), ([0, 100, 40], 100), ([0, 90, 100], 70), ([0, 20, 100], 40)):
+        out, final = torch.full((100, HV, D), 9.0, dtype=BF16, device=DEV), torch.empty(2, HV, D, D, device=DEV)
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        pp.gated_delta_rule_packed_prefill(**dev, out=out, final_state=final, query_start=torch.tensor(start, dtype=torch.int32, device=DEV),
+                                           max_query_len=most, use_qk_l2norm_in_kernel=True, status=status)
+        assert status.item() == _lib.STATUS_BAD_RANGE, (start, most)
+        assert final.isfinite().all() and out.isfinite().all()
+        with pytest.raises(RuntimeError):
+            _lib.raise_for_status(status)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_prompt_in_parts_is_the_prompt(dtype):
+    """Handing the state on at any token, from any of the two ways of working to the other, is within the bounds of one call."""
+    H, HV, D, lengths = 1, 2, 128, [230]
+    c, state = make(lengths, H, HV, D, dtype, True)
+    outs, now, at = [], state.to(DEV), 0
+    for n in (1, 70, 64, 30, 65):
+        part = {k: v[at:at + n] if k in ("mixed_qkv", "a", "b") else v for k, v in c.items()}
+        out, now = run(part, now, [n], HV, D)
+        outs.append(out)
+        at += n
+    check((torch.cat(outs), now), c, state, lengths, H, D, in_chunks=True)
+
+
+def test_launches_that_share_the_workspace_out():
+    """A call too large for the workspace's bound is cut by chunks and by requests: the same numbers as alone."""
+    for D, H, HV, lengths in ((128, 4, 32, [4200, 64, 4500, 4097]), (64, 4, 64, [65] * 130 + [129])):
+        c, state = make(lengths, H, HV, D, BF16, True)
+        out, final = run(c, state, lengths, HV, D)
+        for i in range(0, len(lengths), max(1, len(lengths) // 4)):
+            rows = slice(sum(lengths[:i]), sum(lengths[:i + 1]))
+            part = {k: v[rows] if k in ("mixed_qkv", "a", "b") else v for k, v in c.items()}
+            alone = run(part, state[i:i + 1], lengths[i:i + 1], HV, D, most=None if lengths[i] > 64 else 65)
+            if lengths[i] > 64:
+                assert torch.equal(out[rows], alone[0]) and torch.equal(final[i:i + 1], alone[1])
+
+
+def test_extreme_gates():
+    """Decays of 0 and 1, write strengths of 0 and 1, and products of decays far below fp32."""
+    for lengths in ([30], [140]):
+        H, HV, D = 1, 4, 64
+        c, state = make(lengths, H, HV, D, BF16, True, gates=F32)
+        n = sum(lengths)
+        c["A_log"] = torch.tensor([-30.0, 5.0, 0.0, 60.0])
+        c["dt_bias"] = torch.zeros(HV)
+        c["b"][:, 0], c["b"][n // 2:, 1], c["b"][:, 2] = 100.0, -200.0, torch.where(torch.arange(n) % 2 == 0, 90.0, -90.0)
+        c["a"][:, 2] = torch.where(torch.arange(n) % 7 == 0, 300.0, -300.0)
+        got = run(c, state, lengths, HV, D)
+        check(got, c, state, lengths, H, D, in_chunks=n > 64)
+
+
+def test_alike_keys_and_zero_rows():
+    """A chunk whose keys are all one direction (the triangular system at its fullest), and tokens of zeros."""
+    for lengths in ([30], [150]):
+        H, HV, D = 1, 2, 128
+        c, state = make(lengths, H, HV, D, BF16, True)
+        x = c["mixed_qkv"]
+        x[:, D:2 * D] = x[0, D:2 * D]
+        x[3], x[100:105] = 0.0, 0.0
+        c["a"].fill_(-30.0)
+        c["b"].fill_(3.0)
+        got = run(c, state, lengths, HV, D)
+        check(got, c, state, lengths, H, D, in_chunks=max(lengths) > 64)
+
+
+def test_no_rows_at_all():
+    state = torch.randn(2, 3, 64, 64, device=DEV)
+    for initial, want in ((None, torch.zeros_like(state)), (state, state)):
+        final = torch.full_like(state, 9.0)
+        pp.gated_delta_rule_packed_prefill(torch.empty(0, 5 * 64, dtype=BF16, device=DEV), torch.empty(0, 3, device=DEV), torch.empty(0, 3, device=DEV),
+                                           torch.zeros(3, device=DEV), torch.zeros(3, device=DEV), 1.0, torch.empty(0, 3, 64, dtype=BF16, device=DEV),
+                                           final, initial_state=initial)
+        assert torch.equal(final, want)
+
+
+@pytest.mark.parametrize("n", [16, 150])
+def test_captured_graphs_that_share_a_workspace(n):
+    H, HV, D = 2, 4, 128
+    cases = [make([n, n], H, HV, D, BF16, True, seed=s) for s in (1, 2)]
+    need = pp.prefill_workspace_bytes(cases[0][0]["mixed_qkv"].to(DEV), cases[0][1].to(DEV))
+    assert (need > 0) == (n > 64)
+    work = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    graphs = []
+    for c, state in cases:
+        dev = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in c.items()}
+        out, final, first = torch.zeros(2 * n, HV, D, dtype=BF16, device=DEV), torch.zeros(2, HV, D, D, device=DEV), state.to(DEV)
+        call = lambda: pp.gated_delta_rule_packed_prefill(**dev, out=out, final_state=final, initial_state=first, use_qk_l2norm_in_kernel=True, workspace=work)  # noqa: E731,B023
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        out.zero_(), final.zero_()
+        graphs.append((graph, out, final, dev, first))                             # a graph does not keep its inputs
+    for _ in range(2):
+        for graph, *_ in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for (c, state), (_, out, final, *_) in zip(cases, graphs):
+        alone = run(c, state, [n, n], HV, D)
+        assert torch.equal(out, alone[0]) and torch.equal(final, alone[1])
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    c, _ = make([100], 1, 1, 64, BF16)
+    with pytest.raises(ValueError):
+        run(c, None, [100], 1, 64, workspace=torch.empty(16, dtype=torch.uint8, device=DEV))
+    with pytest.raises(ValueError):
+        run(c, None, [100], 1, 64, workspace=torch.empty(1 << 24, dtype=torch.uint8, device=DEV)[8:])
+
+
+def test_prompt_then_decode_on_the_slot_pool():
+    """A prompt, its state into the requests' slots, and decoded tokens from there: near the recurrence on the unquantized state."""
+    from carrykernel_b200.vllm_integration import quantized_packed_decode as qpd
+    from carrykernel_b200.vllm_integration.state_pool import load_state, store_state
+    H, HV, D, lengths, steps = 2, 4, 128, [100, 131], 4
+    c, _ = make([n + steps for n in lengths], H, HV, D, BF16)
+    c["A_log"], c["dt_bias"] = torch.full((HV,), math.log(0.1)), torch.zeros(HV)
+    first = starts([n + steps for n in lengths])
+    pick = lambda lo, hi: torch.cat([torch.arange(first[i] + lo(n), first[i] + hi(n)) for i, n in enumerate(lengths)])  # noqa: E731
+    prompt = {k: v[pick(lambda n: 0, lambda n: n)] if k in ("mixed_qkv", "a", "b") else v for k, v in c.items()}
+    out, final = run(prompt, None, lengths, HV, D)
+    pool = qpd.init_quantized_state(4, HV, D, D, DEV, resid_fmt=qpd.RESID_INT8)
+    slots = torch.tensor([3, 1], dtype=torch.int32, device=DEV)
+    store_state(final, pool, slots, keep_error=True)
+    back = load_state(pool, slots)
+    assert (back - final).norm() <= 1e-3 * final.norm()          # int8 codes and an int8 residual
+    want = orc.delta_rule(**{k: v for k, v in c.items() if k != "mixed_qkv"}, mixed=c["mixed_qkv"], H=H, D=D, lengths=[n + steps for n in lengths])[0]
+    for t in range(steps):
+        rows = torch.tensor([first[i] + n + t for i, n in enumerate(lengths)])
+        got = torch.empty(2, 1, HV, D, dtype=BF16, device=DEV)
+        qpd.quantized_gated_delta_rule_packed_decode(c["mixed_qkv"][rows].to(DEV), c["a"][rows].to(DEV), c["b"][rows].to(DEV), c["A_log"].to(DEV),
+                                                     c["dt_bias"].to(DEV), c["scale"], *pool, got, slots, use_qk_l2norm_in_kernel=True,
+                                                     resid_fmt=qpd.RESID_INT8)
+        # rows of int8 codes: half a step of 127 against a row's largest number in each of `steps` tokens, and the output's rounding
+        assert (got[:, 0].cpu().double() - want[rows]).norm() <= (steps / 127 + 2 ** -8) * want[rows].norm()
