@@ -15,6 +15,8 @@
 // the sum of two bf16 numbers, in fp32 of three.  What is computed is split too: S, R and U into three, T into two (three with fp32
 // operands), and products of terms are formed down to 2^-18 of the largest.  The final state is then within 1e-6 of the
 // recurrence in 64 bits; two terms throughout would leave it 3.5e-6 off, and one (plain bf16 products) 2.4e-3.
+#include <cuda_pipeline_primitives.h>
+
 #include "carry_delta.cuh"
 #include "carry_tensor.cuh"
 
@@ -50,20 +52,19 @@ template <int DTYPE>
 constexpr int kTermsT = DTYPE == CARRY_F32 ? 3 : 2;
 
 // two numbers' next bf16 term, which is taken off them
-__device__ __forceinline__ uint32_t take_term(float& x, float& y) {
-  const uint32_t u = pack_bf16(x, y);
-  x -= __uint_as_float(u << 16);
-  y -= __uint_as_float(u & 0xffff0000u);
+__device__ __forceinline__ uint32_t take_term(float2& x) {
+  const uint32_t u = pack_bf16(x.x, x.y);
+  x = sub2(x, make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)));
   return u;
 }
 // eight numbers as TERMS chunks of 16 bytes, `apart` bytes from one another
 template <int TERMS>
-__device__ __forceinline__ void store_terms(uint8_t* to, int apart, float (&x)[8]) {
+__device__ __forceinline__ void store_terms(uint8_t* to, int apart, float2 (&x)[4]) {
 #pragma unroll
   for (int t = 0; t < TERMS; ++t) {
     uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = take_term(x[2 * e], x[2 * e + 1]);
+    for (int e = 0; e < 4; ++e) w[e] = take_term(x[e]);
     *reinterpret_cast<uint4*>(to + t * apart) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
@@ -85,33 +86,52 @@ __device__ __forceinline__ Raw<DTYPE> load_row(const void* base, long long at, b
 }
 
 // ---- what does not depend on the state -------------------------------------------------------------------------------
+//
+// With D the inverses of I + L's two 32 x 32 blocks on the diagonal, N its block below them, and Y = N D (of which the first half's columns are
+// not zero): T = D - D Y and P T = P D - (P D) Y.  So two products with 128 rows, [N; P] D and [D; P D] Y, finish both.
 
-constexpr int kPrepareThreads = 256, kPad = 68, kPadX = 36;
+constexpr int kRowWarps = 8, kPrepareThreads = (kRowWarps + 1) * 32, kHalf = kChunk / 2, kPad = 36;
 
-template <int TERMS, int TERMS_T, int D>
+template <int TERMS, int D>
 struct PrepareShared {
-  uint8_t kq[TERMS][D / 64][kPlane];      // rows 0 .. 63 keys, 64 .. 127 queries
-  uint8_t t[TERMS_T][kPlane];             // rows 0 .. 63 T, 64 .. 127 P and then P T
-  alignas(16) float L[kChunk][kPad], T[kChunk][kPad], X[32][kPadX];
-  float2 G[kChunk];                       // running sum of log2 alpha, and what its rounding left out
-  float beta[kChunk], norm[2 * kChunk];   // norm: what makes a key a unit one, and a query one times `scale`
-  uint64_t scored, multiplied;
+  union {
+    uint8_t kq[TERMS][D / 64][kPlane];    // rows 0 .. 63 keys, 64 .. 127 queries
+    uint8_t np[kTerms][kPlane];           // when they are multiplied: rows 0 .. 63 N, then Y; 64 .. 127 P
+  };
+  uint8_t t[kTerms][kPlane];              // rows 0 .. 63 D, then T; 64 .. 127 P D, then P T
+  alignas(16) float L[2][kHalf][kPad];    // the blocks of L on the diagonal
+  // of a token: running sum of log2 alpha within its half; decay from the first half's token to that half's end, or from there to the
+  // second half's token; decays from the chunk's start to the token and from there to the chunk's end; beta
+  alignas(16) float G[kChunk], to_middle[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk];
+  alignas(16) float norm[2 * kChunk];     // what makes a key a unit one, and a query one times `scale`
+  float decay;                            // of the chunk
+  uint64_t done[3];
   uint32_t tmem;
   int poison;
 };
 
-// A chunk's gates and the factors of its rows, by one warp; lane l has tokens 2 l and 2 l + 1.
+__device__ __forceinline__ float exp2_quick(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_of(double x) {
+  const float hi = (float)x;
+  return exp2_quick(hi) * fmaf((float)(x - hi), kLn2, 1.0f);
+}
+
+// A chunk's gates, by one warp; lane l has tokens 2 l and 2 l + 1.  Sums of decays are formed in 64 bits; what fp32 has to hold of them, for
+// differences, is the sum within half a chunk.
 template <class Shared>
-__device__ __forceinline__ void chunk_gates(const ChunkParams& p, Shared& sh, long long row, int n, int hv, float* vec) {
+__device__ __forceinline__ void chunk_gates(const ChunkParams& p, Shared& sh, long long row, int n, int hv) {
   const int lane = threadIdx.x % 32;
   double g[2];
-  float beta[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    float log_alpha = 0.0f;
-    beta[e] = 0.0f;
-    if (2 * lane + e < n) prefill_gates(p.a, row + 2 * lane + e, hv, log_alpha, beta[e]);
+    float log_alpha = 0.0f, beta = 0.0f;
+    if (2 * lane + e < n) prefill_gates(p.a, row + 2 * lane + e, hv, log_alpha, beta);
     g[e] = (double)(log_alpha < kLeastLog ? kLeastLog : log_alpha) * 1.4426950408889634;     // exp(-200) is 0, and sums stay finite
+    sh.beta[2 * lane + e] = beta;
   }
   double sum = g[0] + g[1];
 #pragma unroll
@@ -119,147 +139,114 @@ __device__ __forceinline__ void chunk_gates(const ChunkParams& p, Shared& sh, lo
     const double below = __shfl_up_sync(~0u, sum, d);
     if (lane >= d) sum += below;
   }
-  const double G[2] = {sum - g[1], sum}, last = __shfl_sync(~0u, sum, 31);
-  auto power = [](double x) {
-    const float hi = (float)x;
-    return exp2f(hi) * fmaf((float)(x - hi), kLn2, 1.0f);
-  };
+  const double G[2] = {sum - g[1], sum}, middle = __shfl_sync(~0u, sum, kHalf / 2 - 1), last = __shfl_sync(~0u, sum, 31);
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int i = 2 * lane + e;
-    const bool there = i < n;
-    const float hi = (float)G[e], decay = power(G[e]);
-    sh.G[i] = make_float2(hi, (float)(G[e] - hi));
-    sh.beta[i] = beta[e];
-    vec[i] = there ? beta[e] * decay * sh.norm[i] : 0.0f;
-    vec[kChunk + i] = beta[e];
-    vec[2 * kChunk + i] = there ? power(last - G[e]) * sh.norm[i] : 0.0f;
-    vec[3 * kChunk + i] = there ? decay * sh.norm[kChunk + i] : 0.0f;
+    sh.G[i] = (float)(i < kHalf ? G[e] : G[e] - middle);
+    sh.to_middle[i] = exp2_of(i < kHalf ? middle - G[e] : G[e] - middle);
+    sh.from_start[i] = exp2_of(G[e]);
+    sh.to_end[i] = exp2_of(last - G[e]);
   }
-  if (lane < 8) vec[4 * kChunk + lane] = power(last);
+  if (lane == 0) sh.decay = exp2_of(last);
 }
 
-// T = (I + L)^-1 in fp32: the 16 x 16 blocks on the diagonal by substitution, a column to a thread, then twice
-// T21 = -T22 L21 T11 for neighbouring blocks.  The entries of T are bounded as those of the recurrence are.
+// The inverse of a 32 x 32 block of I + L on the diagonal by substitution, a column to a lane, in fp32; its terms go into the tile of D.
 template <class Shared>
-__device__ __forceinline__ void invert(Shared& sh) {
-  const int tid = threadIdx.x;
-  if (tid < kChunk) {
-    const int b = tid / 16 * 16, j = tid % 16;
-    float x[16];
+__device__ __forceinline__ void invert_block(Shared& sh, int block) {
+  const int lane = threadIdx.x % 32;
+  float x[kHalf];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == j ? 1.0f : 0.0f;
+  for (int i = 0; i < kHalf; ++i) {
+    float s[4] = {i == lane ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < i; ++k) s = fmaf(-sh.L[b + i][b + k], x[k], s);
-      x[i] = s;
-      sh.T[b + i][b + j] = s;
+    for (int k = 0; k < i; k += 4) {
+      const float4 l = *reinterpret_cast<const float4*>(&sh.L[block][i][k]);
+      s[0] = fmaf(-l.x, x[k], s[0]);
+      if (k + 1 < i) s[1] = fmaf(-l.y, x[k + 1], s[1]);
+      if (k + 2 < i) s[2] = fmaf(-l.z, x[k + 2], s[2]);
+      if (k + 3 < i) s[3] = fmaf(-l.w, x[k + 3], s[3]);
     }
-  } else {
-    for (int e = tid - kChunk; e < kChunk * kChunk; e += kPrepareThreads - kChunk)
-      if (e % kChunk / 16 > e / kChunk / 16) sh.T[e / kChunk][e % kChunk] = 0.0f;
+    x[i] = (s[0] + s[1]) + (s[2] + s[3]);
   }
-  __syncthreads();
-  {
-    const int b = tid / 128 * 32, r = tid % 128 / 8, c = tid % 8 * 2, x = tid / 128 * 16;
-    float s[2] = {0.0f, 0.0f};
+  const int chunk = block * kHalf / 8 + lane / 8;
+  uint8_t* to = sh.t[0] + block * kHalf * 128 + lane % 8 * 2;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float l = sh.L[b + 16 + r][b + k];
-      s[0] = fmaf(l, sh.T[b + k][b + c], s[0]);
-      s[1] = fmaf(l, sh.T[b + k][b + c + 1], s[1]);
-    }
-    sh.X[x + r][c] = s[0];
-    sh.X[x + r][c + 1] = s[1];
-    __syncthreads();
-    s[0] = s[1] = 0.0f;
+  for (int i = 0; i < kHalf; i += 2) {
+    float2 y = make_float2(x[i], x[i + 1]);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float l = sh.T[b + 16 + r][b + 16 + k];
-      s[0] = fmaf(-l, sh.X[x + k][c], s[0]);
-      s[1] = fmaf(-l, sh.X[x + k][c + 1], s[1]);
+    for (int t = 0; t < kTerms; ++t) {
+      const uint32_t w = take_term(y);
+      *reinterpret_cast<uint16_t*>(to + t * kPlane + plane_at(i, chunk)) = (uint16_t)w;
+      *reinterpret_cast<uint16_t*>(to + t * kPlane + plane_at(i + 1, chunk)) = (uint16_t)(w >> 16);
     }
-    sh.T[b + 16 + r][b + c] = s[0];
-    sh.T[b + 16 + r][b + c + 1] = s[1];
-    __syncthreads();
   }
-  const int r = tid / 8, c = tid % 8 * 4;
-  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-  for (int k = 0; k < 32; ++k) {
-    const float l = sh.L[32 + r][k];
-    const float4 y = *reinterpret_cast<const float4*>(&sh.T[k][c]);
-    s = make_float4(fmaf(l, y.x, s.x), fmaf(l, y.y, s.y), fmaf(l, y.z, s.z), fmaf(l, y.w, s.w));
-  }
-  *reinterpret_cast<float4*>(&sh.X[r][c]) = s;
-  __syncthreads();
-  s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-  for (int k = 0; k < 32; ++k) {
-    const float l = -sh.T[32 + r][32 + k];
-    const float4 y = *reinterpret_cast<const float4*>(&sh.X[k][c]);
-    s = make_float4(fmaf(l, y.x, s.x), fmaf(l, y.y, s.y), fmaf(l, y.z, s.z), fmaf(l, y.w, s.w));
-  }
-  *reinterpret_cast<float4*>(&sh.T[32 + r][c]) = s;
-  __syncthreads();
 }
 
 template <int DTYPE, int D>
 __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __grid_constant__ ChunkParams p) {
   constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64;
-  using Shared = PrepareShared<kX, kT, D>;
+  using Shared = PrepareShared<kX, D>;
   extern __shared__ uint8_t raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
   depend_release();
   depend_wait();
   const CarryGdnPrefillArgs& a = p.a;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, h = blockIdx.y, group = a.HV / a.H, c = blockIdx.x;
-  const Place place = place_of(p, blockIdx.z, tid == 0 && h == 0 && c == 0 && p.chunk0 == 0 ? a.status : nullptr);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, hv = blockIdx.y, group = a.HV / a.H, h = hv / group, c = blockIdx.x;
+  const Place place = place_of(p, blockIdx.z, tid == 0 && hv == 0 && c == 0 && p.chunk0 == 0 ? a.status : nullptr);
   const int from = (p.chunk0 + c) * kChunk, n = min(place.count - from, kChunk);
   if (n <= 0) return;
   const long long row0 = place.first + from, slot = place.slot0 + c;
-  if (tid == 0) {
-    sh.poison = 0;
-    barrier_init(&sh.scored, 1);
-    barrier_init(&sh.multiplied, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 0) {
+
+  if (warp < kRowWarps) {
+    // keys and queries as operands; rows behind the last token are zeros, whatever memory holds there
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kTurns = 2 * kChunk / (kRowWarps * kRows), kBatch = 4;
+    const int chunk = lane % kLanes, first = warp * kRows + lane / kLanes;
+#pragma unroll
+    for (int t0 = 0; t0 < kTurns; t0 += kBatch) {
+      Raw<DTYPE> x[kBatch];
+#pragma unroll
+      for (int t = 0; t < kBatch; ++t) {
+        const int row = first + (t0 + t) * kRowWarps * kRows, token = row % kChunk;
+        const long long at = (row0 + token) * a.stride_mixed_tok + (row < kChunk ? a.H + h : h) * D + chunk * 8;
+        x[t] = {};
+        if (DTYPE == CARRY_BF16 && p.aligned && token < n)
+          __pipeline_memcpy_async(sh.kq[0][chunk / 8] + plane_at(row, chunk % 8), reinterpret_cast<const uint16_t*>(a.mixed_qkv) + at, 16);
+        else if (token < n)
+          x[t] = load_row<DTYPE>(a.mixed_qkv, at, p.aligned);
+      }
+#pragma unroll
+      for (int t = 0; t < kBatch; ++t) {
+        const int row = first + (t0 + t) * kRowWarps * kRows;
+        if (DTYPE == CARRY_BF16 && p.aligned && row % kChunk < n) continue;
+        Eight e = unpack<DTYPE>(x[t]);
+        store_terms<kX>(sh.kq[0][chunk / 8] + plane_at(row, chunk % 8), kPlanes * kPlane, e.x);
+      }
+    }
+    __pipeline_commit();
+    __pipeline_wait_prior(0);
+    fence_proxy();
+  } else {
+    if (lane == 0) {
+      sh.poison = 0;
+      for (int i = 0; i < 3; ++i) barrier_init(&sh.done[i], 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 128;" ::"r"(smem_addr(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    chunk_gates(p, sh, row0, n, hv);
   }
-
-  // keys and queries as operands, and their norms; rows behind the last token are zeros, whatever memory holds there
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
-#pragma unroll 4
-  for (int row = warp * kRows + lane / kLanes; row < 2 * kChunk; row += kPrepareThreads / 32 * kRows) {
-    const int token = row % kChunk, chunk = lane % kLanes;
-    float x[8] = {};
-    if (token < n) {
-      const Eight e = unpack<DTYPE>(load_row<DTYPE>(a.mixed_qkv, (row0 + token) * a.stride_mixed_tok + (row < kChunk ? a.H + h : h) * D + chunk * 8, p.aligned));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { x[2 * i] = e.x[i].x; x[2 * i + 1] = e.x[i].y; }
-    }
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-    for (int d = kLanes / 2; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-    if (chunk == 0) sh.norm[row] = (a.use_qk_l2norm ? __fdiv_rn(1.0f, sqrtf(sum + kL2Eps)) : 1.0f) * (row < kChunk ? 1.0f : a.scale);
-    store_terms<kX>(sh.kq[0][chunk / 8] + plane_at(row, chunk % 8), kPlanes * kPlane, x);
-  }
-  fence_proxy();
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
   volatile int* poison = &sh.poison;
   // the whole CTA goes on, or none of it
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return !__syncthreads_or(!barrier_wait(bar, parity, poison, a.status)); };
+  auto wait = [&](int i) { return !__syncthreads_or(!barrier_wait(&sh.done[i], 0, poison, a.status)); };
+  const uint32_t elected = warp == kRowWarps ? elect() : 0, base = __shfl_sync(~0u, tmem, 0);
 
-  bool healthy = true;
-  if (warp == 0) {
-    const uint32_t elected = elect(), base = __shfl_sync(~0u, tmem, 0);
+  if (warp == kRowWarps) {                        // [K; Q] [K; Q]^T: the norms are on its diagonal
 #pragma unroll
     for (int x = 0; x < kX; ++x)
 #pragma unroll
@@ -267,137 +254,593 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t step = k / 4 * (kPlane / 16) + k % 4 * 2;
-          mma_shared(elected, base, operand(sh.kq[x], 16) + step, operand(sh.kq[y], 16) + step, instruction_bf16(kChunk, false, false), x + y + k > 0);
+          mma_shared(elected, base, operand(sh.kq[x], 16) + step, operand(sh.kq[y], 16) + step, instruction_bf16(2 * kChunk, false, false), x + y + k > 0);
         }
-    mma_commit(elected, &sh.scored);
-  }
-  if (tid == 0) {
-    bulk_store(p.kq + (slot * a.H + h) * (kX * kPlanes * kPlane), sh.kq, kX * kPlanes * kPlane);
-    bulk_commit();
-  }
-  // products of keys and queries with keys: a row to a thread, half of its columns
-  const int row = warp % 4 * 32 + lane, i = row % kChunk, first = warp / 4 * 32;
-  const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-  float dots[32];
-  healthy = wait(&sh.scored, 0);
-  if (healthy) {
-    fence_after();
-    tmem_load(tmem + lanes + first, dots);
-    wait_loads();
-  }
-  for (int g = 0; g < group && healthy; ++g) {
-    const int hv = h * group + g;
-    if (tid == 0 && g > 0) bulk_wait_read();
-    if (warp == 0) chunk_gates(p, sh, row0, n, hv, p.vec + (slot * a.HV + hv) * kVec);
-    __syncthreads();
-    const float2 G = sh.G[i];
-    const float by = row < kChunk ? sh.beta[i] * sh.norm[i] : sh.norm[row];
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = first + j + e;
-        const float2 to = sh.G[col];
-        const float decay = exp2f((G.x - to.x) + (G.y - to.y));
-        const bool counts = row < kChunk ? col < i : col <= i;
-        x[e] = counts ? dots[j + e] * by * sh.norm[col] * decay : 0.0f;
-      }
-      if (row < kChunk) {
-        *reinterpret_cast<float4*>(&sh.L[i][first + j]) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(&sh.L[i][first + j + 4]) = make_float4(x[4], x[5], x[6], x[7]);
-      } else {
-        store_terms<kT>(sh.t[0] + plane_at(row, (first + j) / 8), kPlane, x);
-      }
-    }
-    __syncthreads();
-    invert(sh);
-    {
-      const int r = tid / 4, q = tid % 4 * 16;
-#pragma unroll
-      for (int j = 0; j < 16; j += 8) {
-        const float4 u = *reinterpret_cast<const float4*>(&sh.T[r][q + j]), v = *reinterpret_cast<const float4*>(&sh.T[r][q + j + 4]);
-        float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-        store_terms<kT>(sh.t[0] + plane_at(r, (q + j) / 8), kPlane, x);
-      }
-    }
-    fence_proxy();
-    fence_before();
-    __syncthreads();
-    fence_after();
-    if (warp == 0) {                              // [T; P] T: of it, P T
-      const uint32_t elected = elect(), base = __shfl_sync(~0u, tmem, 0) + kChunk;
-#pragma unroll
-      for (int x = 0; x < kT; ++x)
-#pragma unroll
-        for (int y = 0; x + y < kT; ++y)
-#pragma unroll
-          for (int k = 0; k < kChunk / 16; ++k)
-            mma_shared(elected, base, operand(sh.t[x], 16) + k * 2, operand(sh.t[y], 16) + k * 128, instruction_bf16(kChunk, false, true), x + y + k > 0);
-      mma_commit(elected, &sh.multiplied);
-    }
-    healthy = wait(&sh.multiplied, g & 1);
-    if (!healthy) break;
-    fence_after();
-    if (row >= kChunk) {
-      float y[32];
-      tmem_load(tmem + lanes + kChunk + first, y);
-      wait_loads();
-#pragma unroll
-      for (int j = 0; j < 32; j += 8) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = y[j + e];
-        store_terms<kT>(sh.t[0] + plane_at(row, (first + j) / 8), kPlane, x);
-      }
-    }
-    fence_proxy();
-    fence_before();
-    __syncthreads();
-    fence_after();
-    if (tid == 0) {
-      bulk_store(p.t + (slot * a.HV + hv) * (kT * kPlane), sh.t, kT * kPlane);
+    mma_commit(elected, &sh.done[0]);
+    if (lane == 0 && hv % group == 0) {
+      bulk_store(p.kq + (slot * a.H + h) * (kX * kPlanes * kPlane), sh.kq, kX * kPlanes * kPlane);
       bulk_commit();
+      bulk_wait_read();
+    }
+    __syncwarp();
+  } else {                                        // zeros beside the blocks of D
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t) {
+      const int row = tid / 4;
+      *reinterpret_cast<uint4*>(sh.t[t] + plane_at(row, (row < kHalf ? 4 : 0) + tid % 4)) = make_uint4(0, 0, 0, 0);
     }
   }
-  if (tid == 0) bulk_wait();
-  if (*poison) {
-    for (int k = 0; k < 1 << 12; ++k) __nanosleep(64);      // products in flight still use shared and tensor memory
+  if (!wait(0)) {
+    if (*poison)
+      for (int k = 0; k < 1 << 12; ++k) __nanosleep(64);    // products in flight still use shared and tensor memory
+    __syncthreads();
+    if (warp == kRowWarps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem) : "memory");
+    return;
+  }
+  fence_after();
+  // a row to a thread, half of its columns
+  const int quarter = warp % 4, row = quarter * 32 + lane, i = row % kChunk, first = warp / 4 * kHalf;
+  const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const bool key = row < kChunk;
+  if (warp < 4) {
+    float x[32], square = 0.0f;
+    tmem_load(at + quarter * 32, x);
+    wait_loads();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) square = j == lane ? x[j] : square;
+    sh.norm[row] = (a.use_qk_l2norm ? __fdiv_rn(1.0f, sqrtf(square + kL2Eps)) : 1.0f) * (key ? 1.0f : a.scale);
+  }
+  __syncthreads();
+  if (warp < kRowWarps) {
+    // L and P.  Between the halves of a chunk a decay is a product of two that end in the middle; both are at most 1.
+    const float G = sh.G[i], by = key ? sh.beta[i] * sh.norm[i] : sh.norm[row];
+    const bool below = first < i / kHalf * kHalf, diagonal = first == i / kHalf * kHalf;    // the same for all lanes
+    float2 x[16];
+    if (below || diagonal) {
+      tmem_load(at + first, *reinterpret_cast<float(*)[32]>(x));
+      wait_loads();
+    }
+    if (diagonal) {
+      const int most = (key ? i - 1 : i) - first;
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 g = *reinterpret_cast<const float4*>(&sh.G[first + j]), m = *reinterpret_cast<const float4*>(&sh.norm[first + j]);
+        const float2 d[2] = {make_float2(exp2_quick(G - g.x), exp2_quick(G - g.y)), make_float2(exp2_quick(G - g.z), exp2_quick(G - g.w))};
+        const float2 f[2] = {make_float2(m.x, m.y), make_float2(m.z, m.w)};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 y = mul2(mul2(x[j / 2 + e], mul2(f[e], make_float2(by, by))), d[e]);
+          x[j / 2 + e] = make_float2(j + 2 * e <= most ? y.x : 0.0f, j + 2 * e + 1 <= most ? y.y : 0.0f);
+        }
+      }
+    } else if (below) {
+      const float f = by * sh.to_middle[i];
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 d = *reinterpret_cast<const float4*>(&sh.to_middle[j]), m = *reinterpret_cast<const float4*>(&sh.norm[j]);
+        x[j / 2] = mul2(mul2(x[j / 2], make_float2(f, f)), make_float2(m.x * d.x, m.y * d.y));
+        x[j / 2 + 1] = mul2(mul2(x[j / 2 + 1], make_float2(f, f)), make_float2(m.z * d.z, m.w * d.w));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = make_float2(0.0f, 0.0f);
+    }
+    auto tile = [&](int to_row, int column) {     // the thread's numbers into the tile of N and P
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        float2 y[4] = {x[j], x[j + 1], x[j + 2], x[j + 3]};
+        store_terms<kTerms>(sh.np[0] + plane_at(to_row, column / 8 + j / 4), kPlane, y);
+      }
+    };
+    if (!key) {
+      tile(row, first);
+    } else if (diagonal) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) *reinterpret_cast<float4*>(&sh.L[i / kHalf][lane][2 * j]) = make_float4(x[j].x, x[j].y, x[j + 1].x, x[j + 1].y);
+    } else if (below) {
+      tile(row, 0);
+    } else {                                      // N's other places
+      tile(lane, 0);
+      tile(lane, kHalf);
+      tile(lane + kHalf, kHalf);
+    }
+  }
+  __syncthreads();
+  if (warp < 2) {
+    invert_block(sh, warp);
+  } else if (warp < 4) {                          // the factors of the chunk's rows
+    const int i = tid - 64;
+    float* vec = p.vec + (slot * a.HV + hv) * kVec;
+    const bool there = i < n;
+    vec[i] = there ? sh.beta[i] * sh.from_start[i] * sh.norm[i] : 0.0f;
+    vec[kChunk + i] = sh.beta[i];
+    vec[2 * kChunk + i] = there ? sh.to_end[i] * sh.norm[i] : 0.0f;
+    vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.norm[kChunk + i] : 0.0f;
+    if (i < 8) vec[4 * kChunk + i] = sh.decay;
+  }
+  fence_proxy();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == kRowWarps) {                        // [N; P] D
+#pragma unroll
+    for (int x = 0; x < kTerms; ++x)
+#pragma unroll
+      for (int y = 0; x + y < kTerms; ++y)
+#pragma unroll
+        for (int k = 0; k < kChunk / 16; ++k)
+          mma_shared(elected, base, operand(sh.np[x], 16) + k * 2, operand(sh.t[y], 16) + k * 128, instruction_bf16(kChunk, false, true), x + y + k > 0);
+    mma_commit(elected, &sh.done[1]);
+  }
+  bool healthy = wait(1);
+  float2 pd[16];
+  if (healthy && warp < kRowWarps && (!key || (quarter == 1 && first == 0))) {
+    fence_after();
+    tmem_load(at + first, *reinterpret_cast<float(*)[32]>(pd));
+    wait_loads();
+    uint8_t* tile = key ? sh.np[0] : sh.t[0];
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      float2 y[4] = {pd[j], pd[j + 1], pd[j + 2], pd[j + 3]};
+      store_terms<kTerms>(tile + plane_at(row, first / 8 + j / 4), kPlane, y);
+    }
+    fence_proxy();
   }
   fence_before();
   __syncthreads();
-  if (warp == 0) {
+  fence_after();
+  if (warp == kRowWarps) {                        // [D; P D] Y, over the second half
+#pragma unroll
+    for (int x = 0; x < kTerms; ++x)
+#pragma unroll
+      for (int y = 0; x + y < kTerms; ++y)
+#pragma unroll
+        for (int k = kHalf / 16; k < kChunk / 16; ++k)
+          mma_shared(elected, base + kChunk, operand(sh.t[x], 16) + k * 2, operand(sh.np[y], 16) + k * 128, instruction_bf16(kHalf, false, true),
+                     x + y + k > kHalf / 16);
+    mma_commit(elected, &sh.done[2]);
+  }
+  healthy = wait(2) && healthy;
+  if (healthy && warp < 4 && quarter > 0) {       // the first half's columns of T's rows below the middle, and of P T
     fence_after();
+    float2 y[16];
+    tmem_load(at + kChunk, *reinterpret_cast<float(*)[32]>(y));
+    wait_loads();
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      float2 z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = sub2(key ? make_float2(0.0f, 0.0f) : pd[j + e], y[j + e]);
+      store_terms<kT>(sh.t[0] + plane_at(row, j / 4), kPlane, z);
+    }
+    fence_proxy();
+  }
+  if (*poison)
+    for (int k = 0; k < 1 << 12; ++k) __nanosleep(64);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == kRowWarps) {
+    if (lane == 0 && healthy) {
+      bulk_store(p.t + (slot * a.HV + hv) * (kT * kPlane), sh.t, kT * kPlane);
+      bulk_commit();
+      bulk_wait_read();
+    }
+    __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem) : "memory");
+  }
+}
+
+// ---- the same, a chunk and head to a warp ----------------------------------------------------------------------------
+//
+// For 16-bit keys and queries.  Everything is a product of 16 x 16 blocks whose operands are registers: a lane's part of a product's result
+// is its part of the next one's left side, or of its right side transposed, so T^T and (P T)^T are built block by block,
+//   W_jj = D_j^T,   W_jb = -(sum over j <= k < b of W_jk L_bk^T) D_b^T  (T_bj = W_jb^T),   (P T)_ij = (sum over j <= k <= i of W_jk P_ik^T)^T,
+// and only the 16 x 16 inverses D_b go through shared memory.  No warp waits for another.  Keys and queries come from memory as they
+// are: a lane has a quarter of a row, and which numbers of a row stand for which step of the sum is the same on both sides.
+
+constexpr int kBlock = 16, kBlocks = kChunk / kBlock, kUnitWarps = 4;
+__host__ __device__ constexpr int pair_of(int i, int k) { return i * (i + 1) / 2 + k; }        // of blocks, k <= i
+
+struct alignas(16) Unit {
+  float2 L[6][4][32], P[10][4][32];       // a lane's numbers of the blocks below the diagonal, and of all
+  float D[kBlocks][kBlock][20];           // the blocks of L on the diagonal, then their inverses
+  uint8_t rows[2][kBlock * 128];          // sixteen rows of a tile on their way out
+  // of a token: running sum of log2 alpha within its block, decay from the block's start, decay to the block's end, decays from the
+  // chunk's start and to its end, beta, norms of key and query
+  float G[kChunk], from_block[kChunk], to_block[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk], key[kChunk], query[kChunk];
+};
+
+template <bool HALF>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (HALF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A lane's part of a 16 x 16 block, of which it has numbers (g, 2t), (g, 2t+1), (g+8, 2t), .. and the same eight columns on: for g = lane / 4,
+// t = lane % 4.
+struct Part {
+  float x[2][4];
+};
+struct Split {
+  uint32_t w[kTerms][4];                  // pairs (g, 2t), (g + 8, 2t), (g, 2t + 8), (g + 8, 2t + 8)
+};
+__device__ __forceinline__ Split split(const Part& p) {
+  Split s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 y = make_float2(p.x[i / 2][i % 2 * 2], p.x[i / 2][i % 2 * 2 + 1]);
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t) s.w[t][i] = take_term(y);
+  }
+  return s;
+}
+// c += a b^T, of terms whose numbers add up to less than TERMS
+template <int TERMS>
+__device__ __forceinline__ void multiply(Part& c, const Split& a, const Split& b) {
+#pragma unroll
+  for (int x = TERMS - 1; x >= 0; --x)
+#pragma unroll
+    for (int y = TERMS - 1 - x; y >= 0; --y) {
+      mma16<false>(c.x[0], a.w[x][0], a.w[x][1], a.w[x][2], a.w[x][3], b.w[y][0], b.w[y][2]);
+      mma16<false>(c.x[1], a.w[x][0], a.w[x][1], a.w[x][2], a.w[x][3], b.w[y][1], b.w[y][3]);
+    }
+}
+__device__ __forceinline__ void store_transposed(uint32_t to, const uint32_t (&w)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+// Gates of a chunk: lane l has tokens 2 l and 2 l + 1.  Sums of decays are formed in 64 bits; what fp32 has to hold of them, for differences,
+// is the sum within a block.  Returns the decays over the second block, over the third, and over the chunk.
+__device__ __forceinline__ float3 unit_gates(const ChunkParams& p, Unit& sh, long long row, int n, int hv) {
+  const int lane = threadIdx.x % 32;
+  double g[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float log_alpha = 0.0f, beta = 0.0f;
+    if (2 * lane + e < n) prefill_gates(p.a, row + 2 * lane + e, hv, log_alpha, beta);
+    g[e] = (double)(log_alpha < kLeastLog ? kLeastLog : log_alpha) * 1.4426950408889634;     // exp(-200) is 0, and sums stay finite
+    sh.beta[2 * lane + e] = beta;
+  }
+  double sum = g[0] + g[1];
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const double below = __shfl_up_sync(~0u, sum, d);
+    if (lane >= d) sum += below;
+  }
+  const double G[2] = {sum - g[1], sum}, last = __shfl_sync(~0u, sum, 31), end = __shfl_sync(~0u, sum, lane | 7);
+  const double before = __shfl_sync(~0u, sum, (lane & 24) - 1 & 31), start = lane < 8 ? 0.0 : before;
+  const double ends[3] = {__shfl_sync(~0u, sum, 7), __shfl_sync(~0u, sum, 15), __shfl_sync(~0u, sum, 23)};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = 2 * lane + e;
+    sh.G[i] = (float)(G[e] - start);
+    sh.from_block[i] = exp2_of(G[e] - start);
+    sh.to_block[i] = exp2_of(end - G[e]);
+    sh.from_start[i] = exp2_of(G[e]);
+    sh.to_end[i] = exp2_of(last - G[e]);
+  }
+  return make_float3(exp2_of(ends[1] - ends[0]), exp2_of(ends[2] - ends[1]), exp2_of(last));
+}
+
+// Rows of keys or queries, for a lane a quarter of row first + 8 r + lane / 4 (r < ROWS), D / 4 numbers as they lie in memory; rows behind the
+// last token are zeros, whatever memory holds there.
+template <int D, int ROWS>
+__device__ __forceinline__ void load_quarters(const ChunkParams& p, long long row0, int n, int first, long long column, uint32_t (&x)[ROWS][D / 8]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int token = first + 8 * r + lane / 4;
+    const long long at = (row0 + token) * p.a.stride_mixed_tok + column + lane % 4 * (D / 4);
+#pragma unroll
+    for (int q = 0; q < D / 32; ++q) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (token < n) u = load_row<CARRY_BF16>(p.a.mixed_qkv, at + q * 8, p.aligned).w[0];
+      x[r][4 * q] = u.x;
+      x[r][4 * q + 1] = u.y;
+      x[r][4 * q + 2] = u.z;
+      x[r][4 * q + 3] = u.w;
+    }
+  }
+}
+// them as operand rows in the workspace; row: of the tile
+template <int DTYPE, int D>
+__device__ __forceinline__ void store_quarter(uint8_t* tile, int row, const uint32_t (&x)[D / 8]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int q = 0; q < D / 32; ++q) {
+    const int chunk = lane % 4 * (D / 32) + q;
+    uint8_t* to = tile + chunk / 8 * kPlane + plane_at(row, chunk % 8);
+    if constexpr (DTYPE == CARRY_BF16) {
+      *reinterpret_cast<uint4*>(to) = make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+    } else {
+      Raw<DTYPE> r;
+      r.w[0] = make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+      Eight e = unpack<DTYPE>(r);
+      store_terms<kTermsX<DTYPE>>(to, D / 64 * kPlane, e.x);
+    }
+  }
+}
+// products of sixteen rows with sixteen
+template <bool HALF, int N>
+__device__ __forceinline__ Part products(const uint32_t (&a0)[N], const uint32_t (&a1)[N], const uint32_t (&b0)[N], const uint32_t (&b1)[N]) {
+  Part c = {};
+#pragma unroll
+  for (int s = 0; s < N; s += 2) {
+    mma16<HALF>(c.x[0], a0[s], a1[s], a0[s + 1], a1[s + 1], b0[s], b0[s + 1]);
+    mma16<HALF>(c.x[1], a0[s], a1[s], a0[s + 1], a1[s + 1], b1[s], b1[s + 1]);
+  }
+  return c;
+}
+
+template <int DTYPE, int D>
+__global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_constant__ ChunkParams p) {
+  constexpr bool kHalfType = DTYPE == CARRY_F16;
+  constexpr int kWords = D / 8;
+  extern __shared__ uint8_t raw[];
+  depend_release();
+  depend_wait();
+  const CarryGdnPrefillArgs& a = p.a;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int hv = blockIdx.y, group = a.HV / a.H, h = hv / group, c = blockIdx.x * kUnitWarps + warp;
+  Unit& sh = reinterpret_cast<Unit*>(raw)[warp];
+  const Place place = place_of(p, blockIdx.z, threadIdx.x == 0 && hv == 0 && c == 0 && p.chunk0 == 0 ? a.status : nullptr);
+  const int from = (p.chunk0 + c) * kChunk, n = c < p.chunks ? min(place.count - from, kChunk) : 0;
+  if (n <= 0) return;
+  const long long row0 = place.first + from, slot = place.slot0 + c;
+  uint8_t* kq = hv % group == 0 ? p.kq + (slot * a.H + h) * (kTermsX<DTYPE> * (D / 64) * kPlane) : nullptr;
+
+  uint32_t k[2 * kBlocks][kWords];
+  load_quarters<D>(p, row0, n, 0, (a.H + h) * D, k);
+  const float3 across = unit_gates(p, sh, row0, n, hv);
+  if (kq) {
+#pragma unroll
+    for (int r = 0; r < 2 * kBlocks; ++r) store_quarter<DTYPE, D>(kq, 8 * r + g, k[r]);
+  }
+
+  // The norms are on the diagonals of products with themselves: of rows g and g + 8, at the lane with t = g / 2.
+  auto norms = [&](const Part& d, float by, float* to) {
+    if (t != g / 2) return;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const float square = g % 2 ? d.x[half][2 * half + 1] : d.x[half][2 * half];
+      to[g + 8 * half] = a.use_qk_l2norm ? __fdiv_rn(by, sqrtf(square + kL2Eps)) : by;
+    }
+  };
+  Part diagonal[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    diagonal[b] = products<kHalfType>(k[2 * b], k[2 * b + 1], k[2 * b], k[2 * b + 1]);
+    norms(diagonal[b], 1.0f, sh.key + b * kBlock);
+  }
+  __syncwarp();
+
+  // L and P, a row of blocks at a time.  Within a block decays are powers of differences; between blocks products of a decay to the one's end, over
+  // what lies between, and from the other's start, all at most 1.
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const int i0 = b * kBlock + g;
+    uint32_t q[2][kWords];
+    load_quarters<D>(p, row0, n, b * kBlock, h * D, q);
+    float decay[2][4];
+    {
+      const float gi[2] = {sh.G[i0], sh.G[i0 + 8]}, by[2] = {sh.beta[i0] * sh.key[i0], sh.beta[i0 + 8] * sh.key[i0 + 8]};
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 8 * x + 2 * t + e % 2, i = g + e / 2 * 8;
+          decay[x][e] = j <= i ? exp2_quick(gi[e / 2] - sh.G[b * kBlock + j]) * sh.key[b * kBlock + j] : 0.0f;
+          sh.D[b][i][j] = j < i ? diagonal[b].x[x][e] * by[e / 2] * decay[x][e] : 0.0f;
+        }
+#pragma unroll
+      for (int m = 0; m < b; ++m) {
+        Part l = products<kHalfType>(k[2 * b], k[2 * b + 1], k[2 * m], k[2 * m + 1]);
+        const float over = m == b - 1 ? 1.0f : b == 2 ? across.x : m == 1 ? across.y : across.x * across.y;
+        const float f[2] = {by[0] * sh.from_block[i0] * over, by[1] * sh.from_block[i0 + 8] * over};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int j = m * kBlock + 8 * x + 2 * t;
+          const float2 to = mul2(*reinterpret_cast<const float2*>(&sh.to_block[j]), *reinterpret_cast<const float2*>(&sh.key[j]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sh.L[pair_of(b - 1, m)][2 * x + e][lane] = mul2(mul2(make_float2(l.x[x][2 * e], l.x[x][2 * e + 1]), make_float2(f[e], f[e])), to);
+        }
+      }
+    }
+    if (kq) {
+      store_quarter<DTYPE, D>(kq, kChunk + i0, q[0]);
+      store_quarter<DTYPE, D>(kq, kChunk + i0 + 8, q[1]);
+    }
+    norms(products<kHalfType>(q[0], q[1], q[0], q[1]), a.scale, sh.query + b * kBlock);
+    __syncwarp();
+    const float by[2] = {sh.query[i0], sh.query[i0 + 8]};
+#pragma unroll
+    for (int m = 0; m <= b; ++m) {
+      Part y = products<kHalfType>(q[0], q[1], k[2 * m], k[2 * m + 1]);
+      const float over = m >= b - 1 ? 1.0f : b == 2 ? across.x : m == 1 ? across.y : across.x * across.y;
+      const float f[2] = {by[0] * sh.from_block[i0] * over, by[1] * sh.from_block[i0 + 8] * over};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int j = m * kBlock + 8 * x + 2 * t;
+        const float2 to = mul2(*reinterpret_cast<const float2*>(&sh.to_block[j]), *reinterpret_cast<const float2*>(&sh.key[j]));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 z = make_float2(y.x[x][2 * e], y.x[x][2 * e + 1]);
+          const float2 d = make_float2(decay[x][2 * e], decay[x][2 * e + 1]), s = make_float2(by[e], by[e]);
+          sh.P[pair_of(b, m)][2 * x + e][lane] = m == b ? make_float2(d.x == 0.0f ? 0.0f : z.x * s.x * d.x, d.y == 0.0f ? 0.0f : z.y * s.y * d.y)
+                                                        : mul2(mul2(z, make_float2(f[e], f[e])), to);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  {
+    // the factors of the chunk's rows
+    float* vec = p.vec + (slot * a.HV + hv) * kVec;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = lane + 32 * e;
+      const bool there = i < n;
+      vec[i] = there ? sh.beta[i] * sh.from_start[i] * sh.key[i] : 0.0f;
+      vec[kChunk + i] = sh.beta[i];
+      vec[2 * kChunk + i] = there ? sh.to_end[i] * sh.key[i] : 0.0f;
+      vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.query[i] : 0.0f;
+    }
+    if (lane < 8) vec[4 * kChunk + lane] = across.z;
+  }
+
+  // The inverses of the blocks on the diagonal, by substitution, a column to a lane, two blocks at a time.
+#pragma unroll
+  for (int b = 0; b < kBlocks; b += 2) {
+    float (&m)[kBlock][20] = sh.D[b + lane / 16];
+    const int j = lane % 16;
+    float x[kBlock];
+#pragma unroll
+    for (int i = 0; i < kBlock; ++i) {
+      float s[4] = {i == j ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int n = 0; n < i; n += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(&m[i][n]);
+        s[0] = fmaf(-l.x, x[n], s[0]);
+        if (n + 1 < i) s[1] = fmaf(-l.y, x[n + 1], s[1]);
+        if (n + 2 < i) s[2] = fmaf(-l.z, x[n + 2], s[2]);
+        if (n + 3 < i) s[3] = fmaf(-l.w, x[n + 3], s[3]);
+      }
+      x[i] = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kBlock; ++i) m[i][j] = x[i];
+  }
+  __syncwarp();
+
+  Split W[10];                                    // W_jb at pair_of(b, j)
+  uint8_t* tile = p.t + (slot * a.HV + hv) * (kTermsT<DTYPE> * kPlane);
+  const uint32_t staged = smem_addr(sh.rows[0]);
+  // sixteen rows, of which blocks 0 .. b are given, into the tile
+  auto put_rows = [&](int b, int row, auto block) {
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) {
+      const int r = lane % 8 + lane / 16 * 8, chunk = 2 * j + lane / 8 % 2;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (j <= b) store_transposed(staged + x * (kBlock * 128) + plane_at(r, chunk), block(j).w[x]);
+        else *reinterpret_cast<uint4*>(sh.rows[x] + plane_at(r, chunk)) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<uint4*>(tile + x * kPlane + row * 128 + (e * 32 + lane) * 16) = *reinterpret_cast<const uint4*>(sh.rows[x] + (e * 32 + lane) * 16);
+    __syncwarp();
+  };
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const float (&m)[kBlock][20] = sh.D[b];
+    Part d, turned;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = g + e / 2 * 8, j = 8 * x + 2 * t + e % 2;
+        d.x[x][e] = m[i][j];
+        turned.x[x][e] = m[j][i];
+      }
+    W[pair_of(b, b)] = split(turned);
+    if (b > 0) {
+      const Split inverse = split(d);
+      Split l[kBlocks];
+#pragma unroll
+      for (int k = 0; k < b; ++k) {
+        Part y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 z = sh.L[pair_of(b - 1, k)][e][lane];
+          y.x[e / 2][e % 2 * 2] = z.x;
+          y.x[e / 2][e % 2 * 2 + 1] = z.y;
+        }
+        l[k] = split(y);
+      }
+#pragma unroll
+      for (int j = 0; j < b; ++j) {
+        Part sum = {}, w = {};
+#pragma unroll
+        for (int k = j; k < b; ++k) multiply<kTerms>(sum, W[pair_of(k, j)], l[k]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum.x[e / 4][e % 4] = -sum.x[e / 4][e % 4];
+        multiply<kTerms>(w, split(sum), inverse);
+        W[pair_of(b, j)] = split(w);
+      }
+    }
+    put_rows(b, b * kBlock, [&](int j) -> const Split& { return W[pair_of(b, j)]; });
+    Split pt[kBlocks];
+    {
+      Part sum[kBlocks] = {};
+#pragma unroll
+      for (int k = 0; k <= b; ++k) {
+        Part y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 z = sh.P[pair_of(b, k)][e][lane];
+          y.x[e / 2][e % 2 * 2] = z.x;
+          y.x[e / 2][e % 2 * 2 + 1] = z.y;
+        }
+        const Split right = split(y);
+#pragma unroll
+        for (int j = 0; j <= k; ++j) multiply<2>(sum[j], W[pair_of(k, j)], right);
+      }
+#pragma unroll
+      for (int j = 0; j <= b; ++j) pt[j] = split(sum[j]);
+    }
+    put_rows(b, kChunk + b * kBlock, [&](int j) -> const Split& { return pt[j]; });
   }
 }
 
 // ---- along a sequence ------------------------------------------------------------------------------------------------
 
-constexpr int kRowThreads = 256, kLoadWarp = kRowThreads / 32, kIssueWarp = kLoadWarp + 1, kSequenceThreads = (kIssueWarp + 1) * 32;
+constexpr int kColumnGroups = 4, kRowThreads = kColumnGroups * 128, kLoadWarp = kRowThreads / 32, kIssueWarp = kLoadWarp + 1, kSequenceThreads = (kIssueWarp + 1) * 32;
 
-template <int TERMS, int TERMS_T, int D, int STAGES>
+// Operands of COLUMNS columns lie with their terms side by side, so that one product takes all terms and reads its left side once;
+// planes have 64 columns.
+template <int COLUMNS>
+constexpr int kPlanesOf = (kTerms * COLUMNS + 63) / 64;
+
+template <int TERMS, int TERMS_T, int D, int COLUMNS, int STAGES>
 struct SequenceShared {
   uint8_t kq[STAGES][TERMS][D / 64][kPlane], t[STAGES][TERMS_T][kPlane];
-  uint8_t s[kTerms][D * 128], u[kTerms][kChunk * 128];    // the state; R, and then U with its decays
+  uint8_t s[kPlanesOf<COLUMNS>][D * 128], u[kPlanesOf<COLUMNS>][kChunk * 128];    // the state; R, and then U with its decays
   alignas(16) float vec[STAGES][kVec];
   uint64_t full[STAGES], free[STAGES], s_ready, r_ready, u_ready, scored, solved, added;
   uint32_t tmem;
   int poison;
 };
 
-template <int W>
-__device__ __forceinline__ void load_columns(uint32_t at, float (&x)[W]) {
-  if constexpr (W == 32) tmem_load(at, x);
-  else tmem_load16(at, reinterpret_cast<uint32_t(&)[16]>(x));
+// this thread's W columns of each term's product, summed, the smallest first
+template <int W, int COLUMNS>
+__device__ __forceinline__ void load_sums(uint32_t at, float2 (&x)[W / 2]) {
+  uint32_t r[kTerms][W];
+#pragma unroll
+  for (int t = 0; t < kTerms; ++t) {
+    if constexpr (W == 8) tmem_load8(at + t * COLUMNS, r[t]);
+    else tmem_load16(at + t * COLUMNS, r[t]);
+  }
   wait_loads();
+  auto two = [&](int t, int j) { return make_float2(__uint_as_float(r[t][j]), __uint_as_float(r[t][j + 1])); };
+#pragma unroll
+  for (int j = 0; j < W; j += 2) x[j / 2] = add2(add2(two(2, j), two(1, j)), two(0, j));
 }
 
 // COLUMNS of a head's state to a CTA
 template <int DTYPE, int D, int COLUMNS, int STAGES>
 __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64, W = COLUMNS / 2;
-  using Shared = SequenceShared<kX, kT, D, STAGES>;
+  constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64, W = COLUMNS / kColumnGroups;
+  using Shared = SequenceShared<kX, kT, D, COLUMNS, STAGES>;
   extern __shared__ uint8_t raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
   depend_release();
@@ -421,7 +864,8 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
     barrier_init(&sh.added, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  constexpr uint32_t kTmem = COLUMNS == 64 ? 256 : 128;
+  // columns 0 and on: [K; Q] S, and, when that is read, K^T U; behind them [T; P T] R
+  constexpr uint32_t kSolvedAt = kTerms * COLUMNS, kTmem = 2 * kSolvedAt <= 256 ? 256 : 512;
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "n"(kTmem) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -431,45 +875,51 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
   fence_after();
   const uint32_t tmem = sh.tmem;
   volatile int* poison = &sh.poison;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, barrier_wait(bar, parity, poison, a.status)) != 0; };
 
   if (tid < kRowThreads) {
-    // ---- a row to a thread, half of its columns: of the products' rows (keys, queries), and of the state's (K) ----
+    // ---- a row to a thread, some of its columns: of the products' rows (keys, queries), and of the state's (K) ----
     const int row = warp % 4 * 32 + lane, first = warp / 4 * W, column0 = blockIdx.x * COLUMNS + first, token = row % kChunk;
     const uint32_t at = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + first;
     const bool key = row < kChunk, has_state = row < D;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, barrier_wait(bar, parity, poison, a.status)) != 0; };
-    // numbers of a row in an operand: TERMS of them, columns first .. first + W - 1
-    auto put = [&](uint8_t* tile, int apart, float (&x)[W]) {
+    // this thread's numbers into an operand with planes of `plane` bytes, as kTerms terms
+    auto put = [&](uint8_t* tile, int plane, float2 (&x)[W / 2]) {
 #pragma unroll
-      for (int j = 0; j < W; j += 8) {
-        float y[8];
+      for (int j = 0; j < W; j += 8)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[j + e];
-        store_terms<kTerms>(tile + plane_at(row, (first + j) / 8), apart, y);
-      }
+        for (int t = 0; t < kTerms; ++t) {
+          const int column = t * COLUMNS + first + j;
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = take_term(x[j / 2 + e]);
+          *reinterpret_cast<uint4*>(tile + column / 64 * plane + plane_at(row, column % 64 / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     };
-    float S[W];
+    float2 S[W / 2];
     {
       const float* state = p.chunk0 > 0 ? a.final_state + b * a.stride_final_req : a.initial_state ? a.initial_state + b * a.stride_initial_req : nullptr;
+      auto number = [&](int j) { return state && has_state ? state[((long long)hv * D + column0 + j) * D + row] : 0.0f; };
 #pragma unroll
-      for (int j = 0; j < W; ++j) S[j] = state && has_state ? state[((long long)hv * D + column0 + j) * D + row] : 0.0f;
+      for (int j = 0; j < W; j += 2) S[j / 2] = make_float2(number(j), number(j + 1));
     }
     auto put_state = [&]() {
       if (has_state) {
-        float x[W];
+        float2 x[W / 2];
 #pragma unroll
-        for (int j = 0; j < W; ++j) x[j] = S[j];
+        for (int j = 0; j < W / 2; ++j) x[j] = S[j];
         put(sh.s[0], D * 128, x);
         fence_proxy();
       }
       fence_before();
       barrier_arrive(&sh.s_ready);
     };
+    // Values of a chunk's tokens, a chunk ahead; rows behind the last token are zeros.
     Raw<DTYPE> v[W / 8];
     auto fetch = [&](int c) {
       const int i = c * kChunk + token;
 #pragma unroll
       for (int j = 0; j < W / 8; ++j) {
+        v[j] = {};
         if (key && i < left) v[j] = load_row<DTYPE>(a.mixed_qkv, (long long)(place.first + from + i) * a.stride_mixed_tok + (2 * a.H + hv) * D + column0 + j * 8, p.aligned);
       }
     };
@@ -480,23 +930,24 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
     }
     for (int c = 0; c < chunks; ++c) {
       const int stage = c % STAGES, parity = c & 1;
-      const bool there = c * kChunk + token < left;
       healthy = wait(&sh.full[stage], c / STAGES & 1);
       if (!healthy) break;
       const float* vec = sh.vec[stage];
-      const float of_state = key ? vec[token] : vec[3 * kChunk + token], beta = vec[kChunk + token], of_added = vec[2 * kChunk + token], decay = vec[4 * kChunk];
-      float x[W], o[W];
+      const float of_state = key ? -vec[token] : vec[3 * kChunk + token], beta = vec[kChunk + token], of_added = vec[2 * kChunk + token], decay = vec[4 * kChunk];
+      float2 x[W / 2], o[W / 2];                  // o: a key's beta v; a query's part of the output that comes from the state
+#pragma unroll
+      for (int j = 0; j < W / 8; ++j) {
+        const Eight e = unpack<DTYPE>(v[j]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[4 * j + k] = mul2(e.x[k], make_float2(beta, beta));
+      }
       healthy = wait(&sh.scored, parity);
       if (!healthy) break;
       fence_after();
-      load_columns<W>(at, x);
+      load_sums<W, COLUMNS>(at, x);
       if (key) {
 #pragma unroll
-        for (int j = 0; j < W; j += 8) {
-          const Eight e = unpack<DTYPE>(v[j / 8]);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[j + k] = there ? fmaf(-of_state, x[j + k], beta * (k % 2 ? e.x[k / 2].y : e.x[k / 2].x)) : 0.0f;
-        }
+        for (int j = 0; j < W / 2; ++j) x[j] = fma2(make_float2(of_state, of_state), x[j], o[j]);
         put(sh.u[0], kChunk * 128, x);
         fence_proxy();
         fence_before();
@@ -504,59 +955,59 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
         if (c + 1 < chunks) fetch(c + 1);
       } else {
 #pragma unroll
-        for (int j = 0; j < W; ++j) o[j] = of_state * x[j];
+        for (int j = 0; j < W / 2; ++j) o[j] = mul2(make_float2(of_state, of_state), x[j]);
         fence_before();
         barrier_arrive(&sh.u_ready);
       }
       healthy = wait(&sh.solved, parity);
       if (!healthy) break;
       fence_after();
-      load_columns<W>(at + COLUMNS, x);
+      load_sums<W, COLUMNS>(at + kSolvedAt, x);
       if (key) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) x[j] *= of_added;
+        for (int j = 0; j < W / 2; ++j) x[j] = mul2(make_float2(of_added, of_added), x[j]);
         put(sh.u[0], kChunk * 128, x);
         fence_proxy();
         fence_before();
         barrier_arrive(&sh.u_ready);
-      } else if (there) {
+      } else if (c * kChunk + token < left) {
         const long long to = (long long)(place.first + from + c * kChunk + token) * a.stride_out_tok + hv * D + column0;
 #pragma unroll
-        for (int j = 0; j < W; ++j) x[j] += o[j];
+        for (int j = 0; j < W / 2; ++j) x[j] = add2(x[j], o[j]);
         if (p.out_aligned) {
 #pragma unroll
-          for (int j = 0; j < W; j += 8) {
+          for (int j = 0; j < W / 2; j += 4) {
             if (a.out_dtype == CARRY_F32) {
-              float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + to + j);
-              q[0] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-              q[1] = make_float4(x[j + 4], x[j + 5], x[j + 6], x[j + 7]);
+              float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + to + 2 * j);
+              q[0] = make_float4(x[j].x, x[j].y, x[j + 1].x, x[j + 1].y);
+              q[1] = make_float4(x[j + 2].x, x[j + 2].y, x[j + 3].x, x[j + 3].y);
             } else {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const __half2 y = __floats2half2_rn(x[j + 2 * e], x[j + 2 * e + 1]);
-                w[e] = a.out_dtype == CARRY_BF16 ? pack_bf16(x[j + 2 * e], x[j + 2 * e + 1]) : *reinterpret_cast<const uint32_t*>(&y);
+                const __half2 y = __float22half2_rn(x[j + e]);
+                w[e] = a.out_dtype == CARRY_BF16 ? pack_bf16(x[j + e].x, x[j + e].y) : *reinterpret_cast<const uint32_t*>(&y);
               }
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + to + j) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + to + 2 * j) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < W; ++j) store_from_float(a.out, to + j, a.out_dtype, x[j]);
+          for (int j = 0; j < W; ++j) store_from_float(a.out, to + j, a.out_dtype, j % 2 ? x[j / 2].y : x[j / 2].x);
         }
       }
       healthy = wait(&sh.added, parity);
       if (!healthy) break;
       fence_after();
-      load_columns<W>(at + 2 * COLUMNS, x);
+      load_sums<W, COLUMNS>(at, x);
 #pragma unroll
-      for (int j = 0; j < W; ++j) S[j] = fmaf(decay, S[j], x[j]);
+      for (int j = 0; j < W / 2; ++j) S[j] = fma2(make_float2(decay, decay), S[j], x[j]);
       if (c + 1 < chunks) put_state();
     }
     if (healthy && has_state) {
       float* state = a.final_state + b * a.stride_final_req;
 #pragma unroll
-      for (int j = 0; j < W; ++j) state[((long long)hv * D + column0 + j) * D + row] = S[j];
+      for (int j = 0; j < W; ++j) state[((long long)hv * D + column0 + j) * D + row] = j % 2 ? S[j / 2].y : S[j / 2].x;
     }
   } else if (warp == kLoadWarp) {
     // ---- tiles and factors out of the workspace ----
@@ -574,11 +1025,9 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
     }
     __syncwarp();
   } else {
-    // ---- products ----
+    // ---- products: a left side's term x with the right side's terms 0 .. kTerms - 1 - x, which are its next columns ----
     const uint32_t elected = elect(), base = __shfl_sync(~0u, tmem, 0);
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, barrier_wait(bar, parity, poison, a.status)) != 0; };
-    const uint32_t state = operand(sh.s, 16), rows = operand(sh.u, 16);
-    constexpr uint32_t kStateTerm = D * 128 / 16, kRowsTerm = kChunk * 128 / 16;
+    const uint32_t state = operand(sh.s, D * 128), rows = operand(sh.u, kChunk * 128);
     for (int c = 0; c < chunks; ++c) {
       const int stage = c % STAGES, parity = c & 1;
       const uint32_t kq = operand(sh.kq[stage], 16), t = operand(sh.t[stage], 16), keys = operand(sh.kq[stage], D == 128 ? kPlane : 0);
@@ -587,32 +1036,25 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
 #pragma unroll
       for (int x = 0; x < kX; ++x)
 #pragma unroll
-        for (int y = 0; x + y < kTerms; ++y)
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_shared(elected, base, kq + x * (kPlanes * kPlane / 16) + k / 4 * (kPlane / 16) + k % 4 * 2, state + y * kStateTerm + k * 128,
-                       instruction_bf16(COLUMNS, false, true), x + y + k > 0);
+        for (int k = 0; k < D / 16; ++k)
+          mma_shared(elected, base, kq + x * (kPlanes * kPlane / 16) + k / 4 * (kPlane / 16) + k % 4 * 2, state + k * 128,
+                     instruction_bf16((kTerms - x) * COLUMNS, false, true), x + k > 0);
       mma_commit(elected, &sh.scored);
       if (!wait(&sh.r_ready, parity)) break;
       fence_after();
 #pragma unroll
       for (int x = 0; x < kT; ++x)
 #pragma unroll
-        for (int y = 0; x + y < kTerms; ++y)
-#pragma unroll
-          for (int k = 0; k < kChunk / 16; ++k)
-            mma_shared(elected, base + COLUMNS, t + x * (kPlane / 16) + k * 2, rows + y * kRowsTerm + k * 128, instruction_bf16(COLUMNS, false, true), x + y + k > 0);
+        for (int k = 0; k < kChunk / 16; ++k)
+          mma_shared(elected, base + kSolvedAt, t + x * (kPlane / 16) + k * 2, rows + k * 128, instruction_bf16((kTerms - x) * COLUMNS, false, true), x + k > 0);
       mma_commit(elected, &sh.solved);
       if (!wait(&sh.u_ready, parity)) break;
       fence_after();
 #pragma unroll
       for (int x = 0; x < kX; ++x)
 #pragma unroll
-        for (int y = 0; x + y < kTerms; ++y)
-#pragma unroll
-          for (int k = 0; k < kChunk / 16; ++k)
-            mma_shared(elected, base + 2 * COLUMNS, keys + x * (kPlanes * kPlane / 16) + k * 128, rows + y * kRowsTerm + k * 128,
-                       instruction_bf16(COLUMNS, true, true), x + y + k > 0);
+        for (int k = 0; k < kChunk / 16; ++k)
+          mma_shared(elected, base, keys + x * (kPlanes * kPlane / 16) + k * 128, rows + k * 128, instruction_bf16((kTerms - x) * COLUMNS, true, true), x + k > 0);
       mma_commit(elected, &sh.added);
       mma_commit(elected, &sh.free[stage]);
     }
@@ -676,7 +1118,7 @@ int allow_shared(K kernel, size_t smem, bool (&ready)[64]) {
 
 template <int DTYPE, int D, int COLUMNS, int STAGES>
 int launch_sequence(const ChunkParams& p, int requests, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(SequenceShared<kTermsX<DTYPE>, kTermsT<DTYPE>, D, STAGES>) + 1024;
+  constexpr size_t smem = sizeof(SequenceShared<kTermsX<DTYPE>, kTermsT<DTYPE>, D, COLUMNS, STAGES>) + 1024;
   static_assert(smem <= 227 * 1024, "a CTA's shared memory");
   static thread_local bool ready[64];
   const int rc = allow_shared(sequence_kernel<DTYPE, D, COLUMNS, STAGES>, smem, ready);
@@ -687,9 +1129,11 @@ int launch_sequence(const ChunkParams& p, int requests, cudaStream_t stream) {
 template <int DTYPE, int D>
 int launch_chunks(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
   constexpr int kSize = DTYPE == CARRY_F32 ? 4 : 2, kX = kTermsX<DTYPE>;
-  constexpr size_t smem = sizeof(PrepareShared<kX, kTermsT<DTYPE>, D>) + 1024;
+  constexpr size_t smem = DTYPE == CARRY_F32 ? sizeof(PrepareShared<kX, D>) + 1024 : kUnitWarps * sizeof(Unit);
   static thread_local bool ready[64];
-  int rc = allow_shared(prepare_kernel<DTYPE, D>, smem, ready);
+  int rc;
+  if constexpr (DTYPE == CARRY_F32) rc = allow_shared(prepare_kernel<DTYPE, D>, smem, ready);
+  else rc = allow_shared(unit_kernel<DTYPE, D>, smem, ready);
   if (rc != CARRY_GDN_OK) return rc;
   const Layout l = lay_out(a);
   ChunkParams p = {};
@@ -707,7 +1151,11 @@ int launch_chunks(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
       p.chunk0 = c;
       p.chunks = l.total - c < l.chunks ? l.total - c : l.chunks;
       const int requests = a.B - b < l.requests ? a.B - b : l.requests;
-      rc = launch_dependent(prepare_kernel<DTYPE, D>, dim3((unsigned)p.chunks, (unsigned)a.H, (unsigned)requests), kPrepareThreads, smem, stream, p);
+      if constexpr (DTYPE == CARRY_F32)
+        rc = launch_dependent(prepare_kernel<DTYPE, D>, dim3((unsigned)p.chunks, (unsigned)a.HV, (unsigned)requests), kPrepareThreads, smem, stream, p);
+      else
+        rc = launch_dependent(unit_kernel<DTYPE, D>, dim3((unsigned)(p.chunks + kUnitWarps - 1) / kUnitWarps, (unsigned)a.HV, (unsigned)requests), kUnitWarps * 32, smem,
+                              stream, p);
       if (rc != CARRY_GDN_OK) return rc;
       const bool narrow = (int64_t)requests * a.HV * (D / 64) < sm_count();
       rc = narrow ? launch_sequence<DTYPE, D, 32, kX == 1 ? 2 : 1>(p, requests, stream) : launch_sequence<DTYPE, D, 64, kX == 1 ? 2 : 1>(p, requests, stream);
