@@ -804,31 +804,31 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
 
 // ---- along a sequence ------------------------------------------------------------------------------------------------
 
-constexpr int kColumnGroups = 4, kRowThreads = kColumnGroups * 128, kLoadWarp = kRowThreads / 32, kIssueWarp = kLoadWarp + 1, kSequenceThreads = (kIssueWarp + 1) * 32;
+constexpr int kColumns = 32;                      // of the state to a CTA
 
-// Operands of COLUMNS columns lie with their terms side by side, so that one product takes all terms and reads its left side once;
-// planes have 64 columns.
-template <int COLUMNS>
-constexpr int kPlanesOf = (kTerms * COLUMNS + 63) / 64;
-
-template <int TERMS, int TERMS_T, int D, int COLUMNS, int STAGES>
+// Right sides lie with their three terms side by side, so that one product takes all terms and reads its left side once: two of them in a
+// plane of 64 columns, the third in the first half of another one.  The second half of the state's other plane has the third term of R and U.
+template <int DTYPE, int D, int STAGES>
 struct SequenceShared {
-  uint8_t kq[STAGES][TERMS][D / 64][kPlane], t[STAGES][TERMS_T][kPlane];
-  uint8_t s[kPlanesOf<COLUMNS>][D * 128], u[kPlanesOf<COLUMNS>][kChunk * 128];    // the state; R, and then U with its decays
-  alignas(16) float vec[STAGES][kVec];
-  uint64_t full[STAGES], free[STAGES], s_ready, r_ready, u_ready, scored, solved, added;
+  uint8_t kq[STAGES][kTermsX<DTYPE>][D / 64][kPlane], t[STAGES][kTermsT<DTYPE>][kPlane];
+  uint8_t u[kChunk * 128], s[2][D * 128];         // R, and then U with its decays; the state
+  alignas(16) uint8_t v[STAGES][kChunk][kColumns * (DTYPE == CARRY_F32 ? 4 : 2)];
+  alignas(16) float vec[2][kVec];
+  // what has come, and what is free again: keys, queries, T and values are each asked for again as soon as they have been used
+  uint64_t k_full[STAGES], q_full[STAGES], t_full[STAGES], v_full[STAGES], vec_full[2], k_free[STAGES], q_free[STAGES], t_free[STAGES], v_free[STAGES];
+  uint64_t s_ready, r_ready, u_ready, scored, solved, added;
   uint32_t tmem;
   int poison;
 };
 
-// this thread's W columns of each term's product, summed, the smallest first
-template <int W, int COLUMNS>
+// this thread's columns of each term's product, summed, the smallest first
+template <int W>
 __device__ __forceinline__ void load_sums(uint32_t at, float2 (&x)[W / 2]) {
   uint32_t r[kTerms][W];
 #pragma unroll
   for (int t = 0; t < kTerms; ++t) {
-    if constexpr (W == 8) tmem_load8(at + t * COLUMNS, r[t]);
-    else tmem_load16(at + t * COLUMNS, r[t]);
+    if constexpr (W == 8) tmem_load8(at + t * kColumns, r[t]);
+    else tmem_load16(at + t * kColumns, r[t]);
   }
   wait_loads();
   auto two = [&](int t, int j) { return make_float2(__uint_as_float(r[t][j]), __uint_as_float(r[t][j + 1])); };
@@ -836,11 +836,12 @@ __device__ __forceinline__ void load_sums(uint32_t at, float2 (&x)[W / 2]) {
   for (int j = 0; j < W; j += 2) x[j / 2] = add2(add2(two(2, j), two(1, j)), two(0, j));
 }
 
-// COLUMNS of a head's state to a CTA
-template <int DTYPE, int D, int COLUMNS, int STAGES>
-__global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64, W = COLUMNS / kColumnGroups;
-  using Shared = SequenceShared<kX, kT, D, COLUMNS, STAGES>;
+// GROUPS of 128 threads share a row's columns.  With two stages of operands a CTA has a processor for itself; with one, two of them share it.
+template <int DTYPE, int D, int GROUPS, int STAGES>
+__global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CARRY_BF16 ? 2 : 1) sequence_kernel(const __grid_constant__ ChunkParams p) {
+  constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64, W = kColumns / GROUPS;
+  constexpr int kRowThreads = GROUPS * 128, kLoadWarp = kRowThreads / 32, kIssueWarp = kLoadWarp + 1, kValueBytes = DTYPE == CARRY_F32 ? 4 : 2;
+  using Shared = SequenceShared<DTYPE, D, STAGES>;
   extern __shared__ uint8_t raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
   depend_release();
@@ -853,9 +854,12 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
   if (tid == 0) {
     sh.poison = 0;
     for (int i = 0; i < STAGES; ++i) {
-      barrier_init(&sh.full[i], 1);
-      barrier_init(&sh.free[i], 1);
+      for (uint64_t* bar : {&sh.k_full[i], &sh.q_full[i], &sh.t_full[i], &sh.k_free[i], &sh.q_free[i], &sh.t_free[i]}) barrier_init(bar, 1);
+      barrier_init(&sh.v_full[i], 32);
+      barrier_init(&sh.v_free[i], kRowThreads / 2);
     }
+    barrier_init(&sh.vec_full[0], 1);
+    barrier_init(&sh.vec_full[1], 1);
     barrier_init(&sh.s_ready, kRowThreads);
     barrier_init(&sh.r_ready, kRowThreads / 2);
     barrier_init(&sh.u_ready, kRowThreads);
@@ -865,7 +869,7 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // columns 0 and on: [K; Q] S, and, when that is read, K^T U; behind them [T; P T] R
-  constexpr uint32_t kSolvedAt = kTerms * COLUMNS, kTmem = 2 * kSolvedAt <= 256 ? 256 : 512;
+  constexpr uint32_t kSolvedAt = kTerms * kColumns, kTmem = 256;
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "n"(kTmem) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -879,20 +883,20 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
 
   if (tid < kRowThreads) {
     // ---- a row to a thread, some of its columns: of the products' rows (keys, queries), and of the state's (K) ----
-    const int row = warp % 4 * 32 + lane, first = warp / 4 * W, column0 = blockIdx.x * COLUMNS + first, token = row % kChunk;
+    const int row = warp % 4 * 32 + lane, first = warp / 4 * W, column0 = blockIdx.x * kColumns + first, token = row % kChunk;
     const uint32_t at = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + first;
     const bool key = row < kChunk, has_state = row < D;
-    // this thread's numbers into an operand with planes of `plane` bytes, as kTerms terms
-    auto put = [&](uint8_t* tile, int plane, float2 (&x)[W / 2]) {
+    // this thread's numbers into an operand's terms; `last`: of the third one
+    auto put = [&](uint8_t* tile, uint8_t* last, int last_column, float2 (&x)[W / 2]) {
 #pragma unroll
       for (int j = 0; j < W; j += 8)
 #pragma unroll
         for (int t = 0; t < kTerms; ++t) {
-          const int column = t * COLUMNS + first + j;
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = take_term(x[j / 2 + e]);
-          *reinterpret_cast<uint4*>(tile + column / 64 * plane + plane_at(row, column % 64 / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+          uint8_t* to = t < 2 ? tile + plane_at(row, (t * kColumns + first + j) / 8) : last + plane_at(row, (last_column + first + j) / 8);
+          *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     };
     float2 S[W / 2];
@@ -907,52 +911,42 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
         float2 x[W / 2];
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = S[j];
-        put(sh.s[0], D * 128, x);
+        put(sh.s[0], sh.s[1], 0, x);
         fence_proxy();
       }
       fence_before();
       barrier_arrive(&sh.s_ready);
     };
-    // Values of a chunk's tokens, a chunk ahead; rows behind the last token are zeros.
-    Raw<DTYPE> v[W / 8];
-    auto fetch = [&](int c) {
-      const int i = c * kChunk + token;
-#pragma unroll
-      for (int j = 0; j < W / 8; ++j) {
-        v[j] = {};
-        if (key && i < left) v[j] = load_row<DTYPE>(a.mixed_qkv, (long long)(place.first + from + i) * a.stride_mixed_tok + (2 * a.H + hv) * D + column0 + j * 8, p.aligned);
-      }
-    };
     bool healthy = true;
-    if (chunks > 0) {
-      fetch(0);
-      put_state();
-    }
+    if (chunks > 0) put_state();
     for (int c = 0; c < chunks; ++c) {
-      const int stage = c % STAGES, parity = c & 1;
-      healthy = wait(&sh.full[stage], c / STAGES & 1);
+      const int parity = c & 1, stage = c % STAGES;
+      healthy = wait(&sh.vec_full[parity], c / 2 & 1) && (!key || wait(&sh.v_full[stage], c / STAGES & 1));    // only keys' threads hold the values back
       if (!healthy) break;
-      const float* vec = sh.vec[stage];
+      const float* vec = sh.vec[parity];
       const float of_state = key ? -vec[token] : vec[3 * kChunk + token], beta = vec[kChunk + token], of_added = vec[2 * kChunk + token], decay = vec[4 * kChunk];
       float2 x[W / 2], o[W / 2];                  // o: a key's beta v; a query's part of the output that comes from the state
+      if (key) {
+        const bool there = c * kChunk + token < left;       // behind the last token lies what an earlier chunk had
 #pragma unroll
-      for (int j = 0; j < W / 8; ++j) {
-        const Eight e = unpack<DTYPE>(v[j]);
+        for (int j = 0; j < W; j += 8) {
+          const Eight e = unpack<DTYPE>(load_raw<DTYPE>(sh.v[stage][token], first + j));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[4 * j + k] = mul2(e.x[k], make_float2(beta, beta));
+          for (int k = 0; k < 4; ++k) o[j / 2 + k] = there ? mul2(e.x[k], make_float2(beta, beta)) : make_float2(0.0f, 0.0f);
+        }
       }
       healthy = wait(&sh.scored, parity);
       if (!healthy) break;
       fence_after();
-      load_sums<W, COLUMNS>(at, x);
+      load_sums<W>(at, x);
       if (key) {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = fma2(make_float2(of_state, of_state), x[j], o[j]);
-        put(sh.u[0], kChunk * 128, x);
+        put(sh.u, sh.s[1], kColumns, x);
         fence_proxy();
         fence_before();
         barrier_arrive(&sh.r_ready);
-        if (c + 1 < chunks) fetch(c + 1);
+        barrier_arrive(&sh.v_free[stage]);        // not before the values have been used: a load that is merely under way may be overtaken by the next copy
       } else {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) o[j] = mul2(make_float2(of_state, of_state), x[j]);
@@ -962,11 +956,11 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
       healthy = wait(&sh.solved, parity);
       if (!healthy) break;
       fence_after();
-      load_sums<W, COLUMNS>(at + kSolvedAt, x);
+      load_sums<W>(at + kSolvedAt, x);
       if (key) {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = mul2(make_float2(of_added, of_added), x[j]);
-        put(sh.u[0], kChunk * 128, x);
+        put(sh.u, sh.s[1], kColumns, x);
         fence_proxy();
         fence_before();
         barrier_arrive(&sh.u_ready);
@@ -999,7 +993,7 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
       healthy = wait(&sh.added, parity);
       if (!healthy) break;
       fence_after();
-      load_sums<W, COLUMNS>(at, x);
+      load_sums<W>(at, x);
 #pragma unroll
       for (int j = 0; j < W / 2; ++j) S[j] = fma2(make_float2(decay, decay), S[j], x[j]);
       if (c + 1 < chunks) put_state();
@@ -1010,53 +1004,88 @@ __global__ void __launch_bounds__(kSequenceThreads, 1) sequence_kernel(const __g
       for (int j = 0; j < W; ++j) state[((long long)hv * D + column0 + j) * D + row] = j % 2 ? S[j / 2].y : S[j / 2].x;
     }
   } else if (warp == kLoadWarp) {
-    // ---- tiles and factors out of the workspace ----
-    if (lane == 0) {
-      constexpr uint32_t kBytesKq = kX * kPlanes * kPlane, kBytesT = kT * kPlane;
-      for (int c = 0; c < chunks; ++c) {
-        const int stage = c % STAGES;
-        if (c >= STAGES && !barrier_wait(&sh.free[stage], c / STAGES - 1 & 1, poison, a.status)) break;
-        barrier_expect(&sh.full[stage], kBytesKq + kBytesT + kVec * 4);
-        const long long slot = place.slot0 + c;
-        bulk_copy(sh.vec[stage], p.vec + (slot * a.HV + hv) * kVec, kVec * 4, &sh.full[stage]);
-        bulk_copy(sh.kq[stage], p.kq + (slot * a.H + h) * kBytesKq, kBytesKq, &sh.full[stage]);
-        bulk_copy(sh.t[stage], p.t + (slot * a.HV + hv) * kBytesT, kBytesT, &sh.full[stage]);
+    // ---- tiles and factors out of the workspace, values out of the rows ----
+    constexpr uint32_t kBytesKq = kX * kPlanes * kPlane, kBytesT = kT * kPlane, kSide = kPlane / 2, kBytesV = kColumns * kValueBytes;
+    auto sides = [&](int c, int side, uint64_t* bar) {      // keys or queries: a half of every plane
+      const uint8_t* tile = p.kq + ((place.slot0 + c) * a.H + h) * kBytesKq;
+      barrier_expect(bar, kBytesKq / 2);
+      for (int i = side * kSide; i < (int)kBytesKq; i += kPlane) bulk_copy(sh.kq[c % STAGES][0][0] + i, tile + i, kSide, bar);
+    };
+    for (int c = 0; c < chunks; ++c) {
+      const int stage = c % STAGES, tokens = min(left - c * kChunk, kChunk);
+      const bool reused = c >= STAGES;
+      const uint32_t turn = (c / STAGES - 1) & 1;           // of the use before
+      const long long place_hv = (place.slot0 + c) * a.HV + hv;
+      // in the order in which what was there is done with
+      if (reused && !wait(&sh.v_free[stage], turn)) break;
+      const long long at = (long long)(place.first + from + c * kChunk) * a.stride_mixed_tok + (2 * a.H + hv) * D + blockIdx.x * kColumns;
+      if (p.aligned) {                            // sixteen bytes at a time: bulk copies of such short rows would hold up the tiles'
+        for (int i = lane; i < tokens * (int)(kBytesV / 16); i += 32) {
+          const int token = i / (kBytesV / 16), part = i % (kBytesV / 16) * 16;
+          __pipeline_memcpy_async(sh.v[stage][token] + part, reinterpret_cast<const uint8_t*>(a.mixed_qkv) + (at + token * a.stride_mixed_tok) * kValueBytes + part, 16);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&sh.v_full[stage])) : "memory");
+      } else {
+        for (int i = 0; i < tokens; ++i) {
+          if constexpr (kValueBytes == 4) reinterpret_cast<float*>(sh.v[stage][i])[lane] = reinterpret_cast<const float*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
+          else reinterpret_cast<uint16_t*>(sh.v[stage][i])[lane] = reinterpret_cast<const uint16_t*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
+        }
+        barrier_arrive(&sh.v_full[stage]);
       }
+      if (reused && !wait(&sh.q_free[stage], turn)) break;
+      if (lane == 0) sides(c, 1, &sh.q_full[stage]);
+      __syncwarp();
+      if (reused && !wait(&sh.t_free[stage], turn)) break;
+      if (lane == 0) {
+        barrier_expect(&sh.t_full[stage], kBytesT);
+        bulk_copy(sh.t[stage], p.t + place_hv * kBytesT, kBytesT, &sh.t_full[stage]);
+      }
+      __syncwarp();
+      if (reused && !wait(&sh.k_free[stage], turn)) break;  // after which nobody reads the factors of the chunk before the last
+      if (lane == 0) {
+        barrier_expect(&sh.vec_full[c & 1], kVec * 4);
+        bulk_copy(sh.vec[c & 1], p.vec + place_hv * kVec, kVec * 4, &sh.vec_full[c & 1]);
+        sides(c, 0, &sh.k_full[stage]);
+      }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // ---- products: a left side's term x with the right side's terms 0 .. kTerms - 1 - x, which are its next columns ----
     const uint32_t elected = elect(), base = __shfl_sync(~0u, tmem, 0);
-    const uint32_t state = operand(sh.s, D * 128), rows = operand(sh.u, kChunk * 128);
+    // the third term lies that far behind the first two
+    const uint32_t state = operand(sh.s[0], D * 128), rows = operand(sh.u, smem_addr(sh.s[1]) + kColumns * 2 - smem_addr(sh.u));
     for (int c = 0; c < chunks; ++c) {
-      const int stage = c % STAGES, parity = c & 1;
+      const int parity = c & 1, stage = c % STAGES;
+      const uint32_t turn = c / STAGES & 1;
       const uint32_t kq = operand(sh.kq[stage], 16), t = operand(sh.t[stage], 16), keys = operand(sh.kq[stage], D == 128 ? kPlane : 0);
-      if (!wait(&sh.full[stage], c / STAGES & 1) || !wait(&sh.s_ready, parity)) break;
+      if (!wait(&sh.k_full[stage], turn) || !wait(&sh.q_full[stage], turn) || !wait(&sh.s_ready, parity)) break;
       fence_after();
 #pragma unroll
       for (int x = 0; x < kX; ++x)
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           mma_shared(elected, base, kq + x * (kPlanes * kPlane / 16) + k / 4 * (kPlane / 16) + k % 4 * 2, state + k * 128,
-                     instruction_bf16((kTerms - x) * COLUMNS, false, true), x + k > 0);
+                     instruction_bf16((kTerms - x) * kColumns, false, true), x + k > 0);
       mma_commit(elected, &sh.scored);
-      if (!wait(&sh.r_ready, parity)) break;
+      mma_commit(elected, &sh.q_free[stage]);
+      if (!wait(&sh.t_full[stage], turn) || !wait(&sh.r_ready, parity)) break;
       fence_after();
 #pragma unroll
       for (int x = 0; x < kT; ++x)
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k)
-          mma_shared(elected, base + kSolvedAt, t + x * (kPlane / 16) + k * 2, rows + k * 128, instruction_bf16((kTerms - x) * COLUMNS, false, true), x + k > 0);
+          mma_shared(elected, base + kSolvedAt, t + x * (kPlane / 16) + k * 2, rows + k * 128, instruction_bf16((kTerms - x) * kColumns, false, true), x + k > 0);
       mma_commit(elected, &sh.solved);
+      mma_commit(elected, &sh.t_free[stage]);
       if (!wait(&sh.u_ready, parity)) break;
       fence_after();
 #pragma unroll
       for (int x = 0; x < kX; ++x)
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k)
-          mma_shared(elected, base, keys + x * (kPlanes * kPlane / 16) + k * 128, rows + k * 128, instruction_bf16((kTerms - x) * COLUMNS, true, true), x + k > 0);
+          mma_shared(elected, base, keys + x * (kPlanes * kPlane / 16) + k * 128, rows + k * 128, instruction_bf16((kTerms - x) * kColumns, true, true), x + k > 0);
       mma_commit(elected, &sh.added);
-      mma_commit(elected, &sh.free[stage]);
+      mma_commit(elected, &sh.k_free[stage]);
     }
   }
   if (*poison) {
@@ -1116,14 +1145,15 @@ int allow_shared(K kernel, size_t smem, bool (&ready)[64]) {
   return CARRY_GDN_OK;
 }
 
-template <int DTYPE, int D, int COLUMNS, int STAGES>
+template <int DTYPE, int D, int GROUPS, int STAGES>
 int launch_sequence(const ChunkParams& p, int requests, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(SequenceShared<kTermsX<DTYPE>, kTermsT<DTYPE>, D, COLUMNS, STAGES>) + 1024;
+  constexpr size_t smem = sizeof(SequenceShared<DTYPE, D, STAGES>) + 1024;
   static_assert(smem <= 227 * 1024, "a CTA's shared memory");
+  static_assert(STAGES == 2 || DTYPE != CARRY_BF16 || 2 * (smem + 1024) <= 228 * 1024, "two CTAs to a processor");
   static thread_local bool ready[64];
-  const int rc = allow_shared(sequence_kernel<DTYPE, D, COLUMNS, STAGES>, smem, ready);
+  const int rc = allow_shared(sequence_kernel<DTYPE, D, GROUPS, STAGES>, smem, ready);
   if (rc != CARRY_GDN_OK) return rc;
-  return launch_dependent(sequence_kernel<DTYPE, D, COLUMNS, STAGES>, dim3(D / COLUMNS, (unsigned)p.a.HV, (unsigned)requests), kSequenceThreads, smem, stream, p);
+  return launch_dependent(sequence_kernel<DTYPE, D, GROUPS, STAGES>, dim3(D / kColumns, (unsigned)p.a.HV, (unsigned)requests), GROUPS * 128 + 64, smem, stream, p);
 }
 
 template <int DTYPE, int D>
@@ -1157,8 +1187,9 @@ int launch_chunks(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
         rc = launch_dependent(unit_kernel<DTYPE, D>, dim3((unsigned)(p.chunks + kUnitWarps - 1) / kUnitWarps, (unsigned)a.HV, (unsigned)requests), kUnitWarps * 32, smem,
                               stream, p);
       if (rc != CARRY_GDN_OK) return rc;
-      const bool narrow = (int64_t)requests * a.HV * (D / 64) < sm_count();
-      rc = narrow ? launch_sequence<DTYPE, D, 32, kX == 1 ? 2 : 1>(p, requests, stream) : launch_sequence<DTYPE, D, 64, kX == 1 ? 2 : 1>(p, requests, stream);
+      // one CTA to a processor while that is all there are
+      if constexpr (DTYPE == CARRY_BF16) rc = (int64_t)requests * a.HV * (D / kColumns) <= sm_count() ? launch_sequence<DTYPE, D, 4, 2>(p, requests, stream) : launch_sequence<DTYPE, D, 2, 1>(p, requests, stream);
+      else rc = launch_sequence<DTYPE, D, 4, 1>(p, requests, stream);
       if (rc != CARRY_GDN_OK) return rc;
     }
   return CARRY_GDN_OK;

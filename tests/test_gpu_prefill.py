@@ -230,6 +230,17 @@ def test_alike_keys_and_zero_rows():
         check(got, c, state, lengths, H, D, in_chunks=max(lengths) > 64)
 
 
+@pytest.mark.parametrize("dtype,D,H,HV,lengths", [(F32, 64, 2, 4, [65]), (BF16, 128, 8, 16, [300, 77, 64, 500]), (F32, 128, 8, 16, [300, 77, 64, 500]),
+                                                  (F16, 128, 16, 32, [130] * 20), (BF16, 64, 1, 2, [700]), (BF16, 128, 16, 32, [1000, 1, 90])])
+def test_repeated_calls_give_the_same_numbers(dtype, D, H, HV, lengths):
+    """Warps and copies that meet at other times: every call's numbers are the first one's."""
+    c, state = make(lengths, H, HV, D, dtype, True)
+    first = run(c, state, lengths, HV, D)
+    for _ in range(40):
+        again = run(c, state, lengths, HV, D)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
 def test_no_rows_at_all():
     state = torch.randn(2, 3, 64, 64, device=DEV)
     for initial, want in ((None, torch.zeros_like(state)), (state, state)):
