@@ -39,6 +39,7 @@ __device__ __forceinline__ void prefill_gates(const CarryGdnPrefillArgs& a, long
 
 int64_t delta_workspace(const CarryGdnPrefillArgs& a);
 int launch_delta(const CarryGdnPrefillArgs& a, cudaStream_t stream);
+bool delta_rows_alone(const CarryGdnPrefillArgs& a);
 int launch_delta_recurrent(const CarryGdnPrefillArgs& a, cudaStream_t stream);
 
 }  // namespace carry

@@ -454,10 +454,10 @@ struct alignas(16) Unit {
 template <bool HALF>
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // A lane's part of a 16 x 16 block, of which it has numbers (g, 2t), (g, 2t+1), (g+8, 2t), .. and the same eight columns on: for g = lane / 4,
@@ -1200,8 +1200,9 @@ int launch_width(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
   return a.K == 64 ? launch_chunks<DTYPE, 64>(a, stream) : launch_chunks<DTYPE, 128>(a, stream);
 }
 
-constexpr int kFewTokens = 64;
-bool in_chunks(const CarryGdnPrefillArgs& a) { return a.max_query > kFewTokens; }
+// Up to so many tokens of a request go token by token.  A token costs 0.35 us where every row of the states has lanes of its own, a chunk 25 us
+// and 2.5 to 4 for each further one; with 128 heads a token 0.85 us, a chunk 36; in fp32, whose products take four times as many, 0.3 to 1.1 and 25 to 90.
+bool in_chunks(const CarryGdnPrefillArgs& a) { return a.max_query > (a.qkv_dtype == CARRY_F32 ? 96 : delta_rows_alone(a) ? 64 : 40); }
 
 }  // namespace
 

@@ -3,7 +3,11 @@
 // Rows of the state do not depend on one another, so a CTA has some of a head's rows, in registers: eight lanes to a row, each with
 // every eighth run of four numbers, so that the state comes and goes in whole lines.  What a token costs is a chain: the products of
 // the state with key and query (formed together from the state as it was, for o = alpha S q + u (k . q)), their sum over eight
-// lanes, and the row that is added.  The next token's numbers are asked for ahead of it.
+// lanes, and the row that is added.  Norms are formed for a block of tokens at a time, and the next block's numbers are asked for ahead of it.
+#include <cuda_pipeline_primitives.h>
+
+#include <type_traits>
+
 #include "carry_delta.cuh"
 
 namespace carry {
@@ -57,16 +61,33 @@ __device__ __forceinline__ float over_lanes(float x) {
   return x;
 }
 
+// Tokens come into shared memory a block at a time, a block ahead.
+constexpr int kTokens = 16;
+template <int DTYPE, int K, int ROWS>
+struct Block {
+  using Number = typename std::conditional<DTYPE == CARRY_F32, float, uint16_t>::type;
+  static constexpr int kRows = kThreads / kLanes * ROWS;      // of the state to a CTA
+  alignas(16) Number q[kTokens][K], k[kTokens][K], v[kTokens][kRows];
+};
+struct alignas(16) Factors {
+  float alpha, beta, query, key;        // query and key: what their numbers are multiplied by
+  float key_query, pad[3];              // product of the two as they are in memory, times both
+};
+
 // ROWS of the state to a group of eight lanes
 template <int DTYPE, int K, int ROWS>
-__global__ void __launch_bounds__(kThreads) recurrent_kernel(const __grid_constant__ CarryGdnPrefillArgs a, bool aligned) {
-  constexpr int kFours = K / 32;
+__global__ void __launch_bounds__(kThreads, ROWS == 4 ? 4 : 1) recurrent_kernel(const __grid_constant__ CarryGdnPrefillArgs a, bool aligned) {
+  using Tokens = Block<DTYPE, K, ROWS>;
+  using Number = typename Tokens::Number;
+  constexpr int kFours = K / 32, kRows = Tokens::kRows;
+  __shared__ Tokens block[2];
+  __shared__ Factors factors[kTokens];
   depend_release();
   depend_wait();
-  const int b = blockIdx.z, hv = blockIdx.y, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, h = hv / (a.HV / a.H);
-  const int row0 = blockIdx.x * (kThreads / kLanes * ROWS) + group * ROWS;
-  const PrefillRequest r = prefill_request(a, b, threadIdx.x == 0 && hv == 0 && blockIdx.x == 0 ? a.status : nullptr);
+  const int b = blockIdx.z, hv = blockIdx.y, tid = threadIdx.x, lane = tid % kLanes, group = tid / kLanes, h = hv / (a.HV / a.H);
+  const int row0 = blockIdx.x * kRows + group * ROWS;
   const long long head = (long long)hv * a.V * K;
+  // the state first: nothing has to be known for it
   float2 S[ROWS][kFours][2];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i)
@@ -77,82 +98,142 @@ __global__ void __launch_bounds__(kThreads) recurrent_kernel(const __grid_consta
       S[i][f][0] = make_float2(u.x, u.y);
       S[i][f][1] = make_float2(u.z, u.w);
     }
+  const PrefillRequest r = prefill_request(a, b, tid == 0 && hv == 0 && blockIdx.x == 0 ? a.status : nullptr);
 
-  struct Token {
-    Four<DTYPE> q[kFours], k[kFours];
-    float v[ROWS];
-  };
-  auto fetch = [&](int t, Token& x) {
-    const long long at = (long long)(r.first + t) * a.stride_mixed_tok;
-#pragma unroll
-    for (int f = 0; f < kFours; ++f) {
-      x.q[f] = load_four<DTYPE>(a.mixed_qkv, at + h * K + f * 32 + lane * 4, aligned);
-      x.k[f] = load_four<DTYPE>(a.mixed_qkv, at + (a.H + h) * K + f * 32 + lane * 4, aligned);
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) x.v[i] = load_as_float(a.mixed_qkv, at + 2LL * a.H * K + (long long)hv * a.V + row0 + i, DTYPE);
-  };
-  Token next;
-  float log_alpha = 0.0f, beta_of = 0.0f;         // of token (t / 32) * 32 + this lane of the warp
-  if (r.count > 0) fetch(0, next);
-  for (int t = 0; t < r.count; ++t) {
-    const Token now = next;
-    if (t % 32 == 0 && t + (int)threadIdx.x % 32 < r.count) {
-      prefill_gates(a, r.first + t + threadIdx.x % 32, hv, log_alpha, beta_of);
-      log_alpha = expf(log_alpha);
-    }
-    if (t + 1 < r.count) fetch(t + 1, next);
-    const float alpha = __shfl_sync(~0u, log_alpha, t % 32), beta = __shfl_sync(~0u, beta_of, t % 32);
-    float2 q[kFours][2], k[kFours][2];
-    float2 qq = make_float2(0.0f, 0.0f), kk = qq, kq = qq;
-#pragma unroll
-    for (int f = 0; f < kFours; ++f) {
-      unpack_four<DTYPE>(now.q[f], q[f]);
-      unpack_four<DTYPE>(now.k[f], k[f]);
-    }
-    float by_q = a.scale, by_k = 1.0f;
-    if (a.use_qk_l2norm) {
-#pragma unroll
-      for (int f = 0; f < kFours; ++f)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          qq = fma2(q[f][e], q[f][e], qq);
-          kk = fma2(k[f][e], k[f][e], kk);
+  auto fetch = [&](int t0) {
+    Tokens& to = block[t0 / kTokens & 1];
+    const int n = min(r.count - t0, kTokens);
+    const Number* rows = reinterpret_cast<const Number*>(a.mixed_qkv) + (long long)(r.first + t0) * a.stride_mixed_tok;
+    auto bring = [&](Number* dst, int stride, const Number* src, int width) {
+      if (aligned) {
+        constexpr int kEach = 16 / sizeof(Number);
+        for (int i = tid; i < n * width / kEach; i += kThreads) {
+          const int t = i / (width / kEach), at = i % (width / kEach) * kEach;
+          __pipeline_memcpy_async(dst + t * stride + at, src + t * a.stride_mixed_tok + at, 16);
         }
-      by_q = __fdiv_rn(a.scale, sqrtf(over_lanes(qq.x + qq.y) + kL2Eps));
-      by_k = __fdiv_rn(1.0f, sqrtf(over_lanes(kk.x + kk.y) + kL2Eps));
-    }
-#pragma unroll
-    for (int f = 0; f < kFours; ++f)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        q[f][e] = mul2(q[f][e], make_float2(by_q, by_q));
-        k[f][e] = mul2(k[f][e], make_float2(by_k, by_k));
-        kq = fma2(k[f][e], q[f][e], kq);
+      } else {
+        for (int i = tid; i < n * width; i += kThreads) dst[i / width * stride + i % width] = src[i / width * a.stride_mixed_tok + i % width];
       }
-    const float k_dot_q = over_lanes(kq.x + kq.y);
-    float out[ROWS];
+    };
+    bring(to.q[0], K, rows + h * K, K);
+    bring(to.k[0], K, rows + (a.H + h) * K, K);
+    bring(to.v[0], kRows, rows + 2LL * a.H * K + (long long)hv * a.V + blockIdx.x * kRows, kRows);
+  };
+  float log_alpha = 0.0f, beta_of = 0.0f;         // of token tid of the block to come
+  auto gates = [&](int t0) {
+    if (tid < kTokens && t0 + tid < r.count) prefill_gates(a, r.first + t0 + tid, hv, log_alpha, beta_of);
+  };
+  if (r.count > 0) fetch(0);
+  __pipeline_commit();
+  if (r.count > kTokens) fetch(kTokens);
+  __pipeline_commit();
+  gates(0);
+
+  for (int t0 = 0; t0 < r.count; t0 += kTokens) {
+    const Tokens& now = block[t0 / kTokens & 1];
+    const int n = min(r.count - t0, kTokens);
+    __pipeline_wait_prior(1);
+    if (tid < kTokens) {
+      factors[tid].alpha = expf(log_alpha);
+      factors[tid].beta = beta_of;
+    }
+    __syncthreads();
+    // norms, and the product of query and key: a token to eight lanes
+    for (int t = group; t < kTokens; t += kThreads / kLanes) {
+      float2 qq = make_float2(0.0f, 0.0f), kk = qq, kq = qq;
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      float2 sk = make_float2(0.0f, 0.0f), sq = sk;
-#pragma unroll
-      for (int f = 0; f < kFours; ++f)
+      for (int f = 0; f < kFours; ++f) {
+        float2 q[2], k[2];
+        unpack_four<DTYPE>(load_four<DTYPE>(now.q[t], f * 32 + lane * 4, true), q);
+        unpack_four<DTYPE>(load_four<DTYPE>(now.k[t], f * 32 + lane * 4, true), k);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          sk = fma2(S[i][f][e], k[f][e], sk);
-          sq = fma2(S[i][f][e], q[f][e], sq);
+          qq = fma2(q[e], q[e], qq);
+          kk = fma2(k[e], k[e], kk);
+          kq = fma2(k[e], q[e], kq);
         }
-      const float u = beta * fmaf(-alpha, over_lanes(sk.x + sk.y), now.v[i]);
-      out[i] = fmaf(u, k_dot_q, alpha * over_lanes(sq.x + sq.y));
-#pragma unroll
-      for (int f = 0; f < kFours; ++f)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) S[i][f][e] = fma2(make_float2(u, u), k[f][e], mul2(make_float2(alpha, alpha), S[i][f][e]));
+      }
+      const float query = a.use_qk_l2norm ? __fdiv_rn(a.scale, sqrtf(over_lanes(qq.x + qq.y) + kL2Eps)) : a.scale;
+      const float key = a.use_qk_l2norm ? __fdiv_rn(1.0f, sqrtf(over_lanes(kk.x + kk.y) + kL2Eps)) : 1.0f;
+      const float product = over_lanes(kq.x + kq.y) * query * key;
+      if (lane == 0) {
+        factors[t].query = query;
+        factors[t].key = key;
+        factors[t].key_query = product;
+      }
     }
-    const long long at = (long long)(r.first + t) * a.stride_out_tok + (long long)hv * a.V + row0;
+    __syncthreads();
+    gates(t0 + kTokens);
+    long long at = (long long)(r.first + t0) * a.stride_out_tok + (long long)hv * a.V + row0;
+    Four<DTYPE> next_q[kFours], next_k[kFours];
+    auto ahead = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-      if (lane == i) store_from_float(a.out, at + i, a.out_dtype, out[i]);
+      for (int f = 0; f < kFours; ++f) {
+        next_q[f] = load_four<DTYPE>(now.q[t], f * 32 + lane * 4, true);
+        next_k[f] = load_four<DTYPE>(now.k[t], f * 32 + lane * 4, true);
+      }
+    };
+    ahead(0);
+    for (int t = 0; t < n; ++t, at += a.stride_out_tok) {
+      const float4 w = *reinterpret_cast<const float4*>(&factors[t]);
+      const float alpha = w.x, beta = w.y, by_q = w.z, by_k = w.w, k_dot_q = factors[t].key_query;
+      float2 q[kFours][2], k[kFours][2];
+#pragma unroll
+      for (int f = 0; f < kFours; ++f) {
+        unpack_four<DTYPE>(next_q[f], q[f]);
+        unpack_four<DTYPE>(next_k[f], k[f]);
+      }
+      ahead(min(t + 1, kTokens - 1));
+      float sk[ROWS], sq[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        float2 x[2] = {}, y[2] = {};
+#pragma unroll
+        for (int f = 0; f < kFours; ++f)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            x[e] = fma2(S[i][f][e], k[f][e], x[e]);
+            y[e] = fma2(S[i][f][e], q[f][e], y[e]);
+          }
+        const float2 z = add2(x[0], x[1]), o = add2(y[0], y[1]);
+        sk[i] = z.x + z.y;
+        sq[i] = o.x + o.y;
+      }
+      float u[ROWS];
+      if constexpr (ROWS == 4) {
+        // eight sums over eight lanes: lane i is left with row i's product with the key, lane 4 + i with the one with the query
+        const bool second = lane & 4, odd_pair = lane & 2, odd = lane & 1;
+        float four[4], two[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) four[i] = (second ? sq[i] : sk[i]) + __shfl_xor_sync(~0u, second ? sk[i] : sq[i], 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) two[i] = (odd_pair ? four[2 + i] : four[i]) + __shfl_xor_sync(~0u, odd_pair ? four[i] : four[2 + i], 2);
+        const float one = (odd ? two[1] : two[0]) + __shfl_xor_sync(~0u, odd ? two[0] : two[1], 1);
+        const float v = load_as_float(now.v[t], group * ROWS + lane % 4, DTYPE);
+        const float added = beta * fmaf(-alpha * by_k, one, v);                   // of use in lanes 0 .. 3
+        const float given = __shfl_xor_sync(~0u, added, 4);
+        if (second) store_from_float(a.out, at + lane % 4, a.out_dtype, fmaf(given, k_dot_q, alpha * by_q * one));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = __shfl_sync(~0u, added, i, kLanes) * by_k;
+      } else {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          const float added = beta * fmaf(-alpha * by_k, over_lanes(sk[i]), load_as_float(now.v[t], group * ROWS + i, DTYPE));
+          const float out = fmaf(added, k_dot_q, alpha * by_q * over_lanes(sq[i]));
+          if (lane == i) store_from_float(a.out, at + i, a.out_dtype, out);
+          u[i] = added * by_k;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (int f = 0; f < kFours; ++f)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) S[i][f][e] = fma2(make_float2(u[i], u[i]), k[f][e], mul2(make_float2(alpha, alpha), S[i][f][e]));
+    }
+    __syncthreads();
+    if (t0 + 2 * kTokens < r.count) fetch(t0 + 2 * kTokens);
+    __pipeline_commit();
   }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i)
@@ -165,15 +246,14 @@ __global__ void __launch_bounds__(kThreads) recurrent_kernel(const __grid_consta
 template <int DTYPE, int K, int ROWS>
 int launch_rows(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
   constexpr int kSize = DTYPE == CARRY_F32 ? 4 : 2;
-  const bool aligned = reinterpret_cast<uintptr_t>(a.mixed_qkv) % (4 * kSize) == 0 && a.stride_mixed_tok % 4 == 0;
+  const bool aligned = reinterpret_cast<uintptr_t>(a.mixed_qkv) % 16 == 0 && a.stride_mixed_tok * kSize % 16 == 0;
   const dim3 grid((unsigned)(a.V / (kThreads / kLanes * ROWS)), (unsigned)a.HV, (unsigned)a.B);
   return launch_dependent(recurrent_kernel<DTYPE, K, ROWS>, grid, kThreads, 0, stream, a, aligned);
 }
 
 template <int DTYPE, int K>
 int launch_heads(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
-  // one row to a group of lanes while that does not fill the processors with four warps to a scheduler
-  return (long long)a.B * a.HV * a.V / 16 <= 4LL * sm_count() ? launch_rows<DTYPE, K, 1>(a, stream) : launch_rows<DTYPE, K, 4>(a, stream);
+  return delta_rows_alone(a) ? launch_rows<DTYPE, K, 1>(a, stream) : launch_rows<DTYPE, K, 4>(a, stream);
 }
 
 template <int DTYPE>
@@ -182,6 +262,9 @@ int launch_width(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// A row of a state to eight lanes, while that fills the processors with no more than four warps to a scheduler; four rows otherwise.
+bool delta_rows_alone(const CarryGdnPrefillArgs& a) { return (int64_t)a.B * a.HV * a.V / 16 <= 4LL * sm_count(); }
 
 int launch_delta_recurrent(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
   return a.qkv_dtype == CARRY_F32 ? launch_width<CARRY_F32>(a, stream)

@@ -80,8 +80,13 @@ def check(got, c, state, lengths, H, D, l2norm=True, in_chunks=None, rows=None, 
     assert off_state[requests].norm() <= mean.expand_as(off_state[requests]).norm() / D ** 0.5
 
 
+def goes_in_chunks(lengths, dtype, many=False):
+    """The rule by which a call of so many tokens a request goes in chunks; `many`: heads, more than a few hundred."""
+    return max(lengths) > (96 if dtype == F32 else 40 if many else 64)
+
+
 FEW = [[1], [3], [1, 1, 1], [5, 0, 2], [33], [64], [1, 64, 17]]
-MANY = [[65], [128], [1, 0, 64, 65, 3], [200, 77], [191, 1]]
+MANY = [[65], [128], [1, 0, 64, 65, 3], [97, 0, 64, 65, 3], [200, 77], [191, 1]]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -92,7 +97,7 @@ def test_against_recurrence(dtype, D, lengths):
     initial = len(lengths) % 2 == 1
     c, state = make(lengths, H, HV, D, dtype, initial)
     got = run(c, state, lengths, HV, D)
-    in_chunks = max(lengths) > 64
+    in_chunks = goes_in_chunks(lengths, dtype)
     assert _lib.load_library().carry_gdn_last_kernel() == (IN_CHUNKS if in_chunks else TOKEN_BY_TOKEN)
     check(got, c, state, lengths, H, D, in_chunks=in_chunks)
 
@@ -103,7 +108,7 @@ def test_head_maps_and_unnormed_keys(lengths, H, HV):
     for dtype, out_dtype, gates in ((BF16, F32, F32), (F16, BF16, BF16), (F32, F16, F16)):
         c, state = make(lengths, H, HV, 64, dtype, True, l2norm=False, seed=H, gates=gates)
         got = run(c, state, lengths, HV, 64, l2norm=False, out_dtype=out_dtype)
-        check(got, c, state, lengths, H, 64, l2norm=False, in_chunks=max(lengths) > 64)
+        check(got, c, state, lengths, H, 64, l2norm=False, in_chunks=goes_in_chunks(lengths, dtype))
 
 
 @pytest.mark.parametrize("lengths", [[3, 20], [100, 70]], ids=str)
@@ -189,6 +194,15 @@ def test_a_prompt_in_parts_is_the_prompt(dtype):
     check((torch.cat(outs), now), c, state, lengths, H, D, in_chunks=True)
 
 
+def test_many_heads_go_in_chunks_sooner():
+    for n, kernel in ((40, TOKEN_BY_TOKEN), (41, IN_CHUNKS)):
+        c, state = make([n] * 40, 16, 32, 64, BF16, True)
+        got = run(c, state, [n] * 40, 32, 64)
+        assert _lib.load_library().carry_gdn_last_kernel() == kernel
+        part = {k: v[:n] if k in ("mixed_qkv", "a", "b") else v for k, v in c.items()}
+        check((got[0][:n], got[1][:1]), part, state[:1], [n], 16, 64, in_chunks=kernel == IN_CHUNKS)
+
+
 def test_launches_that_share_the_workspace_out():
     """A call too large for the workspace's bound is cut by chunks and by requests: the same numbers as alone."""
     for D, H, HV, lengths in ((128, 4, 32, [4200, 64, 4500, 4097]), (64, 4, 64, [65] * 130 + [129])):
@@ -230,7 +244,7 @@ def test_alike_keys_and_zero_rows():
         check(got, c, state, lengths, H, D, in_chunks=max(lengths) > 64)
 
 
-@pytest.mark.parametrize("dtype,D,H,HV,lengths", [(F32, 64, 2, 4, [65]), (BF16, 128, 8, 16, [300, 77, 64, 500]), (F32, 128, 8, 16, [300, 77, 64, 500]),
+@pytest.mark.parametrize("dtype,D,H,HV,lengths", [(F32, 64, 2, 4, [97]), (BF16, 128, 8, 16, [300, 77, 64, 500]), (F32, 128, 8, 16, [300, 77, 64, 500]),
                                                   (F16, 128, 16, 32, [130] * 20), (BF16, 64, 1, 2, [700]), (BF16, 128, 16, 32, [1000, 1, 90])])
 def test_repeated_calls_give_the_same_numbers(dtype, D, H, HV, lengths):
     """Warps and copies that meet at other times: every call's numbers are the first one's."""
