@@ -76,7 +76,7 @@ struct alignas(16) Factors {
 
 // ROWS of the state to a group of eight lanes
 template <int DTYPE, int K, int ROWS>
-__global__ void __launch_bounds__(kThreads, ROWS == 4 ? 4 : 1) recurrent_kernel(const __grid_constant__ CarryGdnPrefillArgs a, bool aligned) {
+__global__ void __launch_bounds__(kThreads, ROWS == 4 || DTYPE == CARRY_F32 ? 4 : 6) recurrent_kernel(const __grid_constant__ CarryGdnPrefillArgs a, bool aligned) {
   using Tokens = Block<DTYPE, K, ROWS>;
   using Number = typename Tokens::Number;
   constexpr int kFours = K / 32, kRows = Tokens::kRows;

@@ -10,6 +10,8 @@
 // (or the four next to them, where pairs are neighbours or nothing is rotated), so that a row is read once, its sum is a few
 // shuffles, and nothing is exchanged for the rotation.  A warp keeps its token's angles and walks over the token's heads, two rows of 128
 // or four of 64 at a time: the table is read once a token and not once a head.  Few tokens are spread over more warps.
+#include <type_traits>
+
 #include "carry_hybrid.cuh"
 
 namespace carry {
@@ -21,21 +23,34 @@ struct Params {
   CarryGdnRotateArgs a;
   int parts;                      // warps to a token
   float inv_width;
+  int runs_whole, table_whole, weights_whole;     // the runs' frequencies are of one axis; tables and weights can be read a run at a time
   int ends[kMaxAxes];             // first frequency beyond each axis
 };
 
+// VE numbers as they lie in memory, and as fp32
 template <int DTYPE, int VE>
-__device__ __forceinline__ void load_numbers(const void* base, long long at, float (&x)[VE]) {
+struct Run {
+  typename std::conditional<VE == 1, float, typename std::conditional<DTYPE == CARRY_F32, float4, typename std::conditional<VE == 8, uint4, uint2>::type>::type>::type u;
+};
+template <int DTYPE, int VE>
+__device__ __forceinline__ Run<DTYPE, VE> load_run(const void* base, long long at) {
+  Run<DTYPE, VE> r;
+  if constexpr (VE == 1) r.u = load_as_float(base, at, DTYPE);
+  else if constexpr (DTYPE == CARRY_F32) r.u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
+  else r.u = *reinterpret_cast<const decltype(r.u)*>(reinterpret_cast<const uint16_t*>(base) + at);
+  return r;
+}
+template <int DTYPE, int VE>
+__device__ __forceinline__ void numbers_of(const Run<DTYPE, VE>& r, float (&x)[VE]) {
   if constexpr (VE == 1) {
-    x[0] = load_as_float(base, at, DTYPE);
+    x[0] = r.u;
   } else if constexpr (DTYPE == CARRY_F32) {
-    const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
-    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    x[0] = r.u.x; x[1] = r.u.y; x[2] = r.u.z; x[3] = r.u.w;
   } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(base) + at);
-    const uint32_t w[2] = {u.x, u.y};
+    uint32_t w[VE / 2];
+    memcpy(w, &r.u, sizeof(w));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < VE / 2; ++i) {
       if constexpr (DTYPE == CARRY_BF16) {
         x[2 * i] = __uint_as_float(w[i] << 16);
         x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
@@ -54,9 +69,9 @@ __device__ __forceinline__ void store_numbers(void* base, long long at, const fl
   } else if constexpr (DTYPE == CARRY_F32) {
     *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + at) = make_float4(x[0], x[1], x[2], x[3]);
   } else {
-    uint32_t w[2];
+    uint32_t w[VE / 2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < VE / 2; ++i) {
       if constexpr (DTYPE == CARRY_BF16) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
         w[i] = *reinterpret_cast<const uint32_t*>(&v);
@@ -65,7 +80,27 @@ __device__ __forceinline__ void store_numbers(void* base, long long at, const fl
         w[i] = *reinterpret_cast<const uint32_t*>(&v);
       }
     }
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(base) + at) = make_uint2(w[0], w[1]);
+    if constexpr (VE == 8) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(base) + at) = make_uint2(w[0], w[1]);
+  }
+}
+
+// VE numbers of a table or a weight, whose type is the call's; `whole`: on the grid of VE numbers
+template <int VE>
+__device__ __forceinline__ void load_factors(const void* base, long long at, int dtype, bool whole, float (&x)[VE]) {
+  if (VE == 1 || !whole) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x[e] = load_as_float(base, at + e, dtype);
+  } else if (dtype == CARRY_F32) {
+#pragma unroll
+    for (int e = 0; e < VE; e += 4) {
+      const Run<CARRY_F32, 4> r = load_run<CARRY_F32, 4>(base, at + e);
+      x[e] = r.u.x; x[e + 1] = r.u.y; x[e + 2] = r.u.z; x[e + 3] = r.u.w;
+    }
+  } else if (dtype == CARRY_BF16) {
+    numbers_of<CARRY_BF16, VE>(load_run<CARRY_BF16, VE>(base, at), x);
+  } else {
+    numbers_of<CARRY_F16, VE>(load_run<CARRY_F16, VE>(base, at), x);
   }
 }
 
@@ -76,18 +111,50 @@ __device__ __forceinline__ float sum_over(float x) {
   return x;
 }
 
-// LANES to a row, each with UNITS times two runs of VE numbers.  VE is 4, or 1 where widths, strides or addresses are off the grid of
-// four numbers.
+// LANES to a row, each with UNITS times two runs of VE numbers: of 16 bytes, of four numbers or of one, as widths, strides and addresses allow.
 template <int DTYPE, int VE, int LANES, int UNITS>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant__ Params p) {
-  constexpr int kRows = 32 / LANES;               // of a warp, at a time
+  constexpr int kRows = 32 / LANES, kBatch = VE == 1 ? 1 : VE == 8 ? 2 : 4 / UNITS;   // rows of a warp at a time; how many times
   const CarryGdnRotateArgs& a = p.a;
   depend_release();
   depend_wait();
   const long long item = (long long)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-  const int token = (int)(item / p.parts), part = (int)(item % p.parts);
-  if (token >= a.N) return;
+  const int token = (int)item, part = blockIdx.y;
+  if (item >= a.N) return;
   const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES, half = a.rotary / 2, units = a.D / (2 * VE), turned = half / VE;
+
+  int first[UNITS], second[UNITS];                // where this lane's runs begin
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int unit = lane + u * LANES;
+    const bool apart = unit < turned && !a.interleaved;
+    first[u] = apart ? unit * VE : unit * 2 * VE;
+    second[u] = apart ? half + unit * VE : unit * 2 * VE + VE;
+  }
+  // the warp's share of the heads, and a batch of rows under way; the first one does not wait for the angles
+  struct Heads {
+    const void *in, *weight;
+    void* out;
+    int from, to;
+    long long in_tok, in_head, out_tok, out_head;
+  };
+  const int each_q = (a.HQ + p.parts - 1) / p.parts, each_k = (a.HK + p.parts - 1) / p.parts;
+  const Heads side[2] = {{a.q, a.q_weight, a.q_out, part * each_q, min((part + 1) * each_q, a.HQ), a.stride_q_tok, a.stride_q_head, a.stride_q_out_tok, a.stride_q_out_head},
+                         {a.k, a.k_weight, a.k_out, part * each_k, min((part + 1) * each_k, a.HK), a.stride_k_tok, a.stride_k_head, a.stride_k_out_tok, a.stride_k_out_head}};
+  Run<DTYPE, VE> rows[kBatch][UNITS][2];
+  auto bring = [&](const Heads& s, int h0) {
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n)
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int h = h0 + n * kRows + group;
+        if (h >= s.to || lane + u * LANES >= units) continue;
+        const long long at = token * s.in_tok + h * s.in_head;
+        rows[n][u][0] = load_run<DTYPE, VE>(s.in, at + first[u]);
+        rows[n][u][1] = load_run<DTYPE, VE>(s.in, at + second[u]);
+      }
+  };
+  bring(side[0], side[0].from);
 
   // the token's place on each axis; one without a place is left alone
   long long place[kMaxAxes];
@@ -104,113 +171,120 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   if (bad && a.status && part == 0 && threadIdx.x % 32 == 0) atomicOr(a.status, CARRY_GDN_STATUS_BAD_RANGE);
   if (!there) return;
 
-  int first[UNITS], second[UNITS];                // where this lane's runs begin
   float cosine[UNITS][VE], sine[UNITS][VE];       // of its pairs; 1 and 0 where nothing is turned
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
     const int unit = lane + u * LANES;
-    const bool turns = unit < turned;
-    const bool apart = turns && !a.interleaved;
-    first[u] = apart ? unit * VE : unit * 2 * VE;
-    second[u] = apart ? half + unit * VE : unit * 2 * VE + VE;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       cosine[u][e] = 1.0f;
       sine[u][e] = 0.0f;
-      if (!turns) continue;
-      const int f = unit * VE + e;
+    }
+    if (unit >= turned) continue;
+    auto row_of = [&](int f) {
       long long row = place[0];
 #pragma unroll
       for (int i = 1; i < kMaxAxes; ++i)
         if (i < a.axes && f >= p.ends[i - 1]) row = place[i];
-      cosine[u][e] = load_as_float(a.cos_sin, row * a.stride_table + f, a.table_dtype);
-      sine[u][e] = load_as_float(a.cos_sin, row * a.stride_table + half + f, a.table_dtype);
+      return row * a.stride_table;
+    };
+    if (p.runs_whole) {                           // a run's frequencies are of one axis
+      const long long at = row_of(unit * VE) + unit * VE;
+      load_factors<VE>(a.cos_sin, at, a.table_dtype, p.table_whole, cosine[u]);
+      load_factors<VE>(a.cos_sin, at + half, a.table_dtype, p.table_whole, sine[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const int f = unit * VE + e;
+        const long long at = row_of(f) + f;
+        cosine[u][e] = load_as_float(a.cos_sin, at, a.table_dtype);
+        sine[u][e] = load_as_float(a.cos_sin, at + half, a.table_dtype);
+      }
     }
   }
 
 #pragma unroll
   for (int which = 0; which < 2; ++which) {       // queries, then keys
-    const void* in = which ? a.k : a.q;
-    void* out = which ? a.k_out : a.q_out;
-    const void* weight = which ? a.k_weight : a.q_weight;
-    const int heads = which ? a.HK : a.HQ, each = (heads + p.parts - 1) / p.parts, from = part * each, to = min(from + each, heads);
-    const long long in_tok = which ? a.stride_k_tok : a.stride_q_tok, in_head = which ? a.stride_k_head : a.stride_q_head;
-    const long long out_tok = which ? a.stride_k_out_tok : a.stride_q_out_tok, out_head = which ? a.stride_k_out_head : a.stride_q_out_head;
-    if (from >= to) continue;
+    const Heads& s = side[which];
+    if (s.from >= s.to) continue;
     float w[UNITS][2][VE];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       if (lane + u * LANES >= units) continue;
+      load_factors<VE>(s.weight, first[u], a.weight_dtype, p.weights_whole, w[u][0]);
+      load_factors<VE>(s.weight, second[u], a.weight_dtype, p.weights_whole, w[u][1]);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        w[u][0][e] = load_as_float(weight, first[u] + e, a.weight_dtype) + a.weight_offset;
-        w[u][1][e] = load_as_float(weight, second[u] + e, a.weight_dtype) + a.weight_offset;
+        w[u][0][e] += a.weight_offset;
+        w[u][1][e] += a.weight_offset;
       }
     }
-#pragma unroll 4
-    for (int h0 = from; h0 < to; h0 += kRows) {
-      const int h = h0 + group;
-      const bool mine = h < to;
-      float x[UNITS][2][VE], sum = 0.0f;
+    for (int h0 = s.from; h0 < s.to; h0 += kRows * kBatch) {
+      if (which > 0 || h0 > s.from) bring(s, h0);
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
+      for (int n = 0; n < kBatch; ++n) {
+        const int h = h0 + n * kRows + group;
+        const bool mine = h < s.to;
+        if (h0 + n * kRows >= s.to) break;        // the same for all lanes
+        float x[UNITS][2][VE], sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) x[u][0][e] = x[u][1][e] = 0.0f;
-        if (!mine || lane + u * LANES >= units) continue;
-        const long long at = token * in_tok + h * in_head;
-        load_numbers<DTYPE, VE>(in, at + first[u], x[u][0]);
-        load_numbers<DTYPE, VE>(in, at + second[u], x[u][1]);
+        for (int u = 0; u < UNITS; ++u) {
+          numbers_of<DTYPE, VE>(rows[n][u][0], x[u][0]);
+          numbers_of<DTYPE, VE>(rows[n][u][1], x[u][1]);
+          if (!mine || lane + u * LANES >= units) continue;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) sum = fmaf(x[u][1][e], x[u][1][e], fmaf(x[u][0][e], x[u][0][e], sum));
-      }
-      sum = sum_over<LANES>(sum);
-      float by = rsqrtf(fmaf(sum, p.inv_width, a.eps)), unit = 1.0f;
-      if (__any_sync(~0u, sum == INFINITY)) {
-        // squares beyond fp32: once more, in units of 2^100 (an infinity among the numbers makes the row NaN)
-        float less = 0.0f;
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float s = x[u][0][e] * 0x1p-100f, t = x[u][1][e] * 0x1p-100f;
-            less = fmaf(t, t, fmaf(s, s, less));
-          }
-        less = sum_over<LANES>(less);
-        if (sum == INFINITY) {
-          by = less == INFINITY ? NAN : rsqrtf(less * p.inv_width);
-          unit = 0x1p-100f;
+          for (int e = 0; e < VE; ++e) sum = fmaf(x[u][1][e], x[u][1][e], fmaf(x[u][0][e], x[u][0][e], sum));
         }
-      }
-      if (!mine) continue;
-      const long long to_at = token * out_tok + h * out_head;
+        sum = sum_over<LANES>(sum);
+        float by = rsqrtf(fmaf(sum, p.inv_width, a.eps)), unit = 1.0f;
+        if (__any_sync(~0u, sum == INFINITY)) {
+          // squares beyond fp32: once more, in units of 2^100 (an infinity among the numbers makes the row NaN)
+          float less = 0.0f;
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        if (lane + u * LANES >= units) continue;
-        float y[2][VE], z[2][VE];
+          for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          y[0][e] = x[u][0][e] * unit * by * w[u][0][e];
-          y[1][e] = x[u][1][e] * unit * by * w[u][1][e];
-        }
-        if (lane + u * LANES >= turned) {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) { z[0][e] = y[0][e]; z[1][e] = y[1][e]; }
-        } else if (a.interleaved && VE > 1) {     // the run's numbers 2i and 2i + 1 are pair i, over both runs
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float one = y[2 * e / VE][2 * e % VE], two = y[2 * e / VE][(2 * e + 1) % VE];
-            z[2 * e / VE][2 * e % VE] = one * cosine[u][e] - two * sine[u][e];
-            z[2 * e / VE][(2 * e + 1) % VE] = two * cosine[u][e] + one * sine[u][e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            z[0][e] = y[0][e] * cosine[u][e] - y[1][e] * sine[u][e];
-            z[1][e] = y[1][e] * cosine[u][e] + y[0][e] * sine[u][e];
+            for (int e = 0; e < VE; ++e) {
+              if (lane + u * LANES >= units) continue;
+              const float s0 = x[u][0][e] * 0x1p-100f, s1 = x[u][1][e] * 0x1p-100f;
+              less = fmaf(s1, s1, fmaf(s0, s0, less));
+            }
+          less = sum_over<LANES>(less);
+          if (sum == INFINITY) {
+            by = less == INFINITY ? NAN : rsqrtf(less * p.inv_width);
+            unit = 0x1p-100f;
           }
         }
-        store_numbers<DTYPE, VE>(out, to_at + first[u], z[0]);
-        store_numbers<DTYPE, VE>(out, to_at + second[u], z[1]);
+        if (!mine) continue;
+        const long long to_at = token * s.out_tok + h * s.out_head;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          if (lane + u * LANES >= units) continue;
+          float y[2][VE], z[2][VE];
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            y[0][e] = x[u][0][e] * unit * by * w[u][0][e];
+            y[1][e] = x[u][1][e] * unit * by * w[u][1][e];
+          }
+          if (lane + u * LANES >= turned) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) { z[0][e] = y[0][e]; z[1][e] = y[1][e]; }
+          } else if (a.interleaved && VE > 1) {   // the run's numbers 2i and 2i + 1 are pair i, over both runs
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const float one = y[2 * e / VE][2 * e % VE], two = y[2 * e / VE][(2 * e + 1) % VE];
+              z[2 * e / VE][2 * e % VE] = one * cosine[u][e] - two * sine[u][e];
+              z[2 * e / VE][(2 * e + 1) % VE] = two * cosine[u][e] + one * sine[u][e];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              z[0][e] = y[0][e] * cosine[u][e] - y[1][e] * sine[u][e];
+              z[1][e] = y[1][e] * cosine[u][e] + y[0][e] * sine[u][e];
+            }
+          }
+          store_numbers<DTYPE, VE>(s.out, to_at + first[u], z[0]);
+          store_numbers<DTYPE, VE>(s.out, to_at + second[u], z[1]);
+        }
       }
     }
   }
@@ -218,26 +292,45 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
 
 template <int DTYPE, int VE, int LANES, int UNITS>
 int launch(Params p, cudaStream_t stream) {
-  // warps to a token: enough for twelve on a processor, a row at a time at least
+  const auto whole = [](const void* t, int64_t stride, int dtype) {
+    const int n = dtype == CARRY_F32 && VE > 4 ? 4 : VE, size = dtype == CARRY_F32 ? 4 : 2;
+    return reinterpret_cast<uintptr_t>(t) % (n * size) == 0 && stride % n == 0;
+  };
+  p.runs_whole = 1;
+  for (int i = 0; i < p.a.axes; ++i) p.runs_whole = p.runs_whole && p.ends[i] % VE == 0;
+  p.table_whole = whole(p.a.cos_sin, p.a.stride_table, p.a.table_dtype);
+  p.weights_whole = whole(p.a.q_weight, 0, p.a.weight_dtype) && whole(p.a.k_weight, 0, p.a.weight_dtype);
+  // warps to a token: enough for 64 on a processor, a row at a time at least
   const int most = (p.a.HQ + 32 / LANES - 1) / (32 / LANES);
-  const long long wanted = (12LL * sm_count() + p.a.N - 1) / p.a.N;
+  const long long wanted = (64LL * sm_count() + p.a.N - 1) / p.a.N;
   p.parts = (int)(wanted < most ? wanted : most);
   if (p.parts < 1) p.parts = 1;
-  const long long ctas = ((long long)p.a.N * p.parts + kThreads / 32 - 1) / (kThreads / 32);
-  if (ctas > 0x7fffffff) return CARRY_GDN_ERR_TOO_LARGE;
-  return launch_dependent(rotate_kernel<DTYPE, VE, LANES, UNITS>, dim3((unsigned)ctas), kThreads, 0, stream, p);
+  const long long ctas = ((long long)p.a.N + kThreads / 32 - 1) / (kThreads / 32);
+  return launch_dependent(rotate_kernel<DTYPE, VE, LANES, UNITS>, dim3((unsigned)ctas, (unsigned)p.parts), kThreads, 0, stream, p);
 }
 
 template <int DTYPE>
 int launch_width(const Params& p, cudaStream_t stream) {
   const CarryGdnRotateArgs& a = p.a;
   constexpr int kSize = DTYPE == CARRY_F32 ? 4 : 2;
-  bool grid = a.D % 8 == 0 && a.rotary % 8 == 0;
-  for (const void* t : {a.q, a.k, (const void*)a.q_out, (const void*)a.k_out}) grid = grid && reinterpret_cast<uintptr_t>(t) % (4 * kSize) == 0;
-  for (int64_t s : {a.stride_q_tok, a.stride_q_head, a.stride_k_tok, a.stride_k_head, a.stride_q_out_tok, a.stride_q_out_head, a.stride_k_out_tok,
-                    a.stride_k_out_head})
-    grid = grid && s % 4 == 0;
-  if (!grid) return launch<DTYPE, 1, 32, 8>(p, stream);
+  // runs of `n` numbers: 16 bytes, or 8 where widths, strides or addresses do not allow it
+  auto fits = [&](int n) {
+    bool yes = a.D % (2 * n) == 0 && a.rotary % (2 * n) == 0;
+    for (const void* t : {a.q, a.k, (const void*)a.q_out, (const void*)a.k_out}) yes = yes && reinterpret_cast<uintptr_t>(t) % (n * kSize) == 0;
+    for (int64_t s : {a.stride_q_tok, a.stride_q_head, a.stride_k_tok, a.stride_k_head, a.stride_q_out_tok, a.stride_q_out_head, a.stride_k_out_tok,
+                      a.stride_k_out_head})
+      yes = yes && s % n == 0;
+    return yes;
+  };
+  if constexpr (kSize == 2) {
+    if (fits(8)) {
+      if (a.D <= 64) return launch<DTYPE, 8, 4, 1>(p, stream);
+      if (a.D <= 128) return launch<DTYPE, 8, 8, 1>(p, stream);
+      if (a.D <= 256) return launch<DTYPE, 8, 16, 1>(p, stream);
+      return launch<DTYPE, 8, 32, 1>(p, stream);
+    }
+  }
+  if (!fits(4)) return launch<DTYPE, 1, 32, 8>(p, stream);
   if (a.D <= 64) return launch<DTYPE, 4, 8, 1>(p, stream);
   if (a.D <= 128) return launch<DTYPE, 4, 16, 1>(p, stream);
   if (a.D <= 256) return launch<DTYPE, 4, 32, 1>(p, stream);
@@ -247,7 +340,7 @@ int launch_width(const Params& p, cudaStream_t stream) {
 }  // namespace
 
 int launch_rotate(const CarryGdnRotateArgs& a, cudaStream_t stream) {
-  Params p = {a, 1, 1.0f / a.D, {}};
+  Params p = {a, 1, 1.0f / a.D, 0, 0, 0, {}};
   for (int i = 0, end = 0; i < kMaxAxes; ++i) p.ends[i] = end += i < a.axes ? a.sections[i] : 0;
   return a.dtype == CARRY_F32 ? launch_width<CARRY_F32>(p, stream)
          : a.dtype == CARRY_BF16 ? launch_width<CARRY_BF16>(p, stream) : launch_width<CARRY_F16>(p, stream);
