@@ -807,15 +807,17 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
 constexpr int kColumns = 32;                      // of the state to a CTA
 
 // Right sides lie with their three terms side by side, so that one product takes all terms and reads its left side once: two of them in a
-// plane of 64 columns, the third in the first half of another one.  The second half of the state's other plane has the third term of R and U.
+// plane of 64 columns, the third in the first half of another one.  Where two CTAs share a processor, the second half of the state's other plane
+// has the third term of R and U.
 template <int DTYPE, int D, int STAGES>
 struct SequenceShared {
+  static constexpr bool kAlone = STAGES == 2;
   uint8_t kq[STAGES][kTermsX<DTYPE>][D / 64][kPlane], t[STAGES][kTermsT<DTYPE>][kPlane];
-  uint8_t u[kChunk * 128], s[2][D * 128];         // R, and then U with its decays; the state
-  alignas(16) uint8_t v[STAGES][kChunk][kColumns * (DTYPE == CARRY_F32 ? 4 : 2)];
+  uint8_t u[kAlone ? 2 : 1][kChunk * 128], s[2][D * 128];     // R, and then U with its decays; the state
+  alignas(16) uint8_t v[kAlone ? 1 : kChunk][kColumns * (DTYPE == CARRY_F32 ? 4 : 2)];
   alignas(16) float vec[2][kVec];
-  // what has come, and what is free again: keys, queries, T and values are each asked for again as soon as they have been used
-  uint64_t k_full[STAGES], q_full[STAGES], t_full[STAGES], v_full[STAGES], vec_full[2], k_free[STAGES], q_free[STAGES], t_free[STAGES], v_free[STAGES];
+  // what has come, and what is free again: with one stage keys, queries, T and values are each asked for again as soon as they have been used
+  uint64_t full[STAGES], free[STAGES], q_full, t_full, v_full, vec_full[2], q_free, t_free, v_free;
   uint64_t s_ready, r_ready, u_ready, scored, solved, added;
   uint32_t tmem;
   int poison;
@@ -836,12 +838,14 @@ __device__ __forceinline__ void load_sums(uint32_t at, float2 (&x)[W / 2]) {
   for (int j = 0; j < W; j += 2) x[j / 2] = add2(add2(two(2, j), two(1, j)), two(0, j));
 }
 
-// GROUPS of 128 threads share a row's columns.  With two stages of operands a CTA has a processor for itself; with one, two of them share it.
+// GROUPS of 128 threads share a row's columns.  With two stages of operands a CTA has a processor for itself, and what counts is the chain of a
+// chunk's products; with one, two CTAs share a processor, and what one waits for the other uses.
 template <int DTYPE, int D, int GROUPS, int STAGES>
 __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CARRY_BF16 ? 2 : 1) sequence_kernel(const __grid_constant__ ChunkParams p) {
   constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64, W = kColumns / GROUPS;
   constexpr int kRowThreads = GROUPS * 128, kLoadWarp = kRowThreads / 32, kIssueWarp = kLoadWarp + 1, kValueBytes = DTYPE == CARRY_F32 ? 4 : 2;
   using Shared = SequenceShared<DTYPE, D, STAGES>;
+  constexpr bool kAlone = Shared::kAlone;
   extern __shared__ uint8_t raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
   depend_release();
@@ -854,10 +858,12 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
   if (tid == 0) {
     sh.poison = 0;
     for (int i = 0; i < STAGES; ++i) {
-      for (uint64_t* bar : {&sh.k_full[i], &sh.q_full[i], &sh.t_full[i], &sh.k_free[i], &sh.q_free[i], &sh.t_free[i]}) barrier_init(bar, 1);
-      barrier_init(&sh.v_full[i], 32);
-      barrier_init(&sh.v_free[i], kRowThreads / 2);
+      barrier_init(&sh.full[i], 1);
+      barrier_init(&sh.free[i], 1);
     }
+    for (uint64_t* bar : {&sh.q_full, &sh.t_full, &sh.q_free, &sh.t_free}) barrier_init(bar, 1);
+    barrier_init(&sh.v_full, 32);
+    barrier_init(&sh.v_free, kRowThreads / 2);
     barrier_init(&sh.vec_full[0], 1);
     barrier_init(&sh.vec_full[1], 1);
     barrier_init(&sh.s_ready, kRowThreads);
@@ -886,6 +892,8 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
     const int row = warp % 4 * 32 + lane, first = warp / 4 * W, column0 = blockIdx.x * kColumns + first, token = row % kChunk;
     const uint32_t at = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + first;
     const bool key = row < kChunk, has_state = row < D;
+    uint8_t* const third = kAlone ? sh.u[kAlone] : sh.s[1];   // where R's and U's third term lies, and its first column there
+    constexpr int kThirdColumn = kAlone ? 0 : kColumns;
     // this thread's numbers into an operand's terms; `last`: of the third one
     auto put = [&](uint8_t* tile, uint8_t* last, int last_column, float2 (&x)[W / 2]) {
 #pragma unroll
@@ -917,36 +925,59 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       fence_before();
       barrier_arrive(&sh.s_ready);
     };
-    bool healthy = true;
-    if (chunks > 0) put_state();
-    for (int c = 0; c < chunks; ++c) {
-      const int parity = c & 1, stage = c % STAGES;
-      healthy = wait(&sh.vec_full[parity], c / 2 & 1) && (!key || wait(&sh.v_full[stage], c / STAGES & 1));    // only keys' threads hold the values back
-      if (!healthy) break;
-      const float* vec = sh.vec[parity];
-      const float of_state = key ? -vec[token] : vec[3 * kChunk + token], beta = vec[kChunk + token], of_added = vec[2 * kChunk + token], decay = vec[4 * kChunk];
-      float2 x[W / 2], o[W / 2];                  // o: a key's beta v; a query's part of the output that comes from the state
-      if (key) {
-        const bool there = c * kChunk + token < left;       // behind the last token lies what an earlier chunk had
+    // A chunk's factors, and a key's beta v.  Values come from memory into registers a chunk ahead, or, where that would be in the other
+    // CTA's way, into shared memory.
+    float of_state = 0.0f, of_added = 0.0f, next_decay = 0.0f;
+    float2 o[W / 2];                              // a key's beta v; a query's part of the output that comes from the state
+    Raw<DTYPE> v[W / 8];
+    auto fetch = [&](int c) {
+      const int i = c * kChunk + token;
 #pragma unroll
-        for (int j = 0; j < W; j += 8) {
-          const Eight e = unpack<DTYPE>(load_raw<DTYPE>(sh.v[stage][token], first + j));
+      for (int j = 0; j < W / 8; ++j)
+        if (key && i < left) v[j] = load_row<DTYPE>(a.mixed_qkv, (long long)(place.first + from + i) * a.stride_mixed_tok + (2 * a.H + hv) * D + column0 + j * 8, p.aligned);
+    };
+    auto begin = [&](int c) {
+      if (!wait(kAlone ? &sh.full[c % STAGES] : &sh.vec_full[c & 1], c / 2 & 1)) return false;
+      const float* vec = sh.vec[c & 1];
+      of_state = key ? -vec[token] : vec[3 * kChunk + token];
+      of_added = vec[2 * kChunk + token];
+      next_decay = vec[4 * kChunk];
+      if (!key) return true;                      // only keys' threads hold the values back
+      const float beta = vec[kChunk + token];
+      if (!kAlone && !wait(&sh.v_full, c & 1)) return false;
+      const bool there = c * kChunk + token < left;         // behind the last token lies what an earlier chunk had
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[j / 2 + k] = there ? mul2(e.x[k], make_float2(beta, beta)) : make_float2(0.0f, 0.0f);
-        }
+      for (int j = 0; j < W; j += 8) {
+        if (!kAlone) v[j / 8] = load_raw<DTYPE>(sh.v[kAlone ? 0 : token], first + j);
+        const Eight e = unpack<DTYPE>(v[j / 8]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[j / 2 + k] = there ? mul2(e.x[k], make_float2(beta, beta)) : make_float2(0.0f, 0.0f);
       }
-      healthy = wait(&sh.scored, parity);
+      return true;
+    };
+    bool healthy = true;
+    if (chunks > 0) {
+      if (kAlone) fetch(0);
+      else healthy = begin(0);
+      put_state();
+    }
+    for (int c = 0; c < chunks && healthy; ++c) {
+      const int parity = c & 1;
+      float2 x[W / 2];
+      if (kAlone) healthy = begin(c);
+      healthy = healthy && wait(&sh.scored, parity);
       if (!healthy) break;
       fence_after();
       load_sums<W>(at, x);
       if (key) {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = fma2(make_float2(of_state, of_state), x[j], o[j]);
-        put(sh.u, sh.s[1], kColumns, x);
+        put(sh.u[0], third, kThirdColumn, x);
         fence_proxy();
         fence_before();
         barrier_arrive(&sh.r_ready);
-        barrier_arrive(&sh.v_free[stage]);        // not before the values have been used: a load that is merely under way may be overtaken by the next copy
+        if (kAlone && c + 1 < chunks) fetch(c + 1);
+        if (!kAlone) barrier_arrive(&sh.v_free);  // not before the values have been used: a load that is merely under way may be overtaken by the next copy
       } else {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) o[j] = mul2(make_float2(of_state, of_state), x[j]);
@@ -960,37 +991,43 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       if (key) {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = mul2(make_float2(of_added, of_added), x[j]);
-        put(sh.u, sh.s[1], kColumns, x);
+        put(sh.u[0], third, kThirdColumn, x);
         fence_proxy();
         fence_before();
         barrier_arrive(&sh.u_ready);
-      } else if (c * kChunk + token < left) {
-        const long long to = (long long)(place.first + from + c * kChunk + token) * a.stride_out_tok + hv * D + column0;
+      } else {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = add2(x[j], o[j]);
-        if (p.out_aligned) {
+        if (!kAlone) healthy = wait(&sh.u_ready, parity);   // stores that are under way hold up the fences of the keys' threads, all the more of two CTAs'
+        if (!healthy) break;
+        if (c * kChunk + token < left) {
+          const long long to = (long long)(place.first + from + c * kChunk + token) * a.stride_out_tok + hv * D + column0;
+          if (p.out_aligned) {
 #pragma unroll
-          for (int j = 0; j < W / 2; j += 4) {
-            if (a.out_dtype == CARRY_F32) {
-              float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + to + 2 * j);
-              q[0] = make_float4(x[j].x, x[j].y, x[j + 1].x, x[j + 1].y);
-              q[1] = make_float4(x[j + 2].x, x[j + 2].y, x[j + 3].x, x[j + 3].y);
-            } else {
-              uint32_t w[4];
+            for (int j = 0; j < W / 2; j += 4) {
+              if (a.out_dtype == CARRY_F32) {
+                float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + to + 2 * j);
+                q[0] = make_float4(x[j].x, x[j].y, x[j + 1].x, x[j + 1].y);
+                q[1] = make_float4(x[j + 2].x, x[j + 2].y, x[j + 3].x, x[j + 3].y);
+              } else {
+                uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __half2 y = __float22half2_rn(x[j + e]);
-                w[e] = a.out_dtype == CARRY_BF16 ? pack_bf16(x[j + e].x, x[j + e].y) : *reinterpret_cast<const uint32_t*>(&y);
+                for (int e = 0; e < 4; ++e) {
+                  const __half2 y = __float22half2_rn(x[j + e]);
+                  w[e] = a.out_dtype == CARRY_BF16 ? pack_bf16(x[j + e].x, x[j + e].y) : *reinterpret_cast<const uint32_t*>(&y);
+                }
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + to + 2 * j) = make_uint4(w[0], w[1], w[2], w[3]);
               }
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + to + 2 * j) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          }
-        } else {
+          } else {
 #pragma unroll
-          for (int j = 0; j < W; ++j) store_from_float(a.out, to + j, a.out_dtype, j % 2 ? x[j / 2].y : x[j / 2].x);
+            for (int j = 0; j < W; ++j) store_from_float(a.out, to + j, a.out_dtype, j % 2 ? x[j / 2].y : x[j / 2].x);
+          }
         }
       }
-      healthy = wait(&sh.added, parity);
+      const float decay = next_decay;
+      if (!kAlone && c + 1 < chunks) healthy = begin(c + 1);
+      healthy = healthy && wait(&sh.added, parity);
       if (!healthy) break;
       fence_after();
       load_sums<W>(at, x);
@@ -1006,59 +1043,72 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
   } else if (warp == kLoadWarp) {
     // ---- tiles and factors out of the workspace, values out of the rows ----
     constexpr uint32_t kBytesKq = kX * kPlanes * kPlane, kBytesT = kT * kPlane, kSide = kPlane / 2, kBytesV = kColumns * kValueBytes;
-    auto sides = [&](int c, int side, uint64_t* bar) {      // keys or queries: a half of every plane
-      const uint8_t* tile = p.kq + ((place.slot0 + c) * a.H + h) * kBytesKq;
-      barrier_expect(bar, kBytesKq / 2);
-      for (int i = side * kSide; i < (int)kBytesKq; i += kPlane) bulk_copy(sh.kq[c % STAGES][0][0] + i, tile + i, kSide, bar);
-    };
     for (int c = 0; c < chunks; ++c) {
-      const int stage = c % STAGES, tokens = min(left - c * kChunk, kChunk);
+      const int stage = c % STAGES;
       const bool reused = c >= STAGES;
       const uint32_t turn = (c / STAGES - 1) & 1;           // of the use before
+      const uint8_t* tile = p.kq + ((place.slot0 + c) * a.H + h) * kBytesKq;
       const long long place_hv = (place.slot0 + c) * a.HV + hv;
+      if constexpr (kAlone) {
+        if (reused && !wait(&sh.free[stage], turn)) break;
+        if (lane == 0) {
+          barrier_expect(&sh.full[stage], kBytesKq + kBytesT + kVec * 4);
+          bulk_copy(sh.vec[stage], p.vec + place_hv * kVec, kVec * 4, &sh.full[stage]);
+          bulk_copy(sh.kq[stage], tile, kBytesKq, &sh.full[stage]);
+          bulk_copy(sh.t[stage], p.t + place_hv * kBytesT, kBytesT, &sh.full[stage]);
+        }
+        __syncwarp();
+        continue;
+      }
+      auto side = [&](int which, uint64_t* bar) {           // keys or queries: a half of every plane
+        barrier_expect(bar, kBytesKq / 2);
+        for (int i = which * kSide; i < (int)kBytesKq; i += kPlane) bulk_copy(sh.kq[0][0][0] + i, tile + i, kSide, bar);
+      };
       // in the order in which what was there is done with
-      if (reused && !wait(&sh.v_free[stage], turn)) break;
+      if (reused && !wait(&sh.v_free, turn)) break;
+      const int tokens = min(left - c * kChunk, kChunk);
       const long long at = (long long)(place.first + from + c * kChunk) * a.stride_mixed_tok + (2 * a.H + hv) * D + blockIdx.x * kColumns;
       if (p.aligned) {                            // sixteen bytes at a time: bulk copies of such short rows would hold up the tiles'
         for (int i = lane; i < tokens * (int)(kBytesV / 16); i += 32) {
           const int token = i / (kBytesV / 16), part = i % (kBytesV / 16) * 16;
-          __pipeline_memcpy_async(sh.v[stage][token] + part, reinterpret_cast<const uint8_t*>(a.mixed_qkv) + (at + token * a.stride_mixed_tok) * kValueBytes + part, 16);
+          __pipeline_memcpy_async(sh.v[token] + part, reinterpret_cast<const uint8_t*>(a.mixed_qkv) + (at + token * a.stride_mixed_tok) * kValueBytes + part, 16);
         }
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&sh.v_full[stage])) : "memory");
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&sh.v_full)) : "memory");
       } else {
         for (int i = 0; i < tokens; ++i) {
-          if constexpr (kValueBytes == 4) reinterpret_cast<float*>(sh.v[stage][i])[lane] = reinterpret_cast<const float*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
-          else reinterpret_cast<uint16_t*>(sh.v[stage][i])[lane] = reinterpret_cast<const uint16_t*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
+          if constexpr (kValueBytes == 4) reinterpret_cast<float*>(sh.v[i])[lane] = reinterpret_cast<const float*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
+          else reinterpret_cast<uint16_t*>(sh.v[i])[lane] = reinterpret_cast<const uint16_t*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
         }
-        barrier_arrive(&sh.v_full[stage]);
+        barrier_arrive(&sh.v_full);
       }
-      if (reused && !wait(&sh.q_free[stage], turn)) break;
-      if (lane == 0) sides(c, 1, &sh.q_full[stage]);
-      __syncwarp();
-      if (reused && !wait(&sh.t_free[stage], turn)) break;
+      if (reused && !wait(&sh.q_free, turn)) break;
       if (lane == 0) {
-        barrier_expect(&sh.t_full[stage], kBytesT);
-        bulk_copy(sh.t[stage], p.t + place_hv * kBytesT, kBytesT, &sh.t_full[stage]);
-      }
-      __syncwarp();
-      if (reused && !wait(&sh.k_free[stage], turn)) break;  // after which nobody reads the factors of the chunk before the last
-      if (lane == 0) {
+        // [K; Q] S of the chunk before is done: the state that it took was ready, and the factors of the chunk before that had been read by then
         barrier_expect(&sh.vec_full[c & 1], kVec * 4);
         bulk_copy(sh.vec[c & 1], p.vec + place_hv * kVec, kVec * 4, &sh.vec_full[c & 1]);
-        sides(c, 0, &sh.k_full[stage]);
+        side(1, &sh.q_full);
       }
+      __syncwarp();
+      if (reused && !wait(&sh.t_free, turn)) break;
+      if (lane == 0) {
+        barrier_expect(&sh.t_full, kBytesT);
+        bulk_copy(sh.t[0], p.t + place_hv * kBytesT, kBytesT, &sh.t_full);
+      }
+      __syncwarp();
+      if (reused && !wait(&sh.free[0], turn)) break;
+      if (lane == 0) side(0, &sh.full[0]);
       __syncwarp();
     }
   } else {
     // ---- products: a left side's term x with the right side's terms 0 .. kTerms - 1 - x, which are its next columns ----
     const uint32_t elected = elect(), base = __shfl_sync(~0u, tmem, 0);
     // the third term lies that far behind the first two
-    const uint32_t state = operand(sh.s[0], D * 128), rows = operand(sh.u, smem_addr(sh.s[1]) + kColumns * 2 - smem_addr(sh.u));
+    const uint32_t state = operand(sh.s[0], D * 128), rows = operand(sh.u[0], kAlone ? kChunk * 128 : smem_addr(sh.s[1]) + kColumns * 2 - smem_addr(sh.u[0]));
     for (int c = 0; c < chunks; ++c) {
       const int parity = c & 1, stage = c % STAGES;
       const uint32_t turn = c / STAGES & 1;
       const uint32_t kq = operand(sh.kq[stage], 16), t = operand(sh.t[stage], 16), keys = operand(sh.kq[stage], D == 128 ? kPlane : 0);
-      if (!wait(&sh.k_full[stage], turn) || !wait(&sh.q_full[stage], turn) || !wait(&sh.s_ready, parity)) break;
+      if (!wait(&sh.full[stage], turn) || (!kAlone && !wait(&sh.q_full, turn)) || !wait(&sh.s_ready, parity)) break;
       fence_after();
 #pragma unroll
       for (int x = 0; x < kX; ++x)
@@ -1067,8 +1117,8 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
           mma_shared(elected, base, kq + x * (kPlanes * kPlane / 16) + k / 4 * (kPlane / 16) + k % 4 * 2, state + k * 128,
                      instruction_bf16((kTerms - x) * kColumns, false, true), x + k > 0);
       mma_commit(elected, &sh.scored);
-      mma_commit(elected, &sh.q_free[stage]);
-      if (!wait(&sh.t_full[stage], turn) || !wait(&sh.r_ready, parity)) break;
+      if (!kAlone) mma_commit(elected, &sh.q_free);
+      if ((!kAlone && !wait(&sh.t_full, turn)) || !wait(&sh.r_ready, parity)) break;
       fence_after();
 #pragma unroll
       for (int x = 0; x < kT; ++x)
@@ -1076,7 +1126,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
         for (int k = 0; k < kChunk / 16; ++k)
           mma_shared(elected, base + kSolvedAt, t + x * (kPlane / 16) + k * 2, rows + k * 128, instruction_bf16((kTerms - x) * kColumns, false, true), x + k > 0);
       mma_commit(elected, &sh.solved);
-      mma_commit(elected, &sh.t_free[stage]);
+      if (!kAlone) mma_commit(elected, &sh.t_free);
       if (!wait(&sh.u_ready, parity)) break;
       fence_after();
 #pragma unroll
@@ -1085,7 +1135,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
         for (int k = 0; k < kChunk / 16; ++k)
           mma_shared(elected, base, keys + x * (kPlanes * kPlane / 16) + k * 128, rows + k * 128, instruction_bf16((kTerms - x) * kColumns, true, true), x + k > 0);
       mma_commit(elected, &sh.added);
-      mma_commit(elected, &sh.k_free[stage]);
+      mma_commit(elected, &sh.free[stage]);
     }
   }
   if (*poison) {
@@ -1108,7 +1158,7 @@ struct Layout {
   bool packed;
   int64_t places, kq, t, vec;   // bytes
 };
-constexpr int64_t kWorkspaceBound = 256LL << 20;
+constexpr int64_t kWorkspaceBound = 1LL << 30;
 
 Layout lay_out(const CarryGdnPrefillArgs& a) {
   const int64_t terms = a.qkv_dtype == CARRY_BF16 ? 1 : a.qkv_dtype == CARRY_F16 ? 2 : 3, terms_t = a.qkv_dtype == CARRY_F32 ? 3 : 2;

@@ -16,16 +16,17 @@ DEV = "cuda"
 TOKEN_BY_TOKEN, IN_CHUNKS = 13, 14
 
 
-def make(lengths, H, HV, D, dtype, initial=False, l2norm=True, seed=0, gates=None):
-    g = torch.Generator().manual_seed(seed)
+def make(lengths, H, HV, D, dtype, initial=False, l2norm=True, seed=0, gates=None, device="cpu"):
+    g = torch.Generator(device=device).manual_seed(seed)
+    new = lambda f, *shape: f(*shape, generator=g, device=device)  # noqa: E731
     N = sum(lengths)
-    x = torch.nn.functional.silu(torch.randn(N, 2 * H * D + HV * D, generator=g))
+    x = torch.nn.functional.silu(new(torch.randn, N, 2 * H * D + HV * D))
     if not l2norm:
         qk = x[:, :2 * H * D].view(N, 2 * H, D)
         qk /= qk.norm(dim=-1, keepdim=True) + 1e-3
-    c = dict(mixed_qkv=x.to(dtype), a=torch.randn(N, HV, generator=g).to(gates or dtype), b=torch.randn(N, HV, generator=g).to(gates or dtype),
-             A_log=torch.log(1 + 15 * torch.rand(HV, generator=g)), dt_bias=torch.randn(HV, generator=g) - 4, scale=D ** -0.5)
-    state = torch.randn(len(lengths), HV, D, D, generator=g) if initial else None
+    c = dict(mixed_qkv=x.to(dtype), a=new(torch.randn, N, HV).to(gates or dtype), b=new(torch.randn, N, HV).to(gates or dtype),
+             A_log=torch.log(1 + 15 * new(torch.rand, HV)), dt_bias=new(torch.randn, HV) - 4, scale=D ** -0.5)
+    state = new(torch.randn, len(lengths), HV, D, D) if initial else None
     return c, state
 
 
@@ -204,14 +205,17 @@ def test_many_heads_go_in_chunks_sooner():
 
 
 def test_launches_that_share_the_workspace_out():
-    """A call too large for the workspace's bound is cut by chunks and by requests: the same numbers as alone."""
-    for D, H, HV, lengths in ((128, 4, 32, [4200, 64, 4500, 4097]), (64, 4, 64, [65] * 130 + [129])):
-        c, state = make(lengths, H, HV, D, BF16, True)
+    """A call too large for the workspace's bound is cut by chunks, or by requests: the same numbers as alone."""
+    for D, H, HV, lengths in ((128, 32, 64, [9000, 64, 9500, 4097]), (64, 4, 64, [65] * 300 + [129])):
+        c, state = make(lengths, H, HV, D, BF16, True, device=DEV)
+        need = pp.prefill_workspace_bytes(c["mixed_qkv"], state, starts(lengths).to(DEV), max(lengths))
+        chunks = sum(-(-n // 64) for n in lengths)
+        assert need < chunks * (H * D * 256 + HV * 32768)          # it does not hold every chunk at once
         out, final = run(c, state, lengths, HV, D)
         for i in range(0, len(lengths), max(1, len(lengths) // 4)):
             rows = slice(sum(lengths[:i]), sum(lengths[:i + 1]))
             part = {k: v[rows] if k in ("mixed_qkv", "a", "b") else v for k, v in c.items()}
-            alone = run(part, state[i:i + 1], lengths[i:i + 1], HV, D, most=None if lengths[i] > 64 else 65)
+            alone = run(part, state[i:i + 1], lengths[i:i + 1], HV, D)
             if lengths[i] > 64:
                 assert torch.equal(out[rows], alone[0]) and torch.equal(final[i:i + 1], alone[1])
 
