@@ -90,7 +90,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
     # the sources whose code differs in the test-only twin (the kernels that wait for bulk copies)
     twin_sources = ("carry_gdn_tile128_vk.cu", "carry_gdn_tile128_kv.cu", "carry_gdn_multi.cu", "carry_gdn_dense128.cu",
-                    "carry_kv_prefill.cu")
+                    "carry_kv_prefill.cu", "carry_delta_chunk.cu")
 
     def compile_one(job):
         src, twin = job
