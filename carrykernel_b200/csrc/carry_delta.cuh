@@ -28,13 +28,23 @@ __device__ __forceinline__ PrefillRequest prefill_request(const CarryGdnPrefillA
   return r;
 }
 
-// log alpha and beta of a token.  The softplus of a large negative number is that number's exponential, of which log(1 + x)
-// would leave few bits; steps of 0.001 are where models begin.
-__device__ __forceinline__ void prefill_gates(const CarryGdnPrefillArgs& a, long long row, int hv, float& log_alpha, float& beta) {
-  const float x = load_as_float(a.a, row * a.stride_a_tok + hv, a.ab_dtype) + load_as_float(a.dt_bias, hv, a.dt_bias_dtype);
+// What a token's gates are made of, and log alpha and beta.  The softplus of a large negative number is that number's exponential, of which
+// log(1 + x) would leave few bits; steps of 0.001 are where models begin.
+struct GateInputs {
+  float a, b, A_log, dt_bias;
+};
+__device__ __forceinline__ GateInputs gate_inputs(const CarryGdnPrefillArgs& a, long long row, int hv) {
+  return {load_as_float(a.a, row * a.stride_a_tok + hv, a.ab_dtype), load_as_float(a.b, row * a.stride_b_tok + hv, a.ab_dtype),
+          load_as_float(a.A_log, hv, a.A_log_dtype), load_as_float(a.dt_bias, hv, a.dt_bias_dtype)};
+}
+__device__ __forceinline__ void gates_of(const GateInputs& g, float& log_alpha, float& beta) {
+  const float x = g.a + g.dt_bias;
   const float softplus = x <= kSoftplusThreshold ? log1pf(expf(x)) : x;
-  log_alpha = -expf(load_as_float(a.A_log, hv, a.A_log_dtype)) * softplus;
-  beta = __fdiv_rn(1.0f, 1.0f + expf(-load_as_float(a.b, row * a.stride_b_tok + hv, a.ab_dtype)));
+  log_alpha = -expf(g.A_log) * softplus;
+  beta = __fdiv_rn(1.0f, 1.0f + expf(-g.b));
+}
+__device__ __forceinline__ void prefill_gates(const CarryGdnPrefillArgs& a, long long row, int hv, float& log_alpha, float& beta) {
+  gates_of(gate_inputs(a, row, hv), log_alpha, beta);
 }
 
 int64_t delta_workspace(const CarryGdnPrefillArgs& a);

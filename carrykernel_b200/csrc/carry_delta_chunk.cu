@@ -35,6 +35,11 @@ struct ChunkParams {
   float* vec;               // [place][HV] factors of a chunk's rows
 };
 
+// A token with a key or a gate that is not a number makes the state so, from there on; products over a whole chunk must not carry that back to
+// the tokens ahead of it.  So from the first such token of a chunk on (`live` are the tokens ahead of it) keys and gates count as absent, and the
+// factors of its outputs and of the state are NaN.  Values are looked after column by column, where they are used.
+constexpr float kNotANumber = __builtin_nanf("");
+
 struct Place {
   int first, count;         // the request's rows
   long long slot0;          // of its chunk chunk0
@@ -104,6 +109,7 @@ struct PrepareShared {
   // second half's token; decays from the chunk's start to the token and from there to the chunk's end; beta
   alignas(16) float G[kChunk], to_middle[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk];
   alignas(16) float norm[2 * kChunk];     // what makes a key a unit one, and a query one times `scale`
+  int live_keys[kRowWarps], live_gates;
   float decay;                            // of the chunk
   uint64_t done[3];
   uint32_t tmem;
@@ -125,13 +131,21 @@ __device__ __forceinline__ float exp2_of(double x) {
 template <class Shared>
 __device__ __forceinline__ void chunk_gates(const ChunkParams& p, Shared& sh, long long row, int n, int hv) {
   const int lane = threadIdx.x % 32;
+  float log_alpha[2] = {}, beta[2] = {};
+  int bad = n;
+#pragma unroll
+  for (int e = 1; e >= 0; --e) {
+    if (2 * lane + e < n) prefill_gates(p.a, row + 2 * lane + e, hv, log_alpha[e], beta[e]);
+    if (isnan(log_alpha[e]) || isnan(beta[e])) bad = 2 * lane + e;
+  }
+  const int live = __reduce_min_sync(~0u, bad);
+  if (lane == 0) sh.live_gates = live;
   double g[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    float log_alpha = 0.0f, beta = 0.0f;
-    if (2 * lane + e < n) prefill_gates(p.a, row + 2 * lane + e, hv, log_alpha, beta);
-    g[e] = (double)(log_alpha < kLeastLog ? kLeastLog : log_alpha) * 1.4426950408889634;     // exp(-200) is 0, and sums stay finite
-    sh.beta[2 * lane + e] = beta;
+    const bool there = 2 * lane + e < live;
+    g[e] = there ? (double)(log_alpha[e] < kLeastLog ? kLeastLog : log_alpha[e]) * 1.4426950408889634 : 0.0;     // exp(-200) is 0, and sums stay finite
+    sh.beta[2 * lane + e] = there ? beta[e] : 0.0f;
   }
   double sum = g[0] + g[1];
 #pragma unroll
@@ -203,6 +217,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
     // keys and queries as operands; rows behind the last token are zeros, whatever memory holds there
     constexpr int kLanes = D / 8, kRows = 32 / kLanes, kTurns = 2 * kChunk / (kRowWarps * kRows), kBatch = 4;
     const int chunk = lane % kLanes, first = warp * kRows + lane / kLanes;
+    int bad = n;
 #pragma unroll
     for (int t0 = 0; t0 < kTurns; t0 += kBatch) {
       Raw<CARRY_F32> x[kBatch];
@@ -216,9 +231,15 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
       for (int t = 0; t < kBatch; ++t) {
         const int row = first + (t0 + t) * kRowWarps * kRows;
         Eight e = unpack<CARRY_F32>(x[t]);
+        if (row < kChunk) {
+          const float2 zero = make_float2(0.0f, 0.0f), none = fma2(e.x[0], zero, fma2(e.x[1], zero, fma2(e.x[2], zero, mul2(e.x[3], zero))));
+          if (!(none.x + none.y == 0.0f)) bad = min(bad, row);
+        }
         store_terms<kX>(sh.kq[0][chunk / 8] + plane_at(row, chunk % 8), kPlanes * kPlane, e.x);
       }
     }
+    bad = __reduce_min_sync(~0u, bad);
+    if (lane == 0) sh.live_keys[warp] = bad;
     fence_proxy();
   } else {
     if (lane == 0) {
@@ -239,6 +260,19 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
   // the whole CTA goes on, or none of it
   auto wait = [&](int i) { return !__syncthreads_or(!barrier_wait(&sh.done[i], 0, poison, a.status)); };
   const uint32_t elected = warp == kRowWarps ? elect() : 0, base = __shfl_sync(~0u, tmem, 0);
+  int live = n;
+#pragma unroll
+  for (int i = 0; i < kRowWarps; ++i) live = min(live, sh.live_keys[i]);
+  if (live < n) {                                 // the same for all
+    if (warp == kRowWarps) chunk_gates(p, sh, row0, live, hv);
+    for (int i = tid; i < kX * kPlanes * kChunk * 8; i += kPrepareThreads)
+      if (i / 8 % kChunk >= live) *reinterpret_cast<uint4*>(sh.kq[0][0] + i / (kChunk * 8) * kPlane + i % (kChunk * 8) * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy();
+    fence_before();
+    __syncthreads();
+    fence_after();
+  }
+  live = min(live, sh.live_gates);
 
   if (warp == kRowWarps) {                        // [K; Q] [K; Q]^T: the norms are on its diagonal
 #pragma unroll
@@ -345,12 +379,12 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
   } else if (warp < 4) {                          // the factors of the chunk's rows
     const int i = tid - 64;
     float* vec = p.vec + (slot * a.HV + hv) * kVec;
-    const bool there = i < n;
+    const bool there = i < live;
     vec[i] = there ? sh.beta[i] * sh.from_start[i] * sh.norm[i] : 0.0f;
     vec[kChunk + i] = sh.beta[i];
     vec[2 * kChunk + i] = there ? sh.to_end[i] * sh.norm[i] : 0.0f;
-    vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.norm[kChunk + i] : 0.0f;
-    if (i < 8) vec[4 * kChunk + i] = sh.decay;
+    vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.norm[kChunk + i] : i < n ? kNotANumber : 0.0f;
+    if (i < 8) vec[4 * kChunk + i] = live < n ? kNotANumber : sh.decay;
   }
   fence_proxy();
   fence_before();
@@ -487,17 +521,25 @@ __device__ __forceinline__ void store_transposed(uint32_t to, const uint32_t (&w
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-// Gates of a chunk: lane l has tokens 2 l and 2 l + 1.  Sums of decays are formed in 64 bits; what fp32 has to hold of them, for differences,
-// is the sum within a block.  Returns the decays over the second block, over the third, and over the chunk.
-__device__ __forceinline__ float3 unit_gates(const ChunkParams& p, Unit& sh, long long row, int n, int hv) {
+// Gates of a chunk: lane l has tokens 2 l and 2 l + 1, whose inputs it has read.  Sums of decays are formed in 64 bits; what fp32 has to hold of
+// them, for differences, is the sum within a block.  `live`: tokens that count; less, when a gate among them is no number.  Returns the decays over
+// the second block, over the third, and over the chunk.
+__device__ __forceinline__ float3 unit_gates(Unit& sh, const GateInputs (&in)[2], int& live) {
   const int lane = threadIdx.x % 32;
+  float log_alpha[2], beta[2];
+  int bad = live;
+#pragma unroll
+  for (int e = 1; e >= 0; --e) {
+    gates_of(in[e], log_alpha[e], beta[e]);
+    if (2 * lane + e < live && (isnan(log_alpha[e]) || isnan(beta[e]))) bad = 2 * lane + e;
+  }
+  live = __reduce_min_sync(~0u, bad);
   double g[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    float log_alpha = 0.0f, beta = 0.0f;
-    if (2 * lane + e < n) prefill_gates(p.a, row + 2 * lane + e, hv, log_alpha, beta);
-    g[e] = (double)(log_alpha < kLeastLog ? kLeastLog : log_alpha) * 1.4426950408889634;     // exp(-200) is 0, and sums stay finite
-    sh.beta[2 * lane + e] = beta;
+    const bool there = 2 * lane + e < live;
+    g[e] = there ? (double)(log_alpha[e] < kLeastLog ? kLeastLog : log_alpha[e]) * 1.4426950408889634 : 0.0;     // exp(-200) is 0, and sums stay finite
+    sh.beta[2 * lane + e] = there ? beta[e] : 0.0f;
   }
   double sum = g[0] + g[1];
 #pragma unroll
@@ -589,27 +631,42 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
 
   uint32_t k[2 * kBlocks][kWords];
   load_quarters<D>(p, row0, n, 0, (a.H + h) * D, k);
-  const float3 across = unit_gates(p, sh, row0, n, hv);
+  GateInputs gate[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) gate[e] = gate_inputs(a, row0 + min(2 * lane + e, n - 1), hv);
+
+  // The norms are on the diagonals of products with themselves: of rows g and g + 8, at the lane with t = g / 2.
+  auto square = [&](const Part& d, int half) { return g % 2 ? d.x[half][2 * half + 1] : d.x[half][2 * half]; };
+  auto norms = [&](const Part& d, float by, float* to) {
+    if (t != g / 2) return;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) to[g + 8 * half] = a.use_qk_l2norm ? __fdiv_rn(by, sqrtf(square(d, half) + kL2Eps)) : by;
+  };
+  Part diagonal[kBlocks];
+  int live = n;
+#pragma unroll
+  for (int b = kBlocks - 1; b >= 0; --b) {
+    diagonal[b] = products<kHalfType>(k[2 * b], k[2 * b + 1], k[2 * b], k[2 * b + 1]);
+#pragma unroll
+    for (int half = 1; half >= 0; --half)
+      if (t == g / 2 && !(square(diagonal[b], half) < INFINITY)) live = b * kBlock + g + 8 * half;
+  }
+  live = __reduce_min_sync(~0u, live);
+  if (live < n) {                                 // the same for all lanes
+#pragma unroll
+    for (int r = 0; r < 2 * kBlocks; ++r)
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) k[r][e] = 8 * r + g < live ? k[r][e] : 0;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) diagonal[b] = products<kHalfType>(k[2 * b], k[2 * b + 1], k[2 * b], k[2 * b + 1]);
+  }
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) norms(diagonal[b], 1.0f, sh.key + b * kBlock);
   if (kq) {
 #pragma unroll
     for (int r = 0; r < 2 * kBlocks; ++r) store_quarter<DTYPE, D>(kq, 8 * r + g, k[r]);
   }
-
-  // The norms are on the diagonals of products with themselves: of rows g and g + 8, at the lane with t = g / 2.
-  auto norms = [&](const Part& d, float by, float* to) {
-    if (t != g / 2) return;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const float square = g % 2 ? d.x[half][2 * half + 1] : d.x[half][2 * half];
-      to[g + 8 * half] = a.use_qk_l2norm ? __fdiv_rn(by, sqrtf(square + kL2Eps)) : by;
-    }
-  };
-  Part diagonal[kBlocks];
-#pragma unroll
-  for (int b = 0; b < kBlocks; ++b) {
-    diagonal[b] = products<kHalfType>(k[2 * b], k[2 * b + 1], k[2 * b], k[2 * b + 1]);
-    norms(diagonal[b], 1.0f, sh.key + b * kBlock);
-  }
+  const float3 across = unit_gates(sh, gate, live);
   __syncwarp();
 
   // L and P, a row of blocks at a time.  Within a block decays are powers of differences; between blocks products of a decay to the one's end, over
@@ -678,13 +735,13 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = lane + 32 * e;
-      const bool there = i < n;
+      const bool there = i < live;
       vec[i] = there ? sh.beta[i] * sh.from_start[i] * sh.key[i] : 0.0f;
       vec[kChunk + i] = sh.beta[i];
       vec[2 * kChunk + i] = there ? sh.to_end[i] * sh.key[i] : 0.0f;
-      vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.query[i] : 0.0f;
+      vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.query[i] : i < n ? kNotANumber : 0.0f;
     }
-    if (lane < 8) vec[4 * kChunk + lane] = across.z;
+    if (lane < 8) vec[4 * kChunk + lane] = live < n ? kNotANumber : across.z;
   }
 
   // The inverses of the blocks on the diagonal, by substitution, a column to a lane, two blocks at a time.
@@ -826,6 +883,9 @@ struct SequenceShared {
   // what has come, and what is free again: with one stage keys, queries, T and values are each asked for again as soon as they have been used
   uint64_t full[STAGES], free[STAGES], q_full, t_full, v_full, vec_full[2], q_free, t_free, v_free;
   uint64_t s_ready, r_ready, u_ready, scored, solved, added;
+  // of a chunk: the first token whose value in a column is not finite, and whether there is one; for three chunks in turn, of which one is being
+  // written, one read and one made ready
+  int bad[3][kColumns], any_bad[3];
   uint32_t tmem;
   int poison;
 };
@@ -880,6 +940,10 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
     barrier_init(&sh.solved, 1);
     barrier_init(&sh.added, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid < 3 * kColumns) {
+    sh.bad[tid / kColumns][tid % kColumns] = kChunk;
+    sh.any_bad[tid / kColumns] = 0;
   }
   // columns 0 and on: [K; Q] S, and, when that is read, K^T U; behind them [T; P T] R
   constexpr uint32_t kSolvedAt = kTerms * kColumns, kTmem = 256;
@@ -960,6 +1024,20 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[j / 2 + k] = there ? mul2(e.x[k], make_float2(beta, beta)) : make_float2(0.0f, 0.0f);
       }
+      // What is not finite would reach the rows ahead of it, as zero times that; its column becomes NaN from its token on instead.
+      float2 none = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < W / 2; ++j) none = fma2(o[j], make_float2(0.0f, 0.0f), none);
+      if (!(none.x + none.y == 0.0f)) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          float& y = j % 2 ? o[j / 2].y : o[j / 2].x;
+          if (isfinite(y)) continue;
+          atomicMin(&sh.bad[c % 3][first + j], token);
+          sh.any_bad[c % 3] = 1;
+          y = 0.0f;
+        }
+      }
       return true;
     };
     bool healthy = true;
@@ -993,8 +1071,12 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
         barrier_arrive(&sh.u_ready);
       }
       test_come_late(warp, c + 1);
+      if (tid < kColumns) sh.bad[(c + 2) % 3][tid] = kChunk;
+      if (tid == 0) sh.any_bad[(c + 2) % 3] = 0;
       healthy = wait(&sh.solved, parity);
       if (!healthy) break;
+      const int* bad = sh.bad[c % 3] + first;
+      const bool spoilt = sh.any_bad[c % 3];
       fence_after();
       load_sums<W>(at + kSolvedAt, x);
       if (key) {
@@ -1007,6 +1089,11 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       } else {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = add2(x[j], o[j]);
+        if (spoilt) {
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            if (bad[j] <= token) (j % 2 ? x[j / 2].y : x[j / 2].x) = kNotANumber;
+        }
         if (!kAlone) healthy = wait(&sh.u_ready, parity);   // stores that are under way hold up the fences of the keys' threads, all the more of two CTAs'
         if (!healthy) break;
         if (c * kChunk + token < left) {
@@ -1043,6 +1130,11 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       load_sums<W>(at, x);
 #pragma unroll
       for (int j = 0; j < W / 2; ++j) S[j] = fma2(make_float2(decay, decay), S[j], x[j]);
+      if (spoilt) {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          if (bad[j] < kChunk) (j % 2 ? S[j / 2].y : S[j / 2].x) = kNotANumber;
+      }
       if (c + 1 < chunks) put_state();
     }
     if (healthy && has_state) {

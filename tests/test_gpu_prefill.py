@@ -166,6 +166,41 @@ def test_a_request_with_numbers_that_are_not_finite_spoils_no_other(n):
     assert torch.equal(got[1][::2], clean[1][::2]) and got[1][1].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,at", [(40, 17), (200, 3), (200, 70), (130, 127), (193, 192)])
+def test_numbers_that_are_not_finite_reach_no_token_ahead_of_them(n, at, dtype):
+    """A value spoils its column of the state from its token on, a key or a gate the heads that read it, a query its token's output."""
+    H, HV, D = 2, 4, 64
+    c, state = make([n], H, HV, D, dtype, True)
+    clean = run(c, state, [n], HV, D)
+    for where, bad in (("value", float("nan")), ("value", float("inf")), ("key", float("nan")), ("key", -float("inf")), ("query", float("nan")),
+                       ("a", float("nan")), ("b", float("nan"))):
+        d = {k: v.clone() if torch.is_tensor(v) else v for k, v in c.items()}
+        heads, columns, rows = slice(2, 4), slice(None), slice(at, None)       # what it may reach: heads 2 and 3 read key head 1
+        if where == "value":
+            d["mixed_qkv"][at, 2 * H * D + 2 * D + 5] = bad
+            heads, columns = slice(2, 3), slice(5, 6)
+        elif where == "key":
+            d["mixed_qkv"][at, H * D + D + 7] = bad
+        elif where == "query":
+            d["mixed_qkv"][at, D + 7] = bad
+            rows = slice(at, at + 1)
+        else:
+            d[where][at, 2] = bad
+            heads = slice(2, 3)
+        out, final = run(d, state, [n], HV, D)
+        reached = torch.zeros_like(out, dtype=torch.bool)
+        reached[rows, heads, columns] = True
+        assert torch.equal(out[~reached], clean[0][~reached]), where
+        assert not out[reached].isfinite().any() or (where == "value" and bad == float("inf")), where
+        if where != "query":
+            spoilt = torch.zeros_like(final, dtype=torch.bool)
+            spoilt[:, heads, columns] = True
+            assert torch.equal(final[~spoilt], clean[1][~spoilt]) and not final[spoilt].isfinite().any(), where
+        else:
+            assert torch.equal(final, clean[1])
+
+
 def test_bad_row_ranges_are_flagged_and_skipped():
     H, HV, D = 1, 1, 64
     c, _ = make([100], H, HV, D, BF16)
