@@ -6,10 +6,18 @@
 // and with T = (I + L)^-1 and P_ij = exp(G_i - G_j) (scale q_i) . k_j for j <= i:
 //   U = T R,   O = diag(exp G) (scale Q) S + (P T) R,   S' = exp(G_64) S + K^T diag(exp(G_64 - G)) U.
 //
-// T and P T do not depend on the state: prepare_kernel forms them for every chunk and head side by side.  sequence_kernel then walks a
-// request's chunks, a CTA for some columns of a head's state, with three products to a chunk that wait for one another:
-//   [K; Q] S  (128 x columns, over K),   [T; P T] R  (128 x columns, over 64 tokens),   K^T U  (K x columns, over 64 tokens).
+// T and P T do not depend on the state: unit_kernel (prepare_kernel for fp32) forms them for every chunk and head side by side.  sequence_kernel
+// then walks a request's chunks, a CTA for 32 columns of a head's state, with three products to a chunk that wait for one another:
+//   [K; Q] S  (128 x 32, over K),   [T; P T] R  (128 x 32, over 64 tokens),   K^T U  (K x 32, over 64 tokens).
 // The state itself stays in registers, in fp32; its products take it as a sum of bf16 numbers.
+//
+// What bounds it.  One prompt of 8192 tokens, 32 heads of 128 over 16: 400 us, of which unit_kernel takes 118 and the 128 steps of sequence_kernel
+// 2.2 us each.  A step is a chain: its products take 1.7 of 3.9 thousand cycles (a left side of 128 rows is 4 KB of shared memory for 16 steps of the
+// sum, whatever the columns, so a product of 32 columns times three terms runs at 60 % of the rate of one of 128), and between them a row's numbers
+// go from tensor memory through the registers of the two schedulers that own the keys' lanes, as three bf16 numbers each, into shared memory.  With
+// two CTAs to a processor (sixteen prompts of 4096: 2.45 ms, 98 TFLOP/s of the recurrence's own operations) the chains overlap, and the same
+// traffic of shared memory bounds: 240 KB a chunk, 1900 cycles of 3300.  Two chains in one CTA that share its tiles came out no faster, nor did
+// truncated terms, stores by a warp of their own, or workspaces that the second-level cache holds (400 us -> 530, for every launch has its own start).
 //
 // Precision.  Keys and queries in bf16 are operands as they are (norms and decays multiply rows of the products, in fp32); in fp16 they are
 // the sum of two bf16 numbers, in fp32 of three.  What is computed is split too: S, R and U into three, T into two (three with fp32
@@ -92,6 +100,7 @@ __device__ __forceinline__ Raw<DTYPE> load_row(const void* base, long long at, b
 
 // ---- what does not depend on the state -------------------------------------------------------------------------------
 //
+// For fp32 keys and queries, three bf16 numbers each, which are too many for a warp's registers.
 // With D the inverses of I + L's two 32 x 32 blocks on the diagonal, N its block below them, and Y = N D (of which the first half's columns are
 // not zero): T = D - D Y and P T = P D - (P D) Y.  So two products with 128 rows, [N; P] D and [D; P D] Y, finish both.
 
@@ -461,7 +470,9 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
 
 // ---- the same, a chunk and head to a warp ----------------------------------------------------------------------------
 //
-// For 16-bit keys and queries.  Everything is a product of 16 x 16 blocks whose operands are registers: a lane's part of a product's result
+// For 16-bit keys and queries; 6200 instructions a warp, two warps to a scheduler (keys alone take half of a thread's registers), 29 ns a chunk and
+// head over the whole GPU.  What bounds it is latency: an instruction in 4.4 cycles.  The form by tensor memory that fp32 has takes 44 ns.
+// Everything is a product of 16 x 16 blocks whose operands are registers: a lane's part of a product's result
 // is its part of the next one's left side, or of its right side transposed, so T^T and (P T)^T are built block by block,
 //   W_jj = D_j^T,   W_jb = -(sum over j <= k < b of W_jk L_bk^T) D_b^T  (T_bj = W_jb^T),   (P T)_ij = (sum over j <= k <= i of W_jk P_ik^T)^T,
 // and only the 16 x 16 inverses D_b go through shared memory.  No warp waits for another.  Keys and queries come from memory as they
