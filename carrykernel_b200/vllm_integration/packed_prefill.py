@@ -99,7 +99,8 @@ def gated_delta_rule_packed_prefill(mixed_qkv, a, b, A_log, dt_bias, scale, out,
     ``scale`` as in ``quantized_gated_delta_rule_packed_decode``; ``out [N, HV, V]``; ``initial_state`` (``None`` for zeros)
     and ``final_state`` fp32 ``[B, HV, V, K]``, which may be one tensor.  Every request has ``N / B`` rows, or, with ``query_start [B + 1]``
     (int32), rows ``query_start[b] .. query_start[b + 1] - 1``, ``max_query_len`` of them at most; a request without rows hands its
-    state on.  ``K = V`` is 64 or 128.
+    state on.  ``K = V`` is 64 or 128.  A key or a gate that is not finite makes the state of the heads that read it NaN from its token on, a
+    value its row of the state; outputs ahead of it are what they were.
 
     ``workspace`` (uint8, at least :func:`prefill_workspace_bytes`) is allocated by the call when it is not given.  ``status`` as in
     ``quantized_packed_decode``: rows beyond ``max_query_len`` or outside of ``mixed_qkv`` are skipped and flagged

@@ -453,11 +453,17 @@ int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* args, void* stream);
  * b are query_start[b] .. query_start[b + 1] - 1 (at most max_query; more, and
  * rows outside 0 .. N - 1, are skipped and flagged with
  * CARRY_GDN_STATUS_BAD_RANGE), or, with query_start NULL, max_query = N / B
- * each.  No two requests share a row.  A request without rows hands its state
- * on.  K and V are 64 or 128 (one width for both), B and HV at most 65535.
+ * each.  No two requests share a row, and other rows are left alone.  A request
+ * without rows hands its state on.  A key or a gate that is not finite makes the
+ * state of the heads that read it NaN from its token on, a value its row of the
+ * state; outputs ahead of it are what they were.  With use_qk_l2norm the squares
+ * of a key's numbers have to add up to less than fp32's largest number.  A token's
+ * decay below exp(-200) is 0.  K and V are 64 or 128 (one width for both), B and HV at most 65535.
  * final_state may be initial_state.  `workspace` is at least
  * carry_gdn_prefill_workspace() bytes, 16-byte aligned; nothing is kept in it
- * between calls.
+ * between calls.  It is at most some 1 GiB: what does not fit is worked off in
+ * turns.  Where a wait runs out (CARRY_GDN_STATUS_TIMEOUT), the head's further
+ * outputs and its state are left as they were.
  */
 typedef struct CarryGdnPrefillArgs {
   const void* mixed_qkv;      /* [N, 2*H*K + HV*V] = q | k | v, as in carry_gdn_packed_decode */
