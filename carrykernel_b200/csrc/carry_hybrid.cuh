@@ -102,7 +102,7 @@ __device__ __forceinline__ KvRequest kv_request(const CarryGdnKvCache& c, const 
   if (r.query_start) {
     const int from = r.query_start[b], to = r.query_start[b + 1];
     q.first = min(max(from, 0), r.N);
-    q.count = max(min(to, r.N) - q.first, 0);
+    q.count = max(min(to, r.N), q.first) - q.first;     // no difference that 32 bits do not hold
     q.todo = min(q.count, r.max_query);
     bad = bad || q.first != from || q.first + q.todo != to;
   } else {
