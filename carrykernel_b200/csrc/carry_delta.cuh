@@ -19,7 +19,7 @@ __device__ __forceinline__ PrefillRequest prefill_request(const CarryGdnPrefillA
   if (a.query_start) {
     const int from = a.query_start[b], to = a.query_start[b + 1];
     r.first = min(max(from, 0), a.N);
-    r.count = min(max(min(to, a.N) - r.first, 0), a.max_query);
+    r.count = min(max(min(to, a.N), r.first) - r.first, a.max_query);   // no difference that 32 bits do not hold
     if (status && (r.first != from || r.first + r.count != to)) atomicOr(status, CARRY_GDN_STATUS_BAD_RANGE);
   } else {
     r.first = b * a.max_query;

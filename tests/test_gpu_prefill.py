@@ -216,6 +216,27 @@ def test_bad_row_ranges_are_flagged_and_skipped():
             _lib.raise_for_status(status)
 
 
+@pytest.mark.parametrize("n", [30, 100])
+def test_row_ranges_at_the_ends_of_32_bits(n):
+    """Starts that are no rows of the call at all: nothing outside of it is read or written, and what has rows is done."""
+    least, most = -2 ** 31, 2 ** 31 - 1
+    H, HV, D = 1, 2, 64
+    c, _ = make([n + 9], H, HV, D, BF16)
+    dev = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in c.items()}
+    alone = run({k: v[:n] if k in ("mixed_qkv", "a", "b") else v for k, v in c.items()}, None, [n], HV, D)
+    for start in ([0, n, least], [0, n, most], [0, n, least, most], [0, n, least, least]):
+        B = len(start) - 1
+        guarded = torch.full((n + 9 + 64, HV, D), 9.0, dtype=BF16, device=DEV)
+        out, final = guarded[32:32 + n + 9], torch.empty(B, HV, D, D, device=DEV)
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        pp.gated_delta_rule_packed_prefill(**dev, out=out, final_state=final, query_start=torch.tensor(start, dtype=torch.int32, device=DEV),
+                                           max_query_len=n, use_qk_l2norm_in_kernel=True, status=status)
+        assert status.item() == _lib.STATUS_BAD_RANGE, start
+        assert (guarded[:32] == 9).all() and (guarded[32 + n + 9:] == 9).all() and torch.equal(final[:1], alone[1])
+        if most not in start:
+            assert torch.equal(out[:n], alone[0]) and (out[n:] == 9).all() and (final[1:] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_a_prompt_in_parts_is_the_prompt(dtype):
     """Handing the state on at any token, from any of the two ways of working to the other, is within the bounds of one call."""
