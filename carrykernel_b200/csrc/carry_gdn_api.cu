@@ -389,7 +389,7 @@ int prefill_ok(const CarryGdnPrefillArgs* a) {
   if (a->B < 0 || a->N < 0 || a->max_query < 0 || a->H <= 0 || a->HV <= 0 || a->HV % a->H) return CARRY_GDN_ERR_SHAPE;
   if (!a->query_start && (long long)a->B * a->max_query != a->N) return CARRY_GDN_ERR_SHAPE;
   if (a->K != a->V || (a->K != 64 && a->K != 128)) return CARRY_GDN_ERR_UNSUPPORTED;
-  if (a->B > 65535 || a->HV > 65535) return CARRY_GDN_ERR_TOO_LARGE;
+  if (a->B > 65535 || a->HV > 65535 || a->N > 1 << 30) return CARRY_GDN_ERR_TOO_LARGE;
   for (int t : {a->qkv_dtype, a->ab_dtype, a->A_log_dtype, a->dt_bias_dtype, a->out_dtype})
     if (!dtype_ok(t)) return CARRY_GDN_ERR_DTYPE;
   return CARRY_GDN_OK;
@@ -439,6 +439,7 @@ int carry_gdn_qk_norm_rope(const CarryGdnRotateArgs* a, void* stream) {
   }
   if (2 * pairs != a->rotary) return CARRY_GDN_ERR_SHAPE;
   if (a->D > 512) return CARRY_GDN_ERR_UNSUPPORTED;
+  if (a->HQ > 65535 || a->HK > 65535) return CARRY_GDN_ERR_TOO_LARGE;
   for (int t : {a->dtype, a->weight_dtype, a->table_dtype})
     if (!dtype_ok(t)) return CARRY_GDN_ERR_DTYPE;
   if (!(a->eps >= 0.0f)) return CARRY_GDN_ERR_SHAPE;

@@ -818,7 +818,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (a.axes < 1 || a.axes > 4 || pos->size(pos->dim() - 1) != N || pos->stride(pos->dim() - 1) != 1) return nullptr;
     a.stride_positions = pos->dim() == 1 ? 0 : pos->stride(0);
     if (o[10] == Py_None) {
-      if (a.axes != 1) return nullptr;
+      if (pos->dim() != 1) return nullptr;
       a.sections[0] = static_cast<int32_t>(table->size(1) / 2);
     } else {
       if (!PyList_Check(o[10]) && !PyTuple_Check(o[10])) return nullptr;

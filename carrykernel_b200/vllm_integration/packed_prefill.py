@@ -102,7 +102,8 @@ def gated_delta_rule_packed_prefill(mixed_qkv, a, b, A_log, dt_bias, scale, out,
     state on.  ``K = V`` is 64 or 128.  A key or a gate that is not finite makes the state of the heads that read it NaN from its token on, a
     value its row of the state; outputs ahead of it are what they were.
 
-    ``workspace`` (uint8, at least :func:`prefill_workspace_bytes`) is allocated by the call when it is not given.  ``status`` as in
+    ``workspace`` (uint8, at least :func:`prefill_workspace_bytes`) is allocated by the call when it is not given; calls that may run at the
+    same time need one each.  ``status`` as in
     ``quantized_packed_decode``: rows beyond ``max_query_len`` or outside of ``mixed_qkv`` are skipped and flagged
     (``STATUS_BAD_RANGE``)."""
     lib = _lib._lib or _lib.load_library()

@@ -28,7 +28,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps: float = 1e-6
     ``sections[0]`` go by the first axis, and so on; they add up to ``R / 2``.
 
     A token with a negative position is left alone; so is one with a position beyond the table, which sets
-    ``STATUS_BAD_RANGE`` in ``status``.  A head with a number that is not finite becomes NaN.  ``q_out`` and ``k_out`` may not overlap
+    ``STATUS_BAD_RANGE`` in ``status``.  A head with a number that is not finite becomes NaN; squares below fp32's range count as 0
+    (``eps`` stands in for them).  ``q_out`` and ``k_out`` may not overlap
     ``q`` and ``k`` other than by being them."""
     lib = _lib._lib or _lib.load_library()
     if lib.native.qk_norm_rope(lib.native_table, q, k, q_weight, k_weight, cos_sin, positions, eps, q_out, k_out, sections, interleaved,

@@ -458,10 +458,10 @@ int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* args, void* stream);
  * state of the heads that read it NaN from its token on, a value its row of the
  * state; outputs ahead of it are what they were.  With use_qk_l2norm the squares
  * of a key's numbers have to add up to less than fp32's largest number.  A token's
- * decay below exp(-200) is 0.  K and V are 64 or 128 (one width for both), B and HV at most 65535.
+ * decay below exp(-200) is 0.  K and V are 64 or 128 (one width for both), B and HV at most 65535, N at most 2^30.
  * final_state may be initial_state.  `workspace` is at least
  * carry_gdn_prefill_workspace() bytes, 16-byte aligned; nothing is kept in it
- * between calls.  It is at most some 1 GiB: what does not fit is worked off in
+ * between calls, and two that may run at a time need one each.  It is at most some 1 GiB: what does not fit is worked off in
  * turns.  Where a wait runs out (CARRY_GDN_STATUS_TIMEOUT), the head's further
  * outputs and its state are left as they were.
  */
@@ -507,8 +507,9 @@ int64_t carry_gdn_prefill_workspace(const CarryGdnPrefillArgs* args);
  * on.  A token with a negative position is left alone (nothing of it is
  * written), and so is one with a position beyond the table, which is flagged
  * with CARRY_GDN_STATUS_BAD_RANGE.  A head with a number that is not finite
- * becomes NaN.  q_out and k_out may be q and k.  D is even and at most 512,
- * rotary even and at most D, axes 1 to 4.
+ * becomes NaN.  Squares below fp32's range count as 0: eps stands in for them.
+ * q_out and k_out may be q and k.  D is even and at most 512, rotary even and at
+ * most D, axes 1 to 4, HQ and HK at most 65535.
  */
 typedef struct CarryGdnRotateArgs {
   const void* q;          /* [N, HQ, D], D contiguous */

@@ -389,3 +389,26 @@ def test_prompt_then_decode_on_the_slot_pool():
                                                      resid_fmt=qpd.RESID_INT8)
         # rows of int8 codes: half a step of 127 against a row's largest number in each of `steps` tokens, and the output's rounding
         assert (got[:, 0].cpu().double() - want[rows]).norm() <= (steps / 127 + 2 ** -8) * want[rows].norm()
+
+
+@pytest.mark.parametrize("lengths", [[20, 7], [200, 90, 130]], ids=str)
+def test_two_streams_at_once_and_a_state_for_all(lengths):
+    """Calls side by side, each with the workspace that it allocates; an initial state that is one tensor for all requests."""
+    H, HV, D, B = 4, 8, 128, len(lengths)
+    cases = [make(lengths, H, HV, D, BF16, True, seed=s) for s in (1, 2)]
+    first = [state[:1].to(DEV).expand(B, -1, -1, -1) for _, state in cases]
+    alone = [run(c, state[:1].expand(B, -1, -1, -1).clone(), lengths, HV, D) for c, state in cases]
+    on = [{k: v.to(DEV) if torch.is_tensor(v) else v for k, v in c.items()} for c, _ in cases]
+    start = starts(lengths).to(DEV)
+    results = [(torch.zeros_like(alone[i][0]), torch.zeros_like(alone[i][1])) for i in (0, 1) for _ in range(8)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for n in range(8):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                out, final = results[8 * i + n]
+                pp.gated_delta_rule_packed_prefill(**on[i], out=out, final_state=final, initial_state=first[i], query_start=start,
+                                                   max_query_len=max(lengths), use_qk_l2norm_in_kernel=True)
+    torch.cuda.synchronize()
+    for j, (out, final) in enumerate(results):
+        assert torch.equal(out, alone[j // 8][0]) and torch.equal(final, alone[j // 8][1]), j

@@ -142,3 +142,27 @@ def test_captured_and_replayed_on_another_stream():
     torch.cuda.synchronize()
     check(out[0], qkv[:, :HQ] * 2, qw, cos_sin, (positions + 17) % 500)
     check(out[1], qkv[:, HQ:HQ + HK], kw, cos_sin, (positions + 17) % 500)
+
+
+def test_one_axis_in_a_row_of_its_own_needs_its_section():
+    N, HQ, HK, D = 9, 2, 1, 64
+    qkv, qw, kw, cos_sin, positions = make(N, HQ, HK, D, D, BF16)
+    q, k = qkv[:, :HQ].to(DEV), qkv[:, HQ:HQ + HK].to(DEV)
+    rest = (qw.to(DEV), kw.to(DEV), cos_sin.to(DEV), positions.to(DEV)[None])
+    out = torch.empty_like(q), torch.empty_like(k)
+    with pytest.raises(ValueError):
+        qk_norm_rope(q, k, *rest, q_out=out[0], k_out=out[1])
+    qk_norm_rope(q, k, *rest, q_out=out[0], k_out=out[1], sections=[D // 2])
+    check(out[0], qkv[:, :HQ], qw, cos_sin, positions)
+    check(out[1], qkv[:, HQ:HQ + HK], kw, cos_sin, positions)
+
+
+def test_numbers_whose_squares_are_below_fp32():
+    """eps stands in for them: numbers come out by their weight over eps's root."""
+    N, HQ, HK, D = 3, 2, 1, 128
+    qkv, qw, kw, cos_sin, positions = make(N, HQ, HK, D, D, F32)
+    qkv = qkv * 1e-25
+    q, k = qkv[:, :HQ].to(DEV), qkv[:, HQ:HQ + HK].to(DEV)
+    qk_norm_rope(q, k, qw.to(DEV), kw.to(DEV), cos_sin.to(DEV), positions.to(DEV))
+    check(q, qkv[:, :HQ], qw, cos_sin, positions)
+    check(k, qkv[:, HQ:HQ + HK], kw, cos_sin, positions)

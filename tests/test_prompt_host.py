@@ -136,6 +136,10 @@ def test_c_entries_refuse_what_they_cannot_index(lib):
         setattr(a, field, value)
         assert lib.carry_gdn_prefill(a, None) == rc == lib.carry_gdn_prefill_workspace(a), field
         setattr(a, field, keep)
+    a.N = a.max_query = 2 ** 30 + 1
+    assert lib.carry_gdn_prefill(a, None) == -8 == lib.carry_gdn_prefill_workspace(a)
+    a.N = a.max_query = 2 ** 30
+    assert 0 < lib.carry_gdn_prefill_workspace(a) <= 1 << 30
     a.B = a.N = a.max_query = 0
     assert lib.carry_gdn_prefill(a, None) == 0 == lib.carry_gdn_prefill_workspace(a)
     r = _lib.RotateArgs()
@@ -143,7 +147,7 @@ def test_c_entries_refuse_what_they_cannot_index(lib):
     r.sections[0] = 32
     assert lib.carry_gdn_qk_norm_rope(r, None) == -1
     for field, value, rc in (("N", -1, -2), ("D", 63, -2), ("D", 600, -5), ("rotary", 66, -2), ("axes", 0, -2), ("axes", 5, -2), ("eps", -1.0, -2),
-                             ("dtype", 7, -3), ("table_dtype", -1, -3)):
+                             ("dtype", 7, -3), ("table_dtype", -1, -3), ("HQ", 65536, -8), ("HK", 65536, -8)):
         keep = getattr(r, field)
         setattr(r, field, value)
         assert lib.carry_gdn_qk_norm_rope(r, None) == rc, field
