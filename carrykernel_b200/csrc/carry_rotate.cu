@@ -6,10 +6,14 @@
 // over pairs of the first `rotary` numbers: neighbours, or number i with i + rotary / 2.  Frequency i takes its angle from the
 // table's row of the token's position on the frequency's axis.
 //
-// A lane has both numbers of its pairs: four neighbouring numbers and the four that are half the rotated width further on
-// (or the four next to them, where pairs are neighbours or nothing is rotated), so that a row is read once, its sum is a few
-// shuffles, and nothing is exchanged for the rotation.  A warp keeps its token's angles and walks over the token's heads, two rows of 128
-// or four of 64 at a time: the table is read once a token and not once a head.  Few tokens are spread over more warps.
+// A lane has both numbers of its pairs: a run of four or eight neighbouring numbers and the run that is half the rotated width further on
+// (or the one next to it, where pairs are neighbours or nothing is rotated), so that a row is read once, its sum is a few
+// shuffles, and nothing is exchanged for the rotation.  A warp keeps its token's angles and walks over the token's heads, four rows of 128
+// or eight of 64 at a time: the table is read once a token and not once a head.  Few tokens are spread over more warps.
+//
+// What bounds it: memory, behind it instructions (13 for a number; two numbers to one where the arithmetic allows).  16384 tokens of
+// 32 and 8 heads of 128: 62 us in bf16, 85 % of a plain copy's rate (68 with eight rows at a time and none ahead), 106 in fp32, 96 %.  One token: 3.6 us,
+// which is the host's call.
 #include <type_traits>
 
 #include "carry_hybrid.cuh"
@@ -104,6 +108,21 @@ __device__ __forceinline__ void load_factors(const void* base, long long at, int
   }
 }
 
+// two numbers to an instruction, where a run has them
+template <int VE, class Two, class One>
+__device__ __forceinline__ void over_run(Two two, One one) {
+  if constexpr (VE == 1) {
+    one(0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; e += 2) two(e);
+  }
+}
+template <int VE>
+__device__ __forceinline__ float2& pair(float (&x)[VE], int e) { return *reinterpret_cast<float2*>(&x[e]); }
+template <int VE>
+__device__ __forceinline__ float2 pair(const float (&x)[VE], int e) { return make_float2(x[e], x[e + 1]); }
+
 template <int LANES>
 __device__ __forceinline__ float sum_over(float x) {
 #pragma unroll
@@ -113,8 +132,12 @@ __device__ __forceinline__ float sum_over(float x) {
 
 // LANES to a row, each with UNITS times two runs of VE numbers: of 16 bytes, of four numbers or of one, as widths, strides and addresses allow.
 template <int DTYPE, int VE, int LANES, int UNITS>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant__ Params p) {
-  constexpr int kRows = 32 / LANES, kBatch = VE == 1 ? 1 : VE == 8 ? 2 : 4 / UNITS;   // rows of a warp at a time; how many times
+__global__ void __launch_bounds__(kThreads, VE == 8 ? 7 : VE == 1 || UNITS > 1 ? 1 : DTYPE == CARRY_F32 ? 5 : 6) rotate_kernel(const __grid_constant__ Params p) {
+  // 16-bit rows: a row's registers take the next one as soon as its numbers have been unpacked, which leaves room for 24 to 28 warps on a
+  // processor (62 us for the tokens above; with four times as many rows under way and 20 warps 65 to 68).  fp32 rows are as many registers as
+  // their numbers, and come four at a time, for 20 warps (106 us; one ahead and 24 warps 112).
+  constexpr bool kAhead = VE > 1 && DTYPE != CARRY_F32;
+  constexpr int kRows = 32 / LANES, kBatch = VE > 1 && !kAhead ? 4 / UNITS : 1;    // rows of a warp at a time; how many times
   const CarryGdnRotateArgs& a = p.a;
   depend_release();
   depend_wait();
@@ -142,19 +165,20 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   const Heads side[2] = {{a.q, a.q_weight, a.q_out, part * each_q, min((part + 1) * each_q, a.HQ), a.stride_q_tok, a.stride_q_head, a.stride_q_out_tok, a.stride_q_out_head},
                          {a.k, a.k_weight, a.k_out, part * each_k, min((part + 1) * each_k, a.HK), a.stride_k_tok, a.stride_k_head, a.stride_k_out_tok, a.stride_k_out_head}};
   Run<DTYPE, VE> rows[kBatch][UNITS][2];
-  auto bring = [&](const Heads& s, int h0) {
+  auto bring = [&](const Heads& s, int h, Run<DTYPE, VE> (&to)[UNITS][2]) {
 #pragma unroll
-    for (int n = 0; n < kBatch; ++n)
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int h = h0 + n * kRows + group;
-        if (h >= s.to || lane + u * LANES >= units) continue;
-        const long long at = token * s.in_tok + h * s.in_head;
-        rows[n][u][0] = load_run<DTYPE, VE>(s.in, at + first[u]);
-        rows[n][u][1] = load_run<DTYPE, VE>(s.in, at + second[u]);
-      }
+    for (int u = 0; u < UNITS; ++u) {
+      if (h >= s.to || lane + u * LANES >= units) continue;
+      const long long at = token * s.in_tok + h * s.in_head;
+      to[u][0] = load_run<DTYPE, VE>(s.in, at + first[u]);
+      to[u][1] = load_run<DTYPE, VE>(s.in, at + second[u]);
+    }
   };
-  bring(side[0], side[0].from);
+#pragma unroll
+  for (int n = 0; n < kBatch; ++n) {
+    if (!kAhead || side[0].from < side[0].to) bring(side[0], side[0].from + n * kRows + group, rows[n]);
+    else bring(side[1], side[1].from + group, rows[n]);
+  }
 
   // the token's place on each axis; one without a place is left alone
   long long place[kMaxAxes];
@@ -171,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   if (bad && a.status && part == 0 && threadIdx.x % 32 == 0) atomicOr(a.status, CARRY_GDN_STATUS_BAD_RANGE);
   if (!there) return;
 
-  float cosine[UNITS][VE], sine[UNITS][VE];       // of its pairs; 1 and 0 where nothing is turned
+  alignas(8) float cosine[UNITS][VE], sine[UNITS][VE];       // of its pairs; 1 and 0 where nothing is turned
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
     const int unit = lane + u * LANES;
@@ -207,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   for (int which = 0; which < 2; ++which) {       // queries, then keys
     const Heads& s = side[which];
     if (s.from >= s.to) continue;
-    float w[UNITS][2][VE];
+    alignas(8) float w[UNITS][2][VE];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       if (lane + u * LANES >= units) continue;
@@ -220,23 +244,36 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
       }
     }
     for (int h0 = s.from; h0 < s.to; h0 += kRows * kBatch) {
-      if (which > 0 || h0 > s.from) bring(s, h0);
+      if (!kAhead && (which > 0 || h0 > s.from)) {
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) bring(s, h0 + n * kRows + group, rows[n]);
+      }
 #pragma unroll
       for (int n = 0; n < kBatch; ++n) {
         const int h = h0 + n * kRows + group;
         const bool mine = h < s.to;
-        if (h0 + n * kRows >= s.to) break;        // the same for all lanes
-        float x[UNITS][2][VE], sum = 0.0f;
+        alignas(8) float x[UNITS][2][VE];
+        float sum = 0.0f;
+        float2 sums = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
           numbers_of<DTYPE, VE>(rows[n][u][0], x[u][0]);
           numbers_of<DTYPE, VE>(rows[n][u][1], x[u][1]);
-          if (!mine || lane + u * LANES >= units) continue;
-#pragma unroll
-          for (int e = 0; e < VE; ++e) sum = fmaf(x[u][1][e], x[u][1][e], fmaf(x[u][0][e], x[u][0][e], sum));
         }
+        if (kAhead) {                             // of the same heads, or the keys' first one
+          if (h0 + kRows < s.to) bring(s, h0 + kRows + group, rows[n]);
+          else if (which == 0) bring(side[1], side[1].from + group, rows[n]);
+        }
+        if (h0 + n * kRows >= s.to) break;        // the same for all lanes
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          if (!mine || lane + u * LANES >= units) continue;
+          over_run<VE>([&](int e) { sums = fma2(pair(x[u][1], e), pair(x[u][1], e), fma2(pair(x[u][0], e), pair(x[u][0], e), sums)); },
+                       [&](int e) { sum = fmaf(x[u][1][e], x[u][1][e], fmaf(x[u][0][e], x[u][0][e], sum)); });
+        }
+        if (VE > 1) sum = sums.x + sums.y;
         sum = sum_over<LANES>(sum);
-        float by = rsqrtf(fmaf(sum, p.inv_width, a.eps)), unit = 1.0f;
+        float by = rsqrtf(fmaf(sum, p.inv_width, a.eps));
         if (__any_sync(~0u, sum == INFINITY)) {
           // squares beyond fp32: once more, in units of 2^100 (an infinity among the numbers makes the row NaN)
           float less = 0.0f;
@@ -245,26 +282,25 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
               if (lane + u * LANES >= units) continue;
-              const float s0 = x[u][0][e] * 0x1p-100f, s1 = x[u][1][e] * 0x1p-100f;
-              less = fmaf(s1, s1, fmaf(s0, s0, less));
+              if (sum == INFINITY) {
+                x[u][0][e] *= 0x1p-100f;
+                x[u][1][e] *= 0x1p-100f;
+              }
+              less = fmaf(x[u][1][e], x[u][1][e], fmaf(x[u][0][e], x[u][0][e], less));
             }
           less = sum_over<LANES>(less);
-          if (sum == INFINITY) {
-            by = less == INFINITY ? NAN : rsqrtf(less * p.inv_width);
-            unit = 0x1p-100f;
-          }
+          if (sum == INFINITY) by = less == INFINITY ? NAN : rsqrtf(less * p.inv_width);
         }
         if (!mine) continue;
         const long long to_at = token * s.out_tok + h * s.out_head;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
           if (lane + u * LANES >= units) continue;
-          float y[2][VE], z[2][VE];
+          alignas(8) float y[2][VE], z[2][VE];
 #pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            y[0][e] = x[u][0][e] * unit * by * w[u][0][e];
-            y[1][e] = x[u][1][e] * unit * by * w[u][1][e];
-          }
+          for (int i = 0; i < 2; ++i)
+            over_run<VE>([&](int e) { pair(y[i], e) = mul2(mul2(pair(x[u][i], e), make_float2(by, by)), pair(w[u][i], e)); },
+                         [&](int e) { y[i][e] = x[u][i][e] * by * w[u][i][e]; });
           if (lane + u * LANES >= turned) {
 #pragma unroll
             for (int e = 0; e < VE; ++e) { z[0][e] = y[0][e]; z[1][e] = y[1][e]; }
@@ -276,11 +312,16 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
               z[2 * e / VE][(2 * e + 1) % VE] = two * cosine[u][e] + one * sine[u][e];
             }
           } else {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              z[0][e] = y[0][e] * cosine[u][e] - y[1][e] * sine[u][e];
-              z[1][e] = y[1][e] * cosine[u][e] + y[0][e] * sine[u][e];
-            }
+            over_run<VE>(
+                [&](int e) {
+                  const float2 c = pair(cosine[u], e), s = pair(sine[u], e), one = pair(y[0], e), two = pair(y[1], e);
+                  pair(z[0], e) = sub2(mul2(one, c), mul2(two, s));
+                  pair(z[1], e) = fma2(two, c, mul2(one, s));
+                },
+                [&](int e) {
+                  z[0][e] = y[0][e] * cosine[u][e] - y[1][e] * sine[u][e];
+                  z[1][e] = y[1][e] * cosine[u][e] + y[0][e] * sine[u][e];
+                });
           }
           store_numbers<DTYPE, VE>(s.out, to_at + first[u], z[0]);
           store_numbers<DTYPE, VE>(s.out, to_at + second[u], z[1]);
