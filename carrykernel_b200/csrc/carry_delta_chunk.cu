@@ -1352,7 +1352,7 @@ int launch_chunks(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
         rc = launch_dependent(unit_kernel<DTYPE, D>, dim3((unsigned)(p.chunks + kUnitWarps - 1) / kUnitWarps, (unsigned)a.HV, (unsigned)requests), kUnitWarps * 32, smem,
                               stream, p);
       if (rc != CARRY_GDN_OK) return rc;
-      // one CTA to a processor while that is all there are
+      // one CTA to a processor while that is all there are (a prompt of 2048 tokens with 32 heads: 117 us, 146 in the other form; two of them 228 and 211)
       if constexpr (DTYPE == CARRY_BF16) rc = (int64_t)requests * a.HV * (D / kColumns) <= sm_count() ? launch_sequence<DTYPE, D, 4, 2>(p, requests, stream) : launch_sequence<DTYPE, D, 2, 1>(p, requests, stream);
       else rc = launch_sequence<DTYPE, D, 4, 1>(p, requests, stream);
       if (rc != CARRY_GDN_OK) return rc;
