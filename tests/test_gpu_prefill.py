@@ -412,3 +412,22 @@ def test_two_streams_at_once_and_a_state_for_all(lengths):
     torch.cuda.synchronize()
     for j, (out, final) in enumerate(results):
         assert torch.equal(out, alone[j // 8][0]) and torch.equal(final, alone[j // 8][1]), j
+
+
+@pytest.mark.parametrize("lengths", [[35, 34, 1], [5, 65, 0]], ids=str)
+def test_offsets_beyond_32_bits(lengths):
+    """Rows, outputs and states that lie more than 2^31 numbers apart."""
+    H, HV, D, N, B = 1, 2, 64, sum(lengths), len(lengths)
+    c, state = make(lengths, H, HV, D, BF16, True)
+    alone = run(c, state, lengths, HV, D)
+    stride, state_stride = 2 ** 25, 2 ** 30 + 4
+    buffer = torch.empty(N * stride, dtype=BF16, device=DEV)
+    width = c["mixed_qkv"].shape[1]
+    mixed, out = buffer.as_strided((N, width), (stride, 1)), buffer.as_strided((N, HV, D), (stride, D, 1), 4096)
+    mixed.copy_(c["mixed_qkv"])
+    states = torch.empty(2 * state_stride + HV * D * D, device=DEV).as_strided((B, HV, D, D), (state_stride, D * D, D, 1))
+    states.copy_(state)
+    dev = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in c.items() if k != "mixed_qkv"}
+    pp.gated_delta_rule_packed_prefill(mixed, **dev, out=out, final_state=states, initial_state=states, query_start=starts(lengths).to(DEV),
+                                       max_query_len=max(lengths), use_qk_l2norm_in_kernel=True)
+    assert (N - 1) * stride > 2 ** 31 and torch.equal(out, alone[0]) and torch.equal(states, alone[1])

@@ -166,3 +166,18 @@ def test_numbers_whose_squares_are_below_fp32():
     qk_norm_rope(q, k, qw.to(DEV), kw.to(DEV), cos_sin.to(DEV), positions.to(DEV))
     check(q, qkv[:, :HQ], qw, cos_sin, positions)
     check(k, qkv[:, HQ:HQ + HK], kw, cos_sin, positions)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_offsets_beyond_32_bits(shift):
+    """Rows and table rows that lie more than 2^31 numbers apart."""
+    N, HQ, HK, D, stride = 70, 3, 2, 64, 2 ** 25 + shift
+    qkv, qw, kw, cos_sin, positions = make(N, HQ, HK, D, D, BF16, P=N)
+    buffer = torch.empty(N * stride, dtype=BF16, device=DEV)
+    q, k = buffer.as_strided((N, HQ, D), (stride, D, 1)), buffer.as_strided((N, HK, D), (stride, D, 1), 512)
+    table = torch.empty(N * stride, device=DEV).as_strided((N, D), (stride, 1))
+    q.copy_(qkv[:, :HQ]), k.copy_(qkv[:, HQ:HQ + HK]), table.copy_(cos_sin)
+    positions[0] = N - 1
+    qk_norm_rope(q, k, qw.to(DEV), kw.to(DEV), table, positions.to(DEV))
+    check(q, qkv[:, :HQ], qw, cos_sin, positions)
+    check(k, qkv[:, HQ:HQ + HK], kw, cos_sin, positions)
