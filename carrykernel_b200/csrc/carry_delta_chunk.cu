@@ -7,7 +7,7 @@
 //   U = T R,   O = diag(exp G) (scale Q) S + (P T) R,   S' = exp(G_64) S + K^T diag(exp(G_64 - G)) U.
 //
 // T and P T do not depend on the state: unit_kernel (prepare_kernel for fp32) forms them for every chunk and head side by side.  sequence_kernel
-// then walks a request's chunks, a CTA for 32 columns of a head's state, with three products to a chunk that wait for one another:
+// then walks a request's chunks, a CTA for 32 or 64 columns of a head's state, with three products to a chunk that wait for one another:
 //   [K; Q] S  (128 x 32, over K),   [T; P T] R  (128 x 32, over 64 tokens),   K^T U  (K x 32, over 64 tokens).
 // The state itself stays in registers, in fp32; its products take it as a sum of bf16 numbers.
 //
@@ -879,36 +879,35 @@ __device__ __forceinline__ void test_come_late(int, int) {}
 __device__ __forceinline__ uint32_t test_extra_bytes(int, int, int) { return 0; }
 #endif
 
-constexpr int kColumns = 32;                      // of the state to a CTA
 
-// Right sides lie with their three terms side by side, so that one product takes all terms and reads its left side once: two of them in a
-// plane of 64 columns, the third in the first half of another one.  Where two CTAs share a processor, the second half of the state's other plane
-// has the third term of R and U.
-template <int DTYPE, int D, int STAGES>
+// A CTA has 32 or 64 columns of a head's state.  Right sides lie with their three terms side by side, so that one product takes all terms and
+// reads its left side once: each in a plane of 64 columns, or two of 32 in one and the third in the first half of another.  Where two CTAs share
+// a processor, the second half of the state's other plane has the third term of R and U.
+template <int DTYPE, int D, int STAGES, int COLUMNS>
 struct SequenceShared {
-  static constexpr bool kAlone = STAGES == 2;
+  static constexpr bool kAlone = STAGES == 2, kWide = COLUMNS == 64;
   uint8_t kq[STAGES][kTermsX<DTYPE>][D / 64][kPlane], t[STAGES][kTermsT<DTYPE>][kPlane];
-  uint8_t u[kAlone ? 2 : 1][kChunk * 128], s[2][D * 128];     // R, and then U with its decays; the state
-  alignas(16) uint8_t v[kAlone ? 1 : kChunk][kColumns * (DTYPE == CARRY_F32 ? 4 : 2)];
+  uint8_t u[kWide ? 3 : kAlone ? 2 : 1][kChunk * 128], s[kWide ? 3 : 2][D * 128];     // R, and then U with its decays; the state
+  alignas(16) uint8_t v[kAlone ? 1 : kChunk][COLUMNS * (DTYPE == CARRY_F32 ? 4 : 2)];
   alignas(16) float vec[2][kVec];
   // what has come, and what is free again: with one stage keys, queries, T and values are each asked for again as soon as they have been used
   uint64_t full[STAGES], free[STAGES], q_full, t_full, v_full, vec_full[2], q_free, t_free, v_free;
   uint64_t s_ready, r_ready, u_ready, scored, solved, added;
   // of a chunk: the first token whose value in a column is not finite, and whether there is one; for three chunks in turn, of which one is being
   // written, one read and one made ready
-  int bad[3][kColumns], any_bad[3];
+  int bad[3][COLUMNS], any_bad[3];
   uint32_t tmem;
   int poison;
 };
 
 // this thread's columns of each term's product, summed, the smallest first
-template <int W>
+template <int W, int COLUMNS>
 __device__ __forceinline__ void load_sums(uint32_t at, float2 (&x)[W / 2]) {
   uint32_t r[kTerms][W];
 #pragma unroll
   for (int t = 0; t < kTerms; ++t) {
-    if constexpr (W == 8) tmem_load8(at + t * kColumns, r[t]);
-    else tmem_load16(at + t * kColumns, r[t]);
+    if constexpr (W == 8) tmem_load8(at + t * COLUMNS, r[t]);
+    else tmem_load16(at + t * COLUMNS, r[t]);
   }
   wait_loads();
   auto two = [&](int t, int j) { return make_float2(__uint_as_float(r[t][j]), __uint_as_float(r[t][j + 1])); };
@@ -918,12 +917,12 @@ __device__ __forceinline__ void load_sums(uint32_t at, float2 (&x)[W / 2]) {
 
 // GROUPS of 128 threads share a row's columns.  With two stages of operands a CTA has a processor for itself, and what counts is the chain of a
 // chunk's products; with one, two CTAs share a processor, and what one waits for the other uses.
-template <int DTYPE, int D, int GROUPS, int STAGES>
+template <int DTYPE, int D, int GROUPS, int STAGES, int COLUMNS>
 __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CARRY_BF16 ? 2 : 1) sequence_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64, W = kColumns / GROUPS;
+  constexpr int kX = kTermsX<DTYPE>, kT = kTermsT<DTYPE>, kPlanes = D / 64, W = COLUMNS / GROUPS;
   constexpr int kRowThreads = GROUPS * 128, kLoadWarp = kRowThreads / 32, kIssueWarp = kLoadWarp + 1, kValueBytes = DTYPE == CARRY_F32 ? 4 : 2;
-  using Shared = SequenceShared<DTYPE, D, STAGES>;
-  constexpr bool kAlone = Shared::kAlone;
+  using Shared = SequenceShared<DTYPE, D, STAGES, COLUMNS>;
+  constexpr bool kAlone = Shared::kAlone, kWide = Shared::kWide;
   extern __shared__ uint8_t raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024 - (smem_addr(raw) & 1023)) & 1023));
   depend_release();
@@ -952,12 +951,12 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
     barrier_init(&sh.added, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid < 3 * kColumns) {
-    sh.bad[tid / kColumns][tid % kColumns] = kChunk;
-    sh.any_bad[tid / kColumns] = 0;
+  if (tid < 3 * COLUMNS) {
+    sh.bad[tid / COLUMNS][tid % COLUMNS] = kChunk;
+    sh.any_bad[tid / COLUMNS] = 0;
   }
   // columns 0 and on: [K; Q] S, and, when that is read, K^T U; behind them [T; P T] R
-  constexpr uint32_t kSolvedAt = kTerms * kColumns, kTmem = 256;
+  constexpr uint32_t kSolvedAt = kTerms * COLUMNS, kTmem = kWide ? 512 : 256;
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "n"(kTmem) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -971,13 +970,13 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
 
   if (tid < kRowThreads) {
     // ---- a row to a thread, some of its columns: of the products' rows (keys, queries), and of the state's (K) ----
-    const int row = warp % 4 * 32 + lane, first = warp / 4 * W, column0 = blockIdx.x * kColumns + first, token = row % kChunk;
+    const int row = warp % 4 * 32 + lane, first = warp / 4 * W, column0 = blockIdx.x * COLUMNS + first, token = row % kChunk;
     const uint32_t at = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + first;
     const bool key = row < kChunk, has_state = row < D;
     uint8_t* const third = kAlone ? sh.u[kAlone] : sh.s[1];   // where R's and U's third term lies, and its first column there
-    constexpr int kThirdColumn = kAlone ? 0 : kColumns;
+    constexpr int kThirdColumn = kAlone ? 0 : COLUMNS;
     // this thread's numbers into an operand's terms; `last`: of the third one
-    auto put = [&](uint8_t* tile, uint8_t* last, int last_column, float2 (&x)[W / 2]) {
+    auto put = [&](uint8_t* tile, int plane, uint8_t* last, int last_column, float2 (&x)[W / 2]) {
 #pragma unroll
       for (int j = 0; j < W; j += 8)
 #pragma unroll
@@ -985,7 +984,8 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = take_term(x[j / 2 + e]);
-          uint8_t* to = t < 2 ? tile + plane_at(row, (t * kColumns + first + j) / 8) : last + plane_at(row, (last_column + first + j) / 8);
+          uint8_t* to = kWide ? tile + t * plane + plane_at(row, (first + j) / 8)
+                        : t < 2 ? tile + plane_at(row, (t * COLUMNS + first + j) / 8) : last + plane_at(row, (last_column + first + j) / 8);
           *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     };
@@ -1001,7 +1001,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
         float2 x[W / 2];
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = S[j];
-        put(sh.s[0], sh.s[1], 0, x);
+        put(sh.s[0], D * 128, sh.s[1], 0, x);
         fence_proxy();
       }
       fence_before();
@@ -1065,11 +1065,11 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       healthy = healthy && wait(&sh.scored, parity);
       if (!healthy) break;
       fence_after();
-      load_sums<W>(at, x);
+      load_sums<W, COLUMNS>(at, x);
       if (key) {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = fma2(make_float2(of_state, of_state), x[j], o[j]);
-        put(sh.u[0], third, kThirdColumn, x);
+        put(sh.u[0], kChunk * 128, third, kThirdColumn, x);
         fence_proxy();
         fence_before();
         barrier_arrive(&sh.r_ready);
@@ -1082,18 +1082,18 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
         barrier_arrive(&sh.u_ready);
       }
       test_come_late(warp, c + 1);
-      if (tid < kColumns) sh.bad[(c + 2) % 3][tid] = kChunk;
+      if (tid < COLUMNS) sh.bad[(c + 2) % 3][tid] = kChunk;
       if (tid == 0) sh.any_bad[(c + 2) % 3] = 0;
       healthy = wait(&sh.solved, parity);
       if (!healthy) break;
       const int* bad = sh.bad[c % 3] + first;
       const bool spoilt = sh.any_bad[c % 3];
       fence_after();
-      load_sums<W>(at + kSolvedAt, x);
+      load_sums<W, COLUMNS>(at + kSolvedAt, x);
       if (key) {
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) x[j] = mul2(make_float2(of_added, of_added), x[j]);
-        put(sh.u[0], third, kThirdColumn, x);
+        put(sh.u[0], kChunk * 128, third, kThirdColumn, x);
         fence_proxy();
         fence_before();
         barrier_arrive(&sh.u_ready);
@@ -1138,7 +1138,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       healthy = healthy && wait(&sh.added, parity);
       if (!healthy) break;
       fence_after();
-      load_sums<W>(at, x);
+      load_sums<W, COLUMNS>(at, x);
 #pragma unroll
       for (int j = 0; j < W / 2; ++j) S[j] = fma2(make_float2(decay, decay), S[j], x[j]);
       if (spoilt) {
@@ -1155,7 +1155,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
     }
   } else if (warp == kLoadWarp) {
     // ---- tiles and factors out of the workspace, values out of the rows ----
-    constexpr uint32_t kBytesKq = kX * kPlanes * kPlane, kBytesT = kT * kPlane, kSide = kPlane / 2, kBytesV = kColumns * kValueBytes;
+    constexpr uint32_t kBytesKq = kX * kPlanes * kPlane, kBytesT = kT * kPlane, kSide = kPlane / 2, kBytesV = COLUMNS * kValueBytes;
     for (int c = 0; c < chunks; ++c) {
       const int stage = c % STAGES;
       const bool reused = c >= STAGES;
@@ -1181,7 +1181,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       // in the order in which what was there is done with
       if (reused && !wait(&sh.v_free, turn)) break;
       const int tokens = min(left - c * kChunk, kChunk);
-      const long long at = (long long)(place.first + from + c * kChunk) * a.stride_mixed_tok + (2 * a.H + hv) * D + blockIdx.x * kColumns;
+      const long long at = (long long)(place.first + from + c * kChunk) * a.stride_mixed_tok + (2 * a.H + hv) * D + blockIdx.x * COLUMNS;
       if (p.aligned) {                            // sixteen bytes at a time: bulk copies of such short rows would hold up the tiles'
         for (int i = lane; i < tokens * (int)(kBytesV / 16); i += 32) {
           const int token = i / (kBytesV / 16), part = i % (kBytesV / 16) * 16;
@@ -1189,9 +1189,12 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&sh.v_full)) : "memory");
       } else {
-        for (int i = 0; i < tokens; ++i) {
-          if constexpr (kValueBytes == 4) reinterpret_cast<float*>(sh.v[i])[lane] = reinterpret_cast<const float*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
-          else reinterpret_cast<uint16_t*>(sh.v[i])[lane] = reinterpret_cast<const uint16_t*>(a.mixed_qkv)[at + i * a.stride_mixed_tok + lane];
+        for (int i = 0; i < tokens * (COLUMNS / 32); ++i) {
+          const int token = i / (COLUMNS / 32), column = i % (COLUMNS / 32) * 32 + lane;
+          if constexpr (kValueBytes == 4)
+            reinterpret_cast<float*>(sh.v[token])[column] = reinterpret_cast<const float*>(a.mixed_qkv)[at + token * a.stride_mixed_tok + column];
+          else
+            reinterpret_cast<uint16_t*>(sh.v[token])[column] = reinterpret_cast<const uint16_t*>(a.mixed_qkv)[at + token * a.stride_mixed_tok + column];
         }
         barrier_arrive(&sh.v_full);
       }
@@ -1217,7 +1220,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
     // ---- products: a left side's term x with the right side's terms 0 .. kTerms - 1 - x, which are its next columns ----
     const uint32_t elected = elect(), base = __shfl_sync(~0u, tmem, 0);
     // the third term lies that far behind the first two
-    const uint32_t state = operand(sh.s[0], D * 128), rows = operand(sh.u[0], kAlone ? kChunk * 128 : smem_addr(sh.s[1]) + kColumns * 2 - smem_addr(sh.u[0]));
+    const uint32_t state = operand(sh.s[0], D * 128), rows = operand(sh.u[0], kAlone || kWide ? kChunk * 128 : smem_addr(sh.s[1]) + COLUMNS * 2 - smem_addr(sh.u[0]));
     for (int c = 0; c < chunks; ++c) {
       const int parity = c & 1, stage = c % STAGES;
       const uint32_t turn = c / STAGES & 1;
@@ -1230,7 +1233,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           mma_shared(elected, base, kq + x * (kPlanes * kPlane / 16) + k / 4 * (kPlane / 16) + k % 4 * 2, state + k * 128,
-                     instruction_bf16((kTerms - x) * kColumns, false, true), x + k > 0);
+                     instruction_bf16((kTerms - x) * COLUMNS, false, true), x + k > 0);
       mma_commit(elected, &sh.scored);
       if (!kAlone) mma_commit(elected, &sh.q_free);
       if ((!kAlone && !wait(&sh.t_full, turn)) || !wait(&sh.r_ready, parity)) break;
@@ -1239,7 +1242,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       for (int x = 0; x < kT; ++x)
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k)
-          mma_shared(elected, base + kSolvedAt, t + x * (kPlane / 16) + k * 2, rows + k * 128, instruction_bf16((kTerms - x) * kColumns, false, true), x + k > 0);
+          mma_shared(elected, base + kSolvedAt, t + x * (kPlane / 16) + k * 2, rows + k * 128, instruction_bf16((kTerms - x) * COLUMNS, false, true), x + k > 0);
       mma_commit(elected, &sh.solved);
       if (!kAlone) mma_commit(elected, &sh.t_free);
       if (!wait(&sh.u_ready, parity)) break;
@@ -1248,7 +1251,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       for (int x = 0; x < kX; ++x)
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k)
-          mma_shared(elected, base, keys + x * (kPlanes * kPlane / 16) + k * 128, rows + k * 128, instruction_bf16((kTerms - x) * kColumns, true, true), x + k > 0);
+          mma_shared(elected, base, keys + x * (kPlanes * kPlane / 16) + k * 128, rows + k * 128, instruction_bf16((kTerms - x) * COLUMNS, true, true), x + k > 0);
       mma_commit(elected, &sh.added);
       mma_commit(elected, &sh.free[stage]);
     }
@@ -1310,15 +1313,15 @@ int allow_shared(K kernel, size_t smem, bool (&ready)[64]) {
   return CARRY_GDN_OK;
 }
 
-template <int DTYPE, int D, int GROUPS, int STAGES>
+template <int DTYPE, int D, int GROUPS, int STAGES, int COLUMNS>
 int launch_sequence(const ChunkParams& p, int requests, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(SequenceShared<DTYPE, D, STAGES>) + 1024;
+  constexpr size_t smem = sizeof(SequenceShared<DTYPE, D, STAGES, COLUMNS>) + 1024;
   static_assert(smem <= 227 * 1024, "a CTA's shared memory");
   static_assert(STAGES == 2 || DTYPE != CARRY_BF16 || 2 * (smem + 1024) <= 228 * 1024, "two CTAs to a processor");
   static thread_local bool ready[64];
-  const int rc = allow_shared(sequence_kernel<DTYPE, D, GROUPS, STAGES>, smem, ready);
+  const int rc = allow_shared(sequence_kernel<DTYPE, D, GROUPS, STAGES, COLUMNS>, smem, ready);
   if (rc != CARRY_GDN_OK) return rc;
-  return launch_dependent(sequence_kernel<DTYPE, D, GROUPS, STAGES>, dim3(D / kColumns, (unsigned)p.a.HV, (unsigned)requests), GROUPS * 128 + 64, smem, stream, p);
+  return launch_dependent(sequence_kernel<DTYPE, D, GROUPS, STAGES, COLUMNS>, dim3(D / COLUMNS, (unsigned)p.a.HV, (unsigned)requests), GROUPS * 128 + 64, smem, stream, p);
 }
 
 template <int DTYPE, int D>
@@ -1353,8 +1356,13 @@ int launch_chunks(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
                               stream, p);
       if (rc != CARRY_GDN_OK) return rc;
       // one CTA to a processor while that is all there are (a prompt of 2048 tokens with 32 heads: 117 us, 146 in the other form; two of them 228 and 211)
-      if constexpr (DTYPE == CARRY_BF16) rc = (int64_t)requests * a.HV * (D / kColumns) <= sm_count() ? launch_sequence<DTYPE, D, 4, 2>(p, requests, stream) : launch_sequence<DTYPE, D, 2, 1>(p, requests, stream);
-      else rc = launch_sequence<DTYPE, D, 4, 1>(p, requests, stream);
+      // More CTAs than that: in bf16 two to a processor (sixteen prompts of 4096 tokens 2.40 ms, 2.59 with 64 columns to one CTA); in fp16, whose keys and
+      // queries fill shared memory, 64 columns, for which the left sides are read once and not twice (two prompts of 3001: 323 us and not 410); in
+      // fp32 as well where there is room, at 64 wide (eight of 1000: 384 us and not 441).
+      const bool alone = (int64_t)requests * a.HV * (D / 32) <= sm_count();
+      if constexpr (DTYPE == CARRY_BF16) rc = alone ? launch_sequence<DTYPE, D, 4, 2, 32>(p, requests, stream) : launch_sequence<DTYPE, D, 2, 1, 32>(p, requests, stream);
+      else if constexpr (DTYPE == CARRY_F16 || D == 64) rc = alone ? launch_sequence<DTYPE, D, 4, 1, 32>(p, requests, stream) : launch_sequence<DTYPE, D, 4, 1, 64>(p, requests, stream);
+      else rc = launch_sequence<DTYPE, D, 4, 1, 32>(p, requests, stream);
       if (rc != CARRY_GDN_OK) return rc;
     }
   return CARRY_GDN_OK;

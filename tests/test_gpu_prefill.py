@@ -305,7 +305,8 @@ def test_alike_keys_and_zero_rows():
 
 
 @pytest.mark.parametrize("dtype,D,H,HV,lengths", [(F32, 64, 2, 4, [97]), (BF16, 128, 8, 16, [300, 77, 64, 500]), (F32, 128, 8, 16, [300, 77, 64, 500]),
-                                                  (F16, 128, 16, 32, [130] * 20), (BF16, 64, 1, 2, [700]), (BF16, 128, 16, 32, [1000, 1, 90])])
+                                                  (F16, 128, 16, 32, [130] * 20), (BF16, 64, 1, 2, [700]), (BF16, 128, 16, 32, [1000, 1, 90]),
+                                                  (F16, 128, 16, 32, [1000, 1, 90]), (F32, 64, 16, 32, [500, 90, 200])])
 def test_repeated_calls_give_the_same_numbers(dtype, D, H, HV, lengths):
     """Warps and copies that meet at other times: every call's numbers are the first one's."""
     c, state = make(lengths, H, HV, D, dtype, True)
@@ -431,3 +432,24 @@ def test_offsets_beyond_32_bits(lengths):
     pp.gated_delta_rule_packed_prefill(mixed, **dev, out=out, final_state=states, initial_state=states, query_start=starts(lengths).to(DEV),
                                        max_query_len=max(lengths), use_qk_l2norm_in_kernel=True)
     assert (N - 1) * stride > 2 ** 31 and torch.equal(out, alone[0]) and torch.equal(states, alone[1])
+
+
+@pytest.mark.parametrize("dtype,D,lengths", [(F16, 128, [130, 77]), (F16, 64, [65, 3, 140]), (F32, 64, [97, 64, 129]), (BF16, 128, [70, 130])], ids=str)
+@pytest.mark.parametrize("shift", [0, 1])
+def test_more_heads_than_processors(dtype, D, lengths, shift):
+    """The forms that share a processor, or have more of a state's columns: aligned rows and others, and a value that is not finite."""
+    H, HV = 16, 32
+    c, state = make(lengths, H, HV, D, dtype, True)
+    width, N = c["mixed_qkv"].shape[1], sum(lengths)
+    rows = torch.empty(N, width + 3, dtype=dtype, device=DEV)[:, shift:shift + width] if shift else torch.empty(N, width, dtype=dtype, device=DEV)
+    rows.copy_(c["mixed_qkv"])
+    got = run(dict(c, mixed_qkv=rows), state, lengths, HV, D)
+    assert _lib.load_library().carry_gdn_last_kernel() == IN_CHUNKS
+    check(got, c, state, lengths, H, D, in_chunks=True)
+    head, column, at = HV - 1, D - 1, lengths[0] - 1
+    rows[at, 2 * H * D + head * D + column] = float("inf")
+    out, final = run(dict(c, mixed_qkv=rows), state, lengths, HV, D)
+    bad, bad_state = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(final, dtype=torch.bool)
+    bad[at, head, column], bad_state[0, head, column] = True, True
+    assert torch.equal(out[~bad], got[0][~bad]) and torch.equal(final[~bad_state], got[1][~bad_state])
+    assert not out[bad].isfinite().any() and not final[bad_state].isfinite().any()
