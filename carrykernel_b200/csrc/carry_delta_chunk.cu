@@ -114,9 +114,9 @@ struct PrepareShared {
   };
   uint8_t t[kTerms][kPlane];              // rows 0 .. 63 D, then T; 64 .. 127 P D, then P T
   alignas(16) float L[2][kHalf][kPad];    // the blocks of L on the diagonal
-  // of a token: running sum of log2 alpha within its half; decay from the first half's token to that half's end, or from there to the
+  // of a token: running sum of log2 alpha within its half, as two numbers; decay from the first half's token to that half's end, or from there to the
   // second half's token; decays from the chunk's start to the token and from there to the chunk's end; beta
-  alignas(16) float G[kChunk], to_middle[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk];
+  alignas(16) float G[kChunk], G_less[kChunk], to_middle[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk];
   alignas(16) float norm[2 * kChunk];     // what makes a key a unit one, and a query one times `scale`
   int live_keys[kRowWarps], live_gates;
   float decay;                            // of the chunk
@@ -135,7 +135,14 @@ __device__ __forceinline__ float exp2_of(double x) {
   return exp2_quick(hi) * fmaf((float)(x - hi), kLn2, 1.0f);
 }
 
-// A chunk's gates, by one warp; lane l has tokens 2 l and 2 l + 1.  Sums of decays are formed in 64 bits; what fp32 has to hold of them, for
+// A running sum of log2 alpha as two fp32 numbers, some 48 bits.  A decay is the exponential of a difference of two such sums, and a strong decay
+// ahead of both tokens makes the sums large without changing the difference: with one number each, of sums near 1000, it would be 6e-5 off.
+__device__ __forceinline__ void two_numbers(double x, float& hi, float& lo) {
+  hi = (float)x;
+  lo = (float)(x - hi);
+}
+
+// A chunk's gates, by one warp; lane l has tokens 2 l and 2 l + 1.  Sums of decays are formed in 64 bits; what is kept of them, for
 // differences, is the sum within half a chunk.
 template <class Shared>
 __device__ __forceinline__ void chunk_gates(const ChunkParams& p, Shared& sh, long long row, int n, int hv) {
@@ -166,7 +173,7 @@ __device__ __forceinline__ void chunk_gates(const ChunkParams& p, Shared& sh, lo
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int i = 2 * lane + e;
-    sh.G[i] = (float)(i < kHalf ? G[e] : G[e] - middle);
+    two_numbers(i < kHalf ? G[e] : G[e] - middle, sh.G[i], sh.G_less[i]);
     sh.to_middle[i] = exp2_of(i < kHalf ? middle - G[e] : G[e] - middle);
     sh.from_start[i] = exp2_of(G[e]);
     sh.to_end[i] = exp2_of(last - G[e]);
@@ -333,7 +340,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
   __syncthreads();
   if (warp < kRowWarps) {
     // L and P.  Between the halves of a chunk a decay is a product of two that end in the middle; both are at most 1.
-    const float G = sh.G[i], by = key ? sh.beta[i] * sh.norm[i] : sh.norm[row];
+    const float G = sh.G[i], G_less = sh.G_less[i], by = key ? sh.beta[i] * sh.norm[i] : sh.norm[row];
     const bool below = first < i / kHalf * kHalf, diagonal = first == i / kHalf * kHalf;    // the same for all lanes
     float2 x[16];
     if (below || diagonal) {
@@ -345,7 +352,9 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {
         const float4 g = *reinterpret_cast<const float4*>(&sh.G[first + j]), m = *reinterpret_cast<const float4*>(&sh.norm[first + j]);
-        const float2 d[2] = {make_float2(exp2_quick(G - g.x), exp2_quick(G - g.y)), make_float2(exp2_quick(G - g.z), exp2_quick(G - g.w))};
+        const float4 l = *reinterpret_cast<const float4*>(&sh.G_less[first + j]);
+        const float2 d[2] = {make_float2(exp2_quick(G - g.x + (G_less - l.x)), exp2_quick(G - g.y + (G_less - l.y))),
+                             make_float2(exp2_quick(G - g.z + (G_less - l.z)), exp2_quick(G - g.w + (G_less - l.w)))};
         const float2 f[2] = {make_float2(m.x, m.y), make_float2(m.z, m.w)};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -489,9 +498,9 @@ struct alignas(16) Unit {
   float2 L[6][4][32], P[10][4][32];       // a lane's numbers of the blocks below the diagonal, and of all
   float D[kBlocks][kBlock][20];           // the blocks of L on the diagonal, then their inverses
   uint8_t rows[2][kBlock * 128];          // sixteen rows of a tile on their way out
-  // of a token: running sum of log2 alpha within its block, decay from the block's start, decay to the block's end, decays from the
+  // of a token: running sum of log2 alpha within its block, as two numbers, decay from the block's start, decay to the block's end, decays from the
   // chunk's start and to its end, beta, norms of key and query
-  float G[kChunk], from_block[kChunk], to_block[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk], key[kChunk], query[kChunk];
+  float G[kChunk], G_less[kChunk], from_block[kChunk], to_block[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk], key[kChunk], query[kChunk];
 };
 
 template <bool HALF>
@@ -536,7 +545,7 @@ __device__ __forceinline__ void store_transposed(uint32_t to, const uint32_t (&w
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-// Gates of a chunk: lane l has tokens 2 l and 2 l + 1, whose inputs it has read.  Sums of decays are formed in 64 bits; what fp32 has to hold of
+// Gates of a chunk: lane l has tokens 2 l and 2 l + 1, whose inputs it has read.  Sums of decays are formed in 64 bits; what is kept of
 // them, for differences, is the sum within a block.  `live`: tokens that count; less, when a gate among them is no number.  Returns the decays over
 // the second block, over the third, and over the chunk.
 __device__ __forceinline__ float3 unit_gates(Unit& sh, const GateInputs (&in)[2], int& live) {
@@ -568,7 +577,7 @@ __device__ __forceinline__ float3 unit_gates(Unit& sh, const GateInputs (&in)[2]
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int i = 2 * lane + e;
-    sh.G[i] = (float)(G[e] - start);
+    two_numbers(G[e] - start, sh.G[i], sh.G_less[i]);
     sh.from_block[i] = exp2_of(G[e] - start);
     sh.to_block[i] = exp2_of(end - G[e]);
     sh.from_start[i] = exp2_of(G[e]);
@@ -693,13 +702,13 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
     load_quarters<D>(p, row0, n, b * kBlock, h * D, q);
     float decay[2][4];
     {
-      const float gi[2] = {sh.G[i0], sh.G[i0 + 8]}, by[2] = {sh.beta[i0] * sh.key[i0], sh.beta[i0 + 8] * sh.key[i0 + 8]};
+      const float gi[2] = {sh.G[i0], sh.G[i0 + 8]}, less[2] = {sh.G_less[i0], sh.G_less[i0 + 8]}, by[2] = {sh.beta[i0] * sh.key[i0], sh.beta[i0 + 8] * sh.key[i0 + 8]};
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = 8 * x + 2 * t + e % 2, i = g + e / 2 * 8;
-          decay[x][e] = j <= i ? exp2_quick(gi[e / 2] - sh.G[b * kBlock + j]) * sh.key[b * kBlock + j] : 0.0f;
+          decay[x][e] = j <= i ? exp2_quick(gi[e / 2] - sh.G[b * kBlock + j] + (less[e / 2] - sh.G_less[b * kBlock + j])) * sh.key[b * kBlock + j] : 0.0f;
           sh.D[b][i][j] = j < i ? diagonal[b].x[x][e] * by[e / 2] * decay[x][e] : 0.0f;
         }
 #pragma unroll
