@@ -31,7 +31,8 @@
 namespace carry {
 namespace {
 
-constexpr int kChunk = 64, kPlane = 128 * 128, kVec = 4 * kChunk + 8, kTerms = 3;
+// of a chunk's factors: its decay, and behind it a number that is not 0 where a wait ran out before T was there
+constexpr int kChunk = 64, kPlane = 128 * 128, kDecayAt = 4 * kChunk, kVec = kDecayAt + 8, kTerms = 3;
 constexpr float kLn2 = 0.69314718055994531f, kLeastLog = -200.0f;
 
 struct ChunkParams {
@@ -57,6 +58,22 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int z, int* stat
   const PrefillRequest r = prefill_request(p.a, b, status);
   return {r.first, r.count, p.packed ? r.first / kChunk + b : (long long)z * p.chunks};
 }
+
+// In the test-only build warps of every kind come late to some of their chunks, by more than the others' work on one: results must not depend on
+// it.  And there, of three value heads, the first copies of head 1's first chunk announce 16 bytes more than they bring: a wait runs out, and the
+// head's rows and state are left as they were.  Of five value heads in fp32, nothing announces the end of the first product of head 1's second chunk,
+// of the second one of head 2's and of the third one of head 3's.
+#ifdef CARRY_TEST_WAIT_EXPIRY
+__device__ __forceinline__ void test_come_late(int warp, int c) {
+  if (warp % 4 == c % 4 || (warp + c) % 5 == 0) __nanosleep(4000);
+}
+__device__ __forceinline__ uint32_t test_extra_bytes(int heads, int hv, int c) { return heads == 3 && hv == 1 && c == 0 ? 16 : 0; }
+__device__ __forceinline__ bool test_no_commit(int heads, int hv, int chunk, int product) { return heads == 5 && hv == 1 + product && chunk == 1; }
+#else
+__device__ __forceinline__ void test_come_late(int, int) {}
+__device__ __forceinline__ uint32_t test_extra_bytes(int, int, int) { return 0; }
+__device__ __forceinline__ bool test_no_commit(int, int, int, int) { return false; }
+#endif
 
 // bf16 numbers that a key's or query's numbers come as, and those of T
 template <int DTYPE>
@@ -303,7 +320,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
           mma_shared(elected, base, operand(sh.kq[x], 16) + step, operand(sh.kq[terms - x], 16) + step, instruction_bf16(2 * kChunk, false, false),
                      terms < 2 * kX - 2 || k > 0);
         }
-    mma_commit(elected, &sh.done[0]);
+    if (!test_no_commit(a.HV, hv, p.chunk0 + c, 0)) mma_commit(elected, &sh.done[0]);
     if (lane == 0 && hv % group == 0) {
       bulk_store(p.kq + (slot * a.H + h) * (kX * kPlanes * kPlane), sh.kq, kX * kPlanes * kPlane);
       bulk_commit();
@@ -317,7 +334,9 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
       *reinterpret_cast<uint4*>(sh.t[t] + plane_at(row, (row < kHalf ? 4 : 0) + tid % 4)) = make_uint4(0, 0, 0, 0);
     }
   }
+  float* const vec = p.vec + (slot * a.HV + hv) * kVec;
   if (!wait(0)) {
+    if (tid == 0) vec[kDecayAt + 1] = 1.0f;
     if (*poison)
       for (int k = 0; k < 1 << 12; ++k) __nanosleep(64);    // products in flight still use shared and tensor memory
     __syncthreads();
@@ -399,13 +418,12 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
     invert_block(sh, warp);
   } else if (warp < 4) {                          // the factors of the chunk's rows
     const int i = tid - 64;
-    float* vec = p.vec + (slot * a.HV + hv) * kVec;
     const bool there = i < live;
     vec[i] = there ? sh.beta[i] * sh.from_start[i] * sh.norm[i] : 0.0f;
     vec[kChunk + i] = sh.beta[i];
     vec[2 * kChunk + i] = there ? sh.to_end[i] * sh.norm[i] : 0.0f;
     vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.norm[kChunk + i] : i < n ? kNotANumber : 0.0f;
-    if (i < 8) vec[4 * kChunk + i] = live < n ? kNotANumber : sh.decay;
+    if (i < 8) vec[kDecayAt + i] = i > 0 ? 0.0f : live < n ? kNotANumber : sh.decay;
   }
   fence_proxy();
   fence_before();
@@ -420,7 +438,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
         for (int k = 0; k < kChunk / 16; ++k)
           mma_shared(elected, base, operand(sh.np[x], 16) + k * 2, operand(sh.t[terms - x], 16) + k * 128, instruction_bf16(kChunk, false, true),
                      terms < kTerms - 1 || x + k > 0);
-    mma_commit(elected, &sh.done[1]);
+    if (!test_no_commit(a.HV, hv, p.chunk0 + c, 1)) mma_commit(elected, &sh.done[1]);
   }
   bool healthy = wait(1);
   float2 pd[16];
@@ -448,7 +466,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
         for (int k = kHalf / 16; k < kChunk / 16; ++k)
           mma_shared(elected, base + kChunk, operand(sh.t[x], 16) + k * 2, operand(sh.np[terms - x], 16) + k * 128, instruction_bf16(kHalf, false, true),
                      terms < kTerms - 1 || x > 0 || k > kHalf / 16);
-    mma_commit(elected, &sh.done[2]);
+    if (!test_no_commit(a.HV, hv, p.chunk0 + c, 2)) mma_commit(elected, &sh.done[2]);
   }
   healthy = wait(2) && healthy;
   if (healthy && warp < 4 && quarter > 0) {       // the first half's columns of T's rows below the middle, and of P T
@@ -470,6 +488,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
   fence_before();
   __syncthreads();
   fence_after();
+  if (tid == 0 && !healthy) vec[kDecayAt + 1] = 1.0f;
   if (warp == kRowWarps) {
     if (lane == 0 && healthy) {
       bulk_store(p.t + (slot * a.HV + hv) * (kT * kPlane), sh.t, kT * kPlane);
@@ -765,7 +784,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
       vec[2 * kChunk + i] = there ? sh.to_end[i] * sh.key[i] : 0.0f;
       vec[3 * kChunk + i] = there ? sh.from_start[i] * sh.query[i] : i < n ? kNotANumber : 0.0f;
     }
-    if (lane < 8) vec[4 * kChunk + lane] = live < n ? kNotANumber : across.z;
+    if (lane < 8) vec[kDecayAt + lane] = lane > 0 ? 0.0f : live < n ? kNotANumber : across.z;
   }
 
   // The inverses of the blocks on the diagonal, by substitution, a column to a lane, two blocks at a time.
@@ -878,20 +897,6 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
 }
 
 // ---- along a sequence ------------------------------------------------------------------------------------------------
-
-// In the test-only build warps of every kind come late to some of their chunks, by more than the others' work on one: results must not depend on
-// it.  And there, of three value heads, the first copies of head 1's first chunk announce 16 bytes more than they bring: a wait runs out, and the
-// head's rows and state are left as they were.
-#ifdef CARRY_TEST_WAIT_EXPIRY
-__device__ __forceinline__ void test_come_late(int warp, int c) {
-  if (warp % 4 == c % 4 || (warp + c) % 5 == 0) __nanosleep(4000);
-}
-__device__ __forceinline__ uint32_t test_extra_bytes(int heads, int hv, int c) { return heads == 3 && hv == 1 && c == 0 ? 16 : 0; }
-#else
-__device__ __forceinline__ void test_come_late(int, int) {}
-__device__ __forceinline__ uint32_t test_extra_bytes(int, int, int) { return 0; }
-#endif
-
 
 // A CTA has 32 or 64 columns of a head's state.  Right sides lie with their three terms side by side, so that one product takes all terms and
 // reads its left side once: each in a plane of 64 columns, or two of 32 in one and the third in the first half of another.  Where two CTAs share
@@ -1036,7 +1041,12 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       const float* vec = sh.vec[c & 1];
       of_state = key ? -vec[token] : vec[3 * kChunk + token];
       of_added = vec[2 * kChunk + token];
-      next_decay = vec[4 * kChunk];
+      const float2 end = *reinterpret_cast<const float2*>(&vec[kDecayAt]);
+      next_decay = end.x;
+      if (end.y != 0.0f) {                        // the chunk's T is not there: the same for all rows, and the other warps stop at their waits
+        *poison = 1;
+        return false;
+      }
       if (!key) return true;                      // only keys' threads hold the values back
       const float beta = vec[kChunk + token];
       if (!kAlone && !wait(&sh.v_full, c & 1)) return false;
