@@ -42,6 +42,7 @@ struct ChunkParams {
   int aligned, out_aligned; // rows are on the grid of 16 bytes
   uint8_t *kq, *t;          // workspace: [place][H] tiles of keys and queries, [place][HV] tiles of T and P T,
   float* vec;               // [place][HV] factors of a chunk's rows
+  int* lost;                // [request of the launch][HV][D / 32] whether a wait ran out for these columns in the launches before; NULL where there is one launch
 };
 
 // A token with a key or a gate that is not a number makes the state so, from there on; products over a whole chunk must not carry that back to
@@ -60,7 +61,7 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int z, int* stat
 }
 
 // In the test-only build warps of every kind come late to some of their chunks, by more than the others' work on one: results must not depend on
-// it.  And there, of three value heads, the first copies of head 1's first chunk announce 16 bytes more than they bring: a wait runs out, and the
+// it.  A workspace is at most 64 MiB, so that calls are worked off in turns sooner.  And there, of three value heads, the first copies of head 1's first chunk announce 16 bytes more than they bring: a wait runs out, and the
 // head's rows and state are left as they were.  Of five value heads in fp32, nothing announces the end of the first product of head 1's second chunk,
 // of the second one of head 2's and of the third one of head 3's.
 #ifdef CARRY_TEST_WAIT_EXPIRY
@@ -950,6 +951,12 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
   const Place place = place_of(p, blockIdx.z, nullptr);
   const int from = p.chunk0 * kChunk, left = place.count - from, chunks = min((left + kChunk - 1) / kChunk, p.chunks);
   if (chunks <= 0 && p.chunk0 > 0) return;                  // the launches before have done with the request
+  auto lost = [&]() -> int& {                               // read anew where it is used: nothing of it takes a register in between
+    uint32_t x, y, z;
+    asm volatile("mov.u32 %0, %%ctaid.x;\nmov.u32 %1, %%ctaid.y;\nmov.u32 %2, %%ctaid.z;" : "=r"(x), "=r"(y), "=r"(z));
+    return p.lost[((int64_t)z * a.HV + y) * (D / 32) + x];
+  };
+  if (p.lost && p.chunk0 > 0 && lost()) return;             // final_state is not where they left off
   if (tid == 0) {
     sh.poison = 0;
     for (int i = 0; i < STAGES; ++i) {
@@ -1284,6 +1291,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
   }
   fence_before();
   __syncthreads();
+  if (p.lost && threadIdx.x == 0) lost() = *poison;
   if (warp == kIssueWarp) {
     __syncwarp();
     fence_after();
@@ -1297,14 +1305,18 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
 struct Layout {
   int requests, chunks, total;  // total: chunks of the longest request
   bool packed;
-  int64_t places, kq, t, vec;   // bytes
+  int64_t places, kq, t, vec, lost;   // bytes
 };
+#ifdef CARRY_TEST_WAIT_EXPIRY
+constexpr int64_t kWorkspaceBound = 1LL << 26;
+#else
 constexpr int64_t kWorkspaceBound = 1LL << 30;
+#endif
 
 Layout lay_out(const CarryGdnPrefillArgs& a) {
   const int64_t terms = a.qkv_dtype == CARRY_BF16 ? 1 : a.qkv_dtype == CARRY_F16 ? 2 : 3, terms_t = a.qkv_dtype == CARRY_F32 ? 3 : 2;
   const int64_t per_kq = a.H * terms * (a.K / 64) * kPlane, per_t = a.HV * terms_t * kPlane, per_vec = (int64_t)a.HV * kVec * 4;
-  const int64_t per = per_kq + per_t + per_vec;
+  const int64_t per_lost = (int64_t)a.HV * (a.K / 32) * 4, per = per_kq + per_t + per_vec + per_lost;
   Layout l;
   l.total = (a.max_query + kChunk - 1) / kChunk;
   const int64_t most = kWorkspaceBound / per > 1 ? kWorkspaceBound / per : 1, follows = a.N / kChunk + a.B, grid = (int64_t)a.B * l.total;
@@ -1321,6 +1333,7 @@ Layout lay_out(const CarryGdnPrefillArgs& a) {
   l.kq = l.places * per_kq;
   l.t = l.places * per_t;
   l.vec = l.places * per_vec;
+  l.lost = l.chunks < l.total ? l.requests * per_lost : 0;     // a launch has no more requests than places
   return l;
 }
 
@@ -1366,6 +1379,7 @@ int launch_chunks(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
   p.kq = static_cast<uint8_t*>(a.workspace);
   p.t = p.kq + l.kq;
   p.vec = reinterpret_cast<float*>(p.t + l.t);
+  if (l.lost) p.lost = reinterpret_cast<int*>(p.t + l.t + l.vec);
   for (int b = 0; b < a.B; b += l.requests)
     for (int c = 0; c < l.total; c += l.chunks) {
       p.b0 = b;
@@ -1405,7 +1419,7 @@ bool in_chunks(const CarryGdnPrefillArgs& a) { return a.max_query > (a.qkv_dtype
 int64_t delta_workspace(const CarryGdnPrefillArgs& a) {
   if (!in_chunks(a)) return 0;
   const Layout l = lay_out(a);
-  return l.kq + l.t + l.vec;
+  return l.kq + l.t + l.vec + l.lost;
 }
 
 int launch_delta(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
