@@ -696,6 +696,20 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
       if (t == g / 2 && !(square(diagonal[b], half) < INFINITY)) live = b * kBlock + g + 8 * half;
   }
   live = __reduce_min_sync(~0u, live);
+  if (!kHalfType && live < n && !a.use_qk_l2norm) {
+    // squares beyond fp32, which fp16's are not, matter to the norm alone: what is not finite is what products with zeros leave
+    live = n;
+#pragma unroll
+    for (int b = kBlocks - 1; b >= 0; --b) {
+      float none[4] = {};
+#pragma unroll
+      for (int s = 0; s < kWords; s += 2) mma16<kHalfType>(none, k[2 * b][s], k[2 * b + 1][s], k[2 * b][s + 1], k[2 * b + 1][s + 1], 0, 0);
+#pragma unroll
+      for (int half = 1; half >= 0; --half)
+        if (none[2 * half] != 0.0f) live = b * kBlock + g + 8 * half;
+    }
+    live = __reduce_min_sync(~0u, live);
+  }
   if (live < n) {                                 // the same for all lanes
 #pragma unroll
     for (int r = 0; r < 2 * kBlocks; ++r)
