@@ -394,6 +394,8 @@ int prefill_ok(const CarryGdnPrefillArgs* a) {
     if (!dtype_ok(t)) return CARRY_GDN_ERR_DTYPE;
   return CARRY_GDN_OK;
 }
+// how far what follows with this stride lies away
+int64_t apart(int64_t stride) { return stride < 0 ? -stride : stride; }
 // No request has more rows than the call: a looser bound costs nothing.
 CarryGdnPrefillArgs prefill_bounded(const CarryGdnPrefillArgs& a) {
   CarryGdnPrefillArgs bounded = a;
@@ -417,6 +419,7 @@ int carry_gdn_prefill(const CarryGdnPrefillArgs* a, void* stream) {
   for (const void* p : {(const void*)a->initial_state, (const void*)a->final_state})
     if (reinterpret_cast<uintptr_t>(p) % 16) return CARRY_GDN_ERR_SHAPE;
   if (a->stride_final_req % 4 || (a->initial_state && a->stride_initial_req % 4)) return CARRY_GDN_ERR_SHAPE;
+  if (a->B > 1 && apart(a->stride_final_req) < (int64_t)a->HV * a->V * a->K) return CARRY_GDN_ERR_SHAPE;     // requests' states would share numbers
   const CarryGdnPrefillArgs bounded = prefill_bounded(*a);
   const int64_t need = carry::delta_workspace(bounded);
   if (need < 0) return static_cast<int>(need);

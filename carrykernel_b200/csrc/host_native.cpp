@@ -734,6 +734,7 @@ PyObject* prefill(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (qk <= 0 || H <= 0 || HV % H || 2 * H * K != qk) return nullptr;
     for (const at::Tensor* t : {last, first})
       if (t && (!is(t, at::kFloat, dev) || !shaped(*t, {B, HV, V, K}) || !dense_inside(*t, {V * K, K, 1}))) return nullptr;
+    if (B > 1 && last->stride(0) < HV * V * K) return nullptr;
     if (!is(mixed, mixed->scalar_type(), dev) || mixed->stride(1) != 1) return nullptr;
     for (const at::Tensor* t : {a, b})
       if (!is(t, a->scalar_type(), dev) || !shaped(*t, {N, HV}) || t->stride(1) != 1) return nullptr;

@@ -45,6 +45,8 @@ def _prefill_args(mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, init
     if H <= 0 or HV % H != 0 or 2 * H * K != qk_dim:
         raise ValueError(f"cannot infer H from mixed_qkv width {width}")
     _state(final_state, (B, HV, V, K), "final_state")
+    if B > 1 and final_state.stride(0) < HV * V * K:
+        raise ValueError("final_state: requests' states must not share memory")
     if initial_state is not None:
         _state(initial_state, (B, HV, V, K), "initial_state")
     _lib.need_shape(a, (N, HV), "a")
