@@ -29,11 +29,10 @@ def _state(t, shape, name):
         raise ValueError(f"{name}: every request's state must start on a 16-byte boundary")
 
 
-def _prefill_args(mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, initial_state, query_start, max_query_len,
-                  use_qk_l2norm_in_kernel, status):
-    """Checks of a call and the filled argument block."""
-    if mixed_qkv.dim() != 2 or mixed_qkv.stride(-1) != 1:
-        raise ValueError("mixed_qkv must be 2-D [N, 2*H*K + HV*V] and contiguous in its last dimension")
+def _prefill_sizes(mixed_qkv, final_state, query_start, max_query_len):
+    """An argument block with a call's sizes, which is all that its workspace goes by."""
+    if mixed_qkv.dim() != 2:
+        raise ValueError("mixed_qkv must be 2-D [N, 2*H*K + HV*V]")
     if final_state.dim() != 4:
         raise ValueError(f"final_state must be 4-D [B, HV, V, K], got {tuple(final_state.shape)}")
     N, width = mixed_qkv.shape
@@ -44,6 +43,33 @@ def _prefill_args(mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, init
     H = qk_dim // (2 * K)
     if H <= 0 or HV % H != 0 or 2 * H * K != qk_dim:
         raise ValueError(f"cannot infer H from mixed_qkv width {width}")
+    args = _lib.PrefillArgs()
+    if query_start is None:
+        if B == 0 or N % B:
+            if N:
+                raise ValueError(f"{N} rows are not the same number for each of {B} requests: give query_start")
+        args.max_query = N // B if B else 0
+        if max_query_len is not None and int(max_query_len) != args.max_query:
+            raise ValueError(f"max_query_len is {max_query_len} but every request has {args.max_query} rows")
+    else:
+        if max_query_len is None or int(max_query_len) < 0:
+            raise ValueError("query_start needs max_query_len, the largest number of rows of a request")
+        if query_start.dtype != torch.int32 or not query_start.is_contiguous() or tuple(query_start.shape) != (B + 1,):
+            raise ValueError(f"query_start must be a contiguous int32 [{B + 1}]")
+        args.max_query = min(int(max_query_len), N)
+        args.query_start = query_start.data_ptr()
+    args.qkv_dtype = _lib.dtype_id(mixed_qkv)
+    args.B, args.N, args.H, args.HV, args.K, args.V = B, N, H, HV, K, V
+    return args
+
+
+def _prefill_args(mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, initial_state, query_start, max_query_len,
+                  use_qk_l2norm_in_kernel, status):
+    """Checks of a call and the filled argument block."""
+    args = _prefill_sizes(mixed_qkv, final_state, query_start, max_query_len)
+    N, (B, HV, V, K) = mixed_qkv.shape[0], final_state.shape
+    if mixed_qkv.stride(-1) != 1:
+        raise ValueError("mixed_qkv must be contiguous in its last dimension")
     _state(final_state, (B, HV, V, K), "final_state")
     if B > 1 and final_state.stride(0) < HV * V * K:
         raise ValueError("final_state: requests' states must not share memory")
@@ -63,22 +89,7 @@ def _prefill_args(mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, init
     dev = final_state.device
     _lib.same_device(dev, mixed_qkv=mixed_qkv, a=a, b=b, A_log=A_log, dt_bias=dt_bias, out=out, initial_state=initial_state,
                      query_start=query_start)
-    args = _lib.PrefillArgs()
-    if query_start is None:
-        if B == 0 or N % B:
-            if N:
-                raise ValueError(f"{N} rows are not the same number for each of {B} requests: give query_start")
-        args.max_query = N // B if B else 0
-        if max_query_len is not None and int(max_query_len) != args.max_query:
-            raise ValueError(f"max_query_len is {max_query_len} but every request has {args.max_query} rows")
-    else:
-        if max_query_len is None or int(max_query_len) < 0:
-            raise ValueError("query_start needs max_query_len, the largest number of rows of a request")
-        if query_start.dtype != torch.int32 or not query_start.is_contiguous() or tuple(query_start.shape) != (B + 1,):
-            raise ValueError(f"query_start must be a contiguous int32 [{B + 1}]")
-        args.max_query = min(int(max_query_len), N)
-        args.query_start = query_start.data_ptr()
-    args.mixed_qkv, args.stride_mixed_tok, args.qkv_dtype = mixed_qkv.data_ptr(), mixed_qkv.stride(0), _lib.dtype_id(mixed_qkv)
+    args.mixed_qkv, args.stride_mixed_tok = mixed_qkv.data_ptr(), mixed_qkv.stride(0)
     args.a, args.stride_a_tok, args.b, args.stride_b_tok = a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0)
     args.ab_dtype = _lib.dtype_id(a)
     args.A_log, args.A_log_dtype = A_log.data_ptr(), _lib.dtype_id(A_log)
@@ -89,7 +100,6 @@ def _prefill_args(mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, init
     args.out, args.stride_out_tok, args.out_dtype = out.data_ptr(), out.stride(0), _lib.dtype_id(out)
     args.status = _lib.status_ptr(status, dev)
     args.scale, args.use_qk_l2norm = float(scale), int(bool(use_qk_l2norm_in_kernel))
-    args.B, args.N, args.H, args.HV, args.K, args.V = B, N, H, HV, K, V
     return args
 
 
@@ -135,13 +145,9 @@ def gated_delta_rule_packed_prefill(mixed_qkv, a, b, A_log, dt_bias, scale, out,
 
 def prefill_workspace_bytes(mixed_qkv, final_state, query_start=None, max_query_len=None) -> int:
     """Bytes of workspace that :func:`gated_delta_rule_packed_prefill` needs for a call of these sizes on the state's device (on the
-    current one, where the state is on none)."""
+    current one, where the state is on none).  Nothing is read or allocated: tensors of no memory (``device="meta"``) will do."""
     lib = _lib._lib or _lib.load_library()
-    N, dev = mixed_qkv.shape[0], final_state.device
-    HV, V = final_state.shape[1:3]
-    gates, per_head = torch.empty((N, HV), device=dev), torch.empty(HV, device=dev)
-    out = mixed_qkv[:, mixed_qkv.shape[1] - HV * V:].unflatten(1, (HV, V))      # of the right shape; nothing is written
-    args = _prefill_args(mixed_qkv, gates, gates, per_head, per_head, 1.0, out, final_state, None, query_start, max_query_len, False, None)
+    args = _prefill_sizes(mixed_qkv, final_state, query_start, max_query_len)
     with torch.cuda.device_of(final_state):
         need = lib.carry_gdn_prefill_workspace(args)
     _lib.check(min(need, 0), "carry_gdn_prefill_workspace")
