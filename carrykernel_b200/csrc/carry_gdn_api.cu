@@ -420,6 +420,7 @@ int carry_gdn_prefill(const CarryGdnPrefillArgs* a, void* stream) {
     if (reinterpret_cast<uintptr_t>(p) % 16) return CARRY_GDN_ERR_SHAPE;
   if (a->stride_final_req % 4 || (a->initial_state && a->stride_initial_req % 4)) return CARRY_GDN_ERR_SHAPE;
   if (a->B > 1 && apart(a->stride_final_req) < (int64_t)a->HV * a->V * a->K) return CARRY_GDN_ERR_SHAPE;     // requests' states would share numbers
+  if (a->N > 1 && apart(a->stride_out_tok) < (int64_t)a->HV * a->V) return CARRY_GDN_ERR_SHAPE;
   const CarryGdnPrefillArgs bounded = prefill_bounded(*a);
   const int64_t need = carry::delta_workspace(bounded);
   if (need < 0) return static_cast<int>(need);

@@ -741,6 +741,7 @@ PyObject* prefill(PyObject*, PyObject* const* o, Py_ssize_t n) {
     for (const at::Tensor* t : {A_log, dt_bias})
       if (!is(t, t->scalar_type(), dev) || !shaped(*t, {HV}) || !t->is_contiguous()) return nullptr;
     if (!is(out, out->scalar_type(), dev) || !shaped(*out, {N, HV, V}) || !dense_inside(*out, {V, 1})) return nullptr;
+    if (N > 1 && out->stride(0) < HV * V) return nullptr;
     CarryGdnPrefillArgs p = {};
     p.qkv_dtype = dtype_id(mixed->scalar_type()); p.ab_dtype = dtype_id(a->scalar_type());
     p.A_log_dtype = dtype_id(A_log->scalar_type()); p.dt_bias_dtype = dtype_id(dt_bias->scalar_type()); p.out_dtype = dtype_id(out->scalar_type());

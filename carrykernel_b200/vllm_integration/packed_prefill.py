@@ -86,6 +86,8 @@ def _prefill_args(mixed_qkv, a, b, A_log, dt_bias, scale, out, final_state, init
     _lib.need_shape(out, (N, HV, V), "out")
     if out.stride()[1:] != (V, 1):
         raise ValueError("out must be dense within a token (only the token stride may vary)")
+    if N > 1 and out.stride(0) < HV * V:
+        raise ValueError("out: tokens' rows must not share memory")
     dev = final_state.device
     _lib.same_device(dev, mixed_qkv=mixed_qkv, a=a, b=b, A_log=A_log, dt_bias=dt_bias, out=out, initial_state=initial_state,
                      query_start=query_start)
