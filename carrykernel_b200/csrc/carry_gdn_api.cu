@@ -396,6 +396,14 @@ int prefill_ok(const CarryGdnPrefillArgs* a) {
 }
 // how far what follows with this stride lies away
 int64_t apart(int64_t stride) { return stride < 0 ? -stride : stride; }
+// Whether runs of `width` numbers lie apart, m of them by one stride and n by another, the smaller stride's within the larger one.
+bool runs_apart(int64_t m, int64_t stride_m, int64_t n, int64_t stride_n, int64_t width) {
+  const int64_t one = apart(stride_m), two = apart(stride_n);
+  if (m == 0 || n == 0) return true;
+  if (m <= 1 || n <= 1) return (m <= 1 || one >= width) && (n <= 1 || two >= width);
+  const int64_t small = one < two ? one : two, large = one < two ? two : one, count = one < two ? m : n;
+  return small >= width && (large - width) / small >= count - 1;
+}
 // No request has more rows than the call: a looser bound costs nothing.
 CarryGdnPrefillArgs prefill_bounded(const CarryGdnPrefillArgs& a) {
   CarryGdnPrefillArgs bounded = a;
@@ -450,6 +458,8 @@ int carry_gdn_qk_norm_rope(const CarryGdnRotateArgs* a, void* stream) {
   if (a->N == 0 || (a->HQ == 0 && a->HK == 0)) return CARRY_GDN_OK;
   if (!a->positions || (a->rotary > 0 && a->table_rows > 0 && !a->cos_sin)) return CARRY_GDN_ERR_NULL;
   if ((a->HQ > 0 && (!a->q || !a->q_out || !a->q_weight)) || (a->HK > 0 && (!a->k || !a->k_out || !a->k_weight))) return CARRY_GDN_ERR_NULL;
+  if (!runs_apart(a->N, a->stride_q_out_tok, a->HQ, a->stride_q_out_head, a->D) || !runs_apart(a->N, a->stride_k_out_tok, a->HK, a->stride_k_out_head, a->D))
+    return CARRY_GDN_ERR_SHAPE;
   const int rc = carry::launch_rotate(*a, static_cast<cudaStream_t>(stream));
   if (rc == CARRY_GDN_OK) g_last_kernel = 12;
   return rc;

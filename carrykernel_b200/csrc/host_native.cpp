@@ -791,6 +791,18 @@ PyObject* prefill(PyObject*, PyObject* const* o, Py_ssize_t n) {
   });
 }
 
+// whether no two rows of [N, heads, D] share memory, the rows along the smaller stride lying within the larger one
+bool rows_apart(const at::Tensor& t) {
+  int64_t within = t.size(2);
+  const int inner = t.stride(0) < t.stride(1) ? 0 : 1;
+  for (int d : {inner, 1 - inner}) {
+    if (t.size(d) <= 1) continue;
+    if (t.stride(d) < within) return false;
+    within = t.stride(d) * (t.size(d) - 1) + t.size(2);
+  }
+  return true;
+}
+
 // (table, q, k, q_weight, k_weight, cos_sin, positions, eps, q_out, k_out, sections, interleaved, weight_offset, status) -> True
 PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -811,6 +823,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
       if (!is(t, q->scalar_type(), dev) || !shaped(*t, {N, HQ, D}) || t->stride(2) != 1) return nullptr;
     for (const at::Tensor* t : {k, k_out})
       if (!is(t, q->scalar_type(), dev) || !shaped(*t, {N, HK, D}) || t->stride(2) != 1) return nullptr;
+    for (const at::Tensor* t : {q_out, k_out})
+      if (!rows_apart(*t)) return nullptr;
     for (const at::Tensor* t : {qw, kw})
       if (!is(t, qw->scalar_type(), dev) || !shaped(*t, {D}) || !t->is_contiguous()) return nullptr;
     if (!is(table, table->scalar_type(), dev) || table->dim() != 2 || table->stride(1) != 1 || table->size(1) > D) return nullptr;

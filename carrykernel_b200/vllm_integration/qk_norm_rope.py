@@ -17,6 +17,12 @@ MAX_WIDTH = 512
 MAX_AXES = 4
 
 
+def _apart(t):
+    """Whether no two rows of ``t [N, heads, D]`` share memory, the rows along the smaller stride lying within the larger one."""
+    steps = sorted((s, n) for s, n in zip(t.stride(), t.shape[:2]) if n > 1)
+    return all(s >= within for (s, _), within in zip(steps, [t.shape[2]] + [s * (n - 1) + t.shape[2] for s, n in steps]))
+
+
 def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps: float = 1e-6, q_out=None, k_out=None, sections=None,
                  interleaved: bool = False, weight_offset: float = 0.0, status=None):
     """``y = x * rsqrt(mean(x ** 2) + eps) * (weight + weight_offset)`` for every head ``x`` of ``q [N, HQ, D]`` and ``k [N, HK, D]``
@@ -49,6 +55,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps: float = 1e-6
             raise ValueError(f"{name} must be contiguous in its last dimension")
         if t.dtype != q.dtype:
             raise ValueError("q, k, q_out and k_out must share a dtype")
+    for name, t in (("q_out", q_out), ("k_out", k_out)):
+        if N and t.shape[1] and not _apart(t):
+            raise ValueError(f"{name}: rows that are written must not share memory")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
         _lib.need_shape(t, (D,), name)
         if not t.is_contiguous() or t.dtype != q_weight.dtype:
