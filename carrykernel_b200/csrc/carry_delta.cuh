@@ -10,6 +10,10 @@ namespace carry {
 
 constexpr float kL2Eps = 1e-6f;
 
+// What makes a key or query with this sum of squares one of length `by`.  Of one whose squares pass fp32 nothing is known: NaN, and not the 0 that a
+// division by infinity gives.
+__device__ __forceinline__ float norm_factor(float squares, float by) { return squares < INFINITY ? __fdiv_rn(by, sqrtf(squares + kL2Eps)) : __builtin_nanf(""); }
+
 // A request's rows, brought into bounds.
 struct PrefillRequest {
   int first, count;

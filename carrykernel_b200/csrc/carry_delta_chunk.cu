@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
     wait_loads();
 #pragma unroll
     for (int j = 0; j < 32; ++j) square = j == lane ? x[j] : square;
-    sh.norm[row] = (a.use_qk_l2norm ? __fdiv_rn(1.0f, sqrtf(square + kL2Eps)) : 1.0f) * (key ? 1.0f : a.scale);
+    sh.norm[row] = (a.use_qk_l2norm ? norm_factor(square, 1.0f) : 1.0f) * (key ? 1.0f : a.scale);
   }
   __syncthreads();
   if (warp < kRowWarps) {
@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(kUnitWarps * 32, 2) unit_kernel(const __grid_c
   auto norms = [&](const Part& d, float by, float* to) {
     if (t != g / 2) return;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) to[g + 8 * half] = a.use_qk_l2norm ? __fdiv_rn(by, sqrtf(square(d, half) + kL2Eps)) : by;
+    for (int half = 0; half < 2; ++half) to[g + 8 * half] = a.use_qk_l2norm ? norm_factor(square(d, half), by) : by;
   };
   Part diagonal[kBlocks];
   int live = n;

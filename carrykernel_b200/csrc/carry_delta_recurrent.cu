@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, ROWS == 4 || DTYPE == CARRY_F32 ? 4 
           kq = fma2(k[e], q[e], kq);
         }
       }
-      const float query = a.use_qk_l2norm ? __fdiv_rn(a.scale, sqrtf(over_lanes(qq.x + qq.y) + kL2Eps)) : a.scale;
-      const float key = a.use_qk_l2norm ? __fdiv_rn(1.0f, sqrtf(over_lanes(kk.x + kk.y) + kL2Eps)) : 1.0f;
+      const float query = a.use_qk_l2norm ? norm_factor(over_lanes(qq.x + qq.y), a.scale) : a.scale;
+      const float key = a.use_qk_l2norm ? norm_factor(over_lanes(kk.x + kk.y), 1.0f) : 1.0f;
       const float product = over_lanes(kq.x + kq.y) * query * key;
       if (lane == 0) {
         factors[t].query = query;

@@ -457,7 +457,8 @@ int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* args, void* stream);
  * without rows hands its state on.  A key or a gate that is not finite makes the
  * state of the heads that read it NaN from its token on, a value its row of the
  * state; outputs ahead of it are what they were.  With use_qk_l2norm the squares
- * of a key's numbers have to add up to less than fp32's largest number.  A token's
+ * of a key's numbers, and of a query's, have to add up to less than fp32's largest number: where a
+ * query's do not, its token's outputs are NaN, and where a key's do not, the state and the outputs from its chunk or token on.  A token's
  * decay below exp(-200) is 0.  K and V are 64 or 128 (one width for both), B and HV at most 65535, N at most 2^30.
  * final_state may be initial_state.  `workspace` is at least
  * carry_gdn_prefill_workspace() bytes, 16-byte aligned; nothing is kept in it
