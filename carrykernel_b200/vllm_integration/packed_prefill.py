@@ -113,8 +113,15 @@ def gated_delta_rule_packed_prefill(mixed_qkv, a, b, A_log, dt_bias, scale, out,
     ``scale`` as in ``quantized_gated_delta_rule_packed_decode``; ``out [N, HV, V]``; ``initial_state`` (``None`` for zeros)
     and ``final_state`` fp32 ``[B, HV, V, K]``, which may be one tensor.  Every request has ``N / B`` rows, or, with ``query_start [B + 1]``
     (int32), rows ``query_start[b] .. query_start[b + 1] - 1``, ``max_query_len`` of them at most; a request without rows hands its
-    state on.  ``K = V`` is 64 or 128.  A key or a gate that is not finite makes the state of the heads that read it NaN from its token on, a
-    value its row of the state; outputs ahead of it are what they were.
+    state on.  ``query_start`` does not fall: where it does, that is flagged, and what the call's rows and states get is not defined.
+    ``K = V`` is 64 or 128.  What is written shares no memory with another part of it or, ``initial_state`` apart, with an input.
+
+    A key that is not finite, and a decay or write strength that is NaN, leave the state of the heads that read them not finite from their token
+    on, a value its row of the state, a number of ``initial_state`` its row; outputs ahead of it are what they were.  With
+    ``use_qk_l2norm_in_kernel`` the squares of a key's numbers, and of a query's, have to add up to less than fp32's largest number.
+
+    Few tokens go one by one, more in chunks (the rule is by ``max_query_len``, the type and the number of heads).  The two ways agree within the
+    precision of each, not to the bit: in bf16 some two of a thousand outputs fall to the neighbouring number.
 
     ``workspace`` (uint8, at least :func:`prefill_workspace_bytes`) is allocated by the call when it is not given; calls that may run at the
     same time need one each.  ``status`` as in

@@ -453,18 +453,27 @@ int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* args, void* stream);
  * b are query_start[b] .. query_start[b + 1] - 1 (at most max_query; more, and
  * rows outside 0 .. N - 1, are skipped and flagged with
  * CARRY_GDN_STATUS_BAD_RANGE), or, with query_start NULL, max_query = N / B
- * each.  No two requests share a row, and other rows are left alone.  A request
- * without rows hands its state on.  A key or a gate that is not finite makes the
- * state of the heads that read it NaN from its token on, a value its row of the
- * state; outputs ahead of it are what they were.  With use_qk_l2norm the squares
+ * each.  query_start does not fall: no two requests share a row, and other rows are left alone.  Where it does fall,
+ * CARRY_GDN_STATUS_BAD_RANGE is set, and what the call's rows and states get is not defined.  A request
+ * without rows hands its state on.
+ *
+ * A key that is not finite, and a decay or a write strength that is NaN, leave the
+ * state of the heads that read them not finite from their token on, a value its row of
+ * the state, a number of initial_state its row; outputs ahead of it and other rows are what
+ * they were.  In chunks such a row is NaN throughout, and states and values count as infinite beyond bf16's largest
+ * number (3.39e38).  With use_qk_l2norm the squares
  * of a key's numbers, and of a query's, have to add up to less than fp32's largest number: where a
  * query's do not, its token's outputs are NaN, and where a key's do not, the state and the outputs from its chunk or token on.  A token's
- * decay below exp(-200) is 0.  K and V are 64 or 128 (one width for both), B and HV at most 65535, N at most 2^30.
- * final_state may be initial_state.  `workspace` is at least
+ * decay below exp(-200) is 0.
+ *
+ * K and V are 64 or 128 (one width for both), B and HV at most 65535, N at most 2^30.
+ * final_state may be initial_state; outputs share no memory with inputs other than that, nor with
+ * one another (a stride of final_state or out below a request's or token's size is refused).
+ * `workspace` is at least
  * carry_gdn_prefill_workspace() bytes, 16-byte aligned; nothing is kept in it
  * between calls, and two that may run at a time need one each.  It is at most some 1 GiB: what does not fit is worked off in
- * turns.  Where a wait runs out (CARRY_GDN_STATUS_TIMEOUT), the head's further
- * outputs and its state are left as they were.
+ * turns.  Where a wait runs out (CARRY_GDN_STATUS_TIMEOUT), the further outputs and the state of the
+ * columns (32 or 64 of a head's V) that waited are left as they were.
  */
 typedef struct CarryGdnPrefillArgs {
   const void* mixed_qkv;      /* [N, 2*H*K + HV*V] = q | k | v, as in carry_gdn_packed_decode */
@@ -510,7 +519,8 @@ int64_t carry_gdn_prefill_workspace(const CarryGdnPrefillArgs* args);
  * with CARRY_GDN_STATUS_BAD_RANGE.  A head with a number that is not finite
  * becomes NaN.  Squares below fp32's range count as 0: eps stands in for them.
  * q_out and k_out may be q and k.  D is even and at most 512, rotary even and at
- * most D, axes 1 to 4, HQ and HK at most 65535.
+ * most D, axes 1 to 4, HQ and HK at most 65535.  Heads that are written share no memory: along the
+ * smaller of an output's two strides they have to lie within the larger one.
  */
 typedef struct CarryGdnRotateArgs {
   const void* q;          /* [N, HQ, D], D contiguous */
