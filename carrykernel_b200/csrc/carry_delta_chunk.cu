@@ -11,18 +11,23 @@
 //   [K; Q] S  (128 x 32, over K),   [T; P T] R  (128 x 32, over 64 tokens),   K^T U  (K x 32, over 64 tokens).
 // The state itself stays in registers, in fp32; its products take it as a sum of bf16 numbers.
 //
-// What bounds it.  One prompt of 8192 tokens, 32 heads of 128 over 16: 400 us, of which unit_kernel takes 118 and the 128 steps of sequence_kernel
+// What bounds it.  One prompt of 8192 tokens, 32 heads of 128 over 16: 400 us, of which unit_kernel takes some 120 and the 128 steps of sequence_kernel
 // 2.2 us each.  A step is a chain: its products take 1.7 of 3.9 thousand cycles (a left side of 128 rows is 4 KB of shared memory for 16 steps of the
 // sum, whatever the columns, so a product of 32 columns times three terms runs at 60 % of the rate of one of 128), and between them a row's numbers
 // go from tensor memory through the registers of the two schedulers that own the keys' lanes, as three bf16 numbers each, into shared memory.  With
-// two CTAs to a processor (sixteen prompts of 4096: 2.45 ms, 98 TFLOP/s of the recurrence's own operations) the chains overlap, and the same
+// two CTAs to a processor (sixteen prompts of 4096: 2.4 to 2.5 ms from box to box, 96 to 99 TFLOP/s of the recurrence's own operations) the chains overlap, and the same
 // traffic of shared memory bounds: 240 KB a chunk, 1900 cycles of 3300.  Two chains in one CTA that share its tiles came out no faster, nor did
 // truncated terms, stores by a warp of their own, or workspaces that the second-level cache holds (400 us -> 530, for every launch has its own start).
 //
 // Precision.  Keys and queries in bf16 are operands as they are (norms and decays multiply rows of the products, in fp32); in fp16 they are
-// the sum of two bf16 numbers, in fp32 of three.  What is computed is split too: S, R and U into three, T into two (three with fp32
-// operands), and products of terms are formed down to 2^-18 of the largest.  The final state is then within 1e-6 of the
-// recurrence in 64 bits; two terms throughout would leave it 3.5e-6 off, and one (plain bf16 products) 2.4e-3.
+// the sum of two bf16 numbers, in fp32 of three.  What is computed is split too: S, R and U into three, of whose products the terms below 2^-18 of the
+// largest are left out, and T and P T into two, or three with fp32 operands.  Two are a choice: a third would be 16 KB more to a chunk, for
+// which two CTAs do not fit a processor, and an entry is 2.4e-6 off in the mean, all of it behind a diagonal that is exact.  P T's products
+// take two terms as well: with all of them outputs are 1.7e-6 off ahead of their rounding and not 2.7e-6 (of bf16 ones 1.3 of a thousand fall to the
+// other side and not 1.9; in plain fp32 arithmetic 0.2), for 27 us more of 8192 tokens.  Beyond that, decays are good to 2^-22 (ex2.approx, of differences
+// that two fp32 numbers hold) and sums on the tensor cores are cut to fp32, not rounded.  The final state is 5e-7 to 7e-7 off the
+// recurrence in 64 bits, in fp32 5e-7 (outputs too; in plain fp32 arithmetic 1.5e-7 to 1.9e-7); behind strong decays among slow ones 6e-7 at most.
+// Two terms throughout would leave it 3.5e-6 off, and one (plain bf16 products) 2.4e-3.
 #include <cuda_pipeline_primitives.h>
 
 #include "carry_delta.cuh"
@@ -503,7 +508,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) prepare_kernel(const __gri
 
 // ---- the same, a chunk and head to a warp ----------------------------------------------------------------------------
 //
-// For 16-bit keys and queries; 6200 instructions a warp, two warps to a scheduler (keys alone take half of a thread's registers), 29 ns a chunk and
+// For 16-bit keys and queries; 6300 instructions a warp, two warps to a scheduler (keys alone take half of a thread's registers), 29 ns a chunk and
 // head over the whole GPU.  What bounds it is latency: an instruction in 4.4 cycles.  The form by tensor memory that fp32 has takes 44 ns.
 // Everything is a product of 16 x 16 blocks whose operands are registers: a lane's part of a product's result
 // is its part of the next one's left side, or of its right side transposed, so T^T and (P T)^T are built block by block,
@@ -550,7 +555,7 @@ __device__ __forceinline__ Split split(const Part& p) {
   }
   return s;
 }
-// c += a b^T, of terms whose numbers add up to less than TERMS
+// c += a b^T, of terms whose numbers add up to less than TERMS: what is left out is 2^-27 of it with three, 2^-18 with two
 template <int TERMS>
 __device__ __forceinline__ void multiply(Part& c, const Split& a, const Split& b) {
 #pragma unroll
@@ -1413,7 +1418,7 @@ int launch_chunks(const CarryGdnPrefillArgs& a, cudaStream_t stream) {
                               stream, p);
       if (rc != CARRY_GDN_OK) return rc;
       // one CTA to a processor while that is all there are (a prompt of 2048 tokens with 32 heads: 117 us, 146 in the other form; two of them 228 and 211)
-      // More CTAs than that: in bf16 two to a processor (sixteen prompts of 4096 tokens 2.40 ms, 2.59 with 64 columns to one CTA); in fp16, whose keys and
+      // More CTAs than that: in bf16 two to a processor (sixteen prompts of 4096 tokens, side by side, 2.40 ms, 2.59 with 64 columns to one CTA); in fp16, whose keys and
       // queries fill shared memory, 64 columns, for which the left sides are read once and not twice (two prompts of 3001: 323 us and not 410); in
       // fp32 as well where there is room, at 64 wide (eight of 1000: 384 us and not 441).
       const bool alone = (int64_t)requests * a.HV * (D / 32) <= sm_count();
