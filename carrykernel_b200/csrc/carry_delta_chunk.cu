@@ -66,19 +66,24 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int z, int* stat
 }
 
 // In the test-only build warps of every kind come late to some of their chunks, by more than the others' work on one: results must not depend on
-// it.  A workspace is at most 64 MiB, so that calls are worked off in turns sooner.  And there, of three value heads, the first copies of head 1's first chunk announce 16 bytes more than they bring: a wait runs out, and the
-// head's rows and state are left as they were.  Of five value heads in fp32, nothing announces the end of the first product of head 1's second chunk,
-// of the second one of head 2's and of the third one of head 3's.
+// it.  A workspace is at most 64 MiB, so that calls are worked off in turns sooner.  And there, of three value heads, the first copies of head 1's first
+// chunk announce 16 bytes more than they bring: a wait runs out, and the head's rows and state are left as they were.  Of five value heads in fp32, nothing announces the end of the first product of head 1's second chunk,
+// of the second one of head 2's and of the third one of head 3's,
+// and some warps hold the others up for longer than a poll takes.
 #ifdef CARRY_TEST_WAIT_EXPIRY
 __device__ __forceinline__ void test_come_late(int warp, int c) {
   if (warp % 4 == c % 4 || (warp + c) % 5 == 0) __nanosleep(4000);
 }
 __device__ __forceinline__ uint32_t test_extra_bytes(int heads, int hv, int c) { return heads == 3 && hv == 1 && c == 0 ? 16 : 0; }
 __device__ __forceinline__ bool test_no_commit(int heads, int hv, int chunk, int product) { return heads == 5 && hv == 1 + product && chunk == 1; }
+__device__ __forceinline__ void test_hold_up(int heads, int warp) {
+  if (heads == 5 && warp % 4 == 1) __nanosleep(500000);
+}
 #else
 __device__ __forceinline__ void test_come_late(int, int) {}
 __device__ __forceinline__ uint32_t test_extra_bytes(int, int, int) { return 0; }
 __device__ __forceinline__ bool test_no_commit(int, int, int, int) { return false; }
+__device__ __forceinline__ void test_hold_up(int, int) {}
 #endif
 
 // bf16 numbers that a key's or query's numbers come as, and those of T
@@ -935,7 +940,7 @@ struct SequenceShared {
   // written, one read and one made ready
   int bad[3][COLUMNS], any_bad[3];
   uint32_t tmem;
-  int poison;
+  int poison, at_end;       // warps of rows that have met a chunk without its T
 };
 
 // this thread's columns of each term's product, summed, the smallest first
@@ -977,7 +982,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
   };
   if (p.lost && p.chunk0 > 0 && lost()) return;             // final_state is not where they left off
   if (tid == 0) {
-    sh.poison = 0;
+    sh.poison = sh.at_end = 0;
     for (int i = 0; i < STAGES; ++i) {
       barrier_init(&sh.full[i], 1);
       barrier_init(&sh.free[i], 1);
@@ -1069,8 +1074,9 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
       of_added = vec[2 * kChunk + token];
       const float2 end = *reinterpret_cast<const float2*>(&vec[kDecayAt]);
       next_decay = end.x;
-      if (end.y != 0.0f) {                        // the chunk's T is not there: the same for all rows, and the other warps stop at their waits
-        *poison = 1;
+      if (end.y != 0.0f) {                        // the chunk's T is not there.  All rows' warps get here, with all done that the chunks ahead give; then the others stop
+        __syncwarp();
+        if (lane == 0 && atomicAdd(&sh.at_end, 1) == kRowThreads / 32 - 1) *poison = 1;
         return false;
       }
       if (!key) return true;                      // only keys' threads hold the values back
@@ -1131,6 +1137,7 @@ __global__ void __launch_bounds__(GROUPS * 128 + 64, STAGES == 1 && DTYPE == CAR
         barrier_arrive(&sh.u_ready);
       }
       test_come_late(warp, c + 1);
+      test_hold_up(a.HV, warp);
       if (tid < COLUMNS) sh.bad[(c + 2) % 3][tid] = kChunk;
       if (tid == 0) sh.any_bad[(c + 2) % 3] = 0;
       healthy = wait(&sh.solved, parity);

@@ -30,3 +30,15 @@ def test_a_chunk_that_was_not_worked_out_is_not_used(D, H, lengths):
     status.zero_()
     again = run(c, state, lengths, HV, D, status=status)
     assert status.item() == 0 and torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+@pytest.mark.parametrize("D,B", [(64, 2), (128, 4)])
+def test_outputs_ahead_of_the_chunk_are_all_there(D, B):
+    """Whichever warp sees first that a chunk was not worked out, all have left what the chunk ahead of it gives."""
+    HV, n = 5, 200
+    c, state = make([n] * B, 1, HV, D, F32, True)
+    want = run(c, state, [n] * B, HV, D)[0].unflatten(0, (B, n))
+    with wait_test_library():
+        for _ in range(30):
+            out = run(c, state, [n] * B, HV, D)[0].unflatten(0, (B, n))
+            assert torch.equal(out[:, :64], want[:, :64]) and out[:, 64:, 1:4].isnan().all()
