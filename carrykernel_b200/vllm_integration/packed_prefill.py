@@ -118,7 +118,8 @@ def gated_delta_rule_packed_prefill(mixed_qkv, a, b, A_log, dt_bias, scale, out,
 
     A key that is not finite, and a decay or write strength that is NaN, leave the state of the heads that read them not finite from their token
     on, a value its row of the state, a number of ``initial_state`` its row; outputs ahead of it are what they were.  With
-    ``use_qk_l2norm_in_kernel`` the squares of a key's numbers, and of a query's, have to add up to less than fp32's largest number.
+    ``use_qk_l2norm_in_kernel`` the squares of a key's numbers, and of a query's, have to add up to less than fp32's largest number; without it
+    products of two keys, and of a key and a query, that are less than 64 tokens apart have to be in its range.
 
     Few tokens go one by one, more in chunks (the rule is by ``max_query_len``, the type and the number of heads).  The two ways agree within the
     precision of each, not to the bit: in bf16 some two of a thousand outputs fall to the neighbouring number.

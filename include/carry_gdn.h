@@ -463,8 +463,9 @@ int carry_gdn_add_rms_norm_quant(const CarryGdnNormArgs* args, void* stream);
  * they were.  In chunks such a row is NaN throughout, and states and values count as infinite beyond bf16's largest
  * number (3.39e38).  With use_qk_l2norm the squares
  * of a key's numbers, and of a query's, have to add up to less than fp32's largest number: where a
- * query's do not, its token's outputs are NaN, and where a key's do not, the state and the outputs from its chunk or token on.  A token's
- * decay below exp(-200) is 0.
+ * query's do not, its token's outputs are NaN, and where a key's do not, the state and the outputs from its chunk or token on.  Without it
+ * the products of a key with the other keys, and with the queries, of its 64 tokens have to be in fp32's range, whatever their write strengths.
+ * A token's decay below exp(-200) is 0.
  *
  * K and V are 64 or 128 (one width for both), B and HV at most 65535, N at most 2^30.
  * final_state may be initial_state; outputs share no memory with inputs other than that, nor with
